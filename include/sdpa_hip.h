@@ -70,7 +70,13 @@ typedef enum {
     SDPA_ERR_WORKSPACE = 22,
     SDPA_ERR_HIP = 23,
     SDPA_ERR_SCRATCH_LIMIT = 24,
-    SDPA_ERR_DS_PATH = 25
+    SDPA_ERR_DS_PATH = 25,
+    SDPA_ERR_ROTARY = 26,
+    SDPA_ERR_PAGE_SIZE = 27,
+    SDPA_ERR_HEADS = 28,
+    SDPA_ERR_LAYOUT = 29,
+    SDPA_ERR_TOO_LARGE = 30,
+    SDPA_ERR_WEIGHT = 31
 } sdpa_status_t;
 
 /* Message for a status code (static storage, never NULL). */
@@ -218,6 +224,77 @@ uint64_t sdpa_hip_drop_threshold(float dropout);
  * [B, S_q, S_kv], computed by the kernels' own hash code.  For tests.       */
 int sdpa_hip_dropout_mask(uint8_t* keep, int B, int S_q, int S_kv, float dropout, uint64_t seed,
                           uint64_t offset, hipStream_t stream);
+
+/* ---- norm and rotation of queries and keys ---------------------------------
+ * No counterpart in the reference: what a layer does to its queries and keys
+ * before Sdpa, in one launch for both.  For every head row x of D features
+ *   n = weight x / sqrt(mean(x^2) + eps)   (norm; else n = x)
+ *   y = n with its first R features turned by the row's position: the pairs
+ *       (i, i + R/2), or (2i, 2i + 1) if interleaved, to
+ *       (a c - b s, b c + a s), c = cos[position][i], s = sin[position][i]
+ * in fp32, rounded once.  q is [B, S, H_q, D], k [B, S, H_kv, D] with dense
+ * features and any other strides ({batch, token, head}, in elements); the
+ * results go where their strides say: {H S D, D, S D} is the [B H, S, D] that
+ * sdpa_hip_fwd reads.  A result may be the input itself (same strides).
+ * cos, sin: float [table_rows, R / 2]; positions: int32 [S] (or [B, S] with
+ * positions_per_batch), NULL for 0 .. S - 1; a position outside the tables
+ * makes its rows NaN.  Weights: [D] of weight_dtype (that of q or
+ * SDPA_DTYPE_F32) or NULL.  H_q or H_kv may be 0.  D <= 128.                  */
+int sdpa_hip_qk_norm_rope(int dtype, const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, void* q_out, const int64_t* q_out_strides, void* k_out,
+                          const int64_t* k_out_strides, const void* q_weight, const void* k_weight,
+                          int weight_dtype, const float* cos, const float* sin, int table_rows,
+                          const int32_t* positions, int positions_per_batch, int B, int S, int H_q, int H_kv,
+                          int D, int R, float eps, int norm, int interleaved, hipStream_t stream);
+
+/* Its gradient: d_q_out and d_k_out as the results were laid out, dq and dk
+ * as their strides say, dq_weight and dk_weight [D] of weight_dtype (NULL: not
+ * wanted; they need no weight in the forward call).  The weights' gradients are
+ * summed in fp32 in a fixed order from the workspace,
+ * sdpa_hip_qk_norm_rope_grad_workspace_bytes(D) bytes, 16-byte aligned; without
+ * them it may be NULL.                                                        */
+size_t sdpa_hip_qk_norm_rope_grad_workspace_bytes(int D);
+
+int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_q_out_strides,
+                               const void* d_k_out, const int64_t* d_k_out_strides, const void* q,
+                               const int64_t* q_strides, const void* k, const int64_t* k_strides, void* dq,
+                               const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dq_weight,
+                               void* dk_weight, const void* q_weight, const void* k_weight, int weight_dtype,
+                               const float* cos, const float* sin, int table_rows, const int32_t* positions,
+                               int positions_per_batch, void* workspace, size_t workspace_bytes, int B, int S,
+                               int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
+                               hipStream_t stream);
+
+/* ---- paged cache -------------------------------------------------------------
+ * No counterpart in the reference.  Keys and values of N sequences lie in pages
+ * of page_size tokens (a power of two, 16 .. 65536): k_cache [pages, H_kv, page_size,
+ * D_qk], v_cache [pages, H_kv, page_size, D_v], dense, so that a page's head is a
+ * dense matrix as the op's k and v are.  T new tokens are packed, sequence after
+ * sequence; device arrays of int32 say what belongs where:
+ *   q_starts [N + 1]    sequence s has the new tokens q_starts[s] ..
+ *                       q_starts[s + 1] - 1 (none: not in this call);
+ *   kv_lens [N]         its cached tokens, the new ones among them, last;
+ *   page_table [N, width] (rows page_table_stride apart): token j of s is row
+ *                       j % page_size of page page_table[s][j / page_size].
+ * They are read on the device only, so a captured call follows them.  Nothing
+ * outside of the T tokens, the width columns and the pages is touched whatever
+ * they hold.                                                                  */
+
+/* Keys and values of the new tokens into their places, k normed (norm) and
+ * rotated by its place in the sequence on the way as above (R = 0: not
+ * rotated), and the queries of the same tokens, normed and rotated, to q_out
+ * (H_q = 0: none).  q, k, v, q_out: [T, H, D] with dense features and strides
+ * {token, head} in elements.  q_out may be q.  Tokens behind the last sequence leave
+ * everything as it was; a token whose place is outside of the table's columns or
+ * of the pages is not appended, and its row of q_out is NaN.  Two tokens of one
+ * call must not have the same place.                                          */
+int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
+                       const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                       const float* cos, const float* sin, int table_rows, const int32_t* page_table,
+                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
+                       int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
+                       int norm, int interleaved, hipStream_t stream);
 
 #ifdef __cplusplus
 }

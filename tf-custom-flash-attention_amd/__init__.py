@@ -13,6 +13,11 @@ Tensors are torch tensors on the GPU (torch is only the device-memory and
 stream plumbing here); all arithmetic runs in the hand-written HIP kernels of
 ``libsdpa_hip.so`` through the C ABI in ``include/sdpa_hip.h``.  There is no
 CPU fallback: if the library is missing, every entry point raises.
+
+Around the op (:mod:`.heads`): ``qk_norm_rope`` and its gradient norm and
+rotate the queries and keys of a layer into the layout that ``sdpa`` reads;
+``kv_append`` puts new tokens into the pages of a cache and ``paged_sdpa``
+attends over them.
 """
 from __future__ import annotations
 
@@ -31,7 +36,7 @@ SDPA_OK = 0
 SDPA_ERR_HIP = 23
 SDPA_ERR_SCRATCH_LIMIT = 24
 SDPA_ERR_DS_PATH = 25
-_ARG_ERRORS = set(range(1, 23)) | {SDPA_ERR_SCRATCH_LIMIT, SDPA_ERR_DS_PATH}
+_ARG_ERRORS = set(range(1, 23)) | {SDPA_ERR_SCRATCH_LIMIT, SDPA_ERR_DS_PATH} | set(range(26, 32))
 
 _lib = None
 
@@ -103,6 +108,19 @@ def library():
     L.sdpa_hip_drop_threshold.argtypes = [f32]
     L.sdpa_hip_dropout_mask.restype = i32
     L.sdpa_hip_dropout_mask.argtypes = [vp, i32, i32, i32, f32, u64, u64, vp]
+    i32p = vp
+    rope = [vp, vp, i32, vp, vp, i32]  # weights, their dtype, tables and their rows
+    L.sdpa_hip_qk_norm_rope.restype = i32
+    L.sdpa_hip_qk_norm_rope.argtypes = [i32] + [vp, i64p] * 4 + rope + [i32p] + [i32] * 7 + [f32, i32, i32, vp]
+    L.sdpa_hip_qk_norm_rope_grad_workspace_bytes.restype = sz
+    L.sdpa_hip_qk_norm_rope_grad_workspace_bytes.argtypes = [i32]
+    L.sdpa_hip_qk_norm_rope_grad.restype = i32
+    L.sdpa_hip_qk_norm_rope_grad.argtypes = ([i32] + [vp, i64p] * 6 + [vp, vp] + rope + [i32p, i32, vp, sz] + [i32] * 6 +
+                                             [f32, i32, i32, vp])
+    batch = [i32p, ctypes.c_int64, i32p, i32p]  # page table and its row stride, q_starts, kv_lens
+    L.sdpa_hip_kv_append.restype = i32
+    L.sdpa_hip_kv_append.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + batch + [i32] * 10 +
+                                     [f32, i32, i32, vp])
     _lib = L
     return L
 
@@ -334,3 +352,7 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
     if _fn is None:
         _fn = _make_function()
     return _fn.apply(q, k, v, seed, offset, dropout, scale, causal_mask)
+
+
+from .heads import (kv_append, qk_norm_rope, qk_norm_rope_autograd,  # noqa: E402
+                    qk_norm_rope_grad)

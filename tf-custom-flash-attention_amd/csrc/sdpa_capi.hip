@@ -14,14 +14,20 @@
 #include "sdpa_parts.h"
 
 namespace {
-
 thread_local int g_last_hip_error = 0;
+}  // namespace
 
+namespace sdpa {
 int hip_status(hipError_t e) {
     if (e == hipSuccess) return SDPA_OK;
     g_last_hip_error = (int)e;
     return SDPA_ERR_HIP;
 }
+}  // namespace sdpa
+
+namespace {
+
+using sdpa::hip_status;
 
 bool aligned16(const void* ptr) { return ((uintptr_t)ptr & 15u) == 0; }
 

@@ -44,6 +44,13 @@ inline const char* status_message(int status) {
         case SDPA_ERR_DS_PATH:
             return "the dS path of the backward needs float16, a feature size over 64, 16-byte aligned tensors "
                    "and a workspace of sdpa_hip_bwd_workspace_bytes_ds bytes";
+        case SDPA_ERR_ROTARY: return "rotated features must be even in number and at most the feature size";
+        case SDPA_ERR_PAGE_SIZE: return "tokens per page must be a power of two from 16 to 65536";
+        case SDPA_ERR_HEADS: return "query heads must be a multiple of key heads";
+        case SDPA_ERR_LAYOUT:
+            return "feature sizes, strides and addresses must be whole 16-byte chunks of at least one feature";
+        case SDPA_ERR_TOO_LARGE: return "too many rows for one call";
+        case SDPA_ERR_WEIGHT: return "a weight needs the norm, and is of dtype T or float32";
         default: return "unknown sdpa status";
     }
 }

@@ -14,6 +14,10 @@ namespace sdpa {
 
 enum class DType : int { F32 = 0, F16 = 1 };
 
+// sdpa_status_t of a launch; a failure is kept for sdpa_hip_last_hip_error
+// (sdpa_capi.hip).
+int hip_status(hipError_t e);
+
 // Padded feature width for D in [0, 128]: the MFMA tiles are 32 wide in the
 // output direction, so every kernel is instantiated for 32, 64 and 128
 // (the reference buckets max(D_qk, D_v) into 8/16/32/64/128,

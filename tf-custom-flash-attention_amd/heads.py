@@ -1,0 +1,317 @@
+"""The steps around ``sdpa`` of a layer of a language model: norm and rotation
+of queries and keys (with the gradient), and a paged cache of keys and values.
+
+As with the op itself, torch tensors are device memory and streams only; the
+arithmetic runs in the HIP kernels behind ``include/sdpa_hip.h``, fp16 or fp32.
+Arguments that the device alone knows (lengths, page tables, positions) are
+checked there, where they are used.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import (DTYPE_F16, DTYPE_F32, InvalidArgumentError, _dtype_code, _raise_for, _stream_handle, library)
+
+_Strides3 = ctypes.c_int64 * 3
+_Strides2 = ctypes.c_int64 * 2
+
+
+def _fail(message):
+    raise InvalidArgumentError(message)
+
+
+def _on_device(device, **tensors):
+    """Every tensor lies on one GPU."""
+    if device.type != "cuda":
+        _fail("tensors must be on the GPU (the op's HIP kernel)")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            _fail(f"{name} is on {t.device}, not on {device}")
+
+
+def _call(entry, device, *args):
+    """``entry(*args, stream)`` with ``device`` current."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        _raise_for(entry(*args, _stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            _raise_for(entry(*args, _stream_handle(device)))
+
+
+def _dense_features(t):
+    """``t`` with its features next to each other."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _int32(name, t, *shape):
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        _fail(f"{name} must be an int32 tensor")
+    if tuple(t.shape) != shape:
+        _fail(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+
+
+def _tables(cos, sin):
+    """Rows and rotated features of the rotation tables (0, 0 without)."""
+    import torch
+    if cos is None and sin is None:
+        return 0, 0
+    if cos is None or sin is None:
+        _fail("cos and sin belong together")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        _fail("cos and sin must be float32")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        _fail("cos and sin must have one shape [positions, rotated features / 2]")
+    if cos.shape[0] > 0x7FFFFFFF:
+        _fail("too many positions in the rotation tables")
+    return cos.shape[0], 2 * cos.shape[1]
+
+
+def _weight_dtype(T, D, q_weight, k_weight, norm):
+    import torch
+    code = None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if not norm:
+            _fail(f"{name} needs the norm")
+        if tuple(w.shape) != (D,):
+            _fail(f"{name} must have shape [{D}], got {list(w.shape)}")
+        if w.dtype not in (T, torch.float32):
+            _fail(f"{name} must be of dtype T or float32, got {w.dtype}")
+        c = DTYPE_F32 if w.dtype == torch.float32 else DTYPE_F16
+        if code is not None and c != code:
+            _fail("q_weight and k_weight must have the same dtype")
+        code = c
+    return DTYPE_F32 if code is None else code
+
+
+def _check_qk(q, k):
+    if q.dim() != 4 or k.dim() != 4:
+        _fail("q and k must be [batch, tokens, heads, features]")
+    if q.dtype != k.dtype:
+        _fail("q and k must have the same dtype T")
+    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        _fail(f"q {list(q.shape)} and k {list(k.shape)} differ in batch, tokens or features")
+
+
+def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm):
+    """Checks of what the forward and the gradient have in common."""
+    _check_qk(q, k)
+    code = _dtype_code(q)
+    B, S, H_q, D = q.shape
+    rows, R = _tables(cos, sin)
+    w_code = _weight_dtype(q.dtype, D, q_weight, k_weight, norm)
+    per_batch = 0
+    if positions is not None:
+        per_batch = int(positions.dim() == 2)
+        _int32("positions", positions, *((B, S) if per_batch else (S,)))
+        positions = positions.contiguous()
+    elif R and S > rows:
+        _fail(f"the rotation tables have {rows} positions, the sequence {S} tokens")
+    _on_device(q.device, k=k, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight, positions=positions)
+    cos, sin, q_weight, k_weight = (None if t is None else t.contiguous() for t in (cos, sin, q_weight, k_weight))
+    return code, (B, S, H_q, k.shape[2], D, R), (cos, sin, rows), (q_weight, k_weight, w_code), positions, per_batch
+
+
+def _out_rows(torch, like, B, S, H, D, fold_heads):
+    """A result [B H, S, D] (folded) or [B, S, H, D], and its strides {batch, token, head}."""
+    if fold_heads:
+        return torch.empty((B * H, S, D), dtype=like.dtype, device=like.device), _Strides3(H * S * D, D, S * D)
+    return torch.empty((B, S, H, D), dtype=like.dtype, device=like.device), _Strides3(S * H * D, H * D, D)
+
+
+def _strides3(t):
+    return _Strides3(t.stride(0), t.stride(1), t.stride(2))
+
+
+def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
+                 norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+    """RMS norm of every head of q and k, and its rotation by position: ``(q_out, k_out)``.
+
+    q [B, S, H_q, D] and k [B, S, H_kv, D] (fp16 or fp32; any strides, so both may be parts of one
+    projection's output; D <= 128).  ``norm``: each row divided by sqrt(mean of its squares + eps)
+    and multiplied by its weight [D] (dtype T or float32), if there is one.  The first R features,
+    R = 2 * cos.shape[1], are rotated by row ``positions`` (int32 [S] or [B, S]; None: 0 .. S - 1) of the float32 tables
+    cos and sin [P, R / 2]: pairs (i, i + R/2), or (2i, 2i + 1) if ``interleaved``; without tables
+    (None) nothing is.  A position outside the tables makes its rows NaN.
+
+    ``fold_heads``: results [B * H, S, D], the layout of ``sdpa``; else [B, S, H, D].
+    """
+    import torch
+    code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
+        q, k, cos, sin, q_weight, k_weight, positions, norm)
+    q, k = _dense_features(q), _dense_features(k)
+    q_out, qos = _out_rows(torch, q, B, S, H_q, D, fold_heads)
+    k_out, kos = _out_rows(torch, k, B, S, H_kv, D, fold_heads)
+    _call(library().sdpa_hip_qk_norm_rope, q.device, code, q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k),
+          q_out.data_ptr(), qos, k_out.data_ptr(), kos, _ptr(weights[0]), _ptr(weights[1]), weights[2],
+          _ptr(tables[0]), _ptr(tables[1]), tables[2], _ptr(positions), per_batch, B, S, H_q, H_kv, D, R, float(eps),
+          int(bool(norm)), int(bool(interleaved)))
+    return q_out, k_out
+
+
+def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=None, positions=None,
+                      eps: float = 1e-6, norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+    """Gradient of ``qk_norm_rope``: ``(dq, dk, dq_weight, dk_weight)``.
+
+    ``d_q_out`` and ``d_k_out`` are laid out as its results; dq and dk come as
+    dense [B, S, H, D], the weights' gradients in their dtype, None for a
+    weight that was not given.
+    """
+    import torch
+    code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
+        q, k, cos, sin, q_weight, k_weight, positions, norm)
+    L = library()
+    _on_device(q.device, d_q_out=d_q_out, d_k_out=d_k_out)
+    grads = []
+    for name, d, H in (("d_q_out", d_q_out, H_q), ("d_k_out", d_k_out, H_kv)):
+        shape = (B * H, S, D) if fold_heads else (B, S, H, D)
+        if tuple(d.shape) != shape or d.dtype != q.dtype:
+            _fail(f"{name} must be {q.dtype} of shape {list(shape)}, got {d.dtype} {list(d.shape)}")
+        d = _dense_features(d)
+        # (batch and head of a folded row are H rows and one row apart)
+        grads.append((d, _Strides3(H * d.stride(0), d.stride(1), d.stride(0)) if fold_heads else _strides3(d)))
+    q, k = _dense_features(q), _dense_features(k)
+    dq = torch.empty((B, S, H_q, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, S, H_kv, D), dtype=q.dtype, device=q.device)
+    dw = [None if w is None else torch.empty_like(w) for w in weights[:2]]
+    ws, ws_bytes = None, 0
+    if dw[0] is not None or dw[1] is not None:
+        ws_bytes = L.sdpa_hip_qk_norm_rope_grad_workspace_bytes(D)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
+    _call(L.sdpa_hip_qk_norm_rope_grad, q.device, code, grads[0][0].data_ptr(), grads[0][1], grads[1][0].data_ptr(),
+          grads[1][1], q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k), dq.data_ptr(), None, dk.data_ptr(),
+          None, _ptr(dw[0]), _ptr(dw[1]), _ptr(weights[0]), _ptr(weights[1]), weights[2], _ptr(tables[0]),
+          _ptr(tables[1]), tables[2], _ptr(positions), per_batch, _ptr(ws), ws_bytes, B, S, H_q, H_kv, D, R,
+          float(eps), int(bool(norm)), int(bool(interleaved)))
+    return dq, dk, dw[0], dw[1]
+
+
+def _make_function():
+    import torch
+
+    class QkNormRopeFunction(torch.autograd.Function):
+        """``qk_norm_rope`` with its gradient for q, k and the weights."""
+
+        @staticmethod
+        def forward(ctx, q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads):
+            ctx.save_for_backward(q, k, cos, sin, q_weight, k_weight, positions)
+            ctx.attrs = dict(eps=eps, norm=norm, interleaved=interleaved, fold_heads=fold_heads)
+            return qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, **ctx.attrs)
+
+        @staticmethod
+        def backward(ctx, d_q_out, d_k_out):
+            dq, dk, dqw, dkw = qk_norm_rope_grad(d_q_out, d_k_out, *ctx.saved_tensors, **ctx.attrs)
+            return dq, dk, None, None, dqw, dkw, None, None, None, None, None
+
+    return QkNormRopeFunction
+
+
+_fn = None
+
+
+def qk_norm_rope_autograd(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
+                          norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+    """Differentiable ``qk_norm_rope`` (no gradient for the tables)."""
+    global _fn
+    if _fn is None:
+        _fn = _make_function()
+    return _fn.apply(q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads)
+
+
+def _check_cache(k_cache, v_cache, T):
+    if k_cache.dim() != 4 or v_cache.dim() != 4:
+        _fail("k_cache and v_cache must be [pages, heads, tokens per page, features]")
+    if k_cache.shape[:3] != v_cache.shape[:3]:
+        _fail(f"k_cache {list(k_cache.shape)} and v_cache {list(v_cache.shape)} differ in pages, heads or page size")
+    if k_cache.dtype != T or v_cache.dtype != T:
+        _fail("the caches must have the same dtype T as the tokens")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        _fail("k_cache and v_cache must be contiguous")
+
+
+def _check_batch(page_table, q_starts, kv_lens):
+    """(N, width) of a batch over the cache."""
+    if page_table.dim() != 2:
+        _fail("page_table must be [sequences, pages per sequence]")
+    N, width = page_table.shape
+    _int32("page_table", page_table, N, width)
+    _int32("q_starts", q_starts, N + 1)
+    _int32("kv_lens", kv_lens, N)
+    if width > 1 and page_table.stride(1) != 1:
+        _fail("the rows of page_table must be contiguous")
+    if (N > 0 and q_starts.stride(0) != 1) or (N > 1 and kv_lens.stride(0) != 1):
+        _fail("q_starts and kv_lens must be contiguous")
+    return N, width
+
+
+def _check_tokens(name, t, T, features=None):
+    if t.dim() != 3 or (features is not None and t.shape[2] != features):
+        _fail(f"{name} must be [tokens, heads{'' if features is None else f', {features}'}], got {list(t.shape)}")
+    if t.dtype != T:
+        _fail(f"{name} must have dtype {T}, got {t.dtype}")
+
+
+def _strides2(t):
+    return _Strides2(t.stride(0), t.stride(1))
+
+
+def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, sin=None, q=None, q_weight=None,
+              k_weight=None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False):
+    """Appends new tokens to a paged cache, in place, and returns their rotated queries.
+
+    k [T, H_kv, D_qk] and v [T, H_kv, D_v] are the packed new tokens of N sequences (any strides):
+    those of sequence s are q_starts[s] .. q_starts[s + 1] - 1 (int32 [N + 1]).  kv_lens (int32 [N])
+    counts its cached tokens with the new ones, which are the last.  Token j of s goes to row j % page of page
+    page_table[s, j // page] (int32 [N, pages per sequence]) of the caches [pages, H_kv, page, D],
+    page a power of two of at least 16.  On the way k is normed (``norm``, ``k_weight``) and rotated
+    by j as in ``qk_norm_rope`` (cos and sin None: not), and so is q [T, H_q, D_qk], where given:
+    the result is [T, H_q, D_qk], else None.
+
+    Tokens behind the last sequence are skipped (their rows of the result are not written).  A token
+    without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
+    of a call may have the same place.
+    """
+    import torch
+    T = k.dtype
+    _check_tokens("k", k, T)
+    _check_tokens("v", v, T)
+    code = _dtype_code(k)
+    _check_cache(k_cache, v_cache, T)
+    N, width = _check_batch(page_table, q_starts, kv_lens)
+    n, H_kv, D_qk = k.shape
+    D_v = v.shape[2]
+    pages, _, page, _ = k_cache.shape
+    if v.shape[:2] != k.shape[:2]:
+        _fail(f"k {list(k.shape)} and v {list(v.shape)} differ in tokens or heads")
+    if k_cache.shape[1] != H_kv or k_cache.shape[3] != D_qk or v_cache.shape[3] != D_v:
+        _fail(f"the caches {list(k_cache.shape)}, {list(v_cache.shape)} do not hold rows of k {list(k.shape)} and v "
+              f"{list(v.shape)}")
+    H_q = 0
+    if q is not None:
+        _check_tokens("q", q, T, D_qk)
+        if q.shape[0] != n:
+            _fail(f"q has {q.shape[0]} tokens, k {n}")
+        H_q = q.shape[1]
+    rows, R = _tables(cos, sin)
+    w_code = _weight_dtype(T, D_qk, q_weight, k_weight, norm)
+    _on_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts,
+               kv_lens=kv_lens, cos=cos, sin=sin, q=q, q_weight=q_weight, k_weight=k_weight)
+    k, v = _dense_features(k), _dense_features(v)
+    cos, sin, q_weight, k_weight = (None if t is None else t.contiguous() for t in (cos, sin, q_weight, k_weight))
+    q_out = None
+    if q is not None:
+        q = _dense_features(q)
+        q_out = torch.empty((n, H_q, D_qk), dtype=T, device=k.device)
+    _call(library().sdpa_hip_kv_append, k.device, code, k.data_ptr(), _strides2(k), v.data_ptr(), _strides2(v),
+          k_cache.data_ptr(), v_cache.data_ptr(), _ptr(q), None if q is None else _strides2(q), _ptr(q_out), None,
+          _ptr(q_weight), _ptr(k_weight), w_code, _ptr(cos), _ptr(sin), rows, page_table.data_ptr(),
+          page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, n, width, pages, page, H_q, H_kv, D_qk,
+          D_v, R, float(eps), int(bool(norm)), int(bool(interleaved)))
+    return q_out
