@@ -296,6 +296,38 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
                        int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
                        int norm, int interleaved, hipStream_t stream);
 
+/* Attention of the new tokens over the cache (after their append): for query
+ * head h of token i of the n new ones of sequence s, over the keys of head
+ * h / (H_q / H_kv),
+ *   o     = softmax(scale q k^T) v      [T, H_q, D_v], strides {token, head}
+ *   stats = log(sum(exp(scale q k^T)))  [T, H_q] fp32, dense
+ * over the cached tokens j < kv_lens[s]; with causal_mask over those with
+ * j <= kv_lens[s] - n + i.  A row that sees no key has o = 0 and stats =
+ * -infinity.  Rows of tokens of no sequence stay as they were.  Where a key that some
+ * row of a sequence may see has no place in the table or on a page, rows of that
+ * sequence are NaN.  What lies in the cache behind a row's last key has no
+ * influence on it, infinities and NaN included; an infinite or NaN value
+ * among its keys makes its feature of o infinite or NaN.
+ * H_q is a multiple of H_kv; feature sizes, strides and addresses must be whole
+ * 16-byte chunks; D_qk, D_v <= 128.
+ * max_q_len: the most new tokens of a sequence, where the caller knows it (1 in
+ * generation), else 0.  It helps to choose kernels; results are right
+ * whatever it is.
+ * The workspace (device memory, 16-byte aligned) holds the parts of tiles whose
+ * keys are divided over workgroups; with less than
+ * sdpa_hip_paged_fwd_workspace_bytes(...), or none, nothing is divided.  The
+ * division goes by all lengths of the call: the last bits of a sequence's
+ * results may differ between batches.  Each call repeats to the bit.         */
+size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
+                                          int D_qk, int D_v, int max_q_len);
+
+int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache,
+                       const void* v_cache, void* o, const int64_t* o_strides, float* stats,
+                       const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
+                       const int32_t* kv_lens, void* workspace, size_t workspace_bytes, int N, int T, int width,
+                       int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int max_q_len, float scale,
+                       int causal_mask, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

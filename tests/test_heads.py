@@ -129,3 +129,49 @@ def test_append_abi_refusals(pkg):
                      (dict(table=None), 20), (dict(width=1 << 27, page=16), 30), (dict(T=1 << 30), 30)):
         assert call(**kw) == code, kw
     assert call(T=0) == 0 and call(N=0) == 0
+
+
+PAGED = dict(q=(6, 4, 32), k_cache=(9, 2, 16, 32), v_cache=(9, 2, 16, 16), page_table=(3, 4), q_starts=(4,), kv_lens=(3,))
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(q=(6, 4)), "q must be"),
+    (dict(q=(6, 4, 24)), "q has 24 features"),
+    (dict(dtype=torch.bfloat16), "T must be half or float"),
+    (dict(cache_dtype=torch.float32), "same dtype T"),
+    (dict(v_cache=(8, 2, 16, 16)), "differ in pages"),
+    (dict(q_starts=(5,)), "q_starts must have shape"),
+    (dict(out=((6, 4, 32), (6, 4))), "out must be"),
+    (dict(out=((6, 4, 16), (6, 3))), "out must be"),
+    ({}, "on the GPU"),
+])
+def test_paged_refusals(pkg, change, message):
+    c = dict(PAGED, dtype=torch.float16, cache_dtype=None, out=None)
+    c.update(change)
+    t = lambda name, d: _meta(*c[name], dtype=d)
+    d = c["cache_dtype"] or c["dtype"]
+    out = None if c["out"] is None else (_meta(*c["out"][0]), _meta(*c["out"][1], dtype=torch.float32))
+    _refused(pkg, message, pkg.paged_sdpa, t("q", c["dtype"]), t("k_cache", d), t("v_cache", d),
+             *(t(n, torch.int32) for n in ("page_table", "q_starts", "kv_lens")), out=out)
+
+
+def test_paged_abi_refusals(pkg):
+    L = pkg.library()
+    some = ctypes.c_void_p(64)
+
+    def call(dtype=1, N=3, T=6, width=4, pages=9, page=16, H_q=4, H_kv=2, D=32, D_v=16, q=some, table=some, stats=some,
+             k=some, strides=None):
+        return L.sdpa_hip_paged_fwd(dtype, q, strides, k, some, some, None, stats, table, width, some, some, None, 0, N, T,
+                                    width, pages, page, H_q, H_kv, D, D_v, 0, 0.5, 1, None)
+
+    odd = (I64 * 2)(132, 32)
+    for kw, code in ((dict(dtype=2), 18), (dict(N=-1), 19), (dict(width=-1), 19), (dict(H_q=-4), 19), (dict(D=136), 16),
+                     (dict(D=0), 29), (dict(D_v=12), 29), (dict(dtype=0, D_v=14), 29), (dict(H_q=3), 28),
+                     (dict(H_kv=0), 28), (dict(page=24), 27), (dict(q=None), 20), (dict(stats=None), 20),
+                     (dict(table=None), 20), (dict(k=None), 20), (dict(q=ctypes.c_void_p(72)), 29),
+                     (dict(k=ctypes.c_void_p(72)), 29), (dict(strides=odd), 29), (dict(T=1 << 30), 30)):
+        assert call(**kw) == code, kw
+    assert call(T=0) == 0 and call(N=0) == 0 and call(H_q=0) == 0
+    need = lambda **k: L.sdpa_hip_paged_fwd_workspace_bytes(*dict(dict(dtype=1, N=3, T=6, width=400, page=16, H_q=4, H_kv=2,
+                                                                       D=32, D_v=16, most=1), **k).values())
+    assert need() > 0 and need(width=1) == 0 and need(H_q=3) == 0 and need(N=0) == 0

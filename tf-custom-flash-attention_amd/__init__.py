@@ -121,6 +121,10 @@ def library():
     L.sdpa_hip_kv_append.restype = i32
     L.sdpa_hip_kv_append.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + batch + [i32] * 10 +
                                      [f32, i32, i32, vp])
+    L.sdpa_hip_paged_fwd_workspace_bytes.restype = sz
+    L.sdpa_hip_paged_fwd_workspace_bytes.argtypes = [i32] * 10
+    L.sdpa_hip_paged_fwd.restype = i32
+    L.sdpa_hip_paged_fwd.argtypes = [i32, vp, i64p, vp, vp, vp, i64p, vp] + batch + [vp, sz] + [i32] * 10 + [f32, i32, vp]
     _lib = L
     return L
 
@@ -354,5 +358,5 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
     return _fn.apply(q, k, v, seed, offset, dropout, scale, causal_mask)
 
 
-from .heads import (kv_append, qk_norm_rope, qk_norm_rope_autograd,  # noqa: E402
+from .heads import (kv_append, paged_sdpa, qk_norm_rope, qk_norm_rope_autograd,  # noqa: E402
                     qk_norm_rope_grad)

@@ -1,0 +1,99 @@
+// sdpa_paged.h -- attention of new tokens over a paged cache: arguments, and
+// how its work is divided over workgroups.
+//
+// Rows.  The G = H_q / H_kv query heads that share a key head read the same
+// keys, so a sequence of n new tokens has, for each key head, n G rows: row
+// i G + g is token i, head h G + g.  A tile is up to BM of them.
+//
+// Division.  The lengths are on the device, so every workgroup forms the plan
+// itself, from sums over the sequences: the cost of a tile is the number of
+// key blocks it walks on average; the keys of a tile are divided into parts of
+// at most `chunk` blocks, chunk being the larger of kPagedMinChunk and the
+// whole cost over `target` workgroups.  So at most target workgroups more than
+// there are tiles have work, whatever the lengths, and at most 2 target
+// parts are of divided tiles: the grid and the workspace go by the call's
+// sizes alone.  Parts are merged in order by a second kernel.
+#pragma once
+
+#include "sdpa_kv_append.h"
+
+namespace sdpa {
+
+struct PagedParams {
+    PagedBatch batch;
+    const void* q;        // [T, H_q, D_qk]
+    const void* k_cache;  // [pages, H_kv, page, D_qk]
+    const void* v_cache;  // [pages, H_kv, page, D_v]
+    void* o;              // [T, H_q, D_v]
+    float* stats;         // [T, H_q] dense
+    TokenStrides qs, os;
+    float* part_o;   // [slot][BM][D_v]: unnormalised O of a part
+    float* part_ml;  // [slot][BM][2]: its running maximum (log2) and sum
+    int H_kv, G, D_qk, D_v;
+    float scale;
+    int causal;
+    int target;              // workgroups to divide for; 0: no workspace, nothing is divided
+    int min_rows, max_rows;  // sequences of min_rows < n G <= max_rows are this launch's
+};
+
+constexpr int kPagedMinChunk = 2;   // key blocks of a part, at least
+constexpr int kPagedMaxParts = 64;  // (the merge walks a row's parts one batch after the other)
+
+// One sequence's part of the plan.
+struct SeqPlan {
+    int q0, n, len;             // first new token, new tokens, cached tokens
+    int tiles, blocks, parts;  // per key head; blocks of a tile on average
+    bool bad;                  // more cached tokens than the table has columns for
+};
+
+// tiles = 0: nothing to do in this launch.  chunk = 0: parts are left at 1.
+__host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const PagedBatch& b, int G, bool causal, int min_rows,
+                                            int max_rows, int BM, int BN, long long chunk) {
+    SeqPlan s{q0, 0, 0, 0, 0, 1, false};
+    if (q0 < 0 || q1 <= q0 || q1 > b.T) return s;
+    const int n = q1 - q0;
+    const long long rows = (long long)n * G;
+    if (rows <= min_rows || rows > max_rows) return s;
+    const int cap = b.width << b.page_log2;
+    s.n = n;
+    s.bad = kv_len > cap;
+    s.len = kv_len < 0 ? 0 : (kv_len > cap ? cap : kv_len);
+    s.tiles = (int)((rows + BM - 1) / BM);
+    const int mean = causal ? s.len - n / 2 : s.len;
+    s.blocks = mean < BN ? 1 : (mean - 1) / BN + 1;
+    if (chunk > 0) {
+        const long long p = (s.blocks + chunk - 1) / chunk;
+        s.parts = (int)(p < kPagedMaxParts ? p : kPagedMaxParts);
+    }
+    return s;
+}
+
+__host__ __device__ inline long long plan_chunk(long long cost, int target) {
+    if (target <= 0) return 0;
+    const long long c = (cost + target - 1) / target;
+    return c < kPagedMinChunk ? kPagedMinChunk : c;
+}
+
+// Tiles of a launch, at most: every sequence ends in one that is not full, and
+// has more than min_rows rows.
+inline long long paged_max_tiles(const PagedParams& p, int BM) {
+    const long long rows = (long long)p.batch.T * p.G;
+    const long long seqs = rows / ((long long)p.min_rows + 1);
+    return (rows / BM + (seqs < p.batch.N ? seqs : p.batch.N)) * p.H_kv;
+}
+
+// Sequences of up to so many rows take the kernel of 32-row tiles, whose waves
+// divide the keys; longer ones that of 128-row tiles.
+constexpr int kPagedSmallRows = 64;
+
+// Workgroups the launches divide for, and the workspace of one launch's parts.
+constexpr int kPagedTarget = 512;
+constexpr int kPagedSmallBM = 32, kPagedBM = 128;
+inline size_t paged_part_bytes(int D_v, int BM) {
+    return 2 * (size_t)kPagedTarget * BM * ((size_t)D_v + 2) * sizeof(float);
+}
+
+hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
+hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream);
+
+}  // namespace sdpa

@@ -7,6 +7,7 @@
 #include "sdpa_hip.h"
 #include "sdpa_kv_append.h"
 #include "sdpa_norm_rope.h"
+#include "sdpa_paged.h"
 
 namespace {
 
@@ -220,6 +221,87 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     add_tokens(ch, v, p.vs);
     p.vec = ch.ok;
     return hip_status(sdpa::launch_kv_append(p, (sdpa::DType)dtype, stream));
+}
+
+}  // extern "C"
+
+namespace {
+
+// Whether the parts of divided tiles can come up at all, and their bytes.
+size_t paged_workspace(int width, int page_size, int D_v) {
+    if (((long long)width * page_size) <= (long long)sdpa::kPagedMinChunk * 64) return 0;
+    return sdpa::paged_part_bytes(D_v, sdpa::kPagedSmallBM);
+}
+
+int check_paged(int dtype, int H_q, int H_kv, int D_qk, int D_v) {
+    if (dtype != SDPA_DTYPE_F32 && dtype != SDPA_DTYPE_F16) return SDPA_ERR_DTYPE;
+    if (H_q < 0 || H_kv < 0 || D_qk < 0 || D_v < 0) return SDPA_ERR_NEGATIVE_DIM;
+    if (D_qk > 128 || D_v > 128) return SDPA_ERR_FEATURE_TOO_LARGE;
+    const int epc = dtype == SDPA_DTYPE_F16 ? 8 : 4;
+    if (D_qk == 0 || D_v == 0 || D_qk % epc != 0 || D_v % epc != 0) return SDPA_ERR_LAYOUT;
+    if (H_q > 0 && (H_kv == 0 || H_q % H_kv != 0)) return SDPA_ERR_HEADS;
+    return SDPA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
+                                          int D_qk, int D_v, int max_q_len) {
+    (void)max_q_len;
+    if (check_paged(dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
+        return 0;
+    return paged_workspace(width, page_size, D_v);
+}
+
+int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
+                       void* o, const int64_t* o_strides, float* stats, const int32_t* page_table,
+                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, void* workspace,
+                       size_t workspace_bytes, int N, int T, int width, int pages, int page_size, int H_q, int H_kv,
+                       int D_qk, int D_v, int max_q_len, float scale, int causal_mask, hipStream_t stream) {
+    int st = check_paged(dtype, H_q, H_kv, D_qk, D_v);
+    if (st != SDPA_OK) return st;
+    sdpa::PagedParams p{};
+    // without pages no column of the table holds any
+    st = make_batch(p.batch, page_table, page_table_stride, q_starts, kv_lens, N, T, pages > 0 ? width : (width < 0 ? -1 : 0),
+                    pages, page_size);
+    if (st != SDPA_OK) return st;
+    if (N == 0 || T == 0 || H_q == 0) return SDPA_OK;
+    if (!q || !o || !stats || (p.batch.width > 0 && (!k_cache || !v_cache))) return SDPA_ERR_NULL_POINTER;
+    p.q = q;
+    p.k_cache = k_cache;
+    p.v_cache = v_cache;
+    p.o = o;
+    p.stats = stats;
+    p.qs = token_strides(q_strides, T, H_q, D_qk);
+    p.os = token_strides(o_strides, T, H_q, D_v);
+    Chunks ch{dtype == SDPA_DTYPE_F16 ? 8 : 4};
+    ch.address(k_cache);
+    ch.address(v_cache);
+    add_tokens(ch, q, p.qs);
+    add_tokens(ch, o, p.os);
+    if (!ch.ok) return SDPA_ERR_LAYOUT;
+    p.H_kv = H_kv;
+    p.G = H_q / H_kv;
+    p.D_qk = D_qk;
+    p.D_v = D_v;
+    p.scale = scale;
+    p.causal = causal_mask != 0;
+    p.min_rows = 0;
+    p.max_rows = 0x7FFFFFFF;
+    const size_t need = paged_workspace(p.batch.width, page_size, D_v);
+    if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
+        p.target = sdpa::kPagedTarget;
+        p.part_o = static_cast<float*>(workspace);
+        p.part_ml = p.part_o + 2 * (size_t)p.target * sdpa::kPagedSmallBM * D_v;
+    }
+    if ((long long)T * p.G > 0x7FFFFFFFLL - 65536 ||
+        sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536)
+        return SDPA_ERR_TOO_LARGE;
+    (void)max_q_len;
+    return hip_status(dtype == SDPA_DTYPE_F16 ? sdpa::launch_paged_f16_small(p, stream)
+                                              : sdpa::launch_paged_f32(p, stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,442 @@
+// sdpa_paged_device.h -- what the kernels of attention over a paged cache
+// share: a workgroup's place in the plan, the pages of its keys, rows done
+// again with care, and the merge of divided tiles.
+#pragma once
+
+#include "sdpa_dma.h"
+#include "sdpa_launch.h"
+#include "sdpa_paged.h"
+#include "sdpa_wave.h"
+
+namespace sdpa {
+namespace {
+
+__device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+__device__ __forceinline__ long long wave_sum64(long long x) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+// One workgroup's work, the same in every lane.
+struct PagedItem {
+    SeqPlan s;
+    int seq, h, tile, part;
+    int slot;  // of this part in the workspace, where the tile is divided
+};
+
+template <int BM, int BN>
+struct PagedPlan {
+    const PagedParams& p;
+    const int lane;
+    long long chunk = 0;
+    int q0 = 0, q1 = 0, len = 0;  // of sequence `lane` (read once where there are up to 64)
+
+    __device__ __forceinline__ void read(int n0) {
+        const int s = n0 + lane;
+        q0 = q1 = len = 0;
+        if (s < p.batch.N) {
+            q0 = p.batch.q_starts[s];
+            q1 = p.batch.q_starts[s + 1];
+            len = p.batch.kv_lens[s];
+        }
+    }
+    __device__ __forceinline__ SeqPlan seq(int n0) {
+        if (p.batch.N > 64) read(n0);
+        return seq_plan(q0, q1, len, p.batch, p.G, p.causal != 0, p.min_rows, p.max_rows, BM, BN, chunk);
+    }
+    __device__ __forceinline__ PagedPlan(const PagedParams& p_) : p(p_), lane(threadIdx.x & 63) {
+        if (p.batch.N <= 64) read(0);
+        if (p.target > 0) {
+            long long cost = 0;
+            for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
+                const SeqPlan s = seq(n0);
+                cost += (long long)s.tiles * s.blocks;
+            }
+            chunk = plan_chunk(wave_sum64(cost) * p.H_kv, p.target);
+        }
+    }
+    // Items of the launch (MERGE: divided tiles).
+    template <bool MERGE>
+    __device__ __forceinline__ static int count(const SeqPlan& s) {
+        return MERGE ? (s.parts > 1 ? s.tiles : 0) : s.tiles * s.parts;
+    }
+    template <bool MERGE>
+    __device__ __forceinline__ int items() {
+        int n = 0;
+        for (int n0 = 0; n0 < p.batch.N; n0 += 64) n += count<MERGE>(seq(n0));
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
+        return __builtin_amdgcn_readfirstlane(n) * p.H_kv;
+    }
+    // Item `at` in the order sequence, key head, tile (last first: under the
+    // causal mask it has the most keys), part.
+    template <bool MERGE>
+    __device__ __forceinline__ bool find(int at, PagedItem& it) {
+        int base = 0, slots = 0;
+        for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
+            const SeqPlan s = seq(n0);
+            const int mine = count<MERGE>(s) * p.H_kv, div = s.parts > 1 ? s.tiles * s.parts * p.H_kv : 0;
+            const int end = wave_scan(mine, lane) + base, slot = wave_scan(div, lane) + slots;
+            const uint64_t over = __builtin_amdgcn_ballot_w64(end > at);
+            if (over != 0) {
+                const int l = __builtin_ctzll(over);
+                const auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+                it.s = SeqPlan{get(s.q0), get(s.n), get(s.len), get(s.tiles), get(s.blocks), get(s.parts), get(s.bad) != 0};
+                it.seq = n0 + l;
+                int i = at - (get(end) - get(mine));
+                const int per_tile = MERGE ? 1 : it.s.parts, per_head = it.s.tiles * per_tile;
+                it.h = i / per_head;
+                i -= it.h * per_head;
+                const int t = i / per_tile;
+                it.tile = it.s.tiles - 1 - t;
+                it.part = i - t * per_tile;
+                it.slot = get(slot) - get(div) + (it.h * it.s.tiles + it.tile) * it.s.parts + it.part;
+                return true;
+            }
+            base = __builtin_amdgcn_readlane(end, 63);
+            slots = __builtin_amdgcn_readlane(slot, 63);
+        }
+        return false;
+    }
+};
+
+// A divided tile's part has room in the workspace.  (It always has, but for
+// q_starts that go back and forth, whose sums may pass 32 bits.)
+__device__ __forceinline__ bool slot_ok(const PagedParams& p, const PagedItem& it) {
+    return it.s.parts == 1 || (it.slot >= 0 && it.slot + it.s.parts <= 2 * p.target + it.part);
+}
+
+// Workgroup id -> item, XCD-major: XCD x takes the items [x n / 8, (x + 1) n / 8),
+// so that the tiles of a sequence's key head, which read the same pages, share an L2.
+__host__ __device__ __forceinline__ int xcd_item(int id, int n) {
+    const int x = id & 7, i = id >> 3;
+    const int lo = (int)((long long)n * x / 8), hi = (int)((long long)n * (x + 1) / 8);
+    return lo + i < hi ? lo + i : -1;
+}
+// Workgroups of a launch of up to n items under that map.
+inline long long xcd_grid(long long n) { return (n + 7) / 8 * 8; }
+
+// A window of 64 columns of a sequence's row of the page table, one in each lane.
+struct PageWindow {
+    const int32_t* row;
+    int pages, columns;  // columns that hold keys of this workgroup
+    int first = -64, id = 0;  // (nothing is held yet)
+    bool bad = false;  // a page that is none has been met (its keys read as zero)
+    __device__ __forceinline__ void load(int column, int lane) {
+        first = column;
+        id = column + lane < columns ? row[column + lane] : 0;
+        const bool none = id < 0 || id >= pages;
+        bad = bad || __builtin_amdgcn_ballot_w64(none && column + lane < columns) != 0;
+        if (none) id = -1;
+    }
+    // wave-uniform column
+    __device__ __forceinline__ int page(int column, int lane) {
+        if (column < first || column >= first + 64) load(column, lane);
+        return __builtin_amdgcn_readlane(id, column - first);
+    }
+};
+
+// Descriptor over the rows of [row, min(row + 16, end)) of one head's matrix of
+// a cache (none of a page that is none); row is a multiple of 16, so these rows
+// share a page.
+struct PagedRows {
+    const unsigned char* base;  // the cache, from this head's matrix of page 0 on
+    long long page_bytes;
+    int row_bytes, log2;
+    __device__ __forceinline__ void init(const void* cache, int H_kv, int h, int D, int esize, int page_log2) {
+        row_bytes = D * esize;
+        log2 = page_log2;
+        const long long m = (long long)row_bytes << page_log2;
+        page_bytes = m * H_kv;
+        base = uniform_ptr(static_cast<const unsigned char*>(cache) + m * h);
+    }
+    __device__ __forceinline__ const unsigned char* at(int page, int row) const {
+        return base + page * page_bytes + (long long)(row & ((1 << log2) - 1)) * row_bytes;
+    }
+    __device__ __forceinline__ rsrc_t rows16(int page, int row, int end) const {
+        const int left = page < 0 ? 0 : end - row;
+        return make_rsrc(at(page < 0 ? 0 : page, row), (long long)(left < 0 ? 0 : (left > 16 ? 16 : left)) * row_bytes);
+    }
+};
+
+// The queries of this lane's row of a tile, and how many keys they see.
+struct PagedRow {
+    int tok, head;  // of the T tokens and H_q heads
+    int see;        // keys [0, see)
+    bool live;
+    __device__ __forceinline__ void init(const PagedParams& p, const PagedItem& it, int row) {
+        live = row < it.s.n * p.G;
+        const int i = live ? (int)((unsigned)row / (unsigned)p.G) : 0;
+        tok = it.s.q0 + i;
+        head = it.h * p.G + (live ? row - i * p.G : 0);
+        const int v = p.causal ? it.s.len - it.s.n + i + 1 : it.s.len;
+        see = live ? (v < 0 ? 0 : v) : 0;
+    }
+};
+// Keys that the last row of a tile sees.
+__device__ __forceinline__ int tile_keys(const PagedParams& p, const PagedItem& it, int BM) {
+    if (!p.causal) return it.s.len;
+    const int rows = it.s.n * p.G, last = min((it.tile + 1) * BM, rows) - 1;
+    return max(0, it.s.len - it.s.n + (int)((unsigned)last / (unsigned)p.G) + 1);
+}
+
+// ---- rows done again ---------------------------------------------------------
+// A product of a masked weight, 0, with an infinite or NaN value is NaN, and
+// tiles are multiplied whole.  A row whose sums come out NaN is therefore done
+// again by one wave, key by key over the keys [lo, hi) it sees: finite values
+// weighted, others added as they are, so that one among the row's own keys makes
+// the result infinite or NaN and one behind the mask nothing.  Lane l returns
+// columns l and l + 64 of the unnormalised sums; m in log2 units.
+struct CareRow {
+    float m, l, o[2], extra[2];
+};
+template <typename T>
+__device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t* table, const PagedRows& K, const PagedRows& V,
+                                         const T* q, int lo, int hi) {
+    const int lane = threadIdx.x & 63;
+    CareRow r{-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}};
+    const float sl2 = p.scale * kLog2e;
+    for (int j0 = lo; j0 < hi; j0 += 64) {
+        const int j = j0 + lane;
+        float s = -INFINITY;
+        int page = 0;
+        if (j < hi) {
+            page = table[j >> K.log2];
+            const T* k = reinterpret_cast<const T*>(K.at(page, j));
+            float dot = 0.f;
+            for (int d = 0; d < p.D_qk; ++d) dot = __builtin_fmaf((float)q[d], (float)k[d], dot);
+            s = dot * sl2;
+        }
+        float mx = s;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+        const float m = fmaxf(r.m, mx), a = m == r.m ? 1.f : fast_exp2(r.m - m);
+        float w = j < hi ? (m == -INFINITY ? (s == s ? 0.f : s) : fast_exp2(s - m)) : 0.f;
+        float sum = w;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+        r.l = __builtin_fmaf(r.l, a, sum);
+        r.m = m;
+        r.o[0] *= a;
+        r.o[1] *= a;
+        for (int i = 0; i < 64 && j0 + i < hi; ++i) {
+            const float wi = __shfl(w, i);
+            const T* v = reinterpret_cast<const T*>(V.at(__shfl(page, i), j0 + i));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int d = lane + 64 * c;
+                if (d >= p.D_v) continue;
+                const float x = (float)v[d];
+                if (__builtin_fabsf(x) < INFINITY) r.o[c] = __builtin_fmaf(wi, x, r.o[c]);
+                else r.extra[c] += x;
+            }
+        }
+    }
+    r.o[0] += r.extra[0];
+    r.o[1] += r.extra[1];
+    return r;
+}
+
+// One row's results of one wave, column d at a time: to o and stats, or (the
+// tile is divided) to the workspace.
+template <typename T, int BM>
+__device__ __forceinline__ void put_care_row(const PagedParams& p, const PagedItem& it, const PagedRow& row, int in_tile,
+                                             const CareRow& r) {
+    const int lane = threadIdx.x & 63;
+    if (it.s.parts > 1) {
+        const size_t at = (size_t)it.slot * BM + in_tile;
+        if (lane == 0) {
+            p.part_ml[2 * at] = r.m;
+            p.part_ml[2 * at + 1] = r.l;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+            if (lane + 64 * c < p.D_v) p.part_o[at * p.D_v + lane + 64 * c] = r.o[c];
+        return;
+    }
+    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+    T* o = static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (lane + 64 * c < p.D_v) o[lane + 64 * c] = (T)(r.o[c] * inv);
+    if (lane == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = r.m * kLn2 + logf(r.l);
+}
+
+// Weight 2^(m - M) of a part (0 where both are -inf: nothing was seen).
+__device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : fast_exp2(m - M); }
+// acc + x w, an infinite or NaN x as it is (w may have vanished)
+__device__ __forceinline__ float add_part(float acc, float x, float w) {
+    return __builtin_fabsf(x) < INFINITY ? __builtin_fmaf(x, w, acc) : acc + x;
+}
+
+// The sums of the NW waves of a workgroup, whose 32 rows and lanes are those of
+// an MFMA accumulator (lane l32: row; features 32 dt + 8 g + 4 hh + e), through
+// LDS in wave order: to o and stats, or to the workspace.  bad: a page of some
+// wave's keys is none; the rows are NaN.  [k0, k1): this workgroup's keys.
+template <typename T, int DV, int NW, int BM>
+__device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const PagedItem& it, float* lds,
+                                                  const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
+                                                  const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
+                                                  int k1) {
+    constexpr int OS = acc_stride(DV), NT = 64 * NW, ITER = (BM * (DV / 4) + NT - 1) / NT;
+    static_assert(BM == 32 && BM * (DV / 4) % NT == 0, "one accumulator tile of rows");
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float* mml = lds + NW * BM * OS;
+    int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);  // rows to do again
+    int* none = again + BM;                                  // waves that met a page that is none
+    if (hh == 0) {
+        mml[(wave * BM + l32) * 2] = m_run;
+        mml[(wave * BM + l32) * 2 + 1] = l_tot;
+    }
+    if (tid < BM) again[tid] = 0;
+    if (lane == 0) none[wave] = bad;
+    acc_to_lds<DV>(lds, wave * BM + l32, oacc, hh);
+    __syncthreads();
+    bad = false;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) bad = bad || none[w] != 0;
+    // one thread per four columns of a row
+    const int rows = min(BM, it.s.n * p.G - it.tile * BM);
+    floatx4 acc[ITER];
+    float M[ITER], L[ITER];
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+        const int i = u * NT + tid, r = i / (DV / 4), c = 4 * (i % (DV / 4));
+        M[u] = -INFINITY;
+        L[u] = 0.f;
+        acc[u] = floatx4{};
+        if (r >= rows || c >= p.D_v) continue;
+        float mw[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            mw[w] = mml[(w * BM + r) * 2];
+            M[u] = fmaxf(M[u], mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = part_weight(mw[w], M[u]);
+            L[u] = __builtin_fmaf(mml[(w * BM + r) * 2 + 1], f, L[u]);
+            const floatx4 x = *reinterpret_cast<const floatx4*>(lds + (w * BM + r) * OS + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[u][e] = __builtin_fmaf(x[e], f, acc[u][e]);
+        }
+        if (bad) {
+            L[u] = __builtin_nanf("");
+            acc[u] = (floatx4){L[u], L[u], L[u], L[u]};
+        } else {
+            bool nan = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan = nan || acc[u][e] != acc[u][e];
+            if (nan) again[r] = 1;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+        const int i = u * NT + tid, r = i / (DV / 4), c = 4 * (i % (DV / 4));
+        if (r >= rows || c >= p.D_v || again[r]) continue;
+        if (it.s.parts > 1) {
+            const size_t at = (size_t)it.slot * BM + r;
+            if (c == 0) {
+                p.part_ml[2 * at] = M[u];
+                p.part_ml[2 * at + 1] = L[u];
+            }
+            *reinterpret_cast<floatx4*>(p.part_o + at * p.D_v + c) = acc[u];
+        } else {
+            PagedRow row;
+            row.init(p, it, it.tile * BM + r);
+            const float inv = L[u] == 0.f ? 0.f : 1.f / L[u];
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            t4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[u][e] * inv);
+            *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
+            if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M[u] * kLn2 + logf(L[u]);
+        }
+    }
+    for (int r = wave; r < rows; r += NW) {
+        if (!__builtin_amdgcn_readfirstlane(again[r])) continue;
+        PagedRow row;
+        row.init(p, it, it.tile * BM + r);
+        const T* q = static_cast<const T*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h;
+        put_care_row<T, BM>(p, it, row, r, care_row<T>(p, table, K, V, q, k0, min(k1, min(row.see, it.s.len))));
+    }
+}
+
+// Merge of the divided tiles: o = sum_i O_i 2^(m_i - M) / l, stats = M ln 2 + log l.
+// One thread per four columns of a row; eight parts at a time, whose loads all
+// go out before the first is used.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
+    PagedPlan<BM, BN> plan(p);
+    PagedItem it;
+    if (!plan.template find<true>((int)blockIdx.x, it) || !slot_ok(p, it)) return;
+    const int np = it.s.parts, cpr = p.D_v / 4, row0 = it.tile * BM;
+    const int rows = min(BM, it.s.n * p.G - row0);
+    constexpr int U = 8;
+    for (int i = threadIdx.x; i < rows * cpr; i += 256) {
+        const int r = i / cpr, c = 4 * (i - r * cpr);
+        float M = -INFINITY, L = 0.f;
+        floatx4 acc = floatx4{};
+        for (int k0 = 0; k0 < np; k0 += U) {
+            floatx2 ml[U];
+            floatx4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t at = (size_t)(it.slot + (k0 + u < np ? k0 + u : np - 1)) * BM + r;
+                ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * at);
+                o[u] = *reinterpret_cast<const floatx4*>(p.part_o + at * p.D_v + c);
+            }
+            float Mn = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) Mn = fmaxf(Mn, ml[u][0]);
+            const float a = M == Mn ? 1.f : part_weight(M, Mn);
+            L *= a;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = add_part(0.f, acc[e], a);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u >= np) break;
+                const float w = part_weight(ml[u][0], Mn);
+                // (a NaN sum has no maximum to weigh it by)
+                L = ml[u][1] == ml[u][1] ? __builtin_fmaf(ml[u][1], w, L) : ml[u][1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = add_part(acc[e], o[u][e], w);
+            }
+            M = Mn;
+        }
+        PagedRow row;
+        row.init(p, it, row0 + r);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
+        *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
+        if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
+    }
+}
+
+template <typename T, int BM, int BN>
+hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
+    // divided tiles have two parts at least
+    return launch_kernel<paged_merge_kernel<T, BM, BN>>(dim3((unsigned)p.target), 256, 0, stream, p);
+}
+
+// Whether a launch may divide anything: some tile can walk more than
+// kPagedMinChunk blocks.
+inline bool paged_may_divide(const PagedParams& p, int BN) {
+    return p.target > 0 && ((long long)p.batch.width << p.batch.page_log2) > (long long)kPagedMinChunk * BN;
+}
+
+}  // namespace
+}  // namespace sdpa

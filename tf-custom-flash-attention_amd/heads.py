@@ -10,7 +10,8 @@ from __future__ import annotations
 
 import ctypes
 
-from . import (DTYPE_F16, DTYPE_F32, InvalidArgumentError, _dtype_code, _raise_for, _stream_handle, library)
+from . import (DTYPE_F16, DTYPE_F32, InvalidArgumentError, _dtype_code, _raise_for, _stream_handle, _workspace,
+               library)
 
 _Strides3 = ctypes.c_int64 * 3
 _Strides2 = ctypes.c_int64 * 2
@@ -315,3 +316,59 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
           page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, R, float(eps), int(bool(norm)), int(bool(interleaved)))
     return q_out
+
+
+def _whole_chunks(t):
+    """``t`` with rows of whole 16-byte chunks (as far as its features allow)."""
+    e = t.element_size()
+    if t.stride(-1) != 1 or t.stride(0) * e % 16 or t.stride(1) * e % 16:
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float = 1.0, causal_mask: bool = True,
+               max_q_len=None, out=None):
+    """Attention of new tokens over a paged cache that holds them already: ``(o, stats)``.
+
+    q [T, H_q, D_qk] and the batch as in ``kv_append``; H_q is a multiple of the caches' heads, and
+    query head h reads key head h // (H_q // H_kv).  Token i of a sequence's n new ones sees its keys
+    j <= kv_len - n + i (``causal_mask``; else all of them).  o [T, H_q, D_v] in T; stats [T, H_q]
+    float32 is the logarithm of the sum of the exponentials of the scaled scores.  A row that sees
+    nothing has o = 0 and stats = -inf.  What the pages hold behind a row's last key has no influence.
+
+    ``max_q_len``: the most new tokens of a sequence, where it is known (1 in generation); it chooses
+    kernels only.  ``out``: (o, stats) to write into; rows of tokens of no sequence stay as they were
+    (in new ones they are arbitrary).  Feature sizes are multiples of 8 (fp16) or 4 (fp32), up to 128.
+    """
+    import torch
+    T = q.dtype
+    _check_tokens("q", q, T)
+    code = _dtype_code(q)
+    _check_cache(k_cache, v_cache, T)
+    N, width = _check_batch(page_table, q_starts, kv_lens)
+    n, H_q, D_qk = q.shape
+    pages, H_kv, page, D_v = v_cache.shape
+    if k_cache.shape[3] != D_qk:
+        _fail(f"q has {D_qk} features, k_cache {k_cache.shape[3]}")
+    if out is None:
+        _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
+        o = torch.empty((n, H_q, D_v), dtype=T, device=q.device)
+        stats = torch.empty((n, H_q), dtype=torch.float32, device=q.device)
+    else:
+        o, stats = out
+        if o.dtype != T or tuple(o.shape) != (n, H_q, D_v) or stats.dtype != torch.float32 or tuple(stats.shape) != (n, H_q):
+            _fail(f"out must be ({T} {[n, H_q, D_v]}, float32 {[n, H_q]})")
+        if not (o.is_contiguous() and stats.is_contiguous()):
+            _fail("out must be contiguous")
+        _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens,
+                   o=o, stats=stats)
+    L = library()
+    longest = 0 if max_q_len is None else int(max_q_len)
+    ws_bytes = L.sdpa_hip_paged_fwd_workspace_bytes(code, N, n, width, page, H_q, H_kv, D_qk, D_v, longest)
+    ws = _workspace(torch, ws_bytes, q.device) if ws_bytes else None
+    q = _whole_chunks(q)
+    _call(L.sdpa_hip_paged_fwd, q.device, code, q.data_ptr(), _strides2(q), k_cache.data_ptr(), v_cache.data_ptr(),
+          o.data_ptr(), None, stats.data_ptr(), page_table.data_ptr(), page_table.stride(0), q_starts.data_ptr(),
+          kv_lens.data_ptr(), _ptr(ws), ws_bytes if ws is not None else 0, N, n, width, pages, page, H_q, H_kv, D_qk,
+          D_v, longest, float(scale), int(bool(causal_mask)))
+    return o, stats
