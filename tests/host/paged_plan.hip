@@ -2,7 +2,7 @@
 // over random batches, garbage ones among them:
 //   - the items of a launch fit its grid, the parts of divided tiles the
 //     workspace, and the divided tiles the merge's grid;
-//   - a sequence is in exactly one of two launches that split at a row count;
+//   - every sequence whose range is one is in the plan, and no other;
 //   - tiles cover the rows, and parts of a tile its blocks, once each;
 //   - tokens and lengths stay inside the batch, whatever the arrays hold;
 //   - workgroup ids map one to one onto the items.
@@ -52,17 +52,13 @@ int main() {
         p.causal = pick(0, 1);
         p.target = pick(0, 5) == 0 ? 0 : kPagedTarget;
         const int cap = p.batch.width << log2;
-        const int split = pick(0, 1) ? kPagedSmallRows : 0x7FFFFFFF;
-        std::vector<int> seen(N, 0);
-        for (int launch = 0; launch < 2; ++launch) {
-            const int BM = launch ? kPagedBM : kPagedSmallBM, BN = launch ? 64 : 128;
-            p.min_rows = launch ? split : 0;
-            p.max_rows = launch ? 0x7FFFFFFF : split;
-            if (p.min_rows >= p.max_rows) continue;
+        for (int kernel = 0; kernel < 2; ++kernel) {
+            const int BM = kernel ? kPagedBM : kPagedSmallBM, BN = kernel ? 64 : 128;
+            std::vector<int> seen(N, 0);
             long long cost = 0, items = 0, slots = 0, divided = 0;
             std::vector<SeqPlan> plans;
             const auto plan = [&](int s, long long chunk) {
-                return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, p.min_rows, p.max_rows, BM, BN, chunk);
+                return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, BM, BN, chunk);
             };
             for (int s = 0; s < N; ++s) cost += (long long)plan(s, 0).tiles * plan(s, 0).blocks;
             const long long chunk = plan_chunk(cost * H_kv, p.target);
@@ -96,11 +92,11 @@ int main() {
                 }
                 for (int i = 0; i < n; ++i) CHECK(hit[i]);
             }
-        }
-        for (int s = 0; s < N; ++s) {
-            const long long n = (long long)starts[s + 1] - starts[s];
-            const bool valid = starts[s] >= 0 && n > 0 && starts[s + 1] <= p.batch.T;
-            CHECK(seen[s] == (valid ? 1 : 0));
+            for (int s = 0; s < N; ++s) {
+                const long long n = (long long)starts[s + 1] - starts[s];
+                const bool valid = starts[s] >= 0 && n > 0 && starts[s + 1] <= p.batch.T;
+                CHECK(seen[s] == (valid ? 1 : 0));
+            }
         }
     }
     printf("ok\n");

@@ -32,8 +32,7 @@ struct PagedParams {
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
-    int target;              // workgroups to divide for; 0: no workspace, nothing is divided
-    int min_rows, max_rows;  // sequences of min_rows < n G <= max_rows are this launch's
+    int target;  // workgroups to divide for; 0: no workspace, nothing is divided
 };
 
 constexpr int kPagedMinChunk = 2;   // key blocks of a part, at least
@@ -46,14 +45,13 @@ struct SeqPlan {
     bool bad;                  // more cached tokens than the table has columns for
 };
 
-// tiles = 0: nothing to do in this launch.  chunk = 0: parts are left at 1.
-__host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const PagedBatch& b, int G, bool causal, int min_rows,
-                                            int max_rows, int BM, int BN, long long chunk) {
+// tiles = 0: nothing to do.  chunk = 0: parts are left at 1.
+__host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const PagedBatch& b, int G, bool causal, int BM,
+                                            int BN, long long chunk) {
     SeqPlan s{q0, 0, 0, 0, 0, 1, false};
     if (q0 < 0 || q1 <= q0 || q1 > b.T) return s;
     const int n = q1 - q0;
     const long long rows = (long long)n * G;
-    if (rows <= min_rows || rows > max_rows) return s;
     const int cap = b.width << b.page_log2;
     s.n = n;
     s.bad = kv_len > cap;
@@ -74,26 +72,29 @@ __host__ __device__ inline long long plan_chunk(long long cost, int target) {
     return c < kPagedMinChunk ? kPagedMinChunk : c;
 }
 
-// Tiles of a launch, at most: every sequence ends in one that is not full, and
-// has more than min_rows rows.
+// Tiles of a launch, at most: every sequence with rows ends in one that is not full.
 inline long long paged_max_tiles(const PagedParams& p, int BM) {
     const long long rows = (long long)p.batch.T * p.G;
-    const long long seqs = rows / ((long long)p.min_rows + 1);
-    return (rows / BM + (seqs < p.batch.N ? seqs : p.batch.N)) * p.H_kv;
+    return (rows / BM + (rows < p.batch.N ? rows : p.batch.N)) * p.H_kv;
 }
 
-// Sequences of up to so many rows take the kernel of 32-row tiles, whose waves
-// divide the keys; longer ones that of 128-row tiles.
-constexpr int kPagedSmallRows = 64;
+// Calls whose sequences have up to so many rows take the kernel of 32-row
+// tiles, whose waves divide the keys; others that of 128-row tiles.
+constexpr int kPagedSmallRows = 32;
 
 // Workgroups the launches divide for, and the workspace of one launch's parts.
 constexpr int kPagedTarget = 512;
 constexpr int kPagedSmallBM = 32, kPagedBM = 128;
+inline bool paged_small(bool f16, long long T, int G, int max_q_len) {
+    const long long most = max_q_len > 0 && max_q_len < T ? max_q_len : T;
+    return !f16 || most * G <= kPagedSmallRows;
+}
 inline size_t paged_part_bytes(int D_v, int BM) {
     return 2 * (size_t)kPagedTarget * BM * ((size_t)D_v + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
+hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream);
 hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream);
 
 }  // namespace sdpa

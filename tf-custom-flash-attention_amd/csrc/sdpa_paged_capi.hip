@@ -228,9 +228,9 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
 namespace {
 
 // Whether the parts of divided tiles can come up at all, and their bytes.
-size_t paged_workspace(int width, int page_size, int D_v) {
+size_t paged_workspace(bool small, int width, int page_size, int D_v) {
     if (((long long)width * page_size) <= (long long)sdpa::kPagedMinChunk * 64) return 0;
-    return sdpa::paged_part_bytes(D_v, sdpa::kPagedSmallBM);
+    return sdpa::paged_part_bytes(D_v, small ? sdpa::kPagedSmallBM : sdpa::kPagedBM);
 }
 
 int check_paged(int dtype, int H_q, int H_kv, int D_qk, int D_v) {
@@ -249,10 +249,9 @@ extern "C" {
 
 size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
                                           int D_qk, int D_v, int max_q_len) {
-    (void)max_q_len;
     if (check_paged(dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
         return 0;
-    return paged_workspace(width, page_size, D_v);
+    return paged_workspace(sdpa::paged_small(dtype == SDPA_DTYPE_F16, T, H_q / H_kv, max_q_len), width, page_size, D_v);
 }
 
 int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -288,20 +287,18 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     p.D_v = D_v;
     p.scale = scale;
     p.causal = causal_mask != 0;
-    p.min_rows = 0;
-    p.max_rows = 0x7FFFFFFF;
-    const size_t need = paged_workspace(p.batch.width, page_size, D_v);
+    if ((long long)T * p.G > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
+    // sequences of few rows, as far as is known here (either kernel takes any)
+    const bool small = sdpa::paged_small(dtype == SDPA_DTYPE_F16, T, p.G, max_q_len);
+    if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
+    const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
         p.target = sdpa::kPagedTarget;
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + 2 * (size_t)p.target * sdpa::kPagedSmallBM * D_v;
+        p.part_ml = p.part_o + 2 * (size_t)p.target * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
     }
-    if ((long long)T * p.G > 0x7FFFFFFFLL - 65536 ||
-        sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536)
-        return SDPA_ERR_TOO_LARGE;
-    (void)max_q_len;
-    return hip_status(dtype == SDPA_DTYPE_F16 ? sdpa::launch_paged_f16_small(p, stream)
-                                              : sdpa::launch_paged_f32(p, stream));
+    if (dtype == SDPA_DTYPE_F32) return hip_status(sdpa::launch_paged_f32(p, stream));
+    return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));
 }
 
 }  // extern "C"

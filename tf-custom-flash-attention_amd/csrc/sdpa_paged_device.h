@@ -11,6 +11,10 @@
 namespace sdpa {
 namespace {
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // v_maximum3_f32: a NaN comes out
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 __device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -50,7 +54,7 @@ struct PagedPlan {
     }
     __device__ __forceinline__ SeqPlan seq(int n0) {
         if (p.batch.N > 64) read(n0);
-        return seq_plan(q0, q1, len, p.batch, p.G, p.causal != 0, p.min_rows, p.max_rows, BM, BN, chunk);
+        return seq_plan(q0, q1, len, p.batch, p.G, p.causal != 0, BM, BN, chunk);
     }
     __device__ __forceinline__ PagedPlan(const PagedParams& p_) : p(p_), lane(threadIdx.x & 63) {
         if (p.batch.N <= 64) read(0);
@@ -144,9 +148,9 @@ struct PageWindow {
     }
 };
 
-// Descriptor over the rows of [row, min(row + 16, end)) of one head's matrix of
-// a cache (none of a page that is none); row is a multiple of 16, so these rows
-// share a page.
+// One head's matrices of a cache.  rows(): a descriptor over the rows [row,
+// min(row + most, end)), which share a page (none of a page that is none): `most` is
+// 16, or more where pages are larger, and row a multiple of it.
 struct PagedRows {
     const unsigned char* base;  // the cache, from this head's matrix of page 0 on
     long long page_bytes;
@@ -161,9 +165,9 @@ struct PagedRows {
     __device__ __forceinline__ const unsigned char* at(int page, int row) const {
         return base + page * page_bytes + (long long)(row & ((1 << log2) - 1)) * row_bytes;
     }
-    __device__ __forceinline__ rsrc_t rows16(int page, int row, int end) const {
+    __device__ __forceinline__ rsrc_t rows(int page, int row, int end, int most) const {
         const int left = page < 0 ? 0 : end - row;
-        return make_rsrc(at(page < 0 ? 0 : page, row), (long long)(left < 0 ? 0 : (left > 16 ? 16 : left)) * row_bytes);
+        return make_rsrc(at(page < 0 ? 0 : page, row), (long long)(left < 0 ? 0 : (left > most ? most : left)) * row_bytes);
     }
 };
 
@@ -373,63 +377,66 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
 }
 
 // Merge of the divided tiles: o = sum_i O_i 2^(m_i - M) / l, stats = M ln 2 + log l.
-// One thread per four columns of a row; eight parts at a time, whose loads all
-// go out before the first is used.
+// A workgroup takes 8 rows of a tile at a time, a thread four columns of a row;
+// four parts' loads go out together.
+constexpr int kMergeRows = 8;
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     PagedPlan<BM, BN> plan(p);
-    PagedItem it;
-    if (!plan.template find<true>((int)blockIdx.x, it) || !slot_ok(p, it)) return;
-    const int np = it.s.parts, cpr = p.D_v / 4, row0 = it.tile * BM;
-    const int rows = min(BM, it.s.n * p.G - row0);
-    constexpr int U = 8;
-    for (int i = threadIdx.x; i < rows * cpr; i += 256) {
-        const int r = i / cpr, c = 4 * (i - r * cpr);
-        float M = -INFINITY, L = 0.f;
-        floatx4 acc = floatx4{};
-        for (int k0 = 0; k0 < np; k0 += U) {
-            floatx2 ml[U];
-            floatx4 o[U];
+    const int units = plan.template items<true>() * (BM / kMergeRows), cpr = p.D_v / 4;
+    constexpr int U = 4;
+    for (int unit = (int)blockIdx.x; unit < units; unit += (int)gridDim.x) {
+        PagedItem it;
+        if (!plan.template find<true>(unit / (BM / kMergeRows), it) || !slot_ok(p, it)) return;
+        const int np = it.s.parts, row0 = unit % (BM / kMergeRows) * kMergeRows;
+        const int rows = min(kMergeRows, it.s.n * p.G - it.tile * BM - row0);
+        for (int i = threadIdx.x; i < rows * cpr; i += 256) {
+            const int r = row0 + i / cpr, c = 4 * (i % cpr);
+            float M = -INFINITY, L = 0.f;
+            floatx4 acc = floatx4{};
+            for (int k0 = 0; k0 < np; k0 += U) {
+                floatx2 ml[U];
+                floatx4 o[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const size_t at = (size_t)(it.slot + (k0 + u < np ? k0 + u : np - 1)) * BM + r;
-                ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * at);
-                o[u] = *reinterpret_cast<const floatx4*>(p.part_o + at * p.D_v + c);
+                for (int u = 0; u < U; ++u) {
+                    const size_t at = (size_t)(it.slot + (k0 + u < np ? k0 + u : np - 1)) * BM + r;
+                    ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * at);
+                    o[u] = *reinterpret_cast<const floatx4*>(p.part_o + at * p.D_v + c);
+                }
+                float Mn = M;
+#pragma unroll
+                for (int u = 0; u < U; ++u) Mn = fmaxf(Mn, ml[u][0]);
+                const float a = M == Mn ? 1.f : part_weight(M, Mn);
+                L *= a;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = add_part(0.f, acc[e], a);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (k0 + u >= np) break;
+                    const float w = part_weight(ml[u][0], Mn);
+                    // (a NaN sum has no maximum to weigh it by)
+                    L = ml[u][1] == ml[u][1] ? __builtin_fmaf(ml[u][1], w, L) : ml[u][1];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = add_part(acc[e], o[u][e], w);
+                }
+                M = Mn;
             }
-            float Mn = M;
+            PagedRow row;
+            row.init(p, it, it.tile * BM + r);
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            t4 v;
 #pragma unroll
-            for (int u = 0; u < U; ++u) Mn = fmaxf(Mn, ml[u][0]);
-            const float a = M == Mn ? 1.f : part_weight(M, Mn);
-            L *= a;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = add_part(0.f, acc[e], a);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (k0 + u >= np) break;
-                const float w = part_weight(ml[u][0], Mn);
-                // (a NaN sum has no maximum to weigh it by)
-                L = ml[u][1] == ml[u][1] ? __builtin_fmaf(ml[u][1], w, L) : ml[u][1];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = add_part(acc[e], o[u][e], w);
-            }
-            M = Mn;
+            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
+            *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
+            if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
         }
-        PagedRow row;
-        row.init(p, it, row0 + r);
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
-        *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
-        if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
     }
 }
 
 template <typename T, int BM, int BN>
 hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
-    // divided tiles have two parts at least
-    return launch_kernel<paged_merge_kernel<T, BM, BN>>(dim3((unsigned)p.target), 256, 0, stream, p);
+    return launch_kernel<paged_merge_kernel<T, BM, BN>>(dim3(1024), 256, 0, stream, p);
 }
 
 // Whether a launch may divide anything: some tile can walk more than

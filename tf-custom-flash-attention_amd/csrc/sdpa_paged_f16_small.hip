@@ -114,8 +114,8 @@ void paged_f16_small_kernel(const PagedParams p) {
         for (int g = 0; g < 2; ++g) {
             const int r0 = blk * BN + 16 * g;
             const int page = r0 < kv_end ? pw.page(r0 >> K.log2, lane) : -1;
-            kc.issue(K.rows16(page, r0, kv_end), ring + so + (uint32_t)(256 * LK * g));
-            vc.issue(V.rows16(page, r0, kv_end), ring + so + (uint32_t)(Cfg::KB + 256 * LV * g));
+            kc.issue(K.rows(page, r0, kv_end, 16), ring + so + (uint32_t)(256 * LK * g));
+            vc.issue(V.rows(page, r0, kv_end, 16), ring + so + (uint32_t)(Cfg::KB + 256 * LV * g));
         }
     };
     prologue_loads_landed();
