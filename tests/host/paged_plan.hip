@@ -5,6 +5,7 @@
 //   - every sequence whose range is one is in the plan, and no other;
 //   - tiles cover the rows, and parts of a tile its blocks, once each;
 //   - tokens and lengths stay inside the batch, whatever the arrays hold;
+//   - shares are in order and equal to one block, and every block has its owner;
 //   - workgroup ids map one to one onto the items.
 #include <cstdio>
 #include <cstdlib>
@@ -82,6 +83,16 @@ int main() {
             }
             CHECK(slots <= 2 * p.target && divided <= p.target);
             if (!garbage) CHECK(items <= paged_max_tiles(p, BM) + p.target);
+            if (cost > 0) {
+                const long long total = cost * H_kv;
+                const int n = (int)(total < kPagedTarget ? total : kPagedTarget);
+                CHECK(share_begin(total, 0, n) == 0 && share_begin(total, n, n) == total);
+                for (int w = 0; w < n; ++w) {
+                    const long long a = share_begin(total, w, n), b = share_begin(total, w + 1, n);
+                    CHECK(b - a >= total / n && b - a <= total / n + 1);
+                    CHECK(share_owner(total, a, n) == w && share_owner(total, b - 1, n) == w);
+                }
+            }
             if (cs % 50 == 0) {
                 const int n = (int)items;
                 std::vector<char> hit(n, 0);

@@ -6,13 +6,20 @@
 // i G + g is token i, head h G + g.  A tile is up to BM of them.
 //
 // Division.  The lengths are on the device, so every workgroup forms the plan
-// itself, from sums over the sequences: the cost of a tile is the number of
-// key blocks it walks on average; the keys of a tile are divided into parts of
-// at most `chunk` blocks, chunk being the larger of kPagedMinChunk and the
-// whole cost over `target` workgroups.  So at most target workgroups more than
-// there are tiles have work, whatever the lengths, and at most 2 target
-// parts are of divided tiles: the grid and the workspace go by the call's
-// sizes alone.  Parts are merged in order by a second kernel.
+// itself, from sums over the sequences; the grid and the workspace go by the call's
+// sizes alone.  Two forms, both merged in order by a second kernel:
+//   parts   The cost of a tile is the number of key blocks it walks on
+//           average; the keys of a tile are divided into parts of at most `chunk`
+//           blocks, chunk being the larger of kPagedMinChunk and the whole cost over
+//           `target` workgroups.  So at most target workgroups more than there
+//           are tiles have work, whatever the lengths, and at most 2 target parts
+//           are of divided tiles.
+//   shares  The key blocks of all tiles, one tile after the other, are cut into
+//           equal shares, one for each of `target` workgroups, which walks the
+//           tiles that its share meets.  It leaves at most two partial tiles: slot
+//           2 w holds one that began before its share, 2 w + 1 one that it begins
+//           and does not end.  For generation, where a workgroup's time is the
+//           keys it reads.
 #pragma once
 
 #include "sdpa_kv_append.h"
@@ -32,7 +39,7 @@ struct PagedParams {
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
-    int target;  // workgroups to divide for; 0: no workspace, nothing is divided
+    int target;  // workgroups to divide for (parts: 0 where nothing is divided)
 };
 
 constexpr int kPagedMinChunk = 2;   // key blocks of a part, at least
@@ -78,16 +85,25 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
     return (rows / BM + (rows < p.batch.N ? rows : p.batch.N)) * p.H_kv;
 }
 
-// Calls whose sequences have up to so many rows take the kernel of 32-row
-// tiles, whose waves divide the keys; others that of 128-row tiles.
+// Calls whose sequences have one tile of 32 rows, as far as is known, take the
+// kernels of such tiles, by shares; others, by parts, that of 128-row tiles (fp32: of 32).
 constexpr int kPagedSmallRows = 32;
+
+// Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)).
+__host__ __device__ inline long long share_begin(long long total, int w, int n) {
+    return total / n * w + (total % n) * w / n;
+}
+// The workgroup whose share holds block u: the largest w with total w / n < u + 1.
+__host__ __device__ inline int share_owner(long long total, long long u, int n) {
+    return (int)(((u + 1) * n - 1) / total);
+}
 
 // Workgroups the launches divide for, and the workspace of one launch's parts.
 constexpr int kPagedTarget = 512;
 constexpr int kPagedSmallBM = 32, kPagedBM = 128;
-inline bool paged_small(bool f16, long long T, int G, int max_q_len) {
+inline bool paged_small(long long T, int G, int max_q_len) {
     const long long most = max_q_len > 0 && max_q_len < T ? max_q_len : T;
-    return !f16 || most * G <= kPagedSmallRows;
+    return most * G <= kPagedSmallRows;
 }
 inline size_t paged_part_bytes(int D_v, int BM) {
     return 2 * (size_t)kPagedTarget * BM * ((size_t)D_v + 2) * sizeof(float);
@@ -95,6 +111,7 @@ inline size_t paged_part_bytes(int D_v, int BM) {
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream);
-hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream);
+// (fp32: by shares, or by parts)
+hipError_t launch_paged_f32(const PagedParams& p, bool shares, hipStream_t stream);
 
 }  // namespace sdpa

@@ -251,7 +251,7 @@ size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, in
                                           int D_qk, int D_v, int max_q_len) {
     if (check_paged(dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
         return 0;
-    return paged_workspace(sdpa::paged_small(dtype == SDPA_DTYPE_F16, T, H_q / H_kv, max_q_len), width, page_size, D_v);
+    return paged_workspace(sdpa::paged_small(T, H_q / H_kv, max_q_len), width, page_size, D_v);
 }
 
 int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -289,15 +289,17 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     p.causal = causal_mask != 0;
     if ((long long)T * p.G > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     // sequences of few rows, as far as is known here (either kernel takes any)
-    const bool small = sdpa::paged_small(dtype == SDPA_DTYPE_F16, T, p.G, max_q_len);
+    const bool small = sdpa::paged_small(T, p.G, max_q_len);
     if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
+    // rows of a tile of the kernel that is taken
+    const int BM = small || dtype == SDPA_DTYPE_F32 ? sdpa::kPagedSmallBM : sdpa::kPagedBM;
+    p.target = sdpa::kPagedTarget;
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
-        p.target = sdpa::kPagedTarget;
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + 2 * (size_t)p.target * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
+        p.part_ml = p.part_o + 2 * (size_t)p.target * BM * D_v;
     }
-    if (dtype == SDPA_DTYPE_F32) return hip_status(sdpa::launch_paged_f32(p, stream));
+    if (dtype == SDPA_DTYPE_F32) return hip_status(sdpa::launch_paged_f32(p, small, stream));
     return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));
 }
 

@@ -29,11 +29,14 @@ __device__ __forceinline__ long long wave_sum64(long long x) {
     return x;
 }
 
-// One workgroup's work, the same in every lane.
+// One workgroup's work, the same in every lane: a tile, or a part of its keys.
 struct PagedItem {
     SeqPlan s;
-    int seq, h, tile, part;
-    int slot;  // of this part in the workspace, where the tile is divided
+    int seq, h, tile;
+    bool divided;
+    int slot;    // of this part in the workspace, where the tile is divided
+    int part;    // (parts) of s.parts
+    int u0, u1;  // (shares) blocks of the tile
 };
 
 template <int BM, int BN>
@@ -103,6 +106,7 @@ struct PagedPlan {
                 it.tile = it.s.tiles - 1 - t;
                 it.part = i - t * per_tile;
                 it.slot = get(slot) - get(div) + (it.h * it.s.tiles + it.tile) * it.s.parts + it.part;
+                it.divided = it.s.parts > 1;
                 return true;
             }
             base = __builtin_amdgcn_readlane(end, 63);
@@ -112,10 +116,102 @@ struct PagedPlan {
     }
 };
 
+// The plan by shares: the blocks of all tiles in the order sequence, key head, tile.
+// Where there are up to 64 sequences their lanes' part of it is kept in LDS (each
+// wave writes the same), as registers are short in the kernels' loops.
+template <int BM, int BN>
+struct PagedShares {
+    struct Lane {
+        SeqPlan s;
+        long long first, last;  // blocks
+    };
+    static constexpr int LDS_BYTES = 64 * (int)sizeof(Lane);
+    const PagedParams& p;
+    Lane* const kept;
+    long long total = 0;
+    int n = 0;  // workgroups
+
+    __device__ __forceinline__ static long long readlane64(long long x, int l) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+        return ((long long)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | lo;
+    }
+    // sequences n0 + lane; base: the blocks before them
+    __device__ __forceinline__ Lane form(int n0, long long base) const {
+        const int lane = threadIdx.x & 63, i = n0 + lane;
+        int q0 = 0, q1 = 0, len = 0;
+        if (i < p.batch.N) {
+            q0 = p.batch.q_starts[i];
+            q1 = p.batch.q_starts[i + 1];
+            len = p.batch.kv_lens[i];
+        }
+        Lane x;
+        // (all tiles of a sequence count as its last one)
+        x.s = seq_plan(q0, q1, len, p.batch, p.G, false, BM, BN, 0);
+        const long long mine = (long long)x.s.tiles * x.s.blocks * p.H_kv;
+        x.last = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const long long y = __shfl_up(x.last, d);
+            if (lane >= d) x.last += y;
+        }
+        x.last += base;
+        x.first = x.last - mine;
+        return x;
+    }
+    __device__ __forceinline__ PagedShares(const PagedParams& p_, void* lds) : p(p_), kept(static_cast<Lane*>(lds)) {
+        for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
+            const Lane x = form(n0, total);
+            total = readlane64(x.last, 63);
+            if (p.batch.N <= 64) kept[threadIdx.x & 63] = x;
+        }
+        n = (int)(total < p.target ? total : p.target);
+    }
+    // The tile that holds block `at` < total, and its first block.
+    __device__ __forceinline__ long long tile(long long at, PagedItem& it) const {
+        long long base = 0;
+        for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
+            const Lane x = p.batch.N <= 64 ? kept[threadIdx.x & 63] : form(n0, base);
+            const uint64_t over = __builtin_amdgcn_ballot_w64(x.last > at);
+            base = readlane64(x.last, 63);
+            if (over == 0) continue;
+            const int l = __builtin_ctzll(over);
+            const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            it.s = SeqPlan{get(x.s.q0), get(x.s.n), get(x.s.len), get(x.s.tiles), get(x.s.blocks), 1, get(x.s.bad) != 0};
+            it.seq = n0 + l;
+            const long long begin = readlane64(x.first, l);
+            const int t = (int)((at - begin) / it.s.blocks);
+            it.h = t / it.s.tiles;
+            it.tile = t - it.h * it.s.tiles;
+            return begin + (long long)t * it.s.blocks;
+        }
+        return at;  // (not reached)
+    }
+    // work(item) for every tile, or part of one, of workgroup w's share.  Without a
+    // workspace the tiles that begin in the share, whole.
+    template <typename F>
+    __device__ __forceinline__ void each(int w, F&& work) const {
+        if (w >= n) return;
+        const long long end = share_begin(total, w + 1, n);
+        for (long long at = share_begin(total, w, n); at < end;) {
+            PagedItem it;
+            const long long t0 = tile(at, it), t1 = t0 + it.s.blocks;
+            const bool divide = p.part_o != nullptr, skip = !divide && t0 != at;
+            const long long stop = divide && end < t1 ? end : t1;
+            it.u0 = (int)(at - t0);
+            it.u1 = (int)(stop - t0);
+            it.divided = it.u0 != 0 || stop != t1;
+            it.slot = 2 * w + (it.u0 == 0 ? 1 : 0);
+            it.part = 0;
+            at = stop;
+            if (!skip) work(it);
+        }
+    }
+};
+
 // A divided tile's part has room in the workspace.  (It always has, but for
 // q_starts that go back and forth, whose sums may pass 32 bits.)
 __device__ __forceinline__ bool slot_ok(const PagedParams& p, const PagedItem& it) {
-    return it.s.parts == 1 || (it.slot >= 0 && it.slot + it.s.parts <= 2 * p.target + it.part);
+    return !it.divided || (it.slot >= 0 && it.slot + it.s.parts <= 2 * p.target + it.part);
 }
 
 // Workgroup id -> item, XCD-major: XCD x takes the items [x n / 8, (x + 1) n / 8),
@@ -255,7 +351,7 @@ template <typename T, int BM>
 __device__ __forceinline__ void put_care_row(const PagedParams& p, const PagedItem& it, const PagedRow& row, int in_tile,
                                              const CareRow& r) {
     const int lane = threadIdx.x & 63;
-    if (it.s.parts > 1) {
+    if (it.divided) {
         const size_t at = (size_t)it.slot * BM + in_tile;
         if (lane == 0) {
             p.part_ml[2 * at] = r.m;
@@ -292,7 +388,11 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
                                                   int k1) {
     constexpr int OS = acc_stride(DV), NT = 64 * NW, ITER = (BM * (DV / 4) + NT - 1) / NT;
     static_assert(BM == 32 && BM * (DV / 4) % NT == 0, "one accumulator tile of rows");
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+    // (opaque: what is formed from it below stays out of the callers' loops, whose
+    // registers it would take)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* mml = lds + NW * BM * OS;
     int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);  // rows to do again
@@ -348,7 +448,7 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
     for (int u = 0; u < ITER; ++u) {
         const int i = u * NT + tid, r = i / (DV / 4), c = 4 * (i % (DV / 4));
         if (r >= rows || c >= p.D_v || again[r]) continue;
-        if (it.s.parts > 1) {
+        if (it.divided) {
             const size_t at = (size_t)it.slot * BM + r;
             if (c == 0) {
                 p.part_ml[2 * at] = M[u];
@@ -434,15 +534,95 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     }
 }
 
+// Merge of the tiles that shares divide.  Workgroup (w, y) looks at the boundary
+// before share w + 1: it merges rows y, y + gridDim.y, ... of the tile that lies
+// across it, if the tile lies across none before.  A row's parts are dealt over
+// groups of D_v / 4 threads (a thread: four columns), whose sums meet in LDS.
+template <typename T, int BM, int BN, int DV>
+__global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParams p) {
+    constexpr int CPR = DV / 4, NG = 256 / CPR;
+    __shared__ floatx4 sum[256];
+    __shared__ floatx2 sml[256];
+    __shared__ typename PagedShares<BM, BN>::Lane lanes[64];
+    const PagedShares<BM, BN> plan(p, lanes);
+    const int w = (int)blockIdx.x;
+    if (w + 1 >= plan.n) return;
+    const long long at = share_begin(plan.total, w + 1, plan.n);
+    PagedItem it;
+    const long long t0 = plan.tile(at, it);
+    if (t0 == at || share_owner(plan.total, t0, plan.n) != w) return;
+    const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n) - w + 1;
+    const int rows = min(BM, it.s.n * p.G - it.tile * BM);
+    const int group = threadIdx.x / CPR, c = 4 * (threadIdx.x % CPR);
+    const auto add = [](float& M, float& L, floatx4& acc, float m, float l, const floatx4& o) {
+        const float Mn = fmaxf(M, m), a = M == Mn ? 1.f : part_weight(M, Mn), b = part_weight(m, Mn);
+        // (a NaN sum has no maximum to weigh it by)
+        L = l == l ? __builtin_fmaf(l, b, L * a) : l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = add_part(add_part(0.f, acc[e], a), o[e], b);
+        M = Mn;
+    };
+    for (int r = (int)blockIdx.y; r < rows; r += (int)gridDim.y) {
+        float M = -INFINITY, L = 0.f;
+        floatx4 acc = floatx4{};
+        constexpr int U = 4;
+        for (int k0 = group; k0 < np; k0 += U * NG) {
+            floatx2 ml[U];
+            floatx4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = min(k0 + u * NG, np - 1);
+                const size_t row = (size_t)(k == 0 ? 2 * w + 1 : 2 * (w + k)) * BM + r;
+                ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * row);
+                o[u] = floatx4{};
+                if (c < p.D_v) o[u] = *reinterpret_cast<const floatx4*>(p.part_o + row * p.D_v + c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (k0 + u * NG < np) add(M, L, acc, ml[u][0], ml[u][1], o[u]);
+        }
+        __syncthreads();  // (the row before has been read)
+        sum[threadIdx.x] = acc;
+        sml[threadIdx.x] = (floatx2){M, L};
+        __syncthreads();
+        if (group == 0 && c < p.D_v) {
+            for (int g = 1; g < min(NG, np); ++g)
+                add(M, L, acc, sml[g * CPR + threadIdx.x][0], sml[g * CPR + threadIdx.x][1], sum[g * CPR + threadIdx.x]);
+            PagedRow row;
+            row.init(p, it, it.tile * BM + r);
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            t4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
+            *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
+            if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
+        }
+    }
+}
+
+template <typename T, int BM, int BN, int DV>
+hipError_t launch_paged_share_merge(const PagedParams& p, hipStream_t stream) {
+    const int rows = (int)(p.G < 8 ? p.G : 8);
+    return launch_kernel<paged_share_merge_kernel<T, BM, BN, DV>>(dim3((unsigned)p.target - 1, (unsigned)rows), 256, 0, stream,
+                                                                 p);
+}
+
 template <typename T, int BM, int BN>
 hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
     return launch_kernel<paged_merge_kernel<T, BM, BN>>(dim3(1024), 256, 0, stream, p);
 }
 
-// Whether a launch may divide anything: some tile can walk more than
-// kPagedMinChunk blocks.
-inline bool paged_may_divide(const PagedParams& p, int BN) {
-    return p.target > 0 && ((long long)p.batch.width << p.batch.page_log2) > (long long)kPagedMinChunk * BN;
+// The arguments of a launch by parts: target 0 where nothing can be divided, for
+// want of a workspace, or as no tile walks more than kPagedMinChunk blocks.
+inline PagedParams paged_parts(const PagedParams& p, int BN) {
+    PagedParams a = p;
+    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)kPagedMinChunk * BN) a.target = 0;
+    return a;
+}
+// Whether a launch by shares may divide a tile.
+inline bool paged_shares_divide(const PagedParams& p, int BN) {
+    return p.part_o && ((long long)p.batch.width << p.batch.page_log2) > BN;
 }
 
 }  // namespace

@@ -321,7 +321,7 @@ void paged_f16_kernel(const PagedParams p) {
     const float nan = __builtin_nanf("");
     if (row.live && !((again >> l32) & 1)) {
         const float m = l_tot == 0.f ? -INFINITY : m_run, l = bad ? nan : l_tot;
-        if (np > 1) {  // this part's unnormalised O, m and l
+        if (it.divided) {  // this part's unnormalised O, m and l
             const size_t at = (size_t)it.slot * BM + in_tile;
             if (hh == 0) {
                 p.part_ml[2 * at] = m;
@@ -361,12 +361,10 @@ hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream) {
         return with_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedCfg<DQK, DV>;
-            const bool divide = paged_may_divide(p, Cfg::BN);
-            PagedParams a = p;
-            if (!divide) a.target = 0;
+            const PagedParams a = paged_parts(p, Cfg::BN);
             const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
             hipError_t e = launch_kernel<paged_f16_kernel<DQK, DV>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES, stream, a);
-            return e == hipSuccess && divide ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;
+            return e == hipSuccess && a.target > 0 ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;
         });
     });
 }

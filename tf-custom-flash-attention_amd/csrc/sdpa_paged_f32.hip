@@ -19,145 +19,163 @@ namespace {
 template <int DQK, int DV>
 struct PagedF32Cfg {
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedSmallBM, BN = 32, PLAN = BN * NW;
-    static constexpr size_t LDS_BYTES = NW * BM * acc_stride(DV) * 4 + NW * BM * 8 + (BM + NW) * 4;
+    static constexpr int PLAN_AT = NW * BM * acc_stride(DV) * 4 + NW * BM * 8 + (BM + NW) * 4;
+    static_assert(PLAN_AT % 16 == 0, "the plan, behind the sums");
+    static constexpr size_t LDS_BYTES = PLAN_AT + PagedShares<BM, PLAN>::LDS_BYTES;
 };
 
-template <int DQK, int DV>
+template <int DQK, int DV, bool SHARES>
 __global__ __launch_bounds__((PagedF32Cfg<DQK, DV>::NT))
 __attribute__((amdgpu_waves_per_eu(DQK + DV > 128 ? 1 : 2, DQK + DV > 128 ? 1 : 2)))
 void paged_f32_kernel(const PagedParams p) {
     using Cfg = PagedF32Cfg<DQK, DV>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW, NKC = DQK / 8, NDT = DV / 32;
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int D_qk = p.D_qk, D_v = p.D_v;
+    const auto work = [&](const PagedItem& it) __attribute__((always_inline)) {
+        int tid = threadIdx.x;  // (opaque: lane terms are formed for each tile, not held across them)
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int kv_end = min(tile_keys(p, it, BM), it.s.len);
+        PagedRow row;
+        row.init(p, it, it.tile * BM + l32);
 
-    PagedPlan<BM, Cfg::PLAN> plan(p);
-    PagedItem it;
-    {
-        const int at = xcd_item(tile_id(), plan.template items<false>());
-        if (at < 0 || !plan.template find<false>(at, it) || !slot_ok(p, it)) return;
-    }
-    const int D_qk = p.D_qk, D_v = p.D_v, np = it.s.parts;
-    const int kv_end = min(tile_keys(p, it, BM), it.s.len);
-    PagedRow row;
-    row.init(p, it, it.tile * BM + l32);
-
-    // the factor goes into the queries: scores come out in the log2 domain
-    const float sl2 = p.scale * kLog2e;
-    floatx4 q[NKC];
-    const float* qrow = static_cast<const float*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h;
-#pragma unroll
-    for (int c = 0; c < NKC; ++c) {
-        const int d = 8 * c + 4 * hh;
-        q[c] = floatx4{};
-        if (row.live && d < D_qk) q[c] = *reinterpret_cast<const floatx4*>(qrow + d) * sl2;
-    }
-
-    const int nblk = (kv_end + BN - 1) / BN;
-    const int lo = part_begin(nblk, it.part, np), hi = part_begin(nblk, it.part + 1, np);
-    PagedRows K, V;
-    K.init(p.k_cache, p.H_kv, it.h, D_qk, 4, p.batch.page_log2);
-    V.init(p.v_cache, p.H_kv, it.h, D_v, 4, p.batch.page_log2);
-    PageWindow pw{uniform_ptr(p.batch.page_table + it.seq * p.batch.table_stride), p.batch.pages,
-                  (min(kv_end, hi * BN) + (1 << K.log2) - 1) >> K.log2};
-    floatx4 k[NKC];
-    float v[16][NDT];
-    // K rows of a block: keys past the last are read as the last (and masked)
-    auto load_k = [&](int blk) {
-        const int key = min(blk * BN + l32, kv_end - 1), column = key >> K.log2;
-        pw.page((blk * BN) >> K.log2, lane);  // the window holds the block's columns
-        const int page = __shfl(pw.id, column - pw.first);
-        const float* src = reinterpret_cast<const float*>(K.at(page < 0 ? 0 : page, key));
+        // the factor goes into the queries: scores come out in the log2 domain
+        const float sl2 = p.scale * kLog2e;
+        floatx4 q[NKC];
+        const float* qrow = static_cast<const float*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h;
 #pragma unroll
         for (int c = 0; c < NKC; ++c) {
             const int d = 8 * c + 4 * hh;
-            k[c] = *reinterpret_cast<const floatx4*>(src + (d < D_qk ? d : 0));
-            if (D_qk < DQK) k[c] = d < D_qk ? k[c] : floatx4{};
+            q[c] = floatx4{};
+            if (row.live && d < D_qk) q[c] = *reinterpret_cast<const floatx4*>(qrow + d) * sl2;
         }
-    };
-    // V rows of a block, zero past the last
-    auto load_v = [&](int blk) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int r0 = blk * BN + 16 * g;
-            const int page = r0 < kv_end ? pw.page(r0 >> K.log2, lane) : -1;
-            const int left = page < 0 ? 0 : min(16, kv_end - r0);
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<unsigned char*>(V.at(page < 0 ? 0 : page, r0)), (short)0, left * V.row_bytes, 0x00020000);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) {
-                    const int d = 32 * dt + l32;
-                    const uint32_t off = d < D_v ? (uint32_t)((8 * (r >> 2) + 4 * hh + (r & 3)) * V.row_bytes + 4 * d) : kOob;
-                    v[8 * g + r][dt] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
-                }
-        }
-    };
-    if (lo + wave < hi) load_k(lo + wave);
 
-    floatx16 oacc[NDT];
+        const int nblk = (kv_end + BN - 1) / BN;
+        const int lo = SHARES ? min(NW * it.u0, nblk) : part_begin(nblk, it.part, it.s.parts);
+        const int hi = SHARES ? min(NW * it.u1, nblk) : part_begin(nblk, it.part + 1, it.s.parts);
+        PagedRows K, V;
+        K.init(p.k_cache, p.H_kv, it.h, D_qk, 4, p.batch.page_log2);
+        V.init(p.v_cache, p.H_kv, it.h, D_v, 4, p.batch.page_log2);
+        PageWindow pw{uniform_ptr(p.batch.page_table + it.seq * p.batch.table_stride), p.batch.pages,
+                      (min(kv_end, hi * BN) + (1 << K.log2) - 1) >> K.log2};
+        floatx4 k[NKC];
+        float v[16][NDT];
+        // K rows of a block: keys past the last are read as the last (and masked)
+        auto load_k = [&](int blk) {
+            const int key = min(blk * BN + l32, kv_end - 1), column = key >> K.log2;
+            pw.page((blk * BN) >> K.log2, lane);  // the window holds the block's columns
+            const int page = __shfl(pw.id, column - pw.first);
+            const float* src = reinterpret_cast<const float*>(K.at(page < 0 ? 0 : page, key));
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) oacc[dt] = floatx16{};
-    float m_run = -INFINITY, l_run = 0.f;
-    for (int blk = lo + wave; blk < hi; blk += NW) {
-        const int kv0 = blk * BN;
-        load_v(blk);
-        floatx16 s = floatx16{};
+            for (int c = 0; c < NKC; ++c) {
+                const int d = 8 * c + 4 * hh;
+                k[c] = *reinterpret_cast<const floatx4*>(src + (d < D_qk ? d : 0));
+                if (D_qk < DQK) k[c] = d < D_qk ? k[c] : floatx4{};
+            }
+        };
+        // V rows of a block, zero past the last
+        auto load_v = [&](int blk) {
 #pragma unroll
-        for (int c = 0; c < NKC; ++c)
+            for (int g = 0; g < 2; ++g) {
+                const int r0 = blk * BN + 16 * g;
+                const int page = r0 < kv_end ? pw.page(r0 >> K.log2, lane) : -1;
+                const int left = page < 0 ? 0 : min(16, kv_end - r0);
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<unsigned char*>(V.at(page < 0 ? 0 : page, r0)), (short)0, left * V.row_bytes, 0x00020000);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = mfma_f32(k[c][e], q[c][e], s);
-        if (blk + NW < hi) load_k(blk + NW);
-        if (wave_any(kv0 + BN > row.see)) {
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt) {
+                        const int d = 32 * dt + l32;
+                        const uint32_t off = d < D_v ? (uint32_t)((8 * (r >> 2) + 4 * hh + (r & 3)) * V.row_bytes + 4 * d) : kOob;
+                        v[8 * g + r][dt] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+                    }
+            }
+        };
+        if (lo + wave < hi) load_k(lo + wave);
+
+        floatx16 oacc[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) oacc[dt] = floatx16{};
+        float m_run = -INFINITY, l_run = 0.f;
+        for (int blk = lo + wave; blk < hi; blk += NW) {
+            const int kv0 = blk * BN;
+            load_v(blk);
+            floatx16 s = floatx16{};
+#pragma unroll
+            for (int c = 0; c < NKC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s = mfma_f32(k[c][e], q[c][e], s);
+            if (blk + NW < hi) load_k(blk + NW);
+            if (wave_any(kv0 + BN > row.see)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = kv0 + 8 * (r >> 2) + 4 * hh + (r & 3);
+                    if (key >= row.see) s[r] = -INFINITY;
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            const float m_use = fmaxf(m_run, xhalf_max(mx));
+            const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
+            const float m0 = m_use == -INFINITY ? 0.f : m_use;
+            float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int key = kv0 + 8 * (r >> 2) + 4 * hh + (r & 3);
-                if (key >= row.see) s[r] = -INFINITY;
+                s[r] = fast_exp2(s[r] - m0);
+                sum += s[r];
             }
+            if (wave_any(alpha != 1.f)) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
+            }
+            l_run = __builtin_fmaf(l_run, alpha, sum);
+            m_run = m_use;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) oacc[dt] = mfma_f32(v[r][dt], s[r], oacc[dt]);
         }
-        float mx = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        const float m_use = fmaxf(m_run, xhalf_max(mx));
-        const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
-        const float m0 = m_use == -INFINITY ? 0.f : m_use;
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = fast_exp2(s[r] - m0);
-            sum += s[r];
-        }
-        if (wave_any(alpha != 1.f)) {
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
-        }
-        l_run = __builtin_fmaf(l_run, alpha, sum);
-        m_run = m_use;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) oacc[dt] = mfma_f32(v[r][dt], s[r], oacc[dt]);
+        merge_paged_waves<float, DV, NW, BM>(p, it, reinterpret_cast<float*>(smem), oacc, m_run, xhalf_sum(l_run),
+                                             pw.bad || it.s.bad, pw.row, K, V, lo * BN, hi * BN);
+    };
+    if constexpr (SHARES) {
+        const PagedShares<BM, Cfg::PLAN> plan(p, smem + Cfg::PLAN_AT);
+        plan.each(tile_id(), [&](const PagedItem& it) __attribute__((always_inline)) {
+            work(it);
+            __syncthreads();
+        });
+    } else {
+        PagedPlan<BM, Cfg::PLAN> plan(p);
+        PagedItem it;
+        const int at = xcd_item(tile_id(), plan.template items<false>());
+        if (at >= 0 && plan.template find<false>(at, it) && slot_ok(p, it)) work(it);
     }
-    merge_paged_waves<float, DV, NW, BM>(p, it, reinterpret_cast<float*>(smem), oacc, m_run, xhalf_sum(l_run),
-                                         pw.bad || it.s.bad, pw.row, K, V, lo * BN, hi * BN);
 }
 
 }  // namespace
 
-hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream) {
+hipError_t launch_paged_f32(const PagedParams& p, bool shares, hipStream_t stream) {
     return with_dim(p.D_qk, [&](auto dqk) {
         return with_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedF32Cfg<DQK, DV>;
-            const bool divide = paged_may_divide(p, Cfg::PLAN);
-            PagedParams a = p;
-            if (!divide) a.target = 0;
+            if (shares) {
+                hipError_t e = launch_kernel<paged_f32_kernel<DQK, DV, true>>(dim3((unsigned)p.target), Cfg::NT,
+                                                                              Cfg::LDS_BYTES, stream, p);
+                return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
+                           ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(p, stream)
+                           : e;
+            }
+            const PagedParams a = paged_parts(p, Cfg::PLAN);
             const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
-            hipError_t e = launch_kernel<paged_f32_kernel<DQK, DV>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES, stream, a);
-            return e == hipSuccess && divide ? launch_paged_merge<float, Cfg::BM, Cfg::PLAN>(a, stream) : e;
+            hipError_t e = launch_kernel<paged_f32_kernel<DQK, DV, false>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES,
+                                                                           stream, a);
+            return e == hipSuccess && a.target > 0 ? launch_paged_merge<float, Cfg::BM, Cfg::PLAN>(a, stream) : e;
         });
     });
 }
