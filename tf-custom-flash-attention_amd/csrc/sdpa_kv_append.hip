@@ -56,7 +56,8 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const Appe
     const unsigned uu = (unsigned)u, tg = uu / (unsigned)m.splits;
     const int group = lane / LPR, tok0 = (int)(tg * (unsigned)m.tpw), mine = group / m.gpt;
     const long long tok = (long long)tok0 + mine;
-    const int h0 = (int)(uu - tg * (unsigned)m.splits) * m.gpt * KU + group % m.gpt;
+    const int first = (int)(uu - tg * (unsigned)m.splits) * m.gpt * KU, h0 = first + group % m.gpt;
+    const int rows = min(KU, (m.H - first + m.gpt - 1) / m.gpt);  // per group, those that some group has
     const bool in_batch = tok < bt.T;
 
     // the rows, before it is known where they go
@@ -65,12 +66,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const Appe
     l.init(lane % LPR, D, kind == 2 ? 0 : p.r.R, p.interleaved != 0);
     const T* x = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v);
     const TokenStrides xs = kind == 0 ? p.qs : kind == 1 ? p.ks : p.vs;
-    float a[KU][EPC], b[KU][EPC];
+    chunk_t<T, EPC> a[KU], b[KU];
 #pragma unroll
-    for (int k = 0; k < KU; ++k) {
-        const int h = h0 + k * m.gpt;
-        load_row<T, EPC, IN>(a[k], b[k], x + tok * xs.t + h * xs.h, in_batch && h < m.H, l);
-    }
+    for (int k = 0; k < KU; ++k)
+        if (k < rows) load_row<T, EPC, IN>(a[k], b[k], x + (in_batch ? tok : bt.T - 1) * xs.t + min(h0 + k * m.gpt, m.H - 1) * xs.h, l);
 
     // sequence of the token: the last that begins at or before it
     int count = 0;
@@ -106,19 +105,16 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const Appe
         hs = (long long)D << bt.page_log2;
         y = static_cast<T*>(kind == 1 ? p.k_cache : p.v_cache) + (long long)page * p.H_kv * hs + slot * D;
     }
+    RowFactors<EPC, IN> f;
+    if (kind != 2) f.init(l, t, wa, wb);
 #pragma unroll
     for (int k = 0; k < KU; ++k) {
+        if (k >= rows) break;
         const int h = h0 + k * m.gpt;
         if (kind != 2) {
-            float r = p.r.norm ? row_rnorm<LPR, EPC>(a[k], b[k], D, p.r.eps) : 1.f;
+            float r = p.r.norm ? row_rnorm<T, LPR, EPC, IN>(a[k], b[k], l, p.r) : 1.f;
             if (t.bad || !placed) r = __builtin_nanf("");
-            if (p.r.norm || r != 1.f)
-#pragma unroll
-                for (int i = 0; i < EPC; ++i) {
-                    a[k][i] = a[k][i] * r * wa[i];
-                    b[k][i] = b[k][i] * r * wb[i];
-                }
-            if (p.r.R > 0) t.template apply<IN, false>(l, a[k], b[k]);
+            f.template apply<T>(l, a[k], b[k], r);
         }
         store_row<T, EPC, IN>(y + h * hs, a[k], b[k], h < m.H, l);
     }

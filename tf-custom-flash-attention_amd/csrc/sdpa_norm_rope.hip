@@ -49,29 +49,28 @@ __host__ __device__ inline SideMap side_map(long long tokens, int H) {
 // Token and first head of this lane's group in unit u; further rows of the
 // group are gpt heads apart.
 struct Place {
-    long long tok;
     int b, s, h;
+    int rows;  // per group, those that some group has (wave-uniform)
     bool live;
     __device__ __forceinline__ Place(const SideMap& m, long long u, int group, long long tokens, int S, int ku) {
         const unsigned uu = (unsigned)u, tg = uu / (unsigned)m.splits;
-        tok = (long long)tg * m.tpw + group / m.gpt;
-        h = (int)(uu - tg * (unsigned)m.splits) * m.gpt * ku + group % m.gpt;
+        long long tok = (long long)tg * m.tpw + group / m.gpt;
+        const int h0 = (int)(uu - tg * (unsigned)m.splits) * m.gpt * ku;
+        h = h0 + group % m.gpt;
+        rows = min(ku, (m.H - h0 + m.gpt - 1) / m.gpt);
         live = tok < tokens;
+        if (!live) tok = tokens - 1;  // (a row that exists is read in its place)
         b = (int)((unsigned)tok / (unsigned)S);
         s = (int)((unsigned)tok - (unsigned)b * (unsigned)S);
     }
 };
 
-__device__ __forceinline__ long long row_at(const RowStrides& st, const Place& at, int h) {
-    return at.b * st.b + at.s * st.s + h * st.h;
-}
-
 __device__ __forceinline__ long long position_of(const NormRopeParams& p, const Place& at) {
-    if (!p.positions || !at.live) return at.s;
+    if (!p.positions) return at.s;
     return p.positions[at.b * p.positions_stride + at.s];
 }
 
-template <typename T, int EPC, int LPR, bool IN, int KU>
+template <typename T, int EPC, int LPR, bool IN, int KU, bool NT>
 __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_kernel(const NormRopeParams p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -82,40 +81,36 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_kernel(const NormRo
     const SideMap m = which ? mk : mq;
     if (which) u -= mq.units;
     if (u >= m.units) return;
-    const NormRopeSide& sd = p.side[which];
+    const NormRopeSide sd = which ? p.side[1] : p.side[0];
 
     RowLane<EPC, IN> l;
     l.init(lane % LPR, p.D, p.r.R, p.interleaved != 0);
     const Place at(m, u, lane / LPR, tokens, p.S, KU);
-    float a[KU][EPC], b[KU][EPC];
-    const T* x = static_cast<const T*>(sd.x);
+    chunk_t<T, EPC> a[KU], b[KU];
+    const T* x = static_cast<const T*>(sd.x) + at.b * sd.xs.b + at.s * sd.xs.s;
 #pragma unroll
-    for (int k = 0; k < KU; ++k) {
-        const int h = at.h + k * m.gpt;
-        load_row<T, EPC, IN>(a[k], b[k], x + row_at(sd.xs, at, h), at.live && h < m.H, l);
-    }
+    for (int k = 0; k < KU; ++k)
+        if (k < at.rows) load_row<T, EPC, IN, NT>(a[k], b[k], x + min(at.h + k * m.gpt, m.H - 1) * sd.xs.h, l);
     RowTurn<EPC> t;
     t.load(p.r, l, position_of(p, at));
     float wa[EPC], wb[EPC];
     load_weight<T, EPC, IN>(wa, wb, sd.w, p.w32 != 0, l);
-    T* y = static_cast<T*>(sd.y);
+    RowFactors<EPC, IN> f;
+    f.init(l, t, wa, wb);
+    T* y = static_cast<T*>(sd.y) + at.b * sd.ys.b + at.s * sd.ys.s;
 #pragma unroll
     for (int k = 0; k < KU; ++k) {
+        if (k >= at.rows) break;
         const int h = at.h + k * m.gpt;
-        float r = p.r.norm ? row_rnorm<LPR, EPC>(a[k], b[k], p.D, p.r.eps) : 1.f;
+        float r = p.r.norm ? row_rnorm<T, LPR, EPC, IN>(a[k], b[k], l, p.r) : 1.f;
         if (t.bad) r = __builtin_nanf("");
-#pragma unroll
-        for (int i = 0; i < EPC; ++i) {
-            a[k][i] = a[k][i] * r * wa[i];
-            b[k][i] = b[k][i] * r * wb[i];
-        }
-        t.template apply<IN, false>(l, a[k], b[k]);
-        store_row<T, EPC, IN>(y + row_at(sd.ys, at, h), a[k], b[k], at.live && h < m.H, l);
+        f.template apply<T>(l, a[k], b[k], r);
+        store_row<T, EPC, IN>(y + h * sd.ys.h, a[k], b[k], at.live && h < m.H, l);
     }
 }
 
 // dx, and this workgroup's sum of dw (blocks of q before those of k).
-template <typename T, int EPC, int LPR, bool IN, int KU>
+template <typename T, int EPC, int LPR, bool IN, int KU, bool NT>
 __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const NormRopeParams p, const int blocks_q,
                                                                          const int blocks_k) {
     __shared__ float sums[kRopeWaves][2 * EPC * LPR];
@@ -124,7 +119,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const N
     const long long tokens = (long long)p.B * p.S;
     const int which = (int)blockIdx.x < blocks_q ? 0 : 1;
     const int block = which ? (int)blockIdx.x - blocks_q : (int)blockIdx.x, blocks = which ? blocks_k : blocks_q;
-    const NormRopeSide& sd = p.side[which];
+    const NormRopeSide sd = which ? p.side[1] : p.side[0];
     const SideMap m = side_map<LPR, KU>(tokens, sd.H);
 
     RowLane<EPC, IN> l;
@@ -133,53 +128,73 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const N
     load_weight<T, EPC, IN>(wa, wb, sd.w, p.w32 != 0, l);
 #pragma unroll
     for (int i = 0; i < EPC; ++i) da[i] = db[i] = 0.f;
-    const T* x = static_cast<const T*>(sd.x);
-    const T* dy = static_cast<const T*>(sd.dy);
-    T* dx = static_cast<T*>(sd.y);
     for (long long u = (long long)block * kRopeWaves + wave; u < m.units; u += (long long)blocks * kRopeWaves) {
         const Place at(m, u, lane / LPR, tokens, p.S, KU);
-        float a[KU][EPC], b[KU][EPC], ga[KU][EPC], gb[KU][EPC];
+        const T* x = static_cast<const T*>(sd.x) + at.b * sd.xs.b + at.s * sd.xs.s;
+        const T* dy = static_cast<const T*>(sd.dy) + at.b * sd.dys.b + at.s * sd.dys.s;
+        T* dx = static_cast<T*>(sd.y) + at.b * sd.ys.b + at.s * sd.ys.s;
+        chunk_t<T, EPC> a[KU], b[KU], ya[KU], yb[KU];
 #pragma unroll
         for (int k = 0; k < KU; ++k) {
-            const int h = at.h + k * m.gpt;
-            const bool live = at.live && h < m.H;
-            load_row<T, EPC, IN>(a[k], b[k], x + row_at(sd.xs, at, h), live, l);
-            load_row<T, EPC, IN>(ga[k], gb[k], dy + row_at(sd.dys, at, h), live, l);
+            if (k >= at.rows) break;
+            const int h = min(at.h + k * m.gpt, m.H - 1);
+            load_row<T, EPC, IN, NT>(a[k], b[k], x + h * sd.xs.h, l);
+            load_row<T, EPC, IN, NT>(ya[k], yb[k], dy + h * sd.dys.h, l);
         }
         RowTurn<EPC> t;
         t.load(p.r, l, position_of(p, at));
 #pragma unroll
         for (int k = 0; k < KU; ++k) {
+            if (k >= at.rows) break;
             const int h = at.h + k * m.gpt;
             const bool live = at.live && h < m.H;
-            t.template apply<IN, true>(l, ga[k], gb[k]);
-            if (t.bad)
+            float ga[EPC], gb[EPC];
 #pragma unroll
-                for (int i = 0; i < EPC; ++i) ga[k][i] = gb[k][i] = __builtin_nanf("");
+            for (int i = 0; i < EPC; ++i) {
+                ga[i] = sdpa::at<T, EPC>(ya[k], i);
+                gb[i] = sdpa::at<T, EPC>(yb[k], i);
+            }
+            t.back(l, ga, gb);
+            float r = 1.f;
             if (p.r.norm) {
-                const float r = row_rnorm<LPR, EPC>(a[k], b[k], p.D, p.r.eps);
-                float dot = 0.f;
+                r = row_rnorm<T, LPR, EPC, IN>(a[k], b[k], l, p.r);
+                float xa[EPC], xb[EPC], sa = 0.f, sb = 0.f;
 #pragma unroll
                 for (int i = 0; i < EPC; ++i) {
-                    a[k][i] *= r;
-                    b[k][i] *= r;
-                    if (live) {
-                        da[i] += ga[k][i] * a[k][i];
-                        db[i] += gb[k][i] * b[k][i];
-                    }
-                    ga[k][i] *= wa[i];
-                    gb[k][i] *= wb[i];
-                    dot += ga[k][i] * a[k][i] + gb[k][i] * b[k][i];
+                    xa[i] = sdpa::at<T, EPC>(a[k], i) * r;
+                    xb[i] = sdpa::at<T, EPC>(b[k], i) * r;
                 }
-                dot = group_sum<LPR>(dot) / (float)p.D;
+                if (live)
+#pragma unroll
+                    for (int i = 0; i < EPC; ++i) {
+                        da[i] = __builtin_fmaf(ga[i], xa[i], da[i]);
+                        db[i] = __builtin_fmaf(gb[i], xb[i], db[i]);
+                    }
 #pragma unroll
                 for (int i = 0; i < EPC; ++i) {
-                    ga[k][i] = r * (ga[k][i] - a[k][i] * dot);
-                    gb[k][i] = r * (gb[k][i] - b[k][i] * dot);
+                    ga[i] *= wa[i];
+                    gb[i] *= wb[i];
+                    sa = __builtin_fmaf(ga[i], xa[i], sa);
+                    sb = __builtin_fmaf(gb[i], xb[i], sb);
+                }
+                const float mean = group_sum<LPR>((l.va ? sa : 0.f) + (l.vb ? sb : 0.f)) * p.r.inv_D;
+#pragma unroll
+                for (int i = 0; i < EPC; ++i) {
+                    ga[i] = __builtin_fmaf(-xa[i], mean, ga[i]);
+                    gb[i] = __builtin_fmaf(-xb[i], mean, gb[i]);
                 }
             }
-            store_row<T, EPC, IN>(dx + row_at(sd.ys, at, h), ga[k], gb[k], live, l);
+            if (t.bad) r = __builtin_nanf("");
+#pragma unroll
+            for (int i = 0; i < EPC; ++i) {
+                ga[i] *= r;
+                gb[i] *= r;
+            }
+            store_row<T, EPC, IN>(dx + h * sd.ys.h, chunk_of<T, EPC>(ga), chunk_of<T, EPC>(gb), live, l);
         }
+        if (t.bad && at.live && at.h < m.H)
+#pragma unroll
+            for (int i = 0; i < EPC; ++i) da[i] = db[i] = __builtin_nanf("");
     }
     if (!p.part_dw || !sd.dw) return;
     // over the groups of the wave, then over the waves
@@ -213,21 +228,31 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const N
     }
 }
 
-// dw[d] = sum over the workgroups of one side: one wave per feature.
+// dw[d] = sum over the workgroups of one side: 16 features a workgroup, whose 1024
+// threads take every 64th partial sum each, then the 64 sums of a feature in order
+// of halves.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_rope_dw_kernel(const NormRopeParams p, const int blocks_q,
-                                                           const int blocks_k) {
-    const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int which = c < p.D ? 0 : 1, d = which ? c - p.D : c;
-    if (d >= p.D || !p.side[which].dw) return;
+__global__ __launch_bounds__(1024) void norm_rope_dw_kernel(const NormRopeParams p, const int blocks_q,
+                                                            const int blocks_k) {
+    __shared__ float sums[64][17];
+    const int which = (int)blockIdx.y, c = threadIdx.x & 15, g = threadIdx.x >> 4, d = (int)blockIdx.x * 16 + c;
+    void* const dw = which ? p.side[1].dw : p.side[0].dw;
+    if (!dw) return;
     const int n = which ? blocks_k : blocks_q;
     const float* src = p.part_dw + (size_t)(which ? blocks_q : 0) * p.D + d;
     float s = 0.f;
-    for (int i = lane; i < n; i += 64) s += src[(size_t)i * p.D];
-    s = group_sum<64>(s);
-    if (lane != 0) return;
-    if (p.w32) static_cast<float*>(p.side[which].dw)[d] = s;
-    else static_cast<T*>(p.side[which].dw)[d] = (T)s;
+    if (d < p.D)
+#pragma unroll 16
+        for (int i = g; i < n; i += 64) s += src[(size_t)i * p.D];
+    sums[g][c] = s;
+    __syncthreads();
+    for (int h = 32; h > 0; h /= 2) {
+        if (g < h) sums[g][c] += sums[g + h][c];
+        __syncthreads();
+    }
+    if (g != 0 || d >= p.D) return;
+    if (p.w32) static_cast<float*>(dw)[d] = sums[0][c];
+    else static_cast<T*>(dw)[d] = (T)sums[0][c];
 }
 
 // f<EPC, LPR, IN>() for the chunks these rows allow.
@@ -260,6 +285,14 @@ int grad_blocks(long long units) {
     return (int)(n < kGradBlocks ? n : kGradBlocks);
 }
 
+// Rows are read past the caches where q and k together outgrow what the 256 MB
+// cache can hold of them beside the results.  268 MB, fp16: plain 126 us, so 114
+// (gradient 232 and 219); 49 MB, fp32, called again and again: plain 21, so 25.
+template <typename T>
+bool past_caches(const NormRopeParams& p) {
+    return (long long)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * (long long)sizeof(T) > (128LL << 20);
+}
+
 template <typename T>
 hipError_t launch_norm_rope_t(const NormRopeParams& p, hipStream_t stream) {
     return with_row<T>(p, [&](auto epc, auto lpr, auto in) {
@@ -270,8 +303,12 @@ hipError_t launch_norm_rope_t(const NormRopeParams& p, hipStream_t stream) {
             constexpr int KU = decltype(ku)::value;
             const long long n = side_map<L, KU>(tokens, p.side[0].H).units + side_map<L, KU>(tokens, p.side[1].H).units;
             if (n == 0) return hipSuccess;
-            return launch_kernel<norm_rope_kernel<T, E, L, IN, KU>>(
-                tile_grid((n + kRopeWaves - 1) / kRopeWaves, 64 * kRopeWaves), 64 * kRopeWaves, 0, stream, p);
+            const dim3 grid = tile_grid((n + kRopeWaves - 1) / kRopeWaves, 64 * kRopeWaves);
+            if constexpr (KU == 4) {
+                if (past_caches<T>(p))
+                    return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, true>>(grid, 64 * kRopeWaves, 0, stream, p);
+            }
+            return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, false>>(grid, 64 * kRopeWaves, 0, stream, p);
         };
         const long long n4 = side_map<L, 4>(tokens, p.side[0].H).units + side_map<L, 4>(tokens, p.side[1].H).units;
         if (n4 >= kRopeFewWaves) return run(std::integral_constant<int, 4>{});
@@ -288,11 +325,14 @@ hipError_t launch_norm_rope_grad_t(const NormRopeParams& p, hipStream_t stream) 
         const int bq = grad_blocks(side_map<L, KU>(tokens, p.side[0].H).units);
         const int bk = grad_blocks(side_map<L, KU>(tokens, p.side[1].H).units);
         hipError_t e = hipSuccess;
+        const dim3 grid((unsigned)(bq + bk));
         if (bq + bk > 0)
-            e = launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU>>(dim3((unsigned)(bq + bk)), 64 * kRopeWaves, 0,
-                                                                      stream, p, bq, bk);
+            e = past_caches<T>(p) ? launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, true>>(grid, 64 * kRopeWaves, 0,
+                                                                                                 stream, p, bq, bk)
+                                  : launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, false>>(grid, 64 * kRopeWaves, 0,
+                                                                                                  stream, p, bq, bk);
         if (e != hipSuccess || (!p.side[0].dw && !p.side[1].dw)) return e;
-        return launch_kernel<norm_rope_dw_kernel<T>>(dim3((unsigned)((2 * p.D + 3) / 4)), 256, 0, stream, p, bq, bk);
+        return launch_kernel<norm_rope_dw_kernel<T>>(dim3((unsigned)((p.D + 15) / 16), 2), 1024, 0, stream, p, bq, bk);
     });
 }
 

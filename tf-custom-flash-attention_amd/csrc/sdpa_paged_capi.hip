@@ -68,6 +68,8 @@ int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64
     ch.rotated(R, interleaved);
     ch.address(cos);
     ch.address(sin);
+    ch.address(w[0]);
+    ch.address(w[1]);
     for (int i = 0; i < 2; ++i) {
         sdpa::NormRopeSide& s = p.side[i];
         s.H = i == 0 ? H_q : H_kv;
@@ -93,7 +95,7 @@ int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64
             return SDPA_ERR_WORKSPACE;
         p.part_dw = static_cast<float*>(workspace);
     }
-    p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps};
+    p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps, 1.f / (float)D};
     p.positions = positions;
     p.positions_stride = positions_per_batch ? S : 0;
     p.B = B;
@@ -198,7 +200,7 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     p.qos = token_strides(q_out_strides, T, H_q, D_qk);
     p.ks = token_strides(k_strides, T, H_kv, D_qk);
     p.vs = token_strides(v_strides, T, H_kv, D_v);
-    p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps};
+    p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps, D_qk > 0 ? 1.f / (float)D_qk : 0.f};
     p.H_q = has_q ? H_q : 0;
     p.H_kv = H_kv;
     p.D_qk = D_qk;
@@ -213,6 +215,8 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     ch.address(sin);
     ch.address(k_cache);
     ch.address(v_cache);
+    ch.address(q_weight);
+    ch.address(k_weight);
     if (has_q) {
         add_tokens(ch, q, p.qs);
         add_tokens(ch, q_out, p.qos);

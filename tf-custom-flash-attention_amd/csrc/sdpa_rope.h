@@ -12,6 +12,8 @@
 // All arithmetic is fp32; a result is rounded once, when it is stored.
 #pragma once
 
+#include <type_traits>
+
 #include "sdpa_device.h"
 
 namespace sdpa {
@@ -28,7 +30,7 @@ struct RopeArgs {
     int rows;  // of the tables: a position outside them makes the row NaN
     int R;     // rotated features (even; 0: none)
     int norm;  // x / sqrt(mean x^2 + eps), then the weight where there is one
-    float eps;
+    float eps, inv_D;
 };
 
 namespace {
@@ -70,23 +72,30 @@ struct Chunk<T, 1> {
     typedef T vec;
 };
 
-// EPC values of type T as fp32, and back.
 template <typename T, int EPC>
-__device__ __forceinline__ void load_chunk(float (&x)[EPC], const T* p) {
-    const auto v = *reinterpret_cast<const typename Chunk<T, EPC>::vec*>(p);
-    if constexpr (EPC == 1) x[0] = (float)v;
-    else
-#pragma unroll
-        for (int i = 0; i < EPC; ++i) x[i] = (float)v[i];
+using chunk_t = typename Chunk<T, EPC>::vec;
+
+// Value i of a chunk as fp32 (an operand that the fused multiply-adds read as it is).
+template <typename T, int EPC>
+__device__ __forceinline__ float at(const chunk_t<T, EPC>& v, int i) {
+    if constexpr (EPC == 1) return (float)v;
+    else return (float)v[i];
 }
 template <typename T, int EPC>
-__device__ __forceinline__ void store_chunk(T* p, const float (&x)[EPC]) {
-    typename Chunk<T, EPC>::vec v;
+__device__ __forceinline__ chunk_t<T, EPC> chunk_of(const float (&x)[EPC]) {
+    chunk_t<T, EPC> v;
     if constexpr (EPC == 1) v = (T)x[0];
     else
 #pragma unroll
         for (int i = 0; i < EPC; ++i) v[i] = (T)x[i];
-    *reinterpret_cast<typename Chunk<T, EPC>::vec*>(p) = v;
+    return v;
+}
+// EPC values of a table.
+template <int EPC>
+__device__ __forceinline__ void load_table(float (&x)[EPC], const float* p) {
+    const chunk_t<float, EPC> v = *reinterpret_cast<const chunk_t<float, EPC>*>(p);
+#pragma unroll
+    for (int i = 0; i < EPC; ++i) x[i] = at<float, EPC>(v, i);
 }
 
 // What lane j of a row's lanes holds: features fa .. + EPC and fb .. + EPC.
@@ -137,52 +146,116 @@ struct RowTurn {
         }
         if constexpr (!IN) {
             if (l.ra && p.rows > 0) {
-                load_chunk<float, EPC>(c, p.cos + row + l.t);
-                load_chunk<float, EPC>(s, p.sin + row + l.t);
+                load_table<EPC>(c, p.cos + row + l.t);
+                load_table<EPC>(s, p.sin + row + l.t);
             }
         } else {
             constexpr int HP = EPC / 2;
             float h[HP];
             if (l.ra && p.rows > 0) {
-                load_chunk<float, HP>(h, p.cos + row + l.t);
+                load_table<HP>(h, p.cos + row + l.t);
 #pragma unroll
                 for (int i = 0; i < HP; ++i) c[i] = h[i];
-                load_chunk<float, HP>(h, p.sin + row + l.t);
+                load_table<HP>(h, p.sin + row + l.t);
 #pragma unroll
                 for (int i = 0; i < HP; ++i) s[i] = h[i];
             }
             if (l.rb && p.rows > 0) {
-                load_chunk<float, HP>(h, p.cos + row + l.t + HP);
+                load_table<HP>(h, p.cos + row + l.t + HP);
 #pragma unroll
                 for (int i = 0; i < HP; ++i) c[HP + i] = h[i];
-                load_chunk<float, HP>(h, p.sin + row + l.t + HP);
+                load_table<HP>(h, p.sin + row + l.t + HP);
 #pragma unroll
                 for (int i = 0; i < HP; ++i) s[HP + i] = h[i];
             }
         }
     }
-    // (x, y) turned by the angle, INV: back
-    template <bool INV>
-    __device__ __forceinline__ void turn(float& x, float& y, int i) const {
-        const float sn = INV ? -s[i] : s[i];
-        const float u = x * c[i] - y * sn, v = y * c[i] + x * sn;
-        x = u;
-        y = v;
-    }
-    template <bool IN, bool INV>
-    __device__ __forceinline__ void apply(const RowLane<EPC, IN>& l, float (&a)[EPC], float (&b)[EPC]) const {
+    // The pairs of (a, b) turned back by the angle.
+    template <bool IN>
+    __device__ __forceinline__ void back(const RowLane<EPC, IN>& l, float (&a)[EPC], float (&b)[EPC]) const {
+        const auto turn = [&](float& x, float& y, int i) {
+            const float u = __builtin_fmaf(y, s[i], x * c[i]), v = __builtin_fmaf(-x, s[i], y * c[i]);
+            x = u;
+            y = v;
+        };
         if constexpr (!IN) {
             if (l.ra)
 #pragma unroll
-                for (int i = 0; i < EPC; ++i) turn<INV>(a[i], b[i], i);
+                for (int i = 0; i < EPC; ++i) turn(a[i], b[i], i);
         } else {
             if (l.ra)
 #pragma unroll
-                for (int i = 0; i < EPC / 2; ++i) turn<INV>(a[2 * i], a[2 * i + 1], i);
+                for (int i = 0; i < EPC / 2; ++i) turn(a[2 * i], a[2 * i + 1], i);
             if (l.rb)
 #pragma unroll
-                for (int i = 0; i < EPC / 2; ++i) turn<INV>(b[2 * i], b[2 * i + 1], EPC / 2 + i);
+                for (int i = 0; i < EPC / 2; ++i) turn(b[2 * i], b[2 * i + 1], EPC / 2 + i);
         }
+    }
+};
+
+// The rotation of a weighted row: for each pair (x, y) of weights (v, w)
+//   x v c - y w s,  y w c + x v s,
+// its four factors formed once for the rows of a token.
+template <int EPC, bool IN>
+struct RowFactors {
+    float xx[EPC], xy[EPC], yx[EPC], yy[EPC];  // pairs of (a, b); IN: of a, then of b
+    __device__ __forceinline__ void pair(int i, float v, float w, const RowTurn<EPC>& t, bool turned) {
+        xx[i] = turned ? v * t.c[i] : v;
+        xy[i] = w * t.s[i];
+        yx[i] = v * t.s[i];
+        yy[i] = turned ? w * t.c[i] : w;
+    }
+    __device__ __forceinline__ void init(const RowLane<EPC, IN>& l, const RowTurn<EPC>& t, const float (&wa)[EPC],
+                                         const float (&wb)[EPC]) {
+        if constexpr (!IN) {
+#pragma unroll
+            for (int i = 0; i < EPC; ++i) pair(i, wa[i], wb[i], t, l.ra);
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPC / 2; ++i) {
+                pair(i, wa[2 * i], wa[2 * i + 1], t, l.ra);
+                pair(EPC / 2 + i, wb[2 * i], wb[2 * i + 1], t, l.rb);
+            }
+        }
+    }
+    // (a plain feature stays clear of its neighbour's infinities.  The products are
+    // fused multiply-adds, which take halves as they are.)
+    template <bool TURNED>
+    __device__ __forceinline__ void one(int i, float x, float y, float r, float& u, float& v) const {
+        if constexpr (TURNED) {
+            u = __builtin_fmaf(x, xx[i], __builtin_fmaf(-y, xy[i], 0.f)) * r;
+            v = __builtin_fmaf(y, yy[i], __builtin_fmaf(x, yx[i], 0.f)) * r;
+        } else {
+            u = __builtin_fmaf(x, xx[i], 0.f) * r;
+            v = __builtin_fmaf(y, yy[i], 0.f) * r;
+        }
+    }
+    // a and b: the row as it lies, the result in place, times r
+    template <typename T>
+    __device__ __forceinline__ void apply(const RowLane<EPC, IN>& l, chunk_t<T, EPC>& a, chunk_t<T, EPC>& b, float r) const {
+        float u[EPC], v[EPC];
+        if constexpr (!IN) {
+            const auto all = [&](auto turned) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < EPC; ++i)
+                    one<decltype(turned)::value>(i, at<T, EPC>(a, i), at<T, EPC>(b, i), r, u[i], v[i]);
+            };
+            if (l.ra) all(std::true_type{});
+            else all(std::false_type{});
+        } else {
+            const auto all = [&](auto turned, const chunk_t<T, EPC>& x, float (&w)[EPC], int i0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < EPC / 2; ++i)
+                    one<decltype(turned)::value>(i0 + i, at<T, EPC>(x, 2 * i), at<T, EPC>(x, 2 * i + 1), r, w[2 * i],
+                                                 w[2 * i + 1]);
+            };
+            if (l.ra) all(std::true_type{}, a, u, 0);
+            else all(std::false_type{}, a, u, 0);
+            if (l.rb) all(std::true_type{}, b, v, EPC / 2);
+            else all(std::false_type{}, b, v, EPC / 2);
+        }
+        a = chunk_of<T, EPC>(u);
+        b = chunk_of<T, EPC>(v);
     }
 };
 
@@ -190,43 +263,58 @@ struct RowTurn {
 template <typename T, int EPC, bool IN>
 __device__ __forceinline__ void load_weight(float (&wa)[EPC], float (&wb)[EPC], const void* w, bool w32,
                                             const RowLane<EPC, IN>& l) {
+    typedef chunk_t<float, EPC> F;
+    F a, b;
+    if (w && w32) {
+        a = *reinterpret_cast<const F*>(static_cast<const float*>(w) + l.fa);
+        b = *reinterpret_cast<const F*>(static_cast<const float*>(w) + l.fb);
+    } else if (w) {
+        const chunk_t<T, EPC> ta = *reinterpret_cast<const chunk_t<T, EPC>*>(static_cast<const T*>(w) + l.fa);
+        const chunk_t<T, EPC> tb = *reinterpret_cast<const chunk_t<T, EPC>*>(static_cast<const T*>(w) + l.fb);
+        if constexpr (EPC == 1) {
+            a = (float)ta;
+            b = (float)tb;
+        } else {
+            a = __builtin_convertvector(ta, F);
+            b = __builtin_convertvector(tb, F);
+        }
+    } else {
+        a = b = F(1.f);
+    }
 #pragma unroll
     for (int i = 0; i < EPC; ++i) {
-        wa[i] = wb[i] = 1.f;
-        if (!w) continue;
-        if (w32) {
-            wa[i] = static_cast<const float*>(w)[l.fa + i];
-            wb[i] = static_cast<const float*>(w)[l.fb + i];
-        } else {
-            wa[i] = (float)static_cast<const T*>(w)[l.fa + i];
-            wb[i] = (float)static_cast<const T*>(w)[l.fb + i];
-        }
+        wa[i] = at<float, EPC>(a, i);
+        wb[i] = at<float, EPC>(b, i);
     }
 }
 
-// A lane's part of a row (0 outside of it).
-template <typename T, int EPC, bool IN>
-__device__ __forceinline__ void load_row(float (&a)[EPC], float (&b)[EPC], const T* row, bool live,
-                                         const RowLane<EPC, IN>& l) {
-#pragma unroll
-    for (int i = 0; i < EPC; ++i) a[i] = b[i] = 0.f;
-    if (live && l.va) load_chunk<T, EPC>(a, row + l.fa);
-    if (live && l.vb) load_chunk<T, EPC>(b, row + l.fb);
+// A lane's part of a row (outside of the row, its first chunk).  NT: past the caches.
+template <typename T, int EPC, bool IN, bool NT = false>
+__device__ __forceinline__ void load_row(chunk_t<T, EPC>& a, chunk_t<T, EPC>& b, const T* row, const RowLane<EPC, IN>& l) {
+    typedef chunk_t<T, EPC> V;
+    const V *pa = reinterpret_cast<const V*>(row + l.fa), *pb = reinterpret_cast<const V*>(row + l.fb);
+    a = NT ? __builtin_nontemporal_load(pa) : *pa;
+    b = NT ? __builtin_nontemporal_load(pb) : *pb;
 }
 template <typename T, int EPC, bool IN>
-__device__ __forceinline__ void store_row(T* row, const float (&a)[EPC], const float (&b)[EPC], bool live,
+__device__ __forceinline__ void store_row(T* row, const chunk_t<T, EPC>& a, const chunk_t<T, EPC>& b, bool live,
                                           const RowLane<EPC, IN>& l) {
-    if (live && l.va) store_chunk<T, EPC>(row + l.fa, a);
-    if (live && l.vb) store_chunk<T, EPC>(row + l.fb, b);
+    typedef chunk_t<T, EPC> V;
+    if (live && l.va) *reinterpret_cast<V*>(row + l.fa) = a;
+    if (live && l.vb) *reinterpret_cast<V*>(row + l.fb) = b;
 }
 
 // 1 / sqrt(mean x^2 + eps) of a row held by LPR lanes.
-template <int LPR, int EPC>
-__device__ __forceinline__ float row_rnorm(const float (&a)[EPC], const float (&b)[EPC], int D, float eps) {
-    float q = 0.f;
+template <typename T, int LPR, int EPC, bool IN>
+__device__ __forceinline__ float row_rnorm(const chunk_t<T, EPC>& a, const chunk_t<T, EPC>& b, const RowLane<EPC, IN>& l,
+                                           const RopeArgs& p) {
+    float qa = 0.f, qb = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPC; ++i) q += a[i] * a[i] + b[i] * b[i];
-    return rsqrtf(group_sum<LPR>(q) / (float)D + eps);
+    for (int i = 0; i < EPC; ++i) {
+        qa = __builtin_fmaf(at<T, EPC>(a, i), at<T, EPC>(a, i), qa);
+        qb = __builtin_fmaf(at<T, EPC>(b, i), at<T, EPC>(b, i), qb);
+    }
+    return rsqrtf(__builtin_fmaf(group_sum<LPR>((l.va ? qa : 0.f) + (l.vb ? qb : 0.f)), p.inv_D, p.eps));
 }
 
 }  // namespace
