@@ -358,5 +358,14 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
     return _fn.apply(q, k, v, seed, offset, dropout, scale, causal_mask)
 
 
-from .heads import (kv_append, paged_sdpa, qk_norm_rope, qk_norm_rope_autograd,  # noqa: E402
-                    qk_norm_rope_grad)
+_HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_append", "paged_sdpa")
+
+
+def __getattr__(name):
+    """The entry points of :mod:`.heads`, loaded when one is first asked for (that
+    module needs torch, which importing this package does not)."""
+    if name not in _HEADS:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import heads
+    globals().update({n: getattr(heads, n) for n in _HEADS})
+    return globals()[name]

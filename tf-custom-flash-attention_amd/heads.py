@@ -9,12 +9,32 @@ checked there, where they are used.
 from __future__ import annotations
 
 import ctypes
+import functools
+
+import torch
 
 from . import (DTYPE_F16, DTYPE_F32, InvalidArgumentError, _dtype_code, _raise_for, _stream_handle, _workspace,
                library)
 
 _Strides3 = ctypes.c_int64 * 3
 _Strides2 = ctypes.c_int64 * 2
+
+
+_F32, _I32 = torch.float32, torch.int32
+_CODES = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
+
+
+# (a ctypes array costs a third of a microsecond, and programs have few layouts)
+@functools.lru_cache(maxsize=512)
+def _strides3(strides):
+    """The first three strides of a [batch, tokens, heads, features] tensor for the C entries."""
+    return _Strides3(*strides[:3])
+
+
+@functools.lru_cache(maxsize=512)
+def _strides2(strides):
+    """The first two strides of a [tokens, heads, features] tensor for the C entries."""
+    return _Strides2(*strides[:2])
 
 
 def _fail(message):
@@ -32,12 +52,13 @@ def _on_device(device, **tensors):
 
 def _call(entry, device, *args):
     """``entry(*args, stream)`` with ``device`` current."""
-    import torch
     if torch.cuda.current_device() == device.index:
-        _raise_for(entry(*args, _stream_handle(device)))
+        code = entry(*args, _stream_handle(device))
     else:
         with torch.cuda.device(device):
-            _raise_for(entry(*args, _stream_handle(device)))
+            code = entry(*args, _stream_handle(device))
+    if code:
+        _raise_for(code)
 
 
 def _dense_features(t):
@@ -45,12 +66,15 @@ def _dense_features(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
 def _int32(name, t, *shape):
-    import torch
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
         _fail(f"{name} must be an int32 tensor")
     if tuple(t.shape) != shape:
@@ -59,7 +83,6 @@ def _int32(name, t, *shape):
 
 def _tables(cos, sin):
     """Rows and rotated features of the rotation tables (0, 0 without)."""
-    import torch
     if cos is None and sin is None:
         return 0, 0
     if cos is None or sin is None:
@@ -74,7 +97,6 @@ def _tables(cos, sin):
 
 
 def _weight_dtype(T, D, q_weight, k_weight, norm):
-    import torch
     code = None
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is None:
@@ -101,8 +123,47 @@ def _check_qk(q, k):
         _fail(f"q {list(q.shape)} and k {list(k.shape)} differ in batch, tokens or features")
 
 
+def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
+    """What ``_rope_args`` returns, of arguments that pass its checks by a few
+    comparisons and need no copies; None of others, which go through them (the
+    checks one by one took half of a small call's host time)."""
+    sq, sk = q.shape, k.shape
+    if cos is None or sin is None or len(sq) != 4 or len(sk) != 4:
+        return None
+    T, device, sc = q.dtype, q.device, cos.shape
+    B, S, H_q, D = sq
+    code = _CODES.get(T)
+    w = q_weight
+    if not (code is not None and k.dtype is T and device.type == "cuda" and k.device == device and cos.device == device
+            and sin.device == device and sk[0] == B and sk[1] == S and sk[3] == D and len(sc) == 2 and sin.shape == sc
+            and cos.dtype is _F32 and sin.dtype is _F32 and sc[0] <= 0x7FFFFFFF and cos.is_contiguous()
+            and sin.is_contiguous()):
+        return None
+    per_batch = 0
+    if positions is None:
+        if S > sc[0]:
+            return None
+    else:
+        sp = positions.shape
+        per_batch = int(len(sp) == 2)
+        if (sp != ((B, S) if per_batch else (S,)) or positions.dtype is not _I32 or positions.device != device
+                or not positions.is_contiguous()):
+            return None
+    w_code = DTYPE_F32
+    if w is not None or k_weight is not None:
+        if (not norm or w is None or k_weight is None or w.dtype is not k_weight.dtype or w.dtype not in (T, _F32)
+                or w.shape != (D,) or k_weight.shape != (D,) or w.device != device or k_weight.device != device
+                or not w.is_contiguous() or not k_weight.is_contiguous()):
+            return None
+        w_code = _CODES[w.dtype]
+    return code, (B, S, H_q, sk[2], D, 2 * sc[1]), (cos, sin, sc[0]), (w, k_weight, w_code), positions, per_batch
+
+
 def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm):
     """Checks of what the forward and the gradient have in common."""
+    plain = _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm)
+    if plain is not None:
+        return plain
     _check_qk(q, k)
     code = _dtype_code(q)
     B, S, H_q, D = q.shape
@@ -116,19 +177,15 @@ def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm):
     elif R and S > rows:
         _fail(f"the rotation tables have {rows} positions, the sequence {S} tokens")
     _on_device(q.device, k=k, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight, positions=positions)
-    cos, sin, q_weight, k_weight = (None if t is None else t.contiguous() for t in (cos, sin, q_weight, k_weight))
+    cos, sin, q_weight, k_weight = _dense(cos), _dense(sin), _dense(q_weight), _dense(k_weight)
     return code, (B, S, H_q, k.shape[2], D, R), (cos, sin, rows), (q_weight, k_weight, w_code), positions, per_batch
 
 
-def _out_rows(torch, like, B, S, H, D, fold_heads):
+def _out_rows(like, B, S, H, D, fold_heads):
     """A result [B H, S, D] (folded) or [B, S, H, D], and its strides {batch, token, head}."""
     if fold_heads:
-        return torch.empty((B * H, S, D), dtype=like.dtype, device=like.device), _Strides3(H * S * D, D, S * D)
-    return torch.empty((B, S, H, D), dtype=like.dtype, device=like.device), _Strides3(S * H * D, H * D, D)
-
-
-def _strides3(t):
-    return _Strides3(t.stride(0), t.stride(1), t.stride(2))
+        return torch.empty((B * H, S, D), dtype=like.dtype, device=like.device), _strides3((H * S * D, D, S * D))
+    return torch.empty((B, S, H, D), dtype=like.dtype, device=like.device), None
 
 
 def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
@@ -144,13 +201,12 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, e
 
     ``fold_heads``: results [B * H, S, D], the layout of ``sdpa``; else [B, S, H, D].
     """
-    import torch
     code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
         q, k, cos, sin, q_weight, k_weight, positions, norm)
     q, k = _dense_features(q), _dense_features(k)
-    q_out, qos = _out_rows(torch, q, B, S, H_q, D, fold_heads)
-    k_out, kos = _out_rows(torch, k, B, S, H_kv, D, fold_heads)
-    _call(library().sdpa_hip_qk_norm_rope, q.device, code, q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k),
+    q_out, qos = _out_rows(q, B, S, H_q, D, fold_heads)
+    k_out, kos = _out_rows(k, B, S, H_kv, D, fold_heads)
+    _call(library().sdpa_hip_qk_norm_rope, q.device, code, q.data_ptr(), _strides3(q.stride()), k.data_ptr(), _strides3(k.stride()),
           q_out.data_ptr(), qos, k_out.data_ptr(), kos, _ptr(weights[0]), _ptr(weights[1]), weights[2],
           _ptr(tables[0]), _ptr(tables[1]), tables[2], _ptr(positions), per_batch, B, S, H_q, H_kv, D, R, float(eps),
           int(bool(norm)), int(bool(interleaved)))
@@ -165,7 +221,6 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
     dense [B, S, H, D], the weights' gradients in their dtype, None for a
     weight that was not given.
     """
-    import torch
     code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
         q, k, cos, sin, q_weight, k_weight, positions, norm)
     L = library()
@@ -177,7 +232,7 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
             _fail(f"{name} must be {q.dtype} of shape {list(shape)}, got {d.dtype} {list(d.shape)}")
         d = _dense_features(d)
         # (batch and head of a folded row are H rows and one row apart)
-        grads.append((d, _Strides3(H * d.stride(0), d.stride(1), d.stride(0)) if fold_heads else _strides3(d)))
+        grads.append((d, _strides3((H * d.stride(0), d.stride(1), d.stride(0)) if fold_heads else d.stride())))
     q, k = _dense_features(q), _dense_features(k)
     dq = torch.empty((B, S, H_q, D), dtype=q.dtype, device=q.device)
     dk = torch.empty((B, S, H_kv, D), dtype=q.dtype, device=q.device)
@@ -187,7 +242,7 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
         ws_bytes = L.sdpa_hip_qk_norm_rope_grad_workspace_bytes(D)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
     _call(L.sdpa_hip_qk_norm_rope_grad, q.device, code, grads[0][0].data_ptr(), grads[0][1], grads[1][0].data_ptr(),
-          grads[1][1], q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k), dq.data_ptr(), None, dk.data_ptr(),
+          grads[1][1], q.data_ptr(), _strides3(q.stride()), k.data_ptr(), _strides3(k.stride()), dq.data_ptr(), None, dk.data_ptr(),
           None, _ptr(dw[0]), _ptr(dw[1]), _ptr(weights[0]), _ptr(weights[1]), weights[2], _ptr(tables[0]),
           _ptr(tables[1]), tables[2], _ptr(positions), per_batch, _ptr(ws), ws_bytes, B, S, H_q, H_kv, D, R,
           float(eps), int(bool(norm)), int(bool(interleaved)))
@@ -195,7 +250,6 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
 
 
 def _make_function():
-    import torch
 
     class QkNormRopeFunction(torch.autograd.Function):
         """``qk_norm_rope`` with its gradient for q, k and the weights."""
@@ -252,6 +306,21 @@ def _check_batch(page_table, q_starts, kv_lens):
     return N, width
 
 
+def _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens):
+    """(N, width) of arguments that pass ``_check_cache``, ``_check_batch`` and
+    ``_on_device`` by a few comparisons, None of others."""
+    st, sk, sv = page_table.shape, k_cache.shape, v_cache.shape
+    if (device.type == "cuda" and k_cache.dtype is T and v_cache.dtype is T and k_cache.device == device
+            and v_cache.device == device and len(sk) == 4 and len(sv) == 4 and sk[:3] == sv[:3]
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and len(st) == 2 and page_table.dtype is _I32
+            and q_starts.dtype is _I32 and kv_lens.dtype is _I32 and page_table.device == device
+            and q_starts.device == device and kv_lens.device == device and q_starts.shape == (st[0] + 1,)
+            and kv_lens.shape == (st[0],) and page_table.is_contiguous() and q_starts.is_contiguous()
+            and kv_lens.is_contiguous()):
+        return st
+    return None
+
+
 def _check_tokens(name, t, T, features=None):
     if t.dim() != 3 or (features is not None and t.shape[2] != features):
         _fail(f"{name} must be [tokens, heads{'' if features is None else f', {features}'}], got {list(t.shape)}")
@@ -259,8 +328,52 @@ def _check_tokens(name, t, T, features=None):
         _fail(f"{name} must have dtype {T}, got {t.dtype}")
 
 
-def _strides2(t):
-    return _Strides2(t.stride(0), t.stride(1))
+def _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm):
+    """Checks of ``kv_append``: (N, width) and (dtype code, table rows, rotated features, weights' code)."""
+    T = k.dtype
+    _check_tokens("k", k, T)
+    _check_tokens("v", v, T)
+    code = _dtype_code(k)
+    _check_cache(k_cache, v_cache, T)
+    batch = _check_batch(page_table, q_starts, kv_lens)
+    n, H_kv, D_qk = k.shape
+    if v.shape[:2] != k.shape[:2]:
+        _fail(f"k {list(k.shape)} and v {list(v.shape)} differ in tokens or heads")
+    if k_cache.shape[1] != H_kv or k_cache.shape[3] != D_qk or v_cache.shape[3] != v.shape[2]:
+        _fail(f"the caches {list(k_cache.shape)}, {list(v_cache.shape)} do not hold rows of k {list(k.shape)} and v "
+              f"{list(v.shape)}")
+    if q is not None:
+        _check_tokens("q", q, T, D_qk)
+        if q.shape[0] != n:
+            _fail(f"q has {q.shape[0]} tokens, k {n}")
+    rows, R = _tables(cos, sin)
+    w_code = _weight_dtype(T, D_qk, q_weight, k_weight, norm)
+    _on_device(k.device, v=v, cos=cos, sin=sin, q=q, q_weight=q_weight, k_weight=k_weight, k_cache=k_cache,
+               v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
+    return batch, (code, rows, R, w_code)
+
+
+def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, norm):
+    """What ``_check_append`` returns second, of usual arguments that pass its
+    checks by a few comparisons; None of others."""
+    sk, sv, T, device = k.shape, v.shape, k.dtype, k.device
+    code = _CODES.get(T)
+    if (code is None or q is None or cos is None or sin is None or len(sk) != 3 or len(sv) != 3 or v.dtype is not T
+            or q.dtype is not T or v.device != device or q.device != device or cos.device != device or sin.device != device):
+        return None
+    n, H_kv, D = sk
+    sq, sc = q.shape, cos.shape
+    if not (sv[0] == n and sv[1] == H_kv == sk_cache[1] and sk_cache[3] == D and sv_cache[3] == sv[2] and len(sq) == 3
+            and sq[0] == n and sq[2] == D and len(sc) == 2 and sin.shape == sc and cos.dtype is _F32 and sin.dtype is _F32
+            and sc[0] <= 0x7FFFFFFF):
+        return None
+    if q_weight is not None or k_weight is not None:
+        if (not norm or q_weight is None or k_weight is None or q_weight.dtype is not k_weight.dtype
+                or q_weight.dtype not in (T, _F32) or q_weight.shape != (D,) or k_weight.shape != (D,)
+                or q_weight.device != device or k_weight.device != device):
+            return None
+        return code, sc[0], 2 * sc[1], _CODES[q_weight.dtype]
+    return code, sc[0], 2 * sc[1], DTYPE_F32
 
 
 def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, sin=None, q=None, q_weight=None,
@@ -279,39 +392,28 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
     of a call may have the same place.
     """
-    import torch
-    T = k.dtype
-    _check_tokens("k", k, T)
-    _check_tokens("v", v, T)
-    code = _dtype_code(k)
-    _check_cache(k_cache, v_cache, T)
-    N, width = _check_batch(page_table, q_starts, kv_lens)
+    T, device = k.dtype, k.device
+    batch = _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
+    checked = None
+    if batch is not None:
+        checked = _plain_append(k, v, k_cache.shape, v_cache.shape, cos, sin, q, q_weight, k_weight, norm)
+    if checked is None:
+        batch, checked = _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight,
+                                       k_weight, norm)
+    N, width = batch
+    code, rows, R, w_code = checked
     n, H_kv, D_qk = k.shape
     D_v = v.shape[2]
     pages, _, page, _ = k_cache.shape
-    if v.shape[:2] != k.shape[:2]:
-        _fail(f"k {list(k.shape)} and v {list(v.shape)} differ in tokens or heads")
-    if k_cache.shape[1] != H_kv or k_cache.shape[3] != D_qk or v_cache.shape[3] != D_v:
-        _fail(f"the caches {list(k_cache.shape)}, {list(v_cache.shape)} do not hold rows of k {list(k.shape)} and v "
-              f"{list(v.shape)}")
-    H_q = 0
-    if q is not None:
-        _check_tokens("q", q, T, D_qk)
-        if q.shape[0] != n:
-            _fail(f"q has {q.shape[0]} tokens, k {n}")
-        H_q = q.shape[1]
-    rows, R = _tables(cos, sin)
-    w_code = _weight_dtype(T, D_qk, q_weight, k_weight, norm)
-    _on_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts,
-               kv_lens=kv_lens, cos=cos, sin=sin, q=q, q_weight=q_weight, k_weight=k_weight)
+    H_q = 0 if q is None else q.shape[1]
     k, v = _dense_features(k), _dense_features(v)
-    cos, sin, q_weight, k_weight = (None if t is None else t.contiguous() for t in (cos, sin, q_weight, k_weight))
+    cos, sin, q_weight, k_weight = _dense(cos), _dense(sin), _dense(q_weight), _dense(k_weight)
     q_out = None
     if q is not None:
         q = _dense_features(q)
-        q_out = torch.empty((n, H_q, D_qk), dtype=T, device=k.device)
-    _call(library().sdpa_hip_kv_append, k.device, code, k.data_ptr(), _strides2(k), v.data_ptr(), _strides2(v),
-          k_cache.data_ptr(), v_cache.data_ptr(), _ptr(q), None if q is None else _strides2(q), _ptr(q_out), None,
+        q_out = torch.empty((n, H_q, D_qk), dtype=T, device=device)
+    _call(library().sdpa_hip_kv_append, device, code, k.data_ptr(), _strides2(k.stride()), v.data_ptr(), _strides2(v.stride()),
+          k_cache.data_ptr(), v_cache.data_ptr(), _ptr(q), None if q is None else _strides2(q.stride()), _ptr(q_out), None,
           _ptr(q_weight), _ptr(k_weight), w_code, _ptr(cos), _ptr(sin), rows, page_table.data_ptr(),
           page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, R, float(eps), int(bool(norm)), int(bool(interleaved)))
@@ -340,18 +442,22 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
     kernels only.  ``out``: (o, stats) to write into; rows of tokens of no sequence stay as they were
     (in new ones they are arbitrary).  Feature sizes are multiples of 8 (fp16) or 4 (fp32), up to 128.
     """
-    import torch
     T = q.dtype
     _check_tokens("q", q, T)
     code = _dtype_code(q)
-    _check_cache(k_cache, v_cache, T)
-    N, width = _check_batch(page_table, q_starts, kv_lens)
+    plain = _plain_batch(q.device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
+    known = plain is not None
+    if not known:
+        _check_cache(k_cache, v_cache, T)
+        plain = _check_batch(page_table, q_starts, kv_lens)
+    N, width = plain
     n, H_q, D_qk = q.shape
     pages, H_kv, page, D_v = v_cache.shape
     if k_cache.shape[3] != D_qk:
         _fail(f"q has {D_qk} features, k_cache {k_cache.shape[3]}")
     if out is None:
-        _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
+        if not known:
+            _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
         o = torch.empty((n, H_q, D_v), dtype=T, device=q.device)
         stats = torch.empty((n, H_q), dtype=torch.float32, device=q.device)
     else:
@@ -367,7 +473,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
     ws_bytes = L.sdpa_hip_paged_fwd_workspace_bytes(code, N, n, width, page, H_q, H_kv, D_qk, D_v, longest)
     ws = _workspace(torch, ws_bytes, q.device) if ws_bytes else None
     q = _whole_chunks(q)
-    _call(L.sdpa_hip_paged_fwd, q.device, code, q.data_ptr(), _strides2(q), k_cache.data_ptr(), v_cache.data_ptr(),
+    _call(L.sdpa_hip_paged_fwd, q.device, code, q.data_ptr(), _strides2(q.stride()), k_cache.data_ptr(), v_cache.data_ptr(),
           o.data_ptr(), None, stats.data_ptr(), page_table.data_ptr(), page_table.stride(0), q_starts.data_ptr(),
           kv_lens.data_ptr(), _ptr(ws), ws_bytes if ws is not None else 0, N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, longest, float(scale), int(bool(causal_mask)))
