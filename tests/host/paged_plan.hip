@@ -62,7 +62,7 @@ int main() {
                 return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, BM, BN, chunk);
             };
             for (int s = 0; s < N; ++s) cost += (long long)plan(s, 0).tiles * plan(s, 0).blocks;
-            const long long chunk = plan_chunk(cost * H_kv, p.target);
+            const long long chunk = plan_chunk(cost * H_kv, p.target, kernel ? kPagedMinChunk16 : kPagedMinChunk32);
             for (int s = 0; s < N; ++s) {
                 const SeqPlan q = plan(s, chunk);
                 if (q.tiles == 0) continue;

@@ -10,7 +10,7 @@
 // sizes alone.  Two forms, both merged in order by a second kernel:
 //   parts   The cost of a tile is the number of key blocks it walks on
 //           average; the keys of a tile are divided into parts of at most `chunk`
-//           blocks, chunk being the larger of kPagedMinChunk and the whole cost over
+//           blocks, chunk being the larger of min_chunk and the whole cost over
 //           `target` workgroups.  So at most target workgroups more than there
 //           are tiles have work, whatever the lengths, and at most 2 target parts
 //           are of divided tiles.
@@ -39,10 +39,14 @@ struct PagedParams {
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
-    int target;  // workgroups to divide for (parts: 0 where nothing is divided)
+    int target;     // workgroups to divide for (parts: 0 where nothing is divided)
+    int min_chunk;  // parts: key blocks of a part, at least
 };
 
-constexpr int kPagedMinChunk = 2;   // key blocks of a part, at least
+// Key blocks of a part, at least.  fp16 (64 keys a block), 300 tokens over 2300, 16
+// heads on 4, D 64: 2 blocks 31.2 us, 4 29.3, 6 25.7, 8 25.8, 16 27.7; over 1150: 24.8,
+// 21.1, 21.9, 23.6, 29.6.  fp32 (128 keys): 2 to 8 alike, 12 and more a quarter slower.
+constexpr int kPagedMinChunk16 = 6, kPagedMinChunk32 = 2;
 constexpr int kPagedMaxParts = 64;  // (the merge walks a row's parts one batch after the other)
 
 // One sequence's part of the plan.
@@ -73,10 +77,10 @@ __host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const Pa
     return s;
 }
 
-__host__ __device__ inline long long plan_chunk(long long cost, int target) {
+__host__ __device__ inline long long plan_chunk(long long cost, int target, int min_chunk) {
     if (target <= 0) return 0;
     const long long c = (cost + target - 1) / target;
-    return c < kPagedMinChunk ? kPagedMinChunk : c;
+    return c < min_chunk ? min_chunk : c;
 }
 
 // Tiles of a launch, at most: every sequence with rows ends in one that is not full.

@@ -233,7 +233,7 @@ namespace {
 
 // Whether the parts of divided tiles can come up at all, and their bytes.
 size_t paged_workspace(bool small, int width, int page_size, int D_v) {
-    if (((long long)width * page_size) <= (long long)sdpa::kPagedMinChunk * 64) return 0;
+    if ((long long)width * page_size <= 128) return 0;  // (one block of the smallest kind)
     return sdpa::paged_part_bytes(D_v, small ? sdpa::kPagedSmallBM : sdpa::kPagedBM);
 }
 

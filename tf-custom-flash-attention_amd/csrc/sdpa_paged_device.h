@@ -67,7 +67,7 @@ struct PagedPlan {
                 const SeqPlan s = seq(n0);
                 cost += (long long)s.tiles * s.blocks;
             }
-            chunk = plan_chunk(wave_sum64(cost) * p.H_kv, p.target);
+            chunk = plan_chunk(wave_sum64(cost) * p.H_kv, p.target, p.min_chunk);
         }
     }
     // Items of the launch (MERGE: divided tiles).
@@ -225,28 +225,30 @@ __host__ __device__ __forceinline__ int xcd_item(int id, int n) {
 inline long long xcd_grid(long long n) { return (n + 7) / 8 * 8; }
 
 // A window of 64 columns of a sequence's row of the page table, one in each lane.
+// A page that is none counts as page 0 and makes the rows NaN in the end (bad).
 struct PageWindow {
     const int32_t* row;
     int pages, columns;  // columns that hold keys of this workgroup
     int first = -64, id = 0;  // (nothing is held yet)
-    bool bad = false;  // a page that is none has been met (its keys read as zero)
+    bool bad = false;
     __device__ __forceinline__ void load(int column, int lane) {
         first = column;
-        id = column + lane < columns ? row[column + lane] : 0;
-        const bool none = id < 0 || id >= pages;
-        bad = bad || __builtin_amdgcn_ballot_w64(none && column + lane < columns) != 0;
-        if (none) id = -1;
+        const bool in = column + lane < columns;
+        id = in ? row[column + lane] : 0;
+        const bool none = in && (id < 0 || id >= pages);
+        bad = bad || __builtin_amdgcn_ballot_w64(none) != 0;
+        if (none) id = 0;
     }
-    // wave-uniform column
-    __device__ __forceinline__ int page(int column, int lane) {
-        if (column < first || column >= first + 64) load(column, lane);
-        return __builtin_amdgcn_readlane(id, column - first);
+    // the window holds `column` (wave-uniform; the blocks of a wave ascend)
+    __device__ __forceinline__ void need(int column, int lane) {
+        if (column >= first + 64) load(column, lane);
     }
+    __device__ __forceinline__ int held(int column) const { return __builtin_amdgcn_readlane(id, column - first); }
 };
 
 // One head's matrices of a cache.  rows(): a descriptor over the rows [row,
-// min(row + most, end)), which share a page (none of a page that is none): `most` is
-// 16, or more where pages are larger, and row a multiple of it.
+// min(row + most, end)), which share a page: `most` is 16, or more where pages are
+// larger, and row a multiple of it.
 struct PagedRows {
     const unsigned char* base;  // the cache, from this head's matrix of page 0 on
     long long page_bytes;
@@ -259,11 +261,13 @@ struct PagedRows {
         base = uniform_ptr(static_cast<const unsigned char*>(cache) + m * h);
     }
     __device__ __forceinline__ const unsigned char* at(int page, int row) const {
-        return base + page * page_bytes + (long long)(row & ((1 << log2) - 1)) * row_bytes;
+        return base + page * page_bytes + (row & ((1 << log2) - 1)) * row_bytes;
     }
     __device__ __forceinline__ rsrc_t rows(int page, int row, int end, int most) const {
-        const int left = page < 0 ? 0 : end - row;
-        return make_rsrc(at(page < 0 ? 0 : page, row), (long long)(left < 0 ? 0 : (left > most ? most : left)) * row_bytes);
+        const uint64_t a = reinterpret_cast<uint64_t>(at(page, row));
+        return (rsrc_t){__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+                        __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
+                        __builtin_amdgcn_readfirstlane(max(0, min(end - row, most)) * row_bytes), 0x00020000};
     }
 };
 
@@ -477,9 +481,9 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
 }
 
 // Merge of the divided tiles: o = sum_i O_i 2^(m_i - M) / l, stats = M ln 2 + log l.
-// A workgroup takes 8 rows of a tile at a time, a thread four columns of a row;
+// A workgroup takes 32 rows of a tile at a time, a thread four columns of a row;
 // four parts' loads go out together.
-constexpr int kMergeRows = 8;
+constexpr int kMergeRows = 32;
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
     PagedPlan<BM, BN> plan(p);
@@ -614,10 +618,11 @@ hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
 }
 
 // The arguments of a launch by parts: target 0 where nothing can be divided, for
-// want of a workspace, or as no tile walks more than kPagedMinChunk blocks.
-inline PagedParams paged_parts(const PagedParams& p, int BN) {
+// want of a workspace, or as no tile walks more than min_chunk blocks.
+inline PagedParams paged_parts(const PagedParams& p, int BN, int min_chunk) {
     PagedParams a = p;
-    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)kPagedMinChunk * BN) a.target = 0;
+    a.min_chunk = min_chunk;
+    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)min_chunk * BN) a.target = 0;
     return a;
 }
 // Whether a launch by shares may divide a tile.

@@ -123,8 +123,9 @@ void paged_f16_kernel(const PagedParams p) {
     auto issue = [&](int step) __attribute__((always_inline)) {
         const int kv0 = step * BN;
         const uint32_t mk = m0w + (uint32_t)((step % NSTAGE) * Cfg::STAGE), mv = mk + (uint32_t)Cfg::KB;
+        pw.need(kv0 >> K.log2, lane);  // (a window holds whole blocks)
         if (K.log2 >= 6) {
-            const int page = pw.page(kv0 >> K.log2, lane);
+            const int page = pw.held(kv0 >> K.log2);
             kc.issue_whole(K.rows(page, kv0, kv_end, BN), mk, K.row_bytes);
             vc.issue_whole(V.rows(page, kv0, kv_end, BN), mv, V.row_bytes);
         } else {
@@ -133,8 +134,7 @@ void paged_f16_kernel(const PagedParams p) {
 #pragma unroll
                 for (int u = 0; u < C::PER_WAVE; ++u) {
                     const int r0 = kv0 + 16 * C::group(u, wave);
-                    const int page = r0 < kv_end ? pw.page(r0 >> m.log2, lane) : -1;
-                    dma16_at(m.rows(page, r0, kv_end, 16), m0 + (uint32_t)(u * 4 * 1024), c.voff);
+                    dma16_at(m.rows(pw.held(r0 >> m.log2), r0, kv_end, 16), m0 + (uint32_t)(u * 4 * 1024), c.voff);
                 }
             };
             copy(K, kc, mk);
@@ -143,6 +143,7 @@ void paged_f16_kernel(const PagedParams p) {
     };
     // copies this wave issues per block (its vmcnt waits count only those)
     constexpr int CPB = PagedTileCopy<LK, false>::PER_WAVE + PagedTileCopy<LV, true>::PER_WAVE;
+    pw.load((lo * BN) >> K.log2, lane);
     prologue_loads_landed();
 #pragma unroll
     for (int i = 0; i < NSTAGE - 1; ++i)
@@ -361,7 +362,7 @@ hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream) {
         return with_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedCfg<DQK, DV>;
-            const PagedParams a = paged_parts(p, Cfg::BN);
+            const PagedParams a = paged_parts(p, Cfg::BN, kPagedMinChunk16);
             const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
             hipError_t e = launch_kernel<paged_f16_kernel<DQK, DV>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES, stream, a);
             return e == hipSuccess && a.target > 0 ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;

@@ -114,14 +114,15 @@ void paged_f16_small_kernel(const PagedParams p) {
         kc.init(lane, D_qk * 2, D_qk / 8);
         vc.init(lane, D_v * 2, D_v / 8);
         auto issue = [&](int blk) __attribute__((always_inline)) {
+            pw.need((blk * BN) >> K.log2, lane);  // (a window holds whole blocks)
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const int r0 = blk * BN + 16 * g;
-                const int page = r0 < kv_end ? pw.page(r0 >> K.log2, lane) : -1;
+                const int r0 = blk * BN + 16 * g, page = pw.held(r0 >> K.log2);
                 kc.issue(K.rows(page, r0, kv_end, 16), ring + (uint32_t)(256 * LK * g));
                 vc.issue(V.rows(page, r0, kv_end, 16), ring + (uint32_t)(Cfg::KB + 256 * LV * g));
             }
         };
+        pw.load((lo * BN) >> K.log2, lane);
         prologue_loads_landed();
         if (lo + wave < hi) issue(lo + wave);
 

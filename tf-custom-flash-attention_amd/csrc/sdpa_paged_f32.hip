@@ -64,9 +64,8 @@ void paged_f32_kernel(const PagedParams p) {
         // K rows of a block: keys past the last are read as the last (and masked)
         auto load_k = [&](int blk) {
             const int key = min(blk * BN + l32, kv_end - 1), column = key >> K.log2;
-            pw.page((blk * BN) >> K.log2, lane);  // the window holds the block's columns
-            const int page = __shfl(pw.id, column - pw.first);
-            const float* src = reinterpret_cast<const float*>(K.at(page < 0 ? 0 : page, key));
+            pw.need((blk * BN) >> K.log2, lane);  // (a window holds whole blocks)
+            const float* src = reinterpret_cast<const float*>(K.at(__shfl(pw.id, column - pw.first), key));
 #pragma unroll
             for (int c = 0; c < NKC; ++c) {
                 const int d = 8 * c + 4 * hh;
@@ -79,10 +78,9 @@ void paged_f32_kernel(const PagedParams p) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int r0 = blk * BN + 16 * g;
-                const int page = r0 < kv_end ? pw.page(r0 >> K.log2, lane) : -1;
-                const int left = page < 0 ? 0 : min(16, kv_end - r0);
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                    const_cast<unsigned char*>(V.at(page < 0 ? 0 : page, r0)), (short)0, left * V.row_bytes, 0x00020000);
+                    const_cast<unsigned char*>(uniform_ptr(V.at(pw.held(r0 >> K.log2), r0))), (short)0,
+                    __builtin_amdgcn_readfirstlane(max(0, min(16, kv_end - r0)) * V.row_bytes), 0x00020000);
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
 #pragma unroll
@@ -93,6 +91,7 @@ void paged_f32_kernel(const PagedParams p) {
                     }
             }
         };
+        pw.load((lo * BN) >> K.log2, lane);
         if (lo + wave < hi) load_k(lo + wave);
 
         floatx16 oacc[NDT];
@@ -171,7 +170,7 @@ hipError_t launch_paged_f32(const PagedParams& p, bool shares, hipStream_t strea
                            ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(p, stream)
                            : e;
             }
-            const PagedParams a = paged_parts(p, Cfg::PLAN);
+            const PagedParams a = paged_parts(p, Cfg::PLAN, kPagedMinChunk32);
             const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
             hipError_t e = launch_kernel<paged_f32_kernel<DQK, DV, false>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES,
                                                                            stream, a);
