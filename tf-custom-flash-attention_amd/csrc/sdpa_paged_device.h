@@ -15,18 +15,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // v_maximum
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
-__device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+// Inclusive sum over the lanes before and up to each (DPP moves inside rows of 16
+// lanes, then the last lane of a row to the rows behind).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_0(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x += dpp_or_0<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+    x += dpp_or_0<0x112, 0xF>(x);
+    x += dpp_or_0<0x114, 0xF>(x);
+    x += dpp_or_0<0x118, 0xF>(x);
+    x += dpp_or_0<0x142, 0xA>(x);  // row_bcast 15, 31
+    x += dpp_or_0<0x143, 0xC>(x);
     return x;
 }
-__device__ __forceinline__ long long wave_sum64(long long x) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+__device__ __forceinline__ long long wave_scan(long long x) {
+    const auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        const uint32_t lo = (uint32_t)dpp_or_0<decltype(ctrl)::value, decltype(rows)::value>((int)x);
+        const int hi = dpp_or_0<decltype(ctrl)::value, decltype(rows)::value>((int)(x >> 32));
+        x += ((long long)hi << 32) | lo;
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
     return x;
+}
+__device__ __forceinline__ long long readlane64(long long x, int l) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+    return ((long long)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | lo;
 }
 
 // One workgroup's work, the same in every lane: a tile, or a part of its keys.
@@ -39,13 +59,23 @@ struct PagedItem {
     int u0, u1;  // (shares) blocks of the tile
 };
 
-template <int BM, int BN>
+// The plan by parts.  MERGE: its items are the divided tiles.
+template <int BM, int BN, bool MERGE = false>
 struct PagedPlan {
     const PagedParams& p;
     const int lane;
     long long chunk = 0;
-    int q0 = 0, q1 = 0, len = 0;  // of sequence `lane` (read once where there are up to 64)
+    // of sequence n0 + lane: q_starts, kv_lens; the items and slots up to it
+    int q0, q1, len, end, slot;
+    int items = 0;  // in all
 
+    __device__ __forceinline__ SeqPlan seq() const {
+        return seq_plan(q0, q1, len, p.batch, p.G, p.causal != 0, BM, BN, chunk);
+    }
+    __device__ __forceinline__ static int count(const SeqPlan& s) {
+        return MERGE ? (s.parts > 1 ? s.tiles : 0) : s.tiles * s.parts;
+    }
+    __device__ __forceinline__ static int slots(const SeqPlan& s) { return s.parts > 1 ? s.tiles * s.parts : 0; }
     __device__ __forceinline__ void read(int n0) {
         const int s = n0 + lane;
         q0 = q1 = len = 0;
@@ -55,62 +85,59 @@ struct PagedPlan {
             len = p.batch.kv_lens[s];
         }
     }
-    __device__ __forceinline__ SeqPlan seq(int n0) {
-        if (p.batch.N > 64) read(n0);
-        return seq_plan(q0, q1, len, p.batch, p.G, p.causal != 0, BM, BN, chunk);
+    __device__ __forceinline__ void scan(int items_before, int slots_before) {
+        const SeqPlan s = seq();
+        end = wave_scan(count(s) * p.H_kv) + items_before;
+        slot = wave_scan(slots(s) * p.H_kv) + slots_before;
     }
     __device__ __forceinline__ PagedPlan(const PagedParams& p_) : p(p_), lane(threadIdx.x & 63) {
-        if (p.batch.N <= 64) read(0);
+        read(0);
         if (p.target > 0) {
             long long cost = 0;
             for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
-                const SeqPlan s = seq(n0);
+                if (n0 > 0) read(n0);
+                const SeqPlan s = seq();
                 cost += (long long)s.tiles * s.blocks;
             }
-            chunk = plan_chunk(wave_sum64(cost) * p.H_kv, p.target, p.min_chunk);
+            chunk = plan_chunk(readlane64(wave_scan(cost), 63) * p.H_kv, p.target, p.min_chunk);
+            if (p.batch.N > 64) read(0);
         }
-    }
-    // Items of the launch (MERGE: divided tiles).
-    template <bool MERGE>
-    __device__ __forceinline__ static int count(const SeqPlan& s) {
-        return MERGE ? (s.parts > 1 ? s.tiles : 0) : s.tiles * s.parts;
-    }
-    template <bool MERGE>
-    __device__ __forceinline__ int items() {
-        int n = 0;
-        for (int n0 = 0; n0 < p.batch.N; n0 += 64) n += count<MERGE>(seq(n0));
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
-        return __builtin_amdgcn_readfirstlane(n) * p.H_kv;
+        scan(0, 0);
+        items = __builtin_amdgcn_readlane(end, 63);
+        for (int n0 = 64; n0 < p.batch.N; n0 += 64) {
+            read(n0);
+            items += __builtin_amdgcn_readlane(wave_scan(count(seq()) * p.H_kv), 63);
+        }
     }
     // Item `at` in the order sequence, key head, tile (last first: under the
     // causal mask it has the most keys), part.
-    template <bool MERGE>
     __device__ __forceinline__ bool find(int at, PagedItem& it) {
-        int base = 0, slots = 0;
+        int base = 0, slots_before = 0;
         for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
-            const SeqPlan s = seq(n0);
-            const int mine = count<MERGE>(s) * p.H_kv, div = s.parts > 1 ? s.tiles * s.parts * p.H_kv : 0;
-            const int end = wave_scan(mine, lane) + base, slot = wave_scan(div, lane) + slots;
+            if (p.batch.N > 64) {
+                read(n0);
+                scan(base, slots_before);
+            }
             const uint64_t over = __builtin_amdgcn_ballot_w64(end > at);
             if (over != 0) {
                 const int l = __builtin_ctzll(over);
                 const auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+                const SeqPlan s = seq();
                 it.s = SeqPlan{get(s.q0), get(s.n), get(s.len), get(s.tiles), get(s.blocks), get(s.parts), get(s.bad) != 0};
                 it.seq = n0 + l;
-                int i = at - (get(end) - get(mine));
+                int i = at - (get(end) - count(it.s) * p.H_kv);
                 const int per_tile = MERGE ? 1 : it.s.parts, per_head = it.s.tiles * per_tile;
                 it.h = i / per_head;
                 i -= it.h * per_head;
                 const int t = i / per_tile;
                 it.tile = it.s.tiles - 1 - t;
                 it.part = i - t * per_tile;
-                it.slot = get(slot) - get(div) + (it.h * it.s.tiles + it.tile) * it.s.parts + it.part;
+                it.slot = get(slot) - slots(it.s) * p.H_kv + (it.h * it.s.tiles + it.tile) * it.s.parts + it.part;
                 it.divided = it.s.parts > 1;
                 return true;
             }
             base = __builtin_amdgcn_readlane(end, 63);
-            slots = __builtin_amdgcn_readlane(slot, 63);
+            slots_before = __builtin_amdgcn_readlane(slot, 63);
         }
         return false;
     }
@@ -131,10 +158,6 @@ struct PagedShares {
     long long total = 0;
     int n = 0;  // workgroups
 
-    __device__ __forceinline__ static long long readlane64(long long x, int l) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
-        return ((long long)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | lo;
-    }
     // sequences n0 + lane; base: the blocks before them
     __device__ __forceinline__ Lane form(int n0, long long base) const {
         const int lane = threadIdx.x & 63, i = n0 + lane;
@@ -148,13 +171,7 @@ struct PagedShares {
         // (all tiles of a sequence count as its last one)
         x.s = seq_plan(q0, q1, len, p.batch, p.G, false, BM, BN, 0);
         const long long mine = (long long)x.s.tiles * x.s.blocks * p.H_kv;
-        x.last = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const long long y = __shfl_up(x.last, d);
-            if (lane >= d) x.last += y;
-        }
-        x.last += base;
+        x.last = wave_scan(mine) + base;
         x.first = x.last - mine;
         return x;
     }
@@ -486,12 +503,12 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
 constexpr int kMergeRows = 32;
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
-    PagedPlan<BM, BN> plan(p);
-    const int units = plan.template items<true>() * (BM / kMergeRows), cpr = p.D_v / 4;
+    PagedPlan<BM, BN, true> plan(p);
+    const int units = plan.items * (BM / kMergeRows), cpr = p.D_v / 4;
     constexpr int U = 4;
     for (int unit = (int)blockIdx.x; unit < units; unit += (int)gridDim.x) {
         PagedItem it;
-        if (!plan.template find<true>(unit / (BM / kMergeRows), it) || !slot_ok(p, it)) return;
+        if (!plan.find(unit / (BM / kMergeRows), it) || !slot_ok(p, it)) return;
         const int np = it.s.parts, row0 = unit % (BM / kMergeRows) * kMergeRows;
         const int rows = min(kMergeRows, it.s.n * p.G - it.tile * BM - row0);
         for (int i = threadIdx.x; i < rows * cpr; i += 256) {

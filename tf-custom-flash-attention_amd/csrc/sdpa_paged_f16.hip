@@ -73,8 +73,8 @@ void paged_f16_kernel(const PagedParams p) {
     PagedItem it;
     {
         PagedPlan<BM, BN> plan(p);
-        const int at = xcd_item(tile_id(), plan.template items<false>());
-        if (at < 0 || !plan.template find<false>(at, it) || !slot_ok(p, it)) return;
+        const int at = xcd_item(tile_id(), plan.items);
+        if (at < 0 || !plan.find(at, it) || !slot_ok(p, it)) return;
     }
     const int D_qk = p.D_qk, D_v = p.D_v, np = it.s.parts;
     const int kv_end = min(tile_keys(p, it, BM), it.s.len);

@@ -151,8 +151,8 @@ void paged_f32_kernel(const PagedParams p) {
     } else {
         PagedPlan<BM, Cfg::PLAN> plan(p);
         PagedItem it;
-        const int at = xcd_item(tile_id(), plan.template items<false>());
-        if (at >= 0 && plan.template find<false>(at, it) && slot_ok(p, it)) work(it);
+        const int at = xcd_item(tile_id(), plan.items);
+        if (at >= 0 && plan.find(at, it) && slot_ok(p, it)) work(it);
     }
 }
 
