@@ -54,7 +54,7 @@ int main() {
         p.target = pick(0, 5) == 0 ? 0 : kPagedTarget;
         const int cap = p.batch.width << log2;
         for (int kernel = 0; kernel < 2; ++kernel) {
-            const int BM = kernel ? kPagedBM : kPagedSmallBM, BN = kernel ? 64 : 128;
+            const int BM = kernel ? kPagedBM : kPagedSmallBM, BN = kernel ? 64 : 32;
             std::vector<int> seen(N, 0);
             long long cost = 0, items = 0, slots = 0, divided = 0;
             std::vector<SeqPlan> plans;
@@ -62,7 +62,7 @@ int main() {
                 return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, BM, BN, chunk);
             };
             for (int s = 0; s < N; ++s) cost += (long long)plan(s, 0).tiles * plan(s, 0).blocks;
-            const long long chunk = plan_chunk(cost * H_kv, p.target, kernel ? kPagedMinChunk16 : kPagedMinChunk32);
+            const long long chunk = plan_chunk(cost * H_kv, p.target, kPagedMinChunk * 64 / BN);
             for (int s = 0; s < N; ++s) {
                 const SeqPlan q = plan(s, chunk);
                 if (q.tiles == 0) continue;

@@ -43,10 +43,10 @@ struct PagedParams {
     int min_chunk;  // parts: key blocks of a part, at least
 };
 
-// Key blocks of a part, at least.  fp16 (64 keys a block), 300 tokens over 2300, 16
-// heads on 4, D 64: 2 blocks 31.2 us, 4 29.3, 6 25.7, 8 25.8, 16 27.7; over 1150: 24.8,
-// 21.1, 21.9, 23.6, 29.6.  fp32 (128 keys): 2 to 8 alike, 12 and more a quarter slower.
-constexpr int kPagedMinChunk16 = 6, kPagedMinChunk32 = 2;
+// Key blocks of 64 of a part, at least.  fp16, 300 tokens over 2300, 16 heads on 4, D
+// 64: 2 blocks 31.2 us, 4 29.3, 6 25.7, 8 25.8, 16 27.7; over 1150: 24.8, 21.1, 21.9,
+// 23.6, 29.6.
+constexpr int kPagedMinChunk = 6;
 constexpr int kPagedMaxParts = 64;  // (the merge walks a row's parts one batch after the other)
 
 // One sequence's part of the plan.
@@ -90,7 +90,7 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
 }
 
 // Calls whose sequences have one tile of 32 rows, as far as is known, take the
-// kernels of such tiles, by shares; others, by parts, that of 128-row tiles (fp32: of 32).
+// kernels of such tiles, by shares; others, by parts, those of 128-row tiles.
 constexpr int kPagedSmallRows = 32;
 
 // Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)).
@@ -115,7 +115,7 @@ inline size_t paged_part_bytes(int D_v, int BM) {
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream);
-// (fp32: by shares, or by parts)
-hipError_t launch_paged_f32(const PagedParams& p, bool shares, hipStream_t stream);
+hipError_t launch_paged_f32_small(const PagedParams& p, hipStream_t stream);
+hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream);
 
 }  // namespace sdpa

@@ -296,14 +296,13 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     const bool small = sdpa::paged_small(T, p.G, max_q_len);
     if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
-    // rows of a tile of the kernel that is taken
-    const int BM = small || dtype == SDPA_DTYPE_F32 ? sdpa::kPagedSmallBM : sdpa::kPagedBM;
     p.target = sdpa::kPagedTarget;
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + 2 * (size_t)p.target * BM * D_v;
+        p.part_ml = p.part_o + 2 * (size_t)p.target * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
     }
-    if (dtype == SDPA_DTYPE_F32) return hip_status(sdpa::launch_paged_f32(p, small, stream));
+    if (dtype == SDPA_DTYPE_F32)
+        return hip_status(small ? sdpa::launch_paged_f32_small(p, stream) : sdpa::launch_paged_f32(p, stream));
     return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));
 }
 

@@ -391,6 +391,62 @@ __device__ __forceinline__ void put_care_row(const PagedParams& p, const PagedIt
     if (lane == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = r.m * kLn2 + logf(r.l);
 }
 
+// Results of a wave of 32 rows (lane l32: row; accumulator tiles over features) of a
+// kernel of 128-row tiles: to o and stats, or to the workspace; rows whose sums hold
+// a NaN or an infinity again with care.  [k0, k1): this workgroup's keys.
+template <typename T, int DV, int BM>
+__device__ __forceinline__ void put_paged_rows(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
+                                               const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
+                                               const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
+                                               int k1) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, in_tile = 32 * wave + l32, D_v = p.D_v;
+    float z = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DV / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(oacc[dt][r], 0.f, z);
+    const uint64_t nan_lanes = __builtin_amdgcn_ballot_w64(z != z && row.live);
+    const uint32_t again = bad ? 0u : (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
+    if (row.live && !((again >> l32) & 1)) {
+        const float m = l_tot == 0.f ? -INFINITY : m_run, l = bad ? __builtin_nanf("") : l_tot;
+        const float f = it.divided ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        const size_t at = (size_t)it.slot * BM + in_tile;
+        if (hh == 0) {
+            if (it.divided) {
+                p.part_ml[2 * at] = m;
+                p.part_ml[2 * at + 1] = l;
+            } else {
+                p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = m * kLn2 + logf(l);
+            }
+        }
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        T* o = static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h;
+#pragma unroll
+        for (int dt = 0; dt < DV / 32; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d0 = 32 * dt + 8 * g + 4 * hh;
+                if (d0 >= D_v) continue;
+                if (it.divided) {
+                    *reinterpret_cast<floatx4*>(p.part_o + at * D_v + d0) =
+                        (floatx4){oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
+                } else {
+                    t4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = (T)(oacc[dt][4 * g + e] * f);
+                    *reinterpret_cast<t4*>(o + d0) = v;
+                }
+            }
+    }
+    for (uint32_t todo = again; todo != 0; todo &= todo - 1) {
+        const int r = 32 * wave + __builtin_ctz(todo);
+        PagedRow rr;
+        rr.init(p, it, it.tile * BM + r);
+        const T* q = static_cast<const T*>(p.q) + rr.tok * p.qs.t + rr.head * p.qs.h;
+        put_care_row<T, BM>(p, it, rr, r, care_row<T>(p, table, K, V, q, k0, min(k1, min(rr.see, it.s.len))));
+    }
+}
+
 // Weight 2^(m - M) of a part (0 where both are -inf: nothing was seen).
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : fast_exp2(m - M); }
 // acc + x w, an infinite or NaN x as it is (w may have vanished)
@@ -636,10 +692,10 @@ hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
 
 // The arguments of a launch by parts: target 0 where nothing can be divided, for
 // want of a workspace, or as no tile walks more than min_chunk blocks.
-inline PagedParams paged_parts(const PagedParams& p, int BN, int min_chunk) {
+inline PagedParams paged_parts(const PagedParams& p, int BN) {
     PagedParams a = p;
-    a.min_chunk = min_chunk;
-    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)min_chunk * BN) a.target = 0;
+    a.min_chunk = kPagedMinChunk * 64 / BN;
+    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)kPagedMinChunk * 64) a.target = 0;
     return a;
 }
 // Whether a launch by shares may divide a tile.

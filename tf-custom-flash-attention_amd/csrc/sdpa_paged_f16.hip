@@ -311,48 +311,7 @@ void paged_f16_kernel(const PagedParams p) {
     if (lane == 0) none[wave] = pw.bad || it.s.bad;
     __syncthreads();
     const bool bad = (none[0] | none[1] | none[2] | none[3]) != 0;
-    // rows with a NaN or infinity in their sums, which are done again
-    float z = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(oacc[dt][r], 0.f, z);
-    const uint64_t nan_lanes = __builtin_amdgcn_ballot_w64(z != z && row.live);
-    const uint32_t again = bad ? 0u : (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
-    const float nan = __builtin_nanf("");
-    if (row.live && !((again >> l32) & 1)) {
-        const float m = l_tot == 0.f ? -INFINITY : m_run, l = bad ? nan : l_tot;
-        if (it.divided) {  // this part's unnormalised O, m and l
-            const size_t at = (size_t)it.slot * BM + in_tile;
-            if (hh == 0) {
-                p.part_ml[2 * at] = m;
-                p.part_ml[2 * at + 1] = l;
-            }
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int d0 = 32 * dt + 8 * g + 4 * hh;
-                    if (d0 < D_v)
-                        *reinterpret_cast<floatx4*>(p.part_o + at * D_v + d0) =
-                            (floatx4){oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
-                }
-        } else {
-            if (hh == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = m * kLn2 + logf(l);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            half_t* o = static_cast<half_t*>(p.o) + row.tok * p.os.t + row.head * p.os.h;
-            if (D_v == DV) store_rows_f16<DV>(o, oacc, inv, hh);
-            else store_rows_f16_n<DV>(o, oacc, inv, hh, D_v);
-        }
-    }
-    for (uint32_t todo = again; todo != 0; todo &= todo - 1) {
-        const int r = 32 * wave + __builtin_ctz(todo);
-        PagedRow rr;
-        rr.init(p, it, it.tile * BM + r);
-        const half_t* q = static_cast<const half_t*>(p.q) + rr.tok * p.qs.t + rr.head * p.qs.h;
-        put_care_row<half_t, BM>(p, it, rr, r,
-                                 care_row<half_t>(p, pw.row, K, V, q, lo * BN, min(nsteps * BN, min(rr.see, it.s.len))));
-    }
+    put_paged_rows<half_t, DV, BM>(p, it, wave, row, oacc, m_run, l_tot, bad, pw.row, K, V, lo * BN, nsteps * BN);
 }
 
 }  // namespace
@@ -362,7 +321,7 @@ hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream) {
         return with_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedCfg<DQK, DV>;
-            const PagedParams a = paged_parts(p, Cfg::BN, kPagedMinChunk16);
+            const PagedParams a = paged_parts(p, Cfg::BN);
             const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
             hipError_t e = launch_kernel<paged_f16_kernel<DQK, DV>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES, stream, a);
             return e == hipSuccess && a.target > 0 ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;
