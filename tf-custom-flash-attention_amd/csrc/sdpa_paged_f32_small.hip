@@ -15,8 +15,14 @@
 namespace sdpa {
 namespace {
 
+// Cache policy of the V loads (nt).  32 sequences of 4096, D 128: 117 us, plain 127; 64 of
+// 2048, D 64: 105 and 116.  K rows are read 32 bytes at a time, their lines again and again:
+// with the hint 132 us there.
+constexpr int kNonTemporal = 2;
+
 template <int DQK, int DV>
 struct PagedF32SmallCfg {
+    static constexpr int WPE = DQK + DV > 128 ? 1 : 2;
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedSmallBM, BN = 32, PLAN = BN * NW;
     static constexpr int PLAN_AT = NW * BM * acc_stride(DV) * 4 + NW * BM * 8 + (BM + NW) * 4;
     static_assert(PLAN_AT % 16 == 0, "the plan, behind the sums");
@@ -25,7 +31,7 @@ struct PagedF32SmallCfg {
 
 template <int DQK, int DV>
 __global__ __launch_bounds__((PagedF32SmallCfg<DQK, DV>::NT))
-__attribute__((amdgpu_waves_per_eu(DQK + DV > 128 ? 1 : 2, DQK + DV > 128 ? 1 : 2)))
+__attribute__((amdgpu_waves_per_eu(PagedF32SmallCfg<DQK, DV>::WPE, PagedF32SmallCfg<DQK, DV>::WPE)))
 void paged_f32_small_kernel(const PagedParams p) {
     using Cfg = PagedF32SmallCfg<DQK, DV>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW, NKC = DQK / 8, NDT = DV / 32;
@@ -86,7 +92,7 @@ void paged_f32_small_kernel(const PagedParams p) {
                     for (int dt = 0; dt < NDT; ++dt) {
                         const int d = 32 * dt + l32;
                         const uint32_t off = d < D_v ? (uint32_t)((8 * (r >> 2) + 4 * hh + (r & 3)) * V.row_bytes + 4 * d) : kOob;
-                        v[8 * g + r][dt] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+                        v[8 * g + r][dt] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, kNonTemporal));
                     }
             }
         };
@@ -151,10 +157,12 @@ hipError_t launch_paged_f32_small(const PagedParams& p, hipStream_t stream) {
         return with_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedF32SmallCfg<DQK, DV>;
-            hipError_t e = launch_kernel<paged_f32_small_kernel<DQK, DV>>(dim3((unsigned)p.target), Cfg::NT, Cfg::LDS_BYTES,
-                                                                         stream, p);
-            return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
-                       ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(p, stream)
+            PagedParams a = p;
+            a.target = min(p.target, 256 * Cfg::WPE);
+            hipError_t e = launch_kernel<paged_f32_small_kernel<DQK, DV>>(dim3((unsigned)a.target), Cfg::NT, Cfg::LDS_BYTES,
+                                                                         stream, a);
+            return e == hipSuccess && paged_shares_divide(a, Cfg::PLAN)
+                       ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(a, stream)
                        : e;
         });
     });
