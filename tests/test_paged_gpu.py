@@ -123,6 +123,13 @@ CASES = [
     (F16, (2, 70) * 40, tuple(range(70, 870, 10)), 4, 1, 32, 32, 16, True, 0, 3),
     (F16, (7, 200), (50, 400), 2, 1, 8, 16, 16, True, 0, 2),                      # a quarter of a tile's width
     (F16, (90,), (90,), 5, 1, 40, 72, 32, True, 0, 3),
+    (F16, (1, 2, 1), (777, 40, 300), 6, 2, 96, 80, 16, True, 0, 3),               # between the widths of tiles
+    (F16, (200, 40), (500, 40), 4, 2, 88, 96, 64, True, 0, 3),
+    (F16, (140,), (300,), 2, 1, 96, 128, 16, False, 0, 3),
+    (F32, (1, 1), (900, 33), 6, 2, 96, 96, 32, True, 0, 3),
+    (F32, (150, 33), (400, 100), 4, 2, 96, 96, 16, True, 0, 3),
+    (F32, (140,), (300,), 2, 1, 128, 92, 16, True, 0, 3),
+    (F32, (140,), (300,), 2, 1, 84, 24, 16, True, 0, 3),
     (F32, (1,), (1,), 1, 1, 64, 64, 16, True, 0, 1),
     (F32, (1, 1, 3), (300, 77, 1500), 8, 2, 128, 128, 16, True, 1, 3),
     (F32, (130, 1, 20), (400, 1111, 20), 6, 3, 64, 32, 64, True, 0, 3),

@@ -28,8 +28,8 @@ constexpr float kTauG = 8.0f;  // lazy-rescale threshold (log2 units)
 template <int DQK, int DV>
 struct PagedCfg {
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedBM, BN = 64;
-    static constexpr int LK = DQK / 8, LV = DV / 8;
-    static constexpr int KB = BN * DQK * 2, VB = BN * DV * 2, STAGE = KB + VB;
+    static constexpr int LK = lds_chunks(DQK), LV = lds_chunks(DV);
+    static constexpr int KB = BN * LK * 16, VB = BN * LV * 16, STAGE = KB + VB;
     static constexpr int NSTAGE = 2 * 3 * STAGE <= 160 * 1024 ? 3 : 2;
     static constexpr size_t LDS_BYTES = NSTAGE * (size_t)STAGE;
     static_assert(2 * LDS_BYTES <= 160 * 1024, "two workgroups per CU in gfx950 LDS");
@@ -317,8 +317,8 @@ void paged_f16_kernel(const PagedParams p) {
 }  // namespace
 
 hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream) {
-    return with_dim(p.D_qk, [&](auto dqk) {
-        return with_dim(p.D_v, [&](auto dv) {
+    return with_paged_dim(p.D_qk, [&](auto dqk) {
+        return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedCfg<DQK, DV>;
             const PagedParams a = paged_parts(p, Cfg::BN);

@@ -38,8 +38,8 @@ constexpr float kTauP = 8.0f;  // lazy-rescale threshold (log2 units)
 template <int DQK, int DV>
 struct PagedSmallCfg {
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedSmallBM, BN = 32, PLAN = BN * NW;
-    static constexpr int LK = DQK / 8, LV = DV / 8;
-    static constexpr int KB = BN * DQK * 2, VB = BN * DV * 2, STAGE = KB + VB;
+    static constexpr int LK = lds_chunks(DQK), LV = lds_chunks(DV);
+    static constexpr int KB = BN * LK * 16, VB = BN * LV * 16, STAGE = KB + VB;
     // merge area (after the loop): O of every wave, m and l, flags of rows and waves
     static constexpr int OS = acc_stride(DV), MERGE = NW * BM * OS * 4 + NW * BM * 8 + (BM + NW) * 4;
     static constexpr int PLAN_AT = NW * STAGE > MERGE ? NW * STAGE : (MERGE + 15) / 16 * 16;  // the plan, behind them
@@ -220,8 +220,8 @@ void paged_f16_small_kernel(const PagedParams p) {
 }  // namespace
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream) {
-    return with_dim(p.D_qk, [&](auto dqk) {
-        return with_dim(p.D_v, [&](auto dv) {
+    return with_paged_dim(p.D_qk, [&](auto dqk) {
+        return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedSmallCfg<DQK, DV>;
             hipError_t e = launch_kernel<paged_f16_small_kernel<DQK, DV>>(dim3((unsigned)p.target), Cfg::NT, Cfg::LDS_BYTES,

@@ -25,9 +25,10 @@ constexpr float kTauP32 = 8.0f;  // lazy-rescale threshold (log2 units)
 
 template <int DQK, int DV>
 struct PagedF32Cfg {
-    static constexpr int NWK = DQK == 128 && DV == 128 ? 1 : 2, NT = 256 * NWK, BM = kPagedBM, BN = 32 * NWK;
-    using KT = Bf3Tile<BN, DQK / 8>;
-    using VT = Bf3Tile<BN, DV / 8>;
+    static constexpr int LK = lds_chunks(DQK), LV = lds_chunks(DV);
+    static constexpr int NWK = LK == 16 && LV == 16 ? 1 : 2, NT = 256 * NWK, BM = kPagedBM, BN = 32 * NWK;
+    using KT = Bf3Tile<BN, LK>;
+    using VT = Bf3Tile<BN, LV>;
     static constexpr int STAGE = KT::BYTES + VT::BYTES;
     static constexpr int OS = DV + 4, MERGE = NWK > 1 ? (BM * OS + BM * 2) * 4 : 0;  // after the loop
     static constexpr size_t LDS_BYTES = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
@@ -57,7 +58,7 @@ struct PagedBf3Stage {
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
             const int c = tid + u * NT;
-            Bf3Tile<ROWS, COLS / 8>::template store4<false>(tile, c / CPR, c % CPR * 4, r[u]);
+            Bf3Tile<ROWS, lds_chunks(COLS)>::template store4<false>(tile, c / CPR, c % CPR * 4, r[u]);
         }
     }
 };
@@ -69,7 +70,7 @@ void paged_f32_kernel(const PagedParams p) {
     using Cfg = PagedF32Cfg<DQK, DV>;
     using KT = typename Cfg::KT;
     using VT = typename Cfg::VT;
-    constexpr int BM = Cfg::BM, BN = Cfg::BN, LK = DQK / 8, LV = DV / 8, NDT = DV / 32;
+    constexpr int BM = Cfg::BM, BN = Cfg::BN, LK = Cfg::LK, LV = Cfg::LV, NDT = DV / 32;
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave & 3, wk = wave >> 2;
 
@@ -244,8 +245,8 @@ void paged_f32_kernel(const PagedParams p) {
 }  // namespace
 
 hipError_t launch_paged_f32(const PagedParams& p, hipStream_t stream) {
-    return with_dim(p.D_qk, [&](auto dqk) {
-        return with_dim(p.D_v, [&](auto dv) {
+    return with_paged_dim(p.D_qk, [&](auto dqk) {
+        return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedF32Cfg<DQK, DV>;
             PagedParams a = paged_parts(p, Cfg::BN);

@@ -153,8 +153,8 @@ void paged_f32_small_kernel(const PagedParams p) {
 }  // namespace
 
 hipError_t launch_paged_f32_small(const PagedParams& p, hipStream_t stream) {
-    return with_dim(p.D_qk, [&](auto dqk) {
-        return with_dim(p.D_v, [&](auto dv) {
+    return with_paged_dim(p.D_qk, [&](auto dqk) {
+        return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedF32SmallCfg<DQK, DV>;
             PagedParams a = p;
