@@ -221,6 +221,32 @@ def test_masked_places_have_no_influence(pkg, T, new, lens, page):
 
 
 @pytest.mark.parametrize("T", [F16, F32])
+@pytest.mark.parametrize("new,lens", [((3,), (300,)), ((150,), (400,))])
+def test_infinite_keys_and_queries(pkg, T, new, lens):
+    """A score of -inf weighs nothing, one of +inf or NaN makes its row NaN, and
+    only rows that see it."""
+    b = Batch(T, new, lens, 2, 1, 64, 64, 16)
+    m, l = new[0], lens[0]
+    b.q = b.q.abs() + T.itemsize / 8  # every product with a key of one sign has its sign
+    b.k[0][7, 0, 11] = -INF            # seen by all
+    ref = b.reference(True)
+    out = pkg.paged_sdpa(*b.args(), scale=b.scale)
+    # (the bound's sum of sizes is infinite for that key: it has no share in any sum)
+    c = Batch(T, new, lens, 2, 1, 64, 64, 16)
+    c.q, c.k, c.v = b.q, [b.k[0].clone()], b.v
+    c.k[0][7] = 0
+    bounds = c.reference(True)[2:]
+    check(out, [ref[0], ref[1], bounds[0], bounds[1]])
+    b.k[0][l - 2, 0, 3] = INF          # seen by the last two tokens
+    o, stats = pkg.paged_sdpa(*b.args(), scale=b.scale)
+    assert bool(torch.isnan(o[m - 2:]).all()) and bool(torch.isnan(stats[m - 2:]).all())
+    check((o[:m - 2], stats[:m - 2]), [ref[0][:m - 2], ref[1][:m - 2], bounds[0][:m - 2], bounds[1][:m - 2]])
+    b.q[0, 1, 5] = NAN
+    o, _ = pkg.paged_sdpa(*b.args(), scale=b.scale)
+    assert bool(torch.isnan(o[0, 1]).all()) and not torch.isnan(o[0, 0]).any()
+
+
+@pytest.mark.parametrize("T", [F16, F32])
 def test_pages_that_are_none(pkg, T):
     """A sequence with a missing page (past the cache, negative, or more tokens
     than columns) is NaN where rows may see it; the others are right."""

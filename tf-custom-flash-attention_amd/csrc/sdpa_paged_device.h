@@ -323,8 +323,8 @@ __device__ __forceinline__ int tile_keys(const PagedParams& p, const PagedItem& 
 
 // ---- rows done again ---------------------------------------------------------
 // A product of a masked weight, 0, with an infinite or NaN value is NaN, and
-// tiles are multiplied whole.  A row whose sums come out NaN is therefore done
-// again by one wave, key by key over the keys [lo, hi) it sees: finite values
+// tiles are multiplied whole.  A row whose sums come out NaN, though the sum of its
+// weights is none, is therefore done again by one wave, key by key over the keys [lo, hi) it sees: finite values
 // weighted, others added as they are, so that one among the row's own keys makes
 // the result infinite or NaN and one behind the mask nothing.  Lane l returns
 // columns l and l + 64 of the unnormalised sums; m in log2 units.
@@ -343,9 +343,13 @@ __device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t*
         int page = 0;
         if (j < hi) {
             page = table[j >> K.log2];
-            const T* k = reinterpret_cast<const T*>(K.at(page, j));
+            typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));
+            const chunk *k = reinterpret_cast<const chunk*>(K.at(page, j)), *qc = reinterpret_cast<const chunk*>(q);
+            constexpr int EPC = 16 / (int)sizeof(T);
             float dot = 0.f;
-            for (int d = 0; d < p.D_qk; ++d) dot = __builtin_fmaf((float)q[d], (float)k[d], dot);
+            for (int d = 0; d < p.D_qk / EPC; ++d)
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) dot = __builtin_fmaf((float)qc[d][e], (float)k[d][e], dot);
             s = dot * sl2;
         }
         float mx = s;
@@ -405,8 +409,10 @@ __device__ __forceinline__ void put_care_row(const PagedParams& p, const PagedIt
 
 // Results of a wave of 32 rows (lane l32: row; accumulator tiles over features) of a
 // kernel of 128-row tiles: to o and stats, or to the workspace; rows whose sums hold
-// a NaN or an infinity again with care.  [k0, k1): this workgroup's keys.
-template <typename T, int DV, int BM>
+// a NaN or an infinity again with care (unless a score was NaN, where they are right;
+// ANY: also then, as a score may be NaN for an infinite factor's sake).  [k0, k1): this
+// workgroup's keys.
+template <typename T, int DV, int BM, bool ANY>
 __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
                                                const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
                                                const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
@@ -417,7 +423,7 @@ __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const Paged
     for (int dt = 0; dt < DV / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z = __builtin_fmaf(oacc[dt][r], 0.f, z);
-    const uint64_t nan_lanes = __builtin_amdgcn_ballot_w64(z != z && row.live);
+    const uint64_t nan_lanes = __builtin_amdgcn_ballot_w64(row.live && (ANY ? z != z || l_tot != l_tot : z != z && l_tot == l_tot));
     const uint32_t again = bad ? 0u : (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
     if (row.live && !((again >> l32) & 1)) {
         const float m = l_tot == 0.f ? -INFINITY : m_run, l = bad ? __builtin_nanf("") : l_tot;
@@ -529,7 +535,7 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
             bool nan = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) nan = nan || acc[u][e] != acc[u][e];
-            if (nan) again[r] = 1;
+            if (nan && L[u] == L[u]) again[r] = 1;
         }
     }
     __syncthreads();

@@ -311,7 +311,7 @@ void paged_f16_kernel(const PagedParams p) {
     if (lane == 0) none[wave] = pw.bad || it.s.bad;
     __syncthreads();
     const bool bad = (none[0] | none[1] | none[2] | none[3]) != 0;
-    put_paged_rows<half_t, DV, BM>(p, it, wave, row, oacc, m_run, l_tot, bad, pw.row, K, V, lo * BN, nsteps * BN);
+    put_paged_rows<half_t, DV, BM, false>(p, it, wave, row, oacc, m_run, l_tot, bad, pw.row, K, V, lo * BN, nsteps * BN);
 }
 
 }  // namespace

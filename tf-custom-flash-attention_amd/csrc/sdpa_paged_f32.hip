@@ -239,7 +239,7 @@ void paged_f32_kernel(const PagedParams p) {
     bool bad = false;
 #pragma unroll
     for (int w = 0; w < 4 * Cfg::NWK; ++w) bad = bad || none[w] != 0;
-    put_paged_rows<float, DV, BM>(p, it, wq, row, oacc, m_run, l_tot, bad, pw.row, K, V, lo * BN, hi * BN);
+    put_paged_rows<float, DV, BM, true>(p, it, wq, row, oacc, m_run, l_tot, bad, pw.row, K, V, lo * BN, hi * BN);
 }
 
 }  // namespace

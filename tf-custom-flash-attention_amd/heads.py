@@ -466,6 +466,8 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
             _fail(f"out must be ({T} {[n, H_q, D_v]}, float32 {[n, H_q]})")
         if not (o.is_contiguous() and stats.is_contiguous()):
             _fail("out must be contiguous")
+        if o.data_ptr() == q.data_ptr() and n > 0:
+            _fail("out must not be q")
         _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens,
                    o=o, stats=stats)
     L = library()
