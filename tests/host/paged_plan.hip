@@ -51,18 +51,20 @@ int main() {
         p.H_kv = H_kv;
         p.G = G;
         p.causal = pick(0, 1);
-        p.target = pick(0, 5) == 0 ? 0 : kPagedTarget;
+        p.target_log2 = kPagedTargetLog2;
+        p.divide = pick(0, 5) != 0;
+        const int target = 1 << p.target_log2;
         const int cap = p.batch.width << log2;
         for (int kernel = 0; kernel < 2; ++kernel) {
             const int BM = kernel ? kPagedBM : kPagedSmallBM, BN = kernel ? 64 : 32;
             std::vector<int> seen(N, 0);
             long long cost = 0, items = 0, slots = 0, divided = 0;
             std::vector<SeqPlan> plans;
-            const auto plan = [&](int s, long long chunk) {
+            const auto plan = [&](int s, int chunk) {
                 return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, BM, BN, chunk);
             };
             for (int s = 0; s < N; ++s) cost += (long long)plan(s, 0).tiles * plan(s, 0).blocks;
-            const long long chunk = plan_chunk(cost * H_kv, p.target, kPagedMinChunk * 64 / BN);
+            const int chunk = p.divide ? plan_chunk(cost * H_kv, p.target_log2, kPagedMinChunk * 64 / BN) : 0;
             for (int s = 0; s < N; ++s) {
                 const SeqPlan q = plan(s, chunk);
                 if (q.tiles == 0) continue;
@@ -71,7 +73,7 @@ int main() {
                 CHECK(q.len >= 0 && q.len <= cap && q.parts >= 1 && q.parts <= kPagedMaxParts && q.blocks >= 1);
                 CHECK(q.bad == (lens[s] > cap));
                 CHECK((long long)q.tiles * BM >= (long long)q.n * G && (long long)(q.tiles - 1) * BM < (long long)q.n * G);
-                CHECK(p.target > 0 || q.parts == 1);
+                CHECK(p.divide || q.parts == 1);
                 items += (long long)q.tiles * q.parts * H_kv;
                 if (q.parts > 1) {
                     slots += (long long)q.tiles * q.parts * H_kv;
@@ -81,16 +83,16 @@ int main() {
                 CHECK(part_begin(nblk, 0, q.parts) == 0 && part_begin(nblk, q.parts, q.parts) == nblk);
                 for (int i = 0; i < q.parts; ++i) CHECK(part_begin(nblk, i, q.parts) <= part_begin(nblk, i + 1, q.parts));
             }
-            CHECK(slots <= 2 * p.target && divided <= p.target);
-            if (!garbage) CHECK(items <= paged_max_tiles(p, BM) + p.target);
+            CHECK(slots <= 2 * target && divided <= target);
+            if (!garbage) CHECK(items <= paged_max_tiles(p, BM) + (p.divide ? target : 0));
             if (cost > 0) {
                 const long long total = cost * H_kv;
-                const int n = (int)(total < kPagedTarget ? total : kPagedTarget);
-                CHECK(share_begin(total, 0, n) == 0 && share_begin(total, n, n) == total);
+                const int n = (int)(total < target ? total : target), l2 = p.target_log2;
+                CHECK(share_begin(total, 0, n, l2) == 0 && share_begin(total, n, n, l2) == total);
                 for (int w = 0; w < n; ++w) {
-                    const long long a = share_begin(total, w, n), b = share_begin(total, w + 1, n);
+                    const long long a = share_begin(total, w, n, l2), b = share_begin(total, w + 1, n, l2);
                     CHECK(b - a >= total / n && b - a <= total / n + 1);
-                    CHECK(share_owner(total, a, n) == w && share_owner(total, b - 1, n) == w);
+                    CHECK(share_owner(total, a, n, l2) == w && share_owner(total, b - 1, n, l2) == w);
                 }
             }
             if (cs % 50 == 0) {

@@ -11,11 +11,11 @@
 //   parts   The cost of a tile is the number of key blocks it walks on
 //           average; the keys of a tile are divided into parts of at most `chunk`
 //           blocks, chunk being the larger of min_chunk and the whole cost over
-//           `target` workgroups.  So at most target workgroups more than there
+//           target = 2^target_log2 workgroups.  So at most target workgroups more than there
 //           are tiles have work, whatever the lengths, and at most 2 target parts
 //           are of divided tiles.
 //   shares  The key blocks of all tiles, one tile after the other, are cut into
-//           equal shares, one for each of `target` workgroups, which walks the
+//           equal shares, one for each of target workgroups, which walks the
 //           tiles that its share meets.  It leaves at most two partial tiles: slot
 //           2 w holds one that began before its share, 2 w + 1 one that it begins
 //           and does not end.  For generation, where a workgroup's time is the
@@ -39,8 +39,9 @@ struct PagedParams {
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
-    int target;     // workgroups to divide for (parts: 0 where nothing is divided)
-    int min_chunk;  // parts: key blocks of a part, at least
+    int target_log2;  // workgroups to divide for: 2^target_log2
+    int divide;       // parts: whether tiles may be divided
+    int min_chunk;    // parts: key blocks of a part, at least
 };
 
 // Key blocks of 64 of a part, at least.  fp16, 300 tokens over 2300, 16 heads on 4, D
@@ -58,7 +59,7 @@ struct SeqPlan {
 
 // tiles = 0: nothing to do.  chunk = 0: parts are left at 1.
 __host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const PagedBatch& b, int G, bool causal, int BM,
-                                            int BN, long long chunk) {
+                                            int BN, int chunk) {
     SeqPlan s{q0, 0, 0, 0, 0, 1, false};
     if (q0 < 0 || q1 <= q0 || q1 > b.T) return s;
     const int n = q1 - q0;
@@ -71,16 +72,21 @@ __host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const Pa
     const int mean = causal ? s.len - n / 2 : s.len;
     s.blocks = mean < BN ? 1 : (mean - 1) / BN + 1;
     if (chunk > 0) {
-        const long long p = (s.blocks + chunk - 1) / chunk;
-        s.parts = (int)(p < kPagedMaxParts ? p : kPagedMaxParts);
+        const unsigned p = ((unsigned)s.blocks + (unsigned)chunk - 1) / (unsigned)chunk;
+        s.parts = p < (unsigned)kPagedMaxParts ? (int)p : kPagedMaxParts;
     }
     return s;
 }
 
-__host__ __device__ inline long long plan_chunk(long long cost, int target, int min_chunk) {
-    if (target <= 0) return 0;
-    const long long c = (cost + target - 1) / target;
-    return c < min_chunk ? min_chunk : c;
+// (Divisions of 64 bits take a microsecond here, which every workgroup would spend:
+// the number of workgroups is a power of two.)
+__host__ __device__ inline int plan_chunk(long long cost, int target_log2, int min_chunk) {
+    const long long c = (cost + (1LL << target_log2) - 1) >> target_log2;
+    return c < min_chunk ? min_chunk : (c < 0x3FFFFFFF ? (int)c : 0x3FFFFFFF);
+}
+// a / b for 0 <= a, 0 < b
+__host__ __device__ inline int div_small(long long a, int b) {
+    return a <= 0xFFFFFFFFLL ? (int)((unsigned)a / (unsigned)b) : (int)(a / b);
 }
 
 // Tiles of a launch, at most: every sequence with rows ends in one that is not full.
@@ -93,24 +99,29 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
 // kernels of such tiles, by shares; others, by parts, those of 128-row tiles.
 constexpr int kPagedSmallRows = 32;
 
-// Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)).
-__host__ __device__ inline long long share_begin(long long total, int w, int n) {
-    return total / n * w + (total % n) * w / n;
+// Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)); n
+// is total itself or a power of two, 2^n_log2, below it.
+__host__ __device__ inline long long share_begin(long long total, int w, int n, int n_log2) {
+    return n == total ? w : (total * w) >> n_log2;
 }
 // The workgroup whose share holds block u: the largest w with total w / n < u + 1.
-__host__ __device__ inline int share_owner(long long total, long long u, int n) {
-    return (int)(((u + 1) * n - 1) / total);
+__host__ __device__ inline int share_owner(long long total, long long u, int n, int n_log2) {
+    if (n == total) return (int)u;
+    int w = (int)((double)u * n / (double)total);  // right or off by one
+    if (share_begin(total, w, n, n_log2) > u) --w;
+    else if (share_begin(total, w + 1, n, n_log2) <= u) ++w;
+    return w;
 }
 
 // Workgroups the launches divide for, and the workspace of one launch's parts.
-constexpr int kPagedTarget = 512;
+constexpr int kPagedTargetLog2 = 9;
 constexpr int kPagedSmallBM = 32, kPagedBM = 128;
 inline bool paged_small(long long T, int G, int max_q_len) {
     const long long most = max_q_len > 0 && max_q_len < T ? max_q_len : T;
     return most * G <= kPagedSmallRows;
 }
 inline size_t paged_part_bytes(int D_v, int BM) {
-    return 2 * (size_t)kPagedTarget * BM * ((size_t)D_v + 2) * sizeof(float);
+    return ((size_t)2 << kPagedTargetLog2) * BM * ((size_t)D_v + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);

@@ -296,10 +296,10 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     const bool small = sdpa::paged_small(T, p.G, max_q_len);
     if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
-    p.target = sdpa::kPagedTarget;
+    p.target_log2 = sdpa::kPagedTargetLog2;
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + 2 * (size_t)p.target * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
+        p.part_ml = p.part_o + ((size_t)2 << p.target_log2) * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
     }
     if (dtype == SDPA_DTYPE_F32)
         return hip_status(small ? sdpa::launch_paged_f32_small(p, stream) : sdpa::launch_paged_f32(p, stream));

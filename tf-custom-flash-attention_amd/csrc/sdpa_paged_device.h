@@ -76,7 +76,7 @@ template <int BM, int BN, bool MERGE = false>
 struct PagedPlan {
     const PagedParams& p;
     const int lane;
-    long long chunk = 0;
+    int chunk = 0;
     // of sequence n0 + lane: q_starts, kv_lens; the items and slots up to it
     int q0, q1, len, end, slot;
     int items = 0;  // in all
@@ -104,14 +104,14 @@ struct PagedPlan {
     }
     __device__ __forceinline__ PagedPlan(const PagedParams& p_) : p(p_), lane(threadIdx.x & 63) {
         read(0);
-        if (p.target > 0) {
+        if (p.divide) {
             long long cost = 0;
             for (int n0 = 0; n0 < p.batch.N; n0 += 64) {
                 if (n0 > 0) read(n0);
                 const SeqPlan s = seq();
                 cost += (long long)s.tiles * s.blocks;
             }
-            chunk = plan_chunk(readlane64(wave_scan(cost), 63) * p.H_kv, p.target, p.min_chunk);
+            chunk = plan_chunk(readlane64(wave_scan(cost), 63) * p.H_kv, p.target_log2, p.min_chunk);
             if (p.batch.N > 64) read(0);
         }
         scan(0, 0);
@@ -193,7 +193,7 @@ struct PagedShares {
             total = readlane64(x.last, 63);
             if (p.batch.N <= 64) kept[threadIdx.x & 63] = x;
         }
-        n = (int)(total < p.target ? total : p.target);
+        n = (int)(total < (1LL << p.target_log2) ? total : 1LL << p.target_log2);
     }
     // The tile that holds block `at` < total, and its first block.
     __device__ __forceinline__ long long tile(long long at, PagedItem& it) const {
@@ -208,7 +208,7 @@ struct PagedShares {
             it.s = SeqPlan{get(x.s.q0), get(x.s.n), get(x.s.len), get(x.s.tiles), get(x.s.blocks), 1, get(x.s.bad) != 0};
             it.seq = n0 + l;
             const long long begin = readlane64(x.first, l);
-            const int t = (int)((at - begin) / it.s.blocks);
+            const int t = div_small(at - begin, it.s.blocks);
             it.h = t / it.s.tiles;
             it.tile = t - it.h * it.s.tiles;
             return begin + (long long)t * it.s.blocks;
@@ -220,8 +220,8 @@ struct PagedShares {
     template <typename F>
     __device__ __forceinline__ void each(int w, F&& work) const {
         if (w >= n) return;
-        const long long end = share_begin(total, w + 1, n);
-        for (long long at = share_begin(total, w, n); at < end;) {
+        const long long end = share_begin(total, w + 1, n, p.target_log2);
+        for (long long at = share_begin(total, w, n, p.target_log2); at < end;) {
             PagedItem it;
             const long long t0 = tile(at, it), t1 = t0 + it.s.blocks;
             const bool divide = p.part_o != nullptr, skip = !divide && t0 != at;
@@ -240,7 +240,7 @@ struct PagedShares {
 // A divided tile's part has room in the workspace.  (It always has, but for
 // q_starts that go back and forth, whose sums may pass 32 bits.)
 __device__ __forceinline__ bool slot_ok(const PagedParams& p, const PagedItem& it) {
-    return !it.divided || (it.slot >= 0 && it.slot + it.s.parts <= 2 * p.target + it.part);
+    return !it.divided || (it.slot >= 0 && it.slot + it.s.parts <= (2 << p.target_log2) + it.part);
 }
 
 // Workgroup id -> item, XCD-major: XCD x takes the items [x n / 8, (x + 1) n / 8),
@@ -642,11 +642,11 @@ __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParam
     const PagedShares<BM, BN> plan(p, lanes);
     const int w = (int)blockIdx.x;
     if (w + 1 >= plan.n) return;
-    const long long at = share_begin(plan.total, w + 1, plan.n);
+    const long long at = share_begin(plan.total, w + 1, plan.n, p.target_log2);
     PagedItem it;
     const long long t0 = plan.tile(at, it);
-    if (t0 == at || share_owner(plan.total, t0, plan.n) != w) return;
-    const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n) - w + 1;
+    if (t0 == at || share_owner(plan.total, t0, plan.n, p.target_log2) != w) return;
+    const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n, p.target_log2) - w + 1;
     const int rows = min(BM, it.s.n * p.G - it.tile * BM);
     const int group = threadIdx.x / CPR, c = 4 * (threadIdx.x % CPR);
     const auto add = [](float& M, float& L, floatx4& acc, float m, float l, const floatx4& o) {
@@ -700,7 +700,7 @@ template <typename T, int BM, int BN, int DV>
 hipError_t launch_paged_share_merge(const PagedParams& p, hipStream_t stream) {
     constexpr int DM = DV == 96 ? 128 : DV;
     const int rows = (int)(p.G < 8 ? p.G : 8);
-    return launch_kernel<paged_share_merge_kernel<T, BM, BN, DM>>(dim3((unsigned)p.target - 1, (unsigned)rows), 256, 0, stream,
+    return launch_kernel<paged_share_merge_kernel<T, BM, BN, DM>>(dim3((1u << p.target_log2) - 1, (unsigned)rows), 256, 0, stream,
                                                                  p);
 }
 
@@ -709,12 +709,13 @@ hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
     return launch_kernel<paged_merge_kernel<T, BM, BN>>(dim3(1024), 256, 0, stream, p);
 }
 
-// The arguments of a launch by parts: target 0 where nothing can be divided, for
-// want of a workspace, or as no tile walks more than min_chunk blocks.
-inline PagedParams paged_parts(const PagedParams& p, int BN) {
+// The arguments of a launch by parts, for so many workgroups a CU: nothing is divided
+// for want of a workspace, or where no tile walks more than min_chunk blocks.
+inline PagedParams paged_parts(const PagedParams& p, int BN, int per_cu) {
     PagedParams a = p;
     a.min_chunk = kPagedMinChunk * 64 / BN;
-    if (!p.part_o || ((long long)p.batch.width << p.batch.page_log2) <= (long long)kPagedMinChunk * 64) a.target = 0;
+    a.target_log2 = per_cu > 1 ? kPagedTargetLog2 : kPagedTargetLog2 - 1;
+    a.divide = p.part_o && ((long long)p.batch.width << p.batch.page_log2) > (long long)kPagedMinChunk * 64;
     return a;
 }
 // Whether a launch by shares may divide a tile.

@@ -321,10 +321,10 @@ hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream) {
         return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedCfg<DQK, DV>;
-            const PagedParams a = paged_parts(p, Cfg::BN);
-            const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + a.target);
+            const PagedParams a = paged_parts(p, Cfg::BN, 2);
+            const long long n = xcd_grid(paged_max_tiles(a, Cfg::BM) + (a.divide ? 1 << a.target_log2 : 0));
             hipError_t e = launch_kernel<paged_f16_kernel<DQK, DV>>(tile_grid(n, Cfg::NT), Cfg::NT, Cfg::LDS_BYTES, stream, a);
-            return e == hipSuccess && a.target > 0 ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;
+            return e == hipSuccess && a.divide ? launch_paged_merge<half_t, Cfg::BM, Cfg::BN>(a, stream) : e;
         });
     });
 }

@@ -224,7 +224,7 @@ hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream) {
         return with_paged_dim(p.D_v, [&](auto dv) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedSmallCfg<DQK, DV>;
-            hipError_t e = launch_kernel<paged_f16_small_kernel<DQK, DV>>(dim3((unsigned)p.target), Cfg::NT, Cfg::LDS_BYTES,
+            hipError_t e = launch_kernel<paged_f16_small_kernel<DQK, DV>>(dim3(1u << p.target_log2), Cfg::NT, Cfg::LDS_BYTES,
                                                                          stream, p);
             return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
                        ? launch_paged_share_merge<half_t, Cfg::BM, Cfg::PLAN, DV>(p, stream)

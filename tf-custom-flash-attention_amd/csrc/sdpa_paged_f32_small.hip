@@ -158,8 +158,8 @@ hipError_t launch_paged_f32_small(const PagedParams& p, hipStream_t stream) {
             constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
             using Cfg = PagedF32SmallCfg<DQK, DV>;
             PagedParams a = p;
-            a.target = min(p.target, 256 * Cfg::WPE);
-            hipError_t e = launch_kernel<paged_f32_small_kernel<DQK, DV>>(dim3((unsigned)a.target), Cfg::NT, Cfg::LDS_BYTES,
+            a.target_log2 = kPagedTargetLog2 - (Cfg::WPE == 1);  // one workgroup per CU, or two
+            hipError_t e = launch_kernel<paged_f32_small_kernel<DQK, DV>>(dim3(1u << a.target_log2), Cfg::NT, Cfg::LDS_BYTES,
                                                                          stream, a);
             return e == hipSuccess && paged_shares_divide(a, Cfg::PLAN)
                        ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(a, stream)
