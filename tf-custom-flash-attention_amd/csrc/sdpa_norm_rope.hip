@@ -14,6 +14,12 @@
 // and the results be laid out [B H, S, D], as attention reads them, without a
 // pass of their own.
 //
+// Rows stay halves until the fused multiply-adds, and a weight's products with cos and
+// sin are formed once for a wave's rows: fp16 is bound by VALU work otherwise (910
+// instructions per four rows 118 us, 740 now).  4 x 4096 tokens, 32 + 32 heads of
+// 128, fp16: forward 91 us, 5.9 TB/s (a bare copy past the caches 5.95; two rows per
+// group of lanes 97 us), gradient 146, 5.5 TB/s (one row 146, four 151).
+//
 // The weight's gradient is summed in registers over the rows of a workgroup,
 // whose number is bounded (kGradBlocks), then over workgroups in order by a
 // second kernel: no atomics, a call repeats to the bit.

@@ -324,7 +324,7 @@ __device__ __forceinline__ int tile_keys(const PagedParams& p, const PagedItem& 
 // ---- rows done again ---------------------------------------------------------
 // A product of a masked weight, 0, with an infinite or NaN value is NaN, and
 // tiles are multiplied whole.  A row whose sums come out NaN, though the sum of its
-// weights is none, is therefore done again by one wave, key by key over the keys [lo, hi) it sees: finite values
+// weights is none, is therefore done again (fp16 chunks: sdpa_paged_f16.hip) by one wave, key by key over the keys [lo, hi) it sees: finite values
 // weighted, others added as they are, so that one among the row's own keys makes
 // the result infinite or NaN and one behind the mask nothing.  Lane l returns
 // columns l and l + 64 of the unnormalised sums; m in log2 units.
@@ -337,6 +337,12 @@ __device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t*
     const int lane = threadIdx.x & 63;
     CareRow r{-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}};
     const float sl2 = p.scale * kLog2e;
+    // (of a NaN query all that sees a key is NaN)
+    const bool none = (lane < p.D_qk && q[lane] != q[lane]) || (lane + 64 < p.D_qk && q[lane + 64] != q[lane + 64]);
+    if (lo < hi && __builtin_amdgcn_ballot_w64(none) != 0) {
+        r.l = __builtin_nanf("");
+        return r;
+    }
     for (int j0 = lo; j0 < hi; j0 += 64) {
         const int j = j0 + lane;
         float s = -INFINITY;
@@ -407,24 +413,32 @@ __device__ __forceinline__ void put_care_row(const PagedParams& p, const PagedIt
     if (lane == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = r.m * kLn2 + logf(r.l);
 }
 
+// Whether an accumulator of this lane holds a NaN or an infinity.
+template <int N>
+__device__ __forceinline__ bool any_nonfinite(const floatx16 (&acc)[N]) {
+    float z = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(acc[dt][r], 0.f, z);
+    return z != z;
+}
+
 // Results of a wave of 32 rows (lane l32: row; accumulator tiles over features) of a
-// kernel of 128-row tiles: to o and stats, or to the workspace; rows whose sums hold
-// a NaN or an infinity again with care (unless a score was NaN, where they are right;
-// ANY: also then, as a score may be NaN for an infinite factor's sake).  [k0, k1): this
+// kernel of 128-row tiles: to o and stats, or to the workspace.  CARE: rows whose sums
+// hold a NaN or an infinity, or whose scores do, again with care.  [k0, k1): this
 // workgroup's keys.
-template <typename T, int DV, int BM, bool ANY>
+template <typename T, int DV, int BM, bool CARE>
 __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
                                                const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
                                                const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
                                                int k1) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, in_tile = 32 * wave + l32, D_v = p.D_v;
-    float z = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DV / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(oacc[dt][r], 0.f, z);
-    const uint64_t nan_lanes = __builtin_amdgcn_ballot_w64(row.live && (ANY ? z != z || l_tot != l_tot : z != z && l_tot == l_tot));
-    const uint32_t again = bad ? 0u : (uint32_t)nan_lanes | (uint32_t)(nan_lanes >> 32);
+    uint32_t again = 0;
+    if constexpr (CARE) {
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(row.live && !bad && (l_tot != l_tot || any_nonfinite<DV / 32>(oacc)));
+        again = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    }
     if (row.live && !((again >> l32) & 1)) {
         const float m = l_tot == 0.f ? -INFINITY : m_run, l = bad ? __builtin_nanf("") : l_tot;
         const float f = it.divided ? 1.f : (l == 0.f ? 0.f : 1.f / l);
@@ -456,6 +470,7 @@ __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const Paged
                 }
             }
     }
+    if constexpr (!CARE) return;
     for (uint32_t todo = again; todo != 0; todo &= todo - 1) {
         const int r = 32 * wave + __builtin_ctz(todo);
         PagedRow rr;
@@ -573,7 +588,8 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
 
 // Merge of the divided tiles: o = sum_i O_i 2^(m_i - M) / l, stats = M ln 2 + log l.
 // A workgroup takes 32 rows of a tile at a time, a thread four columns of a row;
-// four parts' loads go out together.
+// four parts' loads go out together.  512 tokens over 16000, 32 heads, D 128 (128 tiles of
+// four parts, 34 MB): 8 us; 8 rows at a time 12, as each needs the plan's item.
 constexpr int kMergeRows = 32;
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
@@ -632,7 +648,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
 // Merge of the tiles that shares divide.  Workgroup (w, y) looks at the boundary
 // before share w + 1: it merges rows y, y + gridDim.y, ... of the tile that lies
 // across it, if the tile lies across none before.  A row's parts are dealt over
-// groups of D_v / 4 threads (a thread: four columns), whose sums meet in LDS.
+// groups of D_v / 4 threads (a thread: four columns), whose sums meet in LDS.  64 rows of
+// eight parts: 4.6 us, most of it the plan and one trip to memory.
 template <typename T, int BM, int BN, int DV>
 __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParams p) {
     constexpr int CPR = DV / 4, NG = 256 / CPR;  // (DV a power of two)

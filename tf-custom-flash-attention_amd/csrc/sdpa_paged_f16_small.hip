@@ -19,12 +19,12 @@
 //
 // Bound by memory: the cache is read once per key head, with the non-temporal
 // hint (plain loads: 6.0 TB/s where these reach 6.7; copies of 16 KB alone, in no order, 1 GB).
-// 64 sequences of 5120 tokens, 8 key heads, D 128 (1342 MB): 220 us with the
-// merge, 6.1 TB/s; of 600 to 16384 tokens (1328 MB) 232.  Two workgroups per CU
-// hide each other's ends of tiles: 512 sequences of 640 tokens 257 us, with one
-// and a two-stage ring 325 (and 4 sequences of 4096, 16 heads, 32.7 and 31.2).
-// Parts of tiles (sdpa_paged.h) instead of shares: 1328 MB in 218 to 255 us,
-// by the number of parts.
+// 64 sequences of 5120 tokens, 8 key heads, D 128 (1342 MB): 214 us with the
+// merge, 6.3 TB/s; of 600 to 16384 tokens (1328 MB) 219.  Two workgroups per CU hide
+// each other's ends of tiles: 512 sequences of 640 tokens 242 us, where one and a
+// two-stage ring took 325 against 257 (and 4 sequences of 4096, 16 heads, 31.2
+// against 32.7; 30 now).  Parts of tiles (sdpa_paged.h) instead of shares: 1328 MB in 218 to
+// 255 us, by the number of parts, against 232.
 #include "sdpa_launch.h"
 #include "sdpa_paged_device.h"
 #include "sdpa_parts.h"

