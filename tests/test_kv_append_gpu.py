@@ -1,5 +1,7 @@
 """kv_append against the definition in 64 bits (bounds: test_norm_rope_gpu.py),
 and what it must leave alone."""
+import ctypes
+
 import pytest
 import torch
 
@@ -173,3 +175,32 @@ def test_captured_append_follows_the_lengths(pkg):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(q, want) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+def test_layouts_of_the_batch(pkg):
+    """A first sequence that does not begin at the first token, a table that is part
+    of a wider one, results in the place of the queries (C entry)."""
+    page, H, D = 16, 2, 64
+    x = torch.randn((7, 3 * H, D), device=DEV).half()
+    cos, sin = (t.to(DEV) for t in R64.tables(60, D))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    table, starts, lens = i32([[9, 0, 1, 2], [9, 3, 4, 5]]), i32([2, 4, 5]), i32([34, 17])
+    kc, vc = (torch.zeros((6, H, page, D), device=DEV, dtype=F16) for _ in range(2))
+    q = pkg.kv_append(x[:, H:2 * H], x[:, 2 * H:], kc, vc, table[:, 1:], starts, lens, cos, sin, q=x[:, :H])
+    places = [(2, 0), (2, 1), (4, 0)]  # tokens 2, 3 at 32, 33 of the first; 4 at 16 of the second
+    assert (vc != 0).any(-1).any(1).nonzero().tolist() == sorted(map(list, places))
+    for t, (pg, slot) in zip((2, 3, 4), places):
+        assert torch.equal(vc[pg, :, slot], x[t, 2 * H:])
+    y = x.clone()
+    k2, v2 = torch.zeros_like(kc), torch.zeros_like(vc)
+    st = (ctypes.c_int64 * 2)(*y.stride()[:2])
+    part = [y[:, i * H:(i + 1) * H].data_ptr() for i in range(3)]
+    rc = pkg.library().sdpa_hip_kv_append(1, part[1], st, part[2], st, k2.data_ptr(), v2.data_ptr(), part[0], st, part[0], st,
+                                          None, None, 0, cos.data_ptr(), sin.data_ptr(), 60, table[:, 1:].data_ptr(), 4,
+                                          starts.data_ptr(), lens.data_ptr(), 2, 7, 3, 6, page, H, H, D, D, D, 1e-6, 0, 0,
+                                          torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.equal(k2, kc) and torch.equal(v2, vc) and torch.equal(y[2:5, :H], q[2:5])
+    y[2:5, :H] = x[2:5, :H]
+    assert torch.equal(y, x)  # other tokens, keys and values stay

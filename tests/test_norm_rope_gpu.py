@@ -7,6 +7,8 @@ product and one of the sum: together below 32 u of the size of the pair; the
 result is rounded once to T.  Gradient: dn as above (4 u of its pair), the
 mean of w dn x r again 40 u of the mean of the sizes, the rest 4 u.  The
 weight's gradient: chains below 64 additions and 28 u in each term."""
+import ctypes
+
 import pytest
 import torch
 
@@ -285,3 +287,63 @@ def test_captured_forward_and_gradient(pkg):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+def test_in_place(pkg):
+    """The C entry with the inputs as results, dense and as parts of one tensor."""
+    B, S, H, D = 2, 70, 5, 64
+    x = torch.randn((B, S, 2 * H, D), device=DEV).half()
+    cos, sin = (t.to(DEV) for t in R64.tables(S, D))
+    want = pkg.qk_norm_rope(x[:, :, :H], x[:, :, H:], cos, sin, fold_heads=False)
+    q, k = x[:, :, :H], x[:, :, H:]
+    st = (ctypes.c_int64 * 3)(*q.stride()[:3])
+    rc = pkg.library().sdpa_hip_qk_norm_rope(1, q.data_ptr(), st, k.data_ptr(), st, q.data_ptr(), st, k.data_ptr(), st, None,
+                                             None, 0, cos.data_ptr(), sin.data_ptr(), S, None, 0, B, S, H, H, D, D, 1e-6, 1,
+                                             0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.equal(x[:, :, :H], want[0]) and torch.equal(x[:, :, H:], want[1])
+
+
+def test_one_weight_and_one_side(pkg):
+    """A weight for the queries alone; keys without heads."""
+    x = torch.randn((2, 9, 6, 32), device=DEV)
+    w = torch.rand(32, device=DEV) + 0.5
+    cos, sin = (t.to(DEV) for t in R64.tables(9, 32))
+    both = pkg.qk_norm_rope(x, x, cos, sin, w, w)
+    bare = pkg.qk_norm_rope(x, x, cos, sin)
+    one = pkg.qk_norm_rope(x, x, cos, sin, w)
+    assert torch.equal(one[0], both[0]) and torch.equal(one[1], bare[1])
+    g = pkg.qk_norm_rope_grad(*both, x, x, cos, sin, w)
+    assert torch.equal(g[2], pkg.qk_norm_rope_grad(*both, x, x, cos, sin, w, w)[2]) and g[3] is None
+    q_only = pkg.qk_norm_rope(x, x[:, :, :0], cos, sin, w)
+    assert torch.equal(q_only[0], both[0]) and q_only[1].shape == (0, 9, 32)
+
+
+def test_captured_backward(pkg):
+    """Forward and backward of the autograd form in one captured graph."""
+    B, S, H, D = 2, 40, 3, 64
+    x = torch.randn((B, S, 2 * H, D), device=DEV)
+    w = torch.rand(D, device=DEV) + 0.5
+    d = torch.randn((B * H, S, D), device=DEV)
+    cos, sin = (t.to(DEV) for t in R64.tables(S, D))
+
+    def step():
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        q, k = pkg.qk_norm_rope_autograd(a[:, :, :H], a[:, :, H:], cos, sin, b, b)
+        return torch.autograd.grad((q, k), (a, b), (d, d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))

@@ -8,6 +8,8 @@ so are the sum of the weights and, twice (weight and sum), the weighted mean of 
 Sums of n weights or products add n u.  fp16 rounds the weights in the product
 with v to half precision (2^-11 of each, 2^-25 for the smallest, whose number
 is n) and the result once more."""
+import ctypes
+
 import pytest
 import torch
 
@@ -363,3 +365,73 @@ def test_serving_matches_the_dense_path(pkg, T, tol):
             got, want = o[sum(step[:s]):sum(step[:s]) + n], dense[s][done[s] - n:done[s]]
             assert float((got.double() - want.double()).abs().max()) <= tol
     assert done == [L, L]
+
+
+def test_many_shared_heads(pkg):
+    """64 query heads on one key head, 33 tokens a sequence and one."""
+    for T in (F16, F32):
+        for new, lens in (((1, 1), (300, 77)), ((33, 1), (200, 900))):
+            b = Batch(T, new, lens, 64, 1, 64, 64, 16, spread=2)
+            check(pkg.paged_sdpa(*b.args(), scale=b.scale), b.reference(True))
+
+
+@pytest.mark.parametrize("T", [F16, F32])
+@pytest.mark.parametrize("new", [(1, 2), (90, 2)])
+def test_layouts_of_the_batch(pkg, T, new):
+    """A table that is part of a wider one, a first sequence that does not begin at
+    the first token, results that are part of a wider tensor (C entry)."""
+    b = Batch(T, new, (150, 60), 4, 2, 64, 64, 16, behind=3)
+    ref = b.reference(True)
+    q, kc, vc, table, starts, lens = b.args()
+    wide = torch.full((2, table.shape[1] + 5), -3, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + table.shape[1]] = table
+    q = torch.cat([q[-2:], q[:-2]])
+    starts = starts + 2
+    n, m = len(q), sum(new)
+    out = (torch.full((n, 4, 64), 7.0, device=DEV, dtype=T), torch.full((n, 4), 7.0, device=DEV))
+    view = wide[:, 2:2 + table.shape[1]]
+    pkg.paged_sdpa(q, kc, vc, view, starts, lens, scale=b.scale, out=out)
+    check((out[0][2:2 + m], out[1][2:2 + m]), [t[:m] for t in ref])
+    for t in out:
+        assert bool((t[:2] == 7).all()) and bool((t[2 + m:] == 7).all())
+    big = torch.full((n, 6, 80), 7.0, device=DEV, dtype=T)
+    strides = (ctypes.c_int64 * 2)(big.stride(0), big.stride(1))
+    o, stats = big[:, 1:5, 8:72], torch.empty((n, 4), device=DEV)
+    rc = pkg.library().sdpa_hip_paged_fwd(
+        int(T == F16), q.data_ptr(), None, kc.data_ptr(), vc.data_ptr(), o.data_ptr(), strides, stats.data_ptr(),
+        view.data_ptr(), view.stride(0), starts.data_ptr(), lens.data_ptr(), None, 0, 2, n, view.shape[1], b.pages, 16, 4, 2,
+        64, 64, max(new), b.scale, 1, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    check((o[2:2 + m], stats[2:2 + m]), [t[:m] for t in ref])
+    o[2:2 + m] = 7
+    assert bool((big == 7).all())
+
+
+def test_calls_at_once(pkg):
+    """Calls of several batches in flight together on streams of their own."""
+    batches = [Batch(T, new, lens, 8, 2, 128, 128, 16, seed=i) for i, (T, new, lens) in enumerate((
+        (F16, (1, 1, 1), (900, 40, 3000)), (F16, (200, 3), (700, 90)), (F32, (1, 2), (1500, 33)), (F32, (140,), (600,))))]
+    refs, args = [b.reference(True) for b in batches], [b.args() for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    outs = []
+    for _ in range(4):
+        for s, a, b in zip(streams, args, batches):
+            with torch.cuda.stream(s):
+                outs.append(pkg.paged_sdpa(*a, scale=b.scale))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        check(out, refs[i % 4])
+
+
+def test_lengths_of_zero(pkg):
+    """No tokens, no keys, no sequences."""
+    b = Batch(F16, (1, 1, 1), (0, 0, 5), 4, 2, 64, 64, 16)
+    check(pkg.paged_sdpa(*b.args(), scale=b.scale), b.reference(True))
+    q, kc, vc, table, starts, lens = b.args()
+    out = (torch.full((3, 4, 64), 7.0, device=DEV, dtype=F16), torch.full((3, 4), 7.0, device=DEV))
+    pkg.paged_sdpa(q, kc, vc, table[:0], starts[:1], lens[:0], scale=b.scale, out=out)
+    assert bool((out[0] == 7).all()) and bool((out[1] == 7).all())
+    o, stats = pkg.paged_sdpa(q, kc, vc, table[:, :0], starts, lens * 0, scale=b.scale)
+    assert not o.any() and bool(torch.isneginf(stats).all())

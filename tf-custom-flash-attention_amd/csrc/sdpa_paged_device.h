@@ -213,7 +213,10 @@ struct PagedShares {
             it.tile = t - it.h * it.s.tiles;
             return begin + (long long)t * it.s.blocks;
         }
-        return at;  // (not reached)
+        // (not reached, unless the lengths change under the call: nothing, up to the share's end)
+        it.s = SeqPlan{0, 0, 0, 0, 0x7FFFFFFF, 1, false};
+        it.seq = it.h = it.tile = 0;
+        return at;
     }
     // work(item) for every tile, or part of one, of workgroup w's share.  Without a
     // workspace the tiles that begin in the share, whole.
@@ -232,7 +235,7 @@ struct PagedShares {
             it.slot = 2 * w + (it.u0 == 0 ? 1 : 0);
             it.part = 0;
             at = stop;
-            if (!skip) work(it);
+            if (!skip && it.s.n > 0) work(it);
         }
     }
 };
@@ -662,7 +665,7 @@ __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParam
     const long long at = share_begin(plan.total, w + 1, plan.n, p.target_log2);
     PagedItem it;
     const long long t0 = plan.tile(at, it);
-    if (t0 == at || share_owner(plan.total, t0, plan.n, p.target_log2) != w) return;
+    if (it.s.n == 0 || t0 == at || share_owner(plan.total, t0, plan.n, p.target_log2) != w) return;
     const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n, p.target_log2) - w + 1;
     const int rows = min(BM, it.s.n * p.G - it.tile * BM);
     const int group = threadIdx.x / CPR, c = 4 * (threadIdx.x % CPR);
