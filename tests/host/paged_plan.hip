@@ -64,7 +64,8 @@ int main() {
                 return seq_plan(starts[s], starts[s + 1], lens[s], p.batch, G, p.causal != 0, BM, BN, chunk);
             };
             for (int s = 0; s < N; ++s) cost += (long long)plan(s, 0).tiles * plan(s, 0).blocks;
-            const int chunk = p.divide ? plan_chunk(cost * H_kv, p.target_log2, kPagedMinChunk * 64 / BN) : 0;
+            const int one = pick(0, 1) ? kPagedOnePerCu : 0;
+            const int chunk = p.divide ? plan_chunk(cost * H_kv, p.target_log2, kPagedMinChunk * 64 / BN, one) : 0;
             for (int s = 0; s < N; ++s) {
                 const SeqPlan q = plan(s, chunk);
                 if (q.tiles == 0) continue;

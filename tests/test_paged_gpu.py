@@ -435,3 +435,48 @@ def test_lengths_of_zero(pkg):
     assert bool((out[0] == 7).all()) and bool((out[1] == 7).all())
     o, stats = pkg.paged_sdpa(q, kc, vc, table[:, :0], starts, lens * 0, scale=b.scale)
     assert not o.any() and bool(torch.isneginf(stats).all())
+
+
+@pytest.mark.parametrize("case", [
+    (F16, (16,), (50000,), 8, 1, 64, 64, 16, 0),      # one tile of many parts
+    (F16, (40, 1), (30000, 100), 8, 2, 96, 128, 64, 1),
+    (F16, (600,), (9000,), 8, 4, 32, 64, 128, 0),
+    (F32, (20,), (40000,), 8, 1, 64, 64, 64, 0),
+    (F32, (300, 3), (20000, 70), 4, 2, 36, 128, 16, 2),
+], ids=str)
+def test_tiles_of_many_parts(pkg, case):
+    T, new, lens, H_q, H_kv, D, D_v, page, behind = case
+    b = Batch(T, new, lens, H_q, H_kv, D, D_v, page, behind, 3)
+    args = b.args()
+    out = pkg.paged_sdpa(*args, scale=b.scale)
+    check(out, b.reference(True), slice(0, sum(new)))
+    again = pkg.paged_sdpa(*args, scale=b.scale)
+    assert all(torch.equal(x[:sum(new)], y[:sum(new)]) for x, y in zip(out, again))
+
+
+@pytest.mark.parametrize("T", [F16, F32])
+@pytest.mark.parametrize("new,lens,heads,D,page", [
+    ((4,), (5000,), 4, 128, 16), ((1, 3), (2000, 2600), 4, 96, 32), ((90,), (6000,), 4, 128, 64), ((200, 30), (900, 3000), 4, 96, 16)])
+def test_infinite_values_of_divided_tiles(pkg, T, new, lens, heads, D, page):
+    """Infinities of both signs among a row's keys, in keys of other parts than the
+    mask's edge, and NaN behind it."""
+    b = Batch(T, new, lens, heads, 1, D, D, page)
+    ref = b.reference(True)
+    m, l = new[-1], lens[-1]
+    first = sum(new) - m
+    at = m // 2
+    j = l - m + at                       # the key of token `at`
+    v = b.v[-1]
+    v[3, 0, 1], v[l // 3, 0, 2] = -INF, INF       # seen by all
+    v[5, 0, 7], v[j, 0, 7] = INF, -INF            # of both signs from token `at` on
+    v[j, 0, D - 1] = -INF
+    if at + 1 < m:
+        v[j + 1, 0, 11] = NAN
+    o, stats = (t.cpu() for t in pkg.paged_sdpa(*b.args(), scale=b.scale))
+    seq = o[first:]
+    assert bool((seq[..., 1] == -INF).all()) and bool((seq[..., 2] == INF).all())
+    assert bool((seq[:at, :, 7] == INF).all()) and bool(torch.isnan(seq[at:, :, 7]).all())
+    assert bool((seq[at:, :, D - 1] == -INF).all()) and bool(torch.isfinite(seq[:at, :, D - 1]).all())
+    assert bool(torch.isnan(seq[at + 1:, :, 11]).all()) and bool(torch.isfinite(seq[:at + 1, :, 11]).all())
+    others = [f for f in range(D) if f not in (1, 2, 7, 11, D - 1)]
+    check((o[..., others], stats), [ref[0][..., others], ref[1], ref[2][..., others], ref[3]])

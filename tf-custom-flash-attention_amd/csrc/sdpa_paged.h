@@ -10,10 +10,9 @@
 // sizes alone.  Two forms, both merged in order by a second kernel:
 //   parts   The cost of a tile is the number of key blocks it walks on
 //           average; the keys of a tile are divided into parts of at most `chunk`
-//           blocks, chunk being the larger of min_chunk and the whole cost over
-//           target = 2^target_log2 workgroups.  So at most target workgroups more than there
-//           are tiles have work, whatever the lengths, and at most 2 target parts
-//           are of divided tiles.
+//           blocks (plan_chunk), at least the whole cost over target = 2^target_log2
+//           workgroups.  So at most target workgroups more than there are tiles have
+//           work, whatever the lengths, and at most 2 target parts are of divided tiles.
 //   shares  The key blocks of all tiles, one tile after the other, are cut into
 //           equal shares, one for each of target workgroups, which walks the
 //           tiles that its share meets.  It leaves at most two partial tiles: slot
@@ -39,16 +38,23 @@ struct PagedParams {
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
+    int most_rows;    // rows of a sequence and key head, at most as far as is known
     int target_log2;  // workgroups to divide for: 2^target_log2
     int divide;       // parts: whether tiles may be divided
     int min_chunk;    // parts: key blocks of a part, at least
+    int one_per_cu;   // parts: chunks up to this come for half the workgroups (0: not)
 };
 
-// Key blocks of 64 of a part, at least.  fp16, 300 tokens over 2300, 16 heads on 4, D
-// 64: 2 blocks 31.2 us, 4 29.3, 6 25.7, 8 25.8, 16 27.7; over 1150: 24.8, 21.1, 21.9,
-// 23.6, 29.6.
-constexpr int kPagedMinChunk = 6;
-constexpr int kPagedMaxParts = 64;  // (the merge walks a row's parts one batch after the other)
+// Key blocks of 64 of a part, at least.  16 tokens of 8 heads on one, D 128, over 2300:
+// 4 blocks 14.9 us, 6 16.0, 8 17.9; fp32 23.4, 27.0, 31.1.
+constexpr int kPagedMinChunk = 4;
+// Where two workgroups share a CU and chunks would be shorter than this, they are up to
+// twice as long, which leaves one a CU: 300 tokens over 2300, 16 heads on 4, chunks of 4
+// blocks 28.1 us, 6 23.3; 64 over 30000, 8 heads on 4, of 6 28.7, 8 25.8.
+constexpr int kPagedOnePerCu = 8;
+// Parts of a tile.  16 tokens of 8 heads on one over 120000, one tile: 64 parts 50 us, 128
+// 36, 256 27; fp32 202, 114 and 42.
+constexpr int kPagedMaxParts = 256;
 
 // One sequence's part of the plan.
 struct SeqPlan {
@@ -80,8 +86,9 @@ __host__ __device__ inline SeqPlan seq_plan(int q0, int q1, int kv_len, const Pa
 
 // (Divisions of 64 bits take a microsecond here, which every workgroup would spend:
 // the number of workgroups is a power of two.)
-__host__ __device__ inline int plan_chunk(long long cost, int target_log2, int min_chunk) {
-    const long long c = (cost + (1LL << target_log2) - 1) >> target_log2;
+__host__ __device__ inline int plan_chunk(long long cost, int target_log2, int min_chunk, int one_per_cu = 0) {
+    long long c = (cost + (1LL << target_log2) - 1) >> target_log2;
+    if (c < one_per_cu) c = 2 * c < one_per_cu ? 2 * c : one_per_cu;
     return c < min_chunk ? min_chunk : (c < 0x3FFFFFFF ? (int)c : 0x3FFFFFFF);
 }
 // a / b for 0 <= a, 0 < b
@@ -95,9 +102,9 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
     return (rows / BM + (rows < p.batch.N ? rows : p.batch.N)) * p.H_kv;
 }
 
-// Calls whose sequences have one tile of 32 rows, as far as is known, take the
-// kernels of such tiles, by shares; others, by parts, those of 128-row tiles.
-constexpr int kPagedSmallRows = 32;
+// Calls whose sequences have up to so many rows, as far as is known, take the kernels of
+// 32-row tiles, by shares; others, by parts, those of 128-row tiles.
+constexpr int kPagedSmallRowsF16 = 32, kPagedSmallRowsF32 = 32;
 
 // Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)); n
 // is total itself or a power of two, 2^n_log2, below it.
@@ -113,12 +120,15 @@ __host__ __device__ inline int share_owner(long long total, long long u, int n, 
     return w;
 }
 
-// Workgroups the launches divide for, and the workspace of one launch's parts.
+// Rows of a sequence and key head, at most as far as is known; workgroups the launches
+// divide for, and the workspace of one launch's parts.
 constexpr int kPagedTargetLog2 = 9;
 constexpr int kPagedSmallBM = 32, kPagedBM = 128;
-inline bool paged_small(long long T, int G, int max_q_len) {
-    const long long most = max_q_len > 0 && max_q_len < T ? max_q_len : T;
-    return most * G <= kPagedSmallRows;
+inline long long paged_most_rows(long long T, int G, int max_q_len) {
+    return (max_q_len > 0 && max_q_len < T ? max_q_len : T) * G;
+}
+inline bool paged_small(bool f16, long long most_rows) {
+    return most_rows <= (f16 ? kPagedSmallRowsF16 : kPagedSmallRowsF32);
 }
 inline size_t paged_part_bytes(int D_v, int BM) {
     return ((size_t)2 << kPagedTargetLog2) * BM * ((size_t)D_v + 2) * sizeof(float);

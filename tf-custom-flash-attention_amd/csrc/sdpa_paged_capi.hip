@@ -255,7 +255,7 @@ size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, in
                                           int D_qk, int D_v, int max_q_len) {
     if (check_paged(dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
         return 0;
-    return paged_workspace(sdpa::paged_small(T, H_q / H_kv, max_q_len), width, page_size, D_v);
+    return paged_workspace(sdpa::paged_small(dtype == SDPA_DTYPE_F16, sdpa::paged_most_rows(T, H_q / H_kv, max_q_len)), width, page_size, D_v);
 }
 
 int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -293,7 +293,8 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     p.causal = causal_mask != 0;
     if ((long long)T * p.G > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     // sequences of few rows, as far as is known here (either kernel takes any)
-    const bool small = sdpa::paged_small(T, p.G, max_q_len);
+    p.most_rows = (int)sdpa::paged_most_rows(T, p.G, max_q_len);
+    const bool small = sdpa::paged_small(dtype == SDPA_DTYPE_F16, p.most_rows);
     if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
     p.target_log2 = sdpa::kPagedTargetLog2;

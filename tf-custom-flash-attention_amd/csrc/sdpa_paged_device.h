@@ -3,6 +3,8 @@
 // again with care, and the merge of divided tiles.
 #pragma once
 
+#include <algorithm>
+
 #include "sdpa_dma.h"
 #include "sdpa_launch.h"
 #include "sdpa_paged.h"
@@ -111,7 +113,8 @@ struct PagedPlan {
                 const SeqPlan s = seq();
                 cost += (long long)s.tiles * s.blocks;
             }
-            chunk = plan_chunk(readlane64(wave_scan(cost), 63) * p.H_kv, p.target_log2, p.min_chunk);
+            chunk = plan_chunk(readlane64(wave_scan(cost), 63) * p.H_kv, p.target_log2, p.min_chunk,
+                               p.one_per_cu);
             if (p.batch.N > 64) read(0);
         }
         scan(0, 0);
@@ -589,75 +592,124 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
     }
 }
 
-// Merge of the divided tiles: o = sum_i O_i 2^(m_i - M) / l, stats = M ln 2 + log l.
-// A workgroup takes 32 rows of a tile at a time, a thread four columns of a row;
-// four parts' loads go out together.  512 tokens over 16000, 32 heads, D 128 (128 tiles of
-// four parts, 34 MB): 8 us; 8 rows at a time 12, as each needs the plan's item.
-constexpr int kMergeRows = 32;
+// The sums of a row's parts, four columns of them, as they come:
+// o = sum_i O_i 2^(m_i - M) / L, stats = M ln 2 + log L.
+struct MergedRow {
+    float M = -INFINITY, L = 0.f;
+    floatx4 acc = floatx4{};
+    __device__ __forceinline__ void add(float m, float l, const floatx4& o) {
+        const float Mn = fmaxf(M, m), a = M == Mn ? 1.f : part_weight(M, Mn), b = part_weight(m, Mn);
+        // (a NaN sum has no maximum to weigh it by)
+        L = l == l ? __builtin_fmaf(l, b, L * a) : l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = add_part(add_part(0.f, acc[e], a), o[e], b);
+        M = Mn;
+    }
+    // columns c .. c + 3 of row r of a tile
+    template <typename T, int BM>
+    __device__ __forceinline__ void put(const PagedParams& p, const PagedItem& it, int r, int c) const {
+        PagedRow row;
+        row.init(p, it, it.tile * BM + r);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
+        *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
+        if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
+    }
+};
+
+// One row of a tile by a workgroup of 256 threads: its np parts, in slots slot(k), are
+// dealt over groups of D_v / 4 threads (a thread: four columns), whose sums meet in
+// LDS; four parts' loads go out together.
+struct MergeLds {
+    floatx4 sum[256];
+    floatx2 ml[256];
+};
+template <typename T, int BM, typename F>
+__device__ __forceinline__ void merge_row(const PagedParams& p, const PagedItem& it, int r, int np, MergeLds& lds, F&& slot) {
+    const int tid = threadIdx.x, cpr = p.D_v / 4, groups = 256 / cpr, group = tid / cpr, c = 4 * (tid - group * cpr);
+    MergedRow x;
+    constexpr int U = 4;
+    if (group < groups)
+        for (int k0 = group; k0 < np; k0 += U * groups) {
+            floatx2 ml[U];
+            floatx4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t row = (size_t)slot(min(k0 + u * groups, np - 1)) * BM + r;
+                ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * row);
+                o[u] = *reinterpret_cast<const floatx4*>(p.part_o + row * p.D_v + c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (k0 + u * groups < np) x.add(ml[u][0], ml[u][1], o[u]);
+        }
+    __syncthreads();  // (the row before has been read)
+    lds.sum[tid] = x.acc;
+    lds.ml[tid] = (floatx2){x.M, x.L};
+    __syncthreads();
+    if (group != 0) return;
+    for (int g = 1; g < min(groups, np); ++g) x.add(lds.ml[g * cpr + tid][0], lds.ml[g * cpr + tid][1], lds.sum[g * cpr + tid]);
+    x.put<T, BM>(p, it, r, c);
+}
+
+// Merge of the tiles that parts divide.  Many tiles: a workgroup takes 32 rows of a
+// tile at a time, a thread four columns of a row; 128 tiles of four parts (512 tokens over
+// 16000, 32 heads, D 128, 34 MB): 8 us.  Few tiles, which have many parts: a workgroup a
+// row (merge_row).  The whole call of 16 tokens, 16 heads on 4, over 30000 (4 tiles): 106
+// us by 32 rows, 26 by one; 128 tokens over 16000, 32 on 8 (32 tiles): 70 and 66; 256 (64
+// tiles): 95 and 107.
+constexpr int kMergeRows = 32, kMergeRowTiles = 32;
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
+    __shared__ MergeLds lds;
     PagedPlan<BM, BN, true> plan(p);
-    const int units = plan.items * (BM / kMergeRows), cpr = p.D_v / 4;
-    constexpr int U = 4;
+    const bool by_row = plan.items <= kMergeRowTiles;
+    const int per_tile = by_row ? BM : BM / kMergeRows;
+    const int units = plan.items * per_tile, cpr = p.D_v / 4;
     for (int unit = (int)blockIdx.x; unit < units; unit += (int)gridDim.x) {
         PagedItem it;
-        if (!plan.find(unit / (BM / kMergeRows), it) || !slot_ok(p, it)) return;
-        const int np = it.s.parts, row0 = unit % (BM / kMergeRows) * kMergeRows;
-        const int rows = min(kMergeRows, it.s.n * p.G - it.tile * BM - row0);
+        if (!plan.find(unit / per_tile, it) || !slot_ok(p, it)) return;
+        const int np = it.s.parts, row0 = unit % per_tile * (BM / per_tile);
+        const int rows = min(BM / per_tile, it.s.n * p.G - it.tile * BM - row0);
+        if (by_row) {
+            if (rows > 0) merge_row<T, BM>(p, it, row0, np, lds, [&](int k) { return it.slot + k; });
+            continue;
+        }
         for (int i = threadIdx.x; i < rows * cpr; i += 256) {
             const int r = row0 + i / cpr, c = 4 * (i % cpr);
-            float M = -INFINITY, L = 0.f;
-            floatx4 acc = floatx4{};
+            constexpr int U = 4;
+            MergedRow x;
             for (int k0 = 0; k0 < np; k0 += U) {
                 floatx2 ml[U];
                 floatx4 o[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const size_t at = (size_t)(it.slot + (k0 + u < np ? k0 + u : np - 1)) * BM + r;
+                    const size_t at = (size_t)(it.slot + min(k0 + u, np - 1)) * BM + r;
                     ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * at);
                     o[u] = *reinterpret_cast<const floatx4*>(p.part_o + at * p.D_v + c);
                 }
-                float Mn = M;
 #pragma unroll
-                for (int u = 0; u < U; ++u) Mn = fmaxf(Mn, ml[u][0]);
-                const float a = M == Mn ? 1.f : part_weight(M, Mn);
-                L *= a;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = add_part(0.f, acc[e], a);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (k0 + u >= np) break;
-                    const float w = part_weight(ml[u][0], Mn);
-                    // (a NaN sum has no maximum to weigh it by)
-                    L = ml[u][1] == ml[u][1] ? __builtin_fmaf(ml[u][1], w, L) : ml[u][1];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = add_part(acc[e], o[u][e], w);
-                }
-                M = Mn;
+                for (int u = 0; u < U; ++u)
+                    if (k0 + u < np) x.add(ml[u][0], ml[u][1], o[u]);
             }
-            PagedRow row;
-            row.init(p, it, it.tile * BM + r);
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            typedef T t4 __attribute__((ext_vector_type(4)));
-            t4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
-            *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
-            if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
+            x.put<T, BM>(p, it, r, c);
         }
     }
 }
 
 // Merge of the tiles that shares divide.  Workgroup (w, y) looks at the boundary
 // before share w + 1: it merges rows y, y + gridDim.y, ... of the tile that lies
-// across it, if the tile lies across none before.  A row's parts are dealt over
-// groups of D_v / 4 threads (a thread: four columns), whose sums meet in LDS.  64 rows of
-// eight parts: 4.6 us, most of it the plan and one trip to memory.
-template <typename T, int BM, int BN, int DV>
+// across it, if the tile lies across none before.  64 rows of eight parts: 4.6 us, most
+// of it the plan and one trip to memory.  Rows y at most (the whole call of 8 tokens, 16 heads
+// on 4, D 128, for 32 sequences of 4096 and for 4 of 2000): 4 69 and 34 us, 8 63 and 25.6,
+// 16 66 and 23.9, 32 75 and 28.5, as workgroups without rows form the plan too.
+constexpr int kShareMergeRows = 8;
+template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParams p) {
-    constexpr int CPR = DV / 4, NG = 256 / CPR;  // (DV a power of two)
-    __shared__ floatx4 sum[256];
-    __shared__ floatx2 sml[256];
+    __shared__ MergeLds lds;
     __shared__ typename PagedShares<BM, BN>::Lane lanes[64];
     const PagedShares<BM, BN> plan(p, lanes);
     const int w = (int)blockIdx.x;
@@ -668,60 +720,14 @@ __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParam
     if (it.s.n == 0 || t0 == at || share_owner(plan.total, t0, plan.n, p.target_log2) != w) return;
     const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n, p.target_log2) - w + 1;
     const int rows = min(BM, it.s.n * p.G - it.tile * BM);
-    const int group = threadIdx.x / CPR, c = 4 * (threadIdx.x % CPR);
-    const auto add = [](float& M, float& L, floatx4& acc, float m, float l, const floatx4& o) {
-        const float Mn = fmaxf(M, m), a = M == Mn ? 1.f : part_weight(M, Mn), b = part_weight(m, Mn);
-        // (a NaN sum has no maximum to weigh it by)
-        L = l == l ? __builtin_fmaf(l, b, L * a) : l;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = add_part(add_part(0.f, acc[e], a), o[e], b);
-        M = Mn;
-    };
-    for (int r = (int)blockIdx.y; r < rows; r += (int)gridDim.y) {
-        float M = -INFINITY, L = 0.f;
-        floatx4 acc = floatx4{};
-        constexpr int U = 4;
-        for (int k0 = group; k0 < np; k0 += U * NG) {
-            floatx2 ml[U];
-            floatx4 o[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = min(k0 + u * NG, np - 1);
-                const size_t row = (size_t)(k == 0 ? 2 * w + 1 : 2 * (w + k)) * BM + r;
-                ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * row);
-                o[u] = floatx4{};
-                if (c < p.D_v) o[u] = *reinterpret_cast<const floatx4*>(p.part_o + row * p.D_v + c);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (k0 + u * NG < np) add(M, L, acc, ml[u][0], ml[u][1], o[u]);
-        }
-        __syncthreads();  // (the row before has been read)
-        sum[threadIdx.x] = acc;
-        sml[threadIdx.x] = (floatx2){M, L};
-        __syncthreads();
-        if (group == 0 && c < p.D_v) {
-            for (int g = 1; g < min(NG, np); ++g)
-                add(M, L, acc, sml[g * CPR + threadIdx.x][0], sml[g * CPR + threadIdx.x][1], sum[g * CPR + threadIdx.x]);
-            PagedRow row;
-            row.init(p, it, it.tile * BM + r);
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            typedef T t4 __attribute__((ext_vector_type(4)));
-            t4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
-            *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
-            if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
-        }
-    }
+    for (int r = (int)blockIdx.y; r < rows; r += (int)gridDim.y)
+        merge_row<T, BM>(p, it, r, np, lds, [&](int k) { return k == 0 ? 2 * w + 1 : 2 * (w + k); });
 }
 
-template <typename T, int BM, int BN, int DV>
+template <typename T, int BM, int BN>
 hipError_t launch_paged_share_merge(const PagedParams& p, hipStream_t stream) {
-    constexpr int DM = DV == 96 ? 128 : DV;
-    const int rows = (int)(p.G < 8 ? p.G : 8);
-    return launch_kernel<paged_share_merge_kernel<T, BM, BN, DM>>(dim3((1u << p.target_log2) - 1, (unsigned)rows), 256, 0, stream,
-                                                                 p);
+    return launch_kernel<paged_share_merge_kernel<T, BM, BN>>(dim3((1u << p.target_log2) - 1, (unsigned)std::min(p.most_rows, kShareMergeRows)),
+                                                             256, 0, stream, p);
 }
 
 template <typename T, int BM, int BN>
@@ -734,6 +740,7 @@ hipError_t launch_paged_merge(const PagedParams& p, hipStream_t stream) {
 inline PagedParams paged_parts(const PagedParams& p, int BN, int per_cu) {
     PagedParams a = p;
     a.min_chunk = kPagedMinChunk * 64 / BN;
+    a.one_per_cu = per_cu > 1 ? kPagedOnePerCu : 0;
     a.target_log2 = per_cu > 1 ? kPagedTargetLog2 : kPagedTargetLog2 - 1;
     a.divide = p.part_o && ((long long)p.batch.width << p.batch.page_log2) > (long long)kPagedMinChunk * 64;
     return a;

@@ -227,7 +227,7 @@ hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream) {
             hipError_t e = launch_kernel<paged_f16_small_kernel<DQK, DV>>(dim3(1u << p.target_log2), Cfg::NT, Cfg::LDS_BYTES,
                                                                          stream, p);
             return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
-                       ? launch_paged_share_merge<half_t, Cfg::BM, Cfg::PLAN, DV>(p, stream)
+                       ? launch_paged_share_merge<half_t, Cfg::BM, Cfg::PLAN>(p, stream)
                        : e;
         });
     });

@@ -165,7 +165,7 @@ hipError_t launch_paged_f32_small(const PagedParams& p, hipStream_t stream) {
             hipError_t e = launch_kernel<paged_f32_small_kernel<DQK, DV>>(dim3(1u << a.target_log2), Cfg::NT, Cfg::LDS_BYTES,
                                                                          stream, a);
             return e == hipSuccess && paged_shares_divide(a, Cfg::PLAN)
-                       ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN, DV>(a, stream)
+                       ? launch_paged_share_merge<float, Cfg::BM, Cfg::PLAN>(a, stream)
                        : e;
         });
     });
