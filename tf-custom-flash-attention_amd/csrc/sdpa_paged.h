@@ -103,8 +103,14 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
 }
 
 // Calls whose sequences have up to so many rows, as far as is known, take the kernels of
-// 32-row tiles, by shares; others, by parts, those of 128-row tiles.
-constexpr int kPagedSmallRowsF16 = 32, kPagedSmallRowsF32 = 32;
+// 32-row tiles, by shares; others, by parts, those of 128-row tiles.  us by 32-row and by
+// 128-row tiles, D 128:
+//   fp16, 16 rows: 64 sequences of 600 to 16384, 4 key heads 131, 161; 64 of 5120 124, 132;
+//         4 of 2000 19, 22; 32 of 4096 58, 53; 256 of 500 67, 61; one of 30000 36, 24
+//   fp16, 32 rows: 146, 168; 129, 137; 26, 22; 63, 58; 73, 62; 51, 25
+//   fp32, 32 rows: 32 of 4096 126, 215; 4 of 2000 31, 52; one of 30000 62, 64 (D 64: 73,
+//         91; 28, 30; 49, 37); 64 rows, 4 of 2000 37, 53; 32 of 4096 214, 220; one 73, 65
+constexpr int kPagedSmallRowsF16 = 16, kPagedSmallRowsF32 = 32;
 
 // Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)); n
 // is total itself or a power of two, 2^n_log2, below it.
