@@ -250,7 +250,8 @@ int sdpa_hip_qk_norm_rope(int dtype, const void* q, const int64_t* q_strides, co
 /* Its gradient: d_q_out and d_k_out as the results were laid out, dq and dk
  * as their strides say, dq_weight and dk_weight [D] of weight_dtype (NULL: not
  * wanted; they need no weight in the forward call).  The weights' gradients are
- * summed in fp32 in a fixed order from the workspace,
+ * summed in a fixed order, in fp32 over the rows of a workgroup and in fp64 over
+ * the workgroups' sums in the workspace,
  * sdpa_hip_qk_norm_rope_grad_workspace_bytes(D) bytes, 16-byte aligned; without
  * them it may be NULL.                                                        */
 size_t sdpa_hip_qk_norm_rope_grad_workspace_bytes(int D);

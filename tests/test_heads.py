@@ -175,3 +175,31 @@ def test_paged_abi_refusals(pkg):
     need = lambda **k: L.sdpa_hip_paged_fwd_workspace_bytes(*dict(dict(dtype=1, N=3, T=6, width=400, page=16, H_q=4, H_kv=2,
                                                                        D=32, D_v=16, most=1), **k).values())
     assert need() > 0 and need(width=1) == 0 and need(H_q=3) == 0 and need(N=0) == 0
+
+
+def test_sizes_that_pass_64_bits(pkg):
+    """Products of sizes are not formed where they would wrap around."""
+    L, some, most = pkg.library(), ctypes.c_void_p(64), 0x7FFFFFFF
+    rope = lambda B, S, H_q, H_kv: L.sdpa_hip_qk_norm_rope(
+        1, some, None, some, None, some, None, some, None, None, None, 0, some, some, 8, None, 0, B, S, H_q, H_kv, 64, 64,
+        1e-6, 1, 0, None)
+    append = lambda T, H_q, H_kv, N=3: L.sdpa_hip_kv_append(
+        1, some, None, some, None, some, some, some, None, some, None, None, None, 0, some, some, 8, some, 4, some, some,
+        N, T, 4, 9, 16, H_q, H_kv, 64, 64, 64, 1e-6, 0, 0, None)
+    for sizes in ((most, 1, most, most), (1, 1, most, most), (2, 1, most, 1), (most, most, 1, 0)):
+        assert rope(*sizes) == 30, sizes
+    for sizes in ((most, most, most), (1, most, most), (3, 1, most), (1, 0, most)):
+        assert append(*sizes) == 30, sizes
+    assert append(1, 1, 1, N=most) == 30
+    assert L.sdpa_hip_paged_fwd(1, some, None, some, some, some, None, some, some, 4, some, some, None, 0, most, 6, 4, 9, 16,
+                                4, 2, 32, 16, 0, 0.5, 1, None) == 30
+
+
+def test_spans_of_memory():
+    from importlib import import_module
+    share = import_module("tf-custom-flash-attention_amd.heads")._share_memory
+    x = torch.empty((4, 6, 8))
+    a, b = x[:2], x[2:]
+    assert share(a, a) and share(a, x) and share(x, b) and not share(a, b) and not share(b, a)
+    assert share(b, x[:, 1]) and not share(a, x[2:, ::2]) and share(b, x[1:3, ::2])
+    assert not share(x[:0], x) and not share(x, torch.empty((4,)))

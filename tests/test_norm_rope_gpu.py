@@ -347,3 +347,12 @@ def test_captured_backward(pkg):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_gradient_of_a_gradient_is_refused(pkg):
+    x = torch.randn((1, 3, 2, 32), device=DEV, requires_grad=True)
+    cos, sin = (t.to(DEV) for t in R64.tables(3, 32))
+    q, k = pkg.qk_norm_rope_autograd(x, x, cos, sin)
+    (g,) = torch.autograd.grad((q * q).sum() + k.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()

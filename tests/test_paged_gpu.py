@@ -480,3 +480,22 @@ def test_infinite_values_of_divided_tiles(pkg, T, new, lens, heads, D, page):
     assert bool(torch.isnan(seq[at + 1:, :, 11]).all()) and bool(torch.isfinite(seq[:at + 1, :, 11]).all())
     others = [f for f in range(D) if f not in (1, 2, 7, 11, D - 1)]
     check((o[..., others], stats), [ref[0][..., others], ref[1], ref[2][..., others], ref[3]])
+
+
+def test_out_that_shares_memory(pkg):
+    b = Batch(F16, (3, 1), (40, 9), 4, 2, 64, 64, 16)
+    q, kc, vc, *batch = b.args()
+    n = len(q)
+    room = torch.zeros((3 * n, 4, 64), device=DEV, dtype=F16)
+    stats = torch.empty((n, 4), device=DEV)
+    x = room[:n].copy_(q)
+    new = lambda o, s=stats: pkg.paged_sdpa(x, kc, vc, *batch, scale=b.scale, out=(o, s))
+    for bad in (x, room[1:n + 1]):
+        with pytest.raises(pkg.InvalidArgumentError, match="share memory with q"):
+            new(bad)
+    with pytest.raises(pkg.InvalidArgumentError, match="share memory with v_cache"):
+        new(vc.view(-1, 64)[:4 * n].view(n, 4, 64))
+    o = room[n:2 * n]
+    with pytest.raises(pkg.InvalidArgumentError, match="tensors of out"):
+        new(o, o.view(torch.float32).view(-1)[:4 * n].view(n, 4))
+    check(new(o), b.reference(True))

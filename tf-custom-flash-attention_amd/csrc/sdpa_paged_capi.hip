@@ -24,6 +24,9 @@ struct Chunks {
     void rotated(int R, int interleaved) { ok = ok && (interleaved ? R : R / 2) % epc == 0; }
 };
 
+// a (b + c), of sizes, fits into an int
+bool rows_fit(long long a, long long b, long long c) { return a == 0 || b + c <= 0x7FFFFFFFLL / a; }
+
 int check_rows(int dtype, int weight_dtype, const void* w0, const void* w1, const float* cos, const float* sin,
                int table_rows, int D, int R, int norm) {
     if (dtype != SDPA_DTYPE_F32 && dtype != SDPA_DTYPE_F16) return SDPA_ERR_DTYPE;
@@ -59,7 +62,7 @@ int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64
     int st = check_rows(dtype, weight_dtype, any_dw ? (dw[0] ? dw[0] : dw[1]) : w[0], w[1] ? w[1] : w[0], cos, sin,
                         table_rows, D, R, norm);
     if (st != SDPA_OK) return st;
-    if ((long long)B * S > 0x7FFFFFFFLL || (long long)B * S * (H_q + H_kv) > 0x7FFFFFFFLL) return SDPA_ERR_TOO_LARGE;
+    if (!rows_fit(B, S, 0) || !rows_fit((long long)B * S, H_q, H_kv)) return SDPA_ERR_TOO_LARGE;
     if (D == 0) return SDPA_OK;
     const bool rows = B > 0 && S > 0;
     sdpa::NormRopeParams p{};
@@ -113,8 +116,8 @@ int make_batch(sdpa::PagedBatch& b, const int32_t* page_table, int64_t page_tabl
                const int32_t* kv_lens, int N, int T, int width, int pages, int page_size) {
     if (N < 0 || T < 0 || width < 0 || pages < 0) return SDPA_ERR_NEGATIVE_DIM;
     if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)) != 0) return SDPA_ERR_PAGE_SIZE;
-    // token numbers of a sequence stay below 2^31
-    if ((long long)width * page_size > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
+    // token numbers of a sequence, and those of sequences a wave ahead, stay below 2^31
+    if (N > 0x7FFFFFFF - 65536 || (long long)width * page_size > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     if (N > 0 && T > 0 && (!q_starts || !kv_lens || (width > 0 && !page_table))) return SDPA_ERR_NULL_POINTER;
     int l2 = 4;
     while ((1 << l2) < page_size) ++l2;
@@ -182,7 +185,7 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     sdpa::AppendParams p{};
     st = make_batch(p.batch, page_table, page_table_stride, q_starts, kv_lens, N, T, width, pages, page_size);
     if (st != SDPA_OK) return st;
-    if ((long long)T * ((long long)H_q + 2LL * H_kv) > 0x7FFFFFFFLL) return SDPA_ERR_TOO_LARGE;
+    if (!rows_fit(T, H_q, 2LL * H_kv)) return SDPA_ERR_TOO_LARGE;
     if (N == 0 || T == 0) return SDPA_OK;
     const bool has_k = H_kv > 0 && D_qk > 0, has_v = H_kv > 0 && D_v > 0, has_q = H_q > 0 && D_qk > 0;
     if ((has_k && (!k || (pages > 0 && !k_cache))) || (has_v && (!v || (pages > 0 && !v_cache))) ||

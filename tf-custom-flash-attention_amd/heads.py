@@ -261,6 +261,7 @@ def _make_function():
             return qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, **ctx.attrs)
 
         @staticmethod
+        @torch.autograd.function.once_differentiable
         def backward(ctx, d_q_out, d_k_out):
             dq, dk, dqw, dkw = qk_norm_rope_grad(d_q_out, d_k_out, *ctx.saved_tensors, **ctx.attrs)
             return dq, dk, None, None, dqw, dkw, None, None, None, None, None
@@ -273,7 +274,7 @@ _fn = None
 
 def qk_norm_rope_autograd(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
                           norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
-    """Differentiable ``qk_norm_rope`` (no gradient for the tables)."""
+    """Differentiable ``qk_norm_rope`` (once; no gradient for the tables)."""
     global _fn
     if _fn is None:
         _fn = _make_function()
@@ -428,6 +429,14 @@ def _whole_chunks(t):
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _share_memory(a, b):
+    """The spans of ``a`` (contiguous) and ``b`` overlap."""
+    if not a.numel() or not b.numel():
+        return False
+    end = b.data_ptr() + b.element_size() * (1 + sum((n - 1) * s for n, s in zip(b.shape, b.stride())))
+    return a.data_ptr() < end and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
 def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float = 1.0, causal_mask: bool = True,
                max_q_len=None, out=None):
     """Attention of new tokens over a paged cache that holds them already: ``(o, stats)``.
@@ -439,7 +448,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
     nothing has o = 0 and stats = -inf.  What the pages hold behind a row's last key has no influence.
 
     ``max_q_len``: the most new tokens of a sequence, where it is known (1 in generation); it chooses
-    kernels only.  ``out``: (o, stats) to write into; rows of tokens of no sequence stay as they were
+    kernels only.  ``out``: (o, stats) to write into, memory of their own; rows of tokens of no sequence stay as they were
     (in new ones they are arbitrary).  Feature sizes are multiples of 8 (fp16) or 4 (fp32), up to 128.
     """
     T = q.dtype
@@ -466,10 +475,13 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
             _fail(f"out must be ({T} {[n, H_q, D_v]}, float32 {[n, H_q]})")
         if not (o.is_contiguous() and stats.is_contiguous()):
             _fail("out must be contiguous")
-        if o.data_ptr() == q.data_ptr() and n > 0:
-            _fail("out must not be q")
         _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens,
                    o=o, stats=stats)
+        for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)):
+            if _share_memory(o, t) or _share_memory(stats, t):
+                _fail(f"out must not share memory with {name}")
+        if _share_memory(o, stats):
+            _fail("the tensors of out must not share memory")
     L = library()
     longest = 0 if max_q_len is None else int(max_q_len)
     ws_bytes = L.sdpa_hip_paged_fwd_workspace_bytes(code, N, n, width, page, H_q, H_kv, D_qk, D_v, longest)
