@@ -32,9 +32,13 @@ struct NormRopeParams {
 };
 
 // Workgroups that share a side's rows in the gradient, at most: the weight's
-// gradient has one partial sum of each.
+// gradient has one partial sum of each.  Forward and gradient of 4 x 4096 tokens, 32 +
+// 32 heads of 128, fp16: 512 268 us, 1024 259, 2048 261; 2 x 2048, 16 + 16 heads, fp32: 62,
+// 61, 67.
 constexpr int kGradBlocks = 1024;
-// Fewer waves than this of four rows per group of lanes: one row each.
+// Fewer waves than this of four rows per group of lanes: one row each.  32 + 8 heads of
+// 128, fp16: 64 tokens (128 waves of four) 3.5 us with one row, 4.5 with four; 512 (1024)
+// 4.7, 5.2; 1024 (2048) 6.7, 5.9; 2048 10.8, 9.3.
 constexpr int kRopeFewWaves = 2048;
 
 hipError_t launch_norm_rope(const NormRopeParams& p, DType dtype, hipStream_t stream);
