@@ -288,7 +288,8 @@ int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_
  * {token, head} in elements.  q_out may be q.  Tokens behind the last sequence leave
  * everything as it was; a token whose place is outside of the table's columns or
  * of the pages is not appended, and its row of q_out is NaN.  Two tokens of one
- * call must not have the same place.                                          */
+ * call must not have the same place.  D_qk or D_v may be 0: nothing of that width
+ * is read or written, and its pointers may be NULL.                           */
 int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                        void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
                        const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,

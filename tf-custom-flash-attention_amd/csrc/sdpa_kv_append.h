@@ -40,7 +40,9 @@ struct AppendParams {
     const void* k_weight;
     TokenStrides qs, qos, ks, vs;
     RopeArgs r;
-    int H_q, H_kv, D_qk, D_v;
+    int H_kv;           // heads of the caches
+    int H_q, H_k, H_v;  // heads whose rows are taken: none of those without features
+    int D_qk, D_v;
     int interleaved, w32, vec;
 };
 

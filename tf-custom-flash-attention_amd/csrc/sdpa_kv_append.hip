@@ -51,10 +51,14 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const Appe
     int kind = 0;  // 0: q, 1: k, 2: v
     if (u >= m.units) {
         u -= m.units;
-        m = append_map<LPR>(bt.T, p.H_kv);
-        kind = u < m.units ? 1 : 2;
-        if (kind == 2) u -= m.units;
-        if (u >= m.units) return;
+        m = append_map<LPR>(bt.T, p.H_k);
+        kind = 1;
+        if (u >= m.units) {
+            u -= m.units;
+            m = append_map<LPR>(bt.T, p.H_v);
+            kind = 2;
+            if (u >= m.units) return;
+        }
     }
     const unsigned uu = (unsigned)u, tg = uu / (unsigned)m.splits;
     const int group = lane / LPR, tok0 = (int)(tg * (unsigned)m.tpw), mine = group / m.gpt;
@@ -141,7 +145,8 @@ hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
     return with_append_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value;
         constexpr bool IN = decltype(in)::value;
-        const long long n = append_map<L>(p.batch.T, p.H_q).units + 2 * append_map<L>(p.batch.T, p.H_kv).units;
+        const long long n = append_map<L>(p.batch.T, p.H_q).units + append_map<L>(p.batch.T, p.H_k).units +
+                            append_map<L>(p.batch.T, p.H_v).units;
         if (n == 0) return hipSuccess;
         return launch_kernel<kv_append_kernel<T, E, L, IN>>(tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves),
                                                             64 * kAppendWaves, 0, stream, p);

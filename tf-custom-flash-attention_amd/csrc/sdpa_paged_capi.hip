@@ -206,6 +206,8 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps, D_qk > 0 ? 1.f / (float)D_qk : 0.f};
     p.H_q = has_q ? H_q : 0;
     p.H_kv = H_kv;
+    p.H_k = has_k ? H_kv : 0;
+    p.H_v = has_v ? H_kv : 0;
     p.D_qk = D_qk;
     p.D_v = D_v;
     p.interleaved = interleaved != 0;
@@ -224,8 +226,8 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
         add_tokens(ch, q, p.qs);
         add_tokens(ch, q_out, p.qos);
     }
-    add_tokens(ch, k, p.ks);
-    add_tokens(ch, v, p.vs);
+    if (has_k) add_tokens(ch, k, p.ks);
+    if (has_v) add_tokens(ch, v, p.vs);
     p.vec = ch.ok;
     return hip_status(sdpa::launch_kv_append(p, (sdpa::DType)dtype, stream));
 }

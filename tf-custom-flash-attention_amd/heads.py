@@ -391,7 +391,7 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
 
     Tokens behind the last sequence are skipped (their rows of the result are not written).  A token
     without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
-    of a call may have the same place.
+    of a call may have the same place.  D_qk or D_v may be 0 (a cache of keys or of values alone).
     """
     T, device = k.dtype, k.device
     batch = _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
