@@ -34,7 +34,7 @@ struct PagedParams {
     float* stats;         // [T, H_q] dense
     TokenStrides qs, os;
     float* part_o;   // [slot][BM][D_v]: unnormalised O of a part
-    float* part_ml;  // [slot][BM][2]: its running maximum (log2) and sum
+    float* part_ml;  // [slot][BM][2]: the reference of its weights (log2) and their sum
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;

@@ -17,6 +17,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // v_maximum
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+// Weights of the fp16 kernels are 2^(s - m), s in log2 units.  The reference m is taken 7
+// below a row's maximum, and again where the maximum has come 15 above it: weights up to
+// 2^15, the largest of a row at least 2^7, so that fp16 loses those below 2^-32 of the largest
+// (2^-25 with m at the maximum: 400000 keys of 2^-25.25 beside one of 1, a hundredth of
+// the result, vanished).
+constexpr float kTauP = 15.0f, kTopP = 7.0f;
+
 // Inclusive sum over the lanes before and up to each (DPP moves inside rows of 16
 // lanes, then the last lane of a row to the rows behind).
 template <int CTRL, int ROWS>

@@ -27,8 +27,6 @@
 namespace sdpa {
 namespace {
 
-constexpr float kTauG = 8.0f;  // lazy-rescale threshold (log2 units)
-
 template <int DQK, int DV>
 struct PagedCfg {
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedBM, BN = 64;
@@ -65,8 +63,8 @@ struct PagedTileCopy {
 };
 
 // The sums of a wave's 32 rows over the keys [k0, k1) again, where some came out NaN
-// (sdpa_paged_device.h): finite values weighted as before, relative to the final
-// maximum, then the infinite and NaN ones among each row's keys, counted by sign as
+// (sdpa_paged_device.h): finite values weighted as before, by the final
+// reference, then the infinite and NaN ones among each row's keys, counted by sign as
 // products of ones.  Operands straight from the cache; a wave by itself.  4 x 4096
 // tokens with an infinity in the first: 20 ms, where one row after the other took 208.
 template <int NKS, int NDT>
@@ -253,7 +251,7 @@ void paged_f16_kernel(const PagedParams p) {
         mx = __builtin_elementwise_maximum(mx, sc[15]);
         mx = xhalf_max(mx) * sl2;
         mxo = mx;
-        m_use = (mx > m_run + kTauG) ? mx : m_run;
+        m_use = (mx > m_run + kTauP) ? mx - kTopP : m_run;
         alpha = fast_exp2(m_run - m_use);
         const float nm = -m_use;
         uint32_t w[8];

@@ -33,8 +33,6 @@
 namespace sdpa {
 namespace {
 
-constexpr float kTauP = 8.0f;  // lazy-rescale threshold (log2 units)
-
 template <int DQK, int DV>
 struct PagedSmallCfg {
     static constexpr int NW = 4, NT = 64 * NW, BM = kPagedSmallBM, BN = 32, PLAN = BN * NW;
@@ -168,7 +166,7 @@ void paged_f16_small_kernel(const PagedParams p) {
 #pragma unroll
             for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
             mx = xhalf_max(mx) * sl2;
-            const float m_use = (mx > m_run + kTauP) ? mx : m_run;
+            const float m_use = (mx > m_run + kTauP) ? mx - kTopP : m_run;
             const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
             const float nm = m_use == -INFINITY ? 0.f : -m_use;
             float lq[4], pf[16];
