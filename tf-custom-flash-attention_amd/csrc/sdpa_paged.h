@@ -125,6 +125,30 @@ __host__ __device__ inline int share_owner(long long total, long long u, int n, 
     else if (share_begin(total, w + 1, n, n_log2) <= u) ++w;
     return w;
 }
+// The slot of part k of a tile that begins in the share of workgroup w and is cut.
+__host__ __device__ inline int share_slot(int w, int k) { return k == 0 ? 2 * w + 1 : 2 * (w + k); }
+// What workgroup w does with the tile of blocks [t0, t1) that holds block `at` of its share,
+// which ends before block `end`: blocks [u0, u1) of the tile; the walk goes on at `stop`.
+// Without `divide` the tiles that begin in the share, whole.
+struct ShareStep {
+    long long stop;
+    int u0, u1, slot;
+    bool divided, skip;
+};
+__host__ __device__ inline ShareStep share_step(long long at, long long end, long long t0, long long t1, int w,
+                                                bool divide) {
+    const long long stop = divide && end < t1 ? end : t1;
+    const int u0 = (int)(at - t0);
+    return {stop, u0, (int)(stop - t0), u0 == 0 ? share_slot(w, 0) : share_slot(w - 1, 1), u0 != 0 || stop != t1,
+            !divide && t0 != at};
+}
+// The parts that workgroup w merges: those of the tile of `blocks` blocks from t0 on, which holds
+// block `at`, the first of share w + 1, if the tile begins in share w and reaches across; else 0.
+__host__ __device__ inline int share_merge(long long total, long long at, long long t0, int blocks, int w, int n,
+                                           int n_log2) {
+    if (t0 == at || share_owner(total, t0, n, n_log2) != w) return 0;
+    return share_owner(total, t0 + blocks - 1, n, n_log2) - w + 1;
+}
 
 // Rows of a sequence and key head, at most as far as is known; workgroups the launches
 // divide for, and the workspace of one launch's parts.

@@ -237,15 +237,14 @@ struct PagedShares {
         for (long long at = share_begin(total, w, n, p.target_log2); at < end;) {
             PagedItem it;
             const long long t0 = tile(at, it), t1 = t0 + it.s.blocks;
-            const bool divide = p.part_o != nullptr, skip = !divide && t0 != at;
-            const long long stop = divide && end < t1 ? end : t1;
-            it.u0 = (int)(at - t0);
-            it.u1 = (int)(stop - t0);
-            it.divided = it.u0 != 0 || stop != t1;
-            it.slot = 2 * w + (it.u0 == 0 ? 1 : 0);
+            const ShareStep step = share_step(at, end, t0, t1, w, p.part_o != nullptr);
+            it.u0 = step.u0;
+            it.u1 = step.u1;
+            it.divided = step.divided;
+            it.slot = step.slot;
             it.part = 0;
-            at = stop;
-            if (!skip && it.s.n > 0) work(it);
+            at = step.stop;
+            if (!step.skip && it.s.n > 0) work(it);
         }
     }
 };
@@ -724,11 +723,12 @@ __global__ __launch_bounds__(256) void paged_share_merge_kernel(const PagedParam
     const long long at = share_begin(plan.total, w + 1, plan.n, p.target_log2);
     PagedItem it;
     const long long t0 = plan.tile(at, it);
-    if (it.s.n == 0 || t0 == at || share_owner(plan.total, t0, plan.n, p.target_log2) != w) return;
-    const int np = share_owner(plan.total, t0 + it.s.blocks - 1, plan.n, p.target_log2) - w + 1;
+    if (it.s.n == 0) return;
+    const int np = share_merge(plan.total, at, t0, it.s.blocks, w, plan.n, p.target_log2);
+    if (np == 0) return;
     const int rows = min(BM, it.s.n * p.G - it.tile * BM);
     for (int r = (int)blockIdx.y; r < rows; r += (int)gridDim.y)
-        merge_row<T, BM>(p, it, r, np, lds, [&](int k) { return k == 0 ? 2 * w + 1 : 2 * (w + k); });
+        merge_row<T, BM>(p, it, r, np, lds, [&](int k) { return share_slot(w, k); });
 }
 
 template <typename T, int BM, int BN>
