@@ -21,6 +21,7 @@ _Strides2 = ctypes.c_int64 * 2
 
 
 _F32, _I32 = torch.float32, torch.int32
+_MOST = 0x7FFFFFFF  # of any size: the C entries take them as int
 _CODES = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
 
 
@@ -91,8 +92,7 @@ def _tables(cos, sin):
         _fail("cos and sin must be float32")
     if cos.dim() != 2 or cos.shape != sin.shape:
         _fail("cos and sin must have one shape [positions, rotated features / 2]")
-    if cos.shape[0] > 0x7FFFFFFF:
-        _fail("too many positions in the rotation tables")
+    _sizes_fit(cos=cos)
     return cos.shape[0], 2 * cos.shape[1]
 
 
@@ -114,6 +114,12 @@ def _weight_dtype(T, D, q_weight, k_weight, norm):
     return DTYPE_F32 if code is None else code
 
 
+def _sizes_fit(**tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dim() and max(t.shape) > _MOST:
+            _fail(f"{name} {list(t.shape)} is too large for one call")
+
+
 def _check_qk(q, k):
     if q.dim() != 4 or k.dim() != 4:
         _fail("q and k must be [batch, tokens, heads, features]")
@@ -121,6 +127,7 @@ def _check_qk(q, k):
         _fail("q and k must have the same dtype T")
     if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         _fail(f"q {list(q.shape)} and k {list(k.shape)} differ in batch, tokens or features")
+    _sizes_fit(q=q, k=k)
 
 
 def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
@@ -136,7 +143,7 @@ def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
     w = q_weight
     if not (code is not None and k.dtype is T and device.type == "cuda" and k.device == device and cos.device == device
             and sin.device == device and sk[0] == B and sk[1] == S and sk[3] == D and len(sc) == 2 and sin.shape == sc
-            and cos.dtype is _F32 and sin.dtype is _F32 and sc[0] <= 0x7FFFFFFF and cos.is_contiguous()
+            and cos.dtype is _F32 and sin.dtype is _F32 and B + S + H_q + sk[2] + D + sc[0] + sc[1] <= _MOST and cos.is_contiguous()
             and sin.is_contiguous()):
         return None
     per_batch = 0
@@ -290,6 +297,7 @@ def _check_cache(k_cache, v_cache, T):
         _fail("the caches must have the same dtype T as the tokens")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         _fail("k_cache and v_cache must be contiguous")
+    _sizes_fit(k_cache=k_cache, v_cache=v_cache)
 
 
 def _check_batch(page_table, q_starts, kv_lens):
@@ -304,6 +312,7 @@ def _check_batch(page_table, q_starts, kv_lens):
         _fail("the rows of page_table must be contiguous")
     if (N > 0 and q_starts.stride(0) != 1) or (N > 1 and kv_lens.stride(0) != 1):
         _fail("q_starts and kv_lens must be contiguous")
+    _sizes_fit(page_table=page_table)
     return N, width
 
 
@@ -313,7 +322,7 @@ def _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens):
     st, sk, sv = page_table.shape, k_cache.shape, v_cache.shape
     if (device.type == "cuda" and k_cache.dtype is T and v_cache.dtype is T and k_cache.device == device
             and v_cache.device == device and len(sk) == 4 and len(sv) == 4 and sk[:3] == sv[:3]
-            and k_cache.is_contiguous() and v_cache.is_contiguous() and len(st) == 2 and page_table.dtype is _I32
+            and sum(sk) + sv[3] + sum(st) <= _MOST and k_cache.is_contiguous() and v_cache.is_contiguous() and len(st) == 2 and page_table.dtype is _I32
             and q_starts.dtype is _I32 and kv_lens.dtype is _I32 and page_table.device == device
             and q_starts.device == device and kv_lens.device == device and q_starts.shape == (st[0] + 1,)
             and kv_lens.shape == (st[0],) and page_table.is_contiguous() and q_starts.is_contiguous()
@@ -327,6 +336,8 @@ def _check_tokens(name, t, T, features=None):
         _fail(f"{name} must be [tokens, heads{'' if features is None else f', {features}'}], got {list(t.shape)}")
     if t.dtype != T:
         _fail(f"{name} must have dtype {T}, got {t.dtype}")
+    if sum(t.shape) > _MOST:
+        _sizes_fit(**{name: t})
 
 
 def _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm):
@@ -366,7 +377,7 @@ def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, nor
     sq, sc = q.shape, cos.shape
     if not (sv[0] == n and sv[1] == H_kv == sk_cache[1] and sk_cache[3] == D and sv_cache[3] == sv[2] and len(sq) == 3
             and sq[0] == n and sq[2] == D and len(sc) == 2 and sin.shape == sc and cos.dtype is _F32 and sin.dtype is _F32
-            and sc[0] <= 0x7FFFFFFF):
+            and sum(sq) + sum(sc) <= _MOST):
         return None
     if q_weight is not None or k_weight is not None:
         if (not norm or q_weight is None or k_weight is None or q_weight.dtype is not k_weight.dtype
