@@ -2,14 +2,17 @@
 // cache, keys normed (where asked) and rotated on the way, and the queries of
 // the same tokens rotated beside them, in one launch, for gfx950.
 //
-// Bound by memory, and in generation by latency: each row is read and written
-// once, by lanes that hold it as in sdpa_rope.h.  A wave takes q, k or v heads of one
+// Each row is read and written once, by lanes that hold it as in sdpa_rope.h.  Prompts
+// wait for memory, generation for a chain of dependent loads (start, length, page, row).
+//  A wave takes q, k or v heads of one
 // token (of several where heads are few), one row per group of lanes; it finds its tokens' sequences by counting, a wave's width of
 // q_starts at a time, those that begin at or before the token.
 //
-// 8643 tokens of 4 sequences, 32 + 8 + 8 heads of 128, fp16 (217 MB): 42.5 us, 5.1
-// TB/s, 53 from HBM; up to four rows per group of lanes 45 and 53.  64 single tokens:
-// 4.6 us.
+// 8643 tokens of 4 sequences, 32 + 8 + 8 heads of 128, fp16 (217 MB): 43 us, 5.1
+// TB/s, where the rows lie in the last-level cache, 53 us, 4.1 TB/s, from HBM; up to four
+// rows per group of lanes 45 and 53.  The forward of sdpa_norm_rope.hip, whose reads and
+// writes are alike, reaches 5.9 with loads past the caches; here they have not been tried.
+// 64 single tokens: 4.6 us.
 //
 // A token of no sequence (behind the last) leaves everything as it was.  One
 // whose place is outside the table's columns or the cache's pages is not

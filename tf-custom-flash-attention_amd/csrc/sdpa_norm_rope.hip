@@ -292,8 +292,10 @@ int grad_blocks(long long units) {
 }
 
 // Rows are read past the caches where q and k together outgrow what the 256 MB
-// cache can hold of them beside the results.  268 MB, fp16: plain 126 us, so 114
-// (gradient 232 and 219); 49 MB, fp32, called again and again: plain 21, so 25.
+// cache can hold of them beside the results.  Forward, fp16 and fp32 alike, called again
+// and again: 268 MB of q and k plain 103 us, so 89; 134 MB 44 and 47; 67 MB 22 and 26.  Forward
+// and gradient: 268 MB 274 and 262, 134 MB 143 and 127, 67 MB 63 and 71 (the gradient alone,
+// which reads dy too, would gain from 134 MB on; one rule serves both).
 template <typename T>
 bool past_caches(const NormRopeParams& p) {
     return (long long)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * (long long)sizeof(T) > (128LL << 20);

@@ -110,6 +110,9 @@ inline long long paged_max_tiles(const PagedParams& p, int BM) {
 //   fp16, 32 rows: 146, 168; 129, 137; 26, 22; 63, 58; 73, 62; 51, 25
 //   fp32, 32 rows: 32 of 4096 126, 215; 4 of 2000 31, 52; one of 30000 62, 64 (D 64: 73,
 //         91; 28, 30; 49, 37); 64 rows, 4 of 2000 37, 53; 32 of 4096 214, 220; one 73, 65
+// At 16 fp16 rows each wins three of the six (435 and 453 us together), at 32 the 128-row
+// tiles four of six; one long sequence loses most by the small ones (36 for 24).  The rule goes
+// by rows alone: lengths are on the device.
 constexpr int kPagedSmallRowsF16 = 16, kPagedSmallRowsF32 = 32;
 
 // Shares: of `total` blocks, workgroup w of n takes [share_begin(w), share_begin(w + 1)); n
@@ -151,7 +154,10 @@ __host__ __device__ inline int share_merge(long long total, long long at, long l
 }
 
 // Rows of a sequence and key head, at most as far as is known; workgroups the launches
-// divide for, and the workspace of one launch's parts.
+// divide for, and the workspace of one launch's parts: by the kernel and D_v alone (D_v 128:
+// 17 MB and 68 MB), as much for a short call as for a long one.  Launches that divide for
+// half as many workgroups (fp32 chunks, fp32 generation of more than 128 features in all) use
+// half of it.
 constexpr int kPagedTargetLog2 = 9;
 constexpr int kPagedSmallBM = 32, kPagedBM = 128;
 inline long long paged_most_rows(long long T, int G, int max_q_len) {

@@ -663,7 +663,7 @@ __device__ __forceinline__ void merge_row(const PagedParams& p, const PagedItem&
 
 // Merge of the tiles that parts divide.  Many tiles: a workgroup takes 32 rows of a
 // tile at a time, a thread four columns of a row; 128 tiles of four parts (512 tokens over
-// 16000, 32 heads, D 128, 34 MB): 8 us.  Few tiles, which have many parts: a workgroup a
+// 16000, 32 heads, D 128, 34 MB): 11 us.  Few tiles, which have many parts: a workgroup a
 // row (merge_row).  The whole call of 16 tokens, 16 heads on 4, over 30000 (4 tiles): 106
 // us by 32 rows, 26 by one; 128 tokens over 16000, 32 on 8 (32 tiles): 70 and 66; 256 (64
 // tiles): 95 and 107.

@@ -15,9 +15,9 @@
 // Where a page holds whole blocks, one descriptor serves a block's copies;
 // else each copy has its own.  A descriptor ends at the tile's last key.
 //
-// Bound by issue, as the dense forward is.  4 x 4096 tokens, 32 heads on 8, D 128: 611
-// us, 900 TFLOP/s (a product of 8192^3 1159), pages of 16 instead of 64: 656; 512
-// tokens over 16000 (four parts a tile) 148 us and 8 for the merge.  A short call is a
+// Bound by issue, as the dense forward is.  4 x 4096 tokens, 32 heads on 8, D 128: 618
+// us a call, 890 TFLOP/s (a product of 8192^3 1159), pages of 16 instead of 64: 654; 512
+// tokens over 16000 (four parts a tile) 159 us, 11 of it the merge.  A short call is a
 // chain: 1.5 us for the plan, 0.9 for queries and page table, 0.5 for the first block,
 // 1 for each block of a workgroup alone on its CU, 1 for the results.
 #include "sdpa_launch.h"

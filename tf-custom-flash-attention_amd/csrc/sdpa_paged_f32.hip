@@ -13,8 +13,8 @@
 // by themselves (sdpa_paged_device.h).
 //
 // What bounds it: VALU work beside the MFMAs, as in the dense forward.  2048 tokens
-// over 4096, 16 heads on 4, D 128: 417 us, 124 TFLOP/s; 512 over 8192, D 64: 103 us,
-// 161 TFLOP/s (32-row tiles on v_mfma_f32_32x32x2_f32, as for generation: 647 and 175).
+// over 4096, 16 heads on 4, D 128: 425 us, 121 TFLOP/s; 512 over 8192, D 64: 102 us,
+// 163 TFLOP/s (32-row tiles on v_mfma_f32_32x32x2_f32, as for generation: 647 and 175).
 #include "sdpa_bf3.h"
 #include "sdpa_launch.h"
 #include "sdpa_paged_device.h"

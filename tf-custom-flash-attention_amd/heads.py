@@ -403,6 +403,7 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     Tokens behind the last sequence are skipped (their rows of the result are not written).  A token
     without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
     of a call may have the same place.  D_qk or D_v may be 0 (a cache of keys or of values alone).
+    Any width up to 128 can be cached; ``paged_sdpa`` reads multiples of 8 (fp16) or 4 (fp32).
     """
     T, device = k.dtype, k.device
     batch = _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
