@@ -311,6 +311,7 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
  * sequence are NaN.  What lies in the cache behind a row's last key has no
  * influence on it, infinities and NaN included; an infinite or NaN value
  * among its keys makes its feature of o infinite or NaN.
+ * o, stats and the workspace share no memory with each other or with the inputs.
  * H_q is a multiple of H_kv; feature sizes, strides and addresses must be whole
  * 16-byte chunks; D_qk, D_v <= 128.
  * max_q_len: the most new tokens of a sequence, where the caller knows it (1 in
