@@ -76,7 +76,9 @@ typedef enum {
     SDPA_ERR_HEADS = 28,
     SDPA_ERR_LAYOUT = 29,
     SDPA_ERR_TOO_LARGE = 30,
-    SDPA_ERR_WEIGHT = 31
+    SDPA_ERR_WEIGHT = 31,
+    SDPA_ERR_AXES = 32,
+    SDPA_ERR_FP4_WIDTH = 33
 } sdpa_status_t;
 
 /* Message for a status code (static storage, never NULL). */
@@ -266,6 +268,30 @@ int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_
                                int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
                                hipStream_t stream);
 
+/* The same where the pairs follow several positions of a token (time, height,
+ * width of image and video patches): pair i, of the R / 2 rotated ones, is turned
+ * by row positions[pair_axes[i]] of the tables.  positions: int32 [n_axes, S] (or
+ * [n_axes, B, S] with positions_per_batch) on the device, dense; pair_axes: R / 2
+ * bytes on the host, read before the call returns, each below n_axes and 4.  A
+ * position outside the tables, on an axis that some pair follows, makes its rows NaN. */
+int sdpa_hip_qk_norm_rope_axes(int dtype, const void* q, const int64_t* q_strides, const void* k,
+                               const int64_t* k_strides, void* q_out, const int64_t* q_out_strides, void* k_out,
+                               const int64_t* k_out_strides, const void* q_weight, const void* k_weight,
+                               int weight_dtype, const float* cos, const float* sin, int table_rows,
+                               const int32_t* positions, int positions_per_batch, const uint8_t* pair_axes, int n_axes,
+                               int B, int S, int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
+                               hipStream_t stream);
+
+int sdpa_hip_qk_norm_rope_axes_grad(int dtype, const void* d_q_out, const int64_t* d_q_out_strides,
+                                    const void* d_k_out, const int64_t* d_k_out_strides, const void* q,
+                                    const int64_t* q_strides, const void* k, const int64_t* k_strides, void* dq,
+                                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dq_weight,
+                                    void* dk_weight, const void* q_weight, const void* k_weight, int weight_dtype,
+                                    const float* cos, const float* sin, int table_rows, const int32_t* positions,
+                                    int positions_per_batch, const uint8_t* pair_axes, int n_axes, void* workspace,
+                                    size_t workspace_bytes, int B, int S, int H_q, int H_kv, int D, int R, float eps,
+                                    int norm, int interleaved, hipStream_t stream);
+
 /* ---- paged cache -------------------------------------------------------------
  * No counterpart in the reference.  Keys and values of N sequences lie in pages
  * of page_size tokens (a power of two, 16 .. 65536): k_cache [pages, H_kv, page_size,
@@ -280,6 +306,29 @@ int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_
  * They are read on the device only, so a captured call follows them.  Nothing
  * outside of the T tokens, the width columns and the pages is touched whatever
  * they hold.                                                                  */
+
+/* Pages for the new tokens of a batch, and where each token goes: what a server
+ * does between two steps, on the device.  free_pages [capacity] is a stack of pages
+ * that no sequence holds, its first *free_count entries.
+ *   1. Sequences with finished[s] != 0 (NULL: none) give back the pages of their
+ *      kv_lens[s] tokens, in the order sequence, column (entries below 0 are left
+ *      out, and what would pass capacity), and have no tokens then; their rows of the
+ *      table are left as they are.
+ *   2. new_lens[s] tokens are added to every sequence (a finished one begins
+ *      anew).  Each column that they are the first to need gets the top page of the
+ *      stack, in the order sequence, column; -1 once the stack is empty, and what
+ *      lies behind the table's columns gets none.
+ * Out: q_starts [N + 1] and kv_lens_out [N] as below (kv_lens_out may be kv_lens);
+ * free_count_out (may be free_count); for every one of the T packed tokens its
+ * place in the sequence, positions [T], and slots [T], page * page_size + row, -1 for
+ * a token without a page; both -1 behind the last sequence.  Lengths below 0 count as
+ * 0, cached ones above width * page_size and new ones above T as those.  No two
+ * rows of the table may overlap.  T <= 2^30 - 1, width * page_size + T below 2^31.  */
+int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                        const int32_t* new_lens, const uint8_t* finished, int32_t* free_pages,
+                        const int32_t* free_count, int32_t* q_starts, int32_t* kv_lens_out, int32_t* free_count_out,
+                        int32_t* positions, int64_t* slots, int N, int T, int width, int page_size, int capacity,
+                        hipStream_t stream);
 
 /* Keys and values of the new tokens into their places, k normed (norm) and
  * rotated by its place in the sequence on the way as above (R = 0: not
@@ -298,6 +347,17 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
                        int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
                        int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
                        int norm, int interleaved, hipStream_t stream);
+
+/* The same, rotated by positions [n_axes, T] instead of the places in the
+ * sequences (as in sdpa_hip_qk_norm_rope_axes).                               */
+int sdpa_hip_kv_append_axes(int dtype, const void* k, const int64_t* k_strides, const void* v,
+                            const int64_t* v_strides, void* k_cache, void* v_cache, const void* q,
+                            const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* q_weight,
+                            const void* k_weight, int weight_dtype, const float* cos, const float* sin, int table_rows,
+                            const int32_t* positions, const uint8_t* pair_axes, int n_axes, const int32_t* page_table,
+                            int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
+                            int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
+                            int norm, int interleaved, hipStream_t stream);
 
 /* Attention of the new tokens over the cache (after their append): for query
  * head h of token i of the n new ones of sequence s, over the keys of head

@@ -36,7 +36,7 @@ SDPA_OK = 0
 SDPA_ERR_HIP = 23
 SDPA_ERR_SCRATCH_LIMIT = 24
 SDPA_ERR_DS_PATH = 25
-_ARG_ERRORS = set(range(1, 23)) | {SDPA_ERR_SCRATCH_LIMIT, SDPA_ERR_DS_PATH} | set(range(26, 32))
+_ARG_ERRORS = set(range(1, 23)) | {SDPA_ERR_SCRATCH_LIMIT, SDPA_ERR_DS_PATH} | set(range(26, 34))
 
 _lib = None
 
@@ -117,10 +117,21 @@ def library():
     L.sdpa_hip_qk_norm_rope_grad.restype = i32
     L.sdpa_hip_qk_norm_rope_grad.argtypes = ([i32] + [vp, i64p] * 6 + [vp, vp] + rope + [i32p, i32, vp, sz] + [i32] * 6 +
                                              [f32, i32, i32, vp])
+    axes = [i32p, i32, vp, i32]  # positions, whether per batch, axes of the pairs and their number
+    L.sdpa_hip_qk_norm_rope_axes.restype = i32
+    L.sdpa_hip_qk_norm_rope_axes.argtypes = [i32] + [vp, i64p] * 4 + rope + axes + [i32] * 6 + [f32, i32, i32, vp]
+    L.sdpa_hip_qk_norm_rope_axes_grad.restype = i32
+    L.sdpa_hip_qk_norm_rope_axes_grad.argtypes = ([i32] + [vp, i64p] * 6 + [vp, vp] + rope + axes + [vp, sz] + [i32] * 6 +
+                                                  [f32, i32, i32, vp])
     batch = [i32p, ctypes.c_int64, i32p, i32p]  # page table and its row stride, q_starts, kv_lens
+    L.sdpa_hip_kv_reserve.restype = i32
+    L.sdpa_hip_kv_reserve.argtypes = [i32p, ctypes.c_int64] + [vp] * 10 + [i32] * 5 + [vp]
     L.sdpa_hip_kv_append.restype = i32
     L.sdpa_hip_kv_append.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + batch + [i32] * 10 +
                                      [f32, i32, i32, vp])
+    L.sdpa_hip_kv_append_axes.restype = i32
+    L.sdpa_hip_kv_append_axes.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + [i32p, vp, i32] + batch +
+                                          [i32] * 10 + [f32, i32, i32, vp])
     L.sdpa_hip_paged_fwd_workspace_bytes.restype = sz
     L.sdpa_hip_paged_fwd_workspace_bytes.argtypes = [i32] * 10
     L.sdpa_hip_paged_fwd.restype = i32
@@ -358,7 +369,7 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
     return _fn.apply(q, k, v, seed, offset, dropout, scale, causal_mask)
 
 
-_HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_append", "paged_sdpa")
+_HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_reserve", "Reserved", "kv_append", "paged_sdpa")
 
 
 def __getattr__(name):

@@ -51,6 +51,8 @@ inline const char* status_message(int status) {
             return "feature sizes, strides and addresses must be whole 16-byte chunks of at least one feature";
         case SDPA_ERR_TOO_LARGE: return "too many rows for one call";
         case SDPA_ERR_WEIGHT: return "a weight needs the norm, and is of dtype T or float32";
+        case SDPA_ERR_AXES: return "the axes of rotated pairs must be below 4 and below the number of axes of the positions";
+        case SDPA_ERR_FP4_WIDTH: return "feature sizes of a cache in 4 bits must be multiples of 32, up to 128";
         default: return "unknown sdpa status";
     }
 }

@@ -44,7 +44,7 @@ __host__ __device__ inline AppendMap append_map(int tokens, int H) {
     return m;
 }
 
-template <typename T, int EPC, int LPR, bool IN>
+template <typename T, int EPC, int LPR, bool IN, bool AX>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const AppendParams p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -98,7 +98,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const Appe
     const bool placed = page >= 0 && page < bt.pages;
 
     RowTurn<EPC> t;
-    if (kind != 2) t.load(p.r, l, pos);
+    if (kind != 2) {
+        if constexpr (AX) t.load_axes(p.r, p.axes, l, p.axes.positions + tok);
+        else t.load(p.r, l, pos);
+    }
     float wa[EPC], wb[EPC];
     load_weight<T, EPC, IN>(wa, wb, kind == 2 ? nullptr : kind == 0 ? p.q_weight : p.k_weight, p.w32 != 0, l);
     const long long slot = pos & ((1LL << bt.page_log2) - 1);
@@ -143,7 +146,7 @@ hipError_t with_append_row(const AppendParams& p, F&& f) {
     return lpr(std::integral_constant<int, V>{}, std::false_type{});
 }
 
-template <typename T>
+template <typename T, bool AX>
 hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
     return with_append_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value;
@@ -151,7 +154,7 @@ hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
         const long long n = append_map<L>(p.batch.T, p.H_q).units + append_map<L>(p.batch.T, p.H_k).units +
                             append_map<L>(p.batch.T, p.H_v).units;
         if (n == 0) return hipSuccess;
-        return launch_kernel<kv_append_kernel<T, E, L, IN>>(tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves),
+        return launch_kernel<kv_append_kernel<T, E, L, IN, AX>>(tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves),
                                                             64 * kAppendWaves, 0, stream, p);
     });
 }
@@ -159,7 +162,10 @@ hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_kv_append(const AppendParams& p, DType dtype, hipStream_t stream) {
-    return dtype == DType::F16 ? launch_kv_append_t<half_t>(p, stream) : launch_kv_append_t<float>(p, stream);
+    return with_bool(p.axes.used != 0, [&](auto ax) {
+        constexpr bool AX = decltype(ax)::value;
+        return dtype == DType::F16 ? launch_kv_append_t<half_t, AX>(p, stream) : launch_kv_append_t<float, AX>(p, stream);
+    });
 }
 
 }  // namespace sdpa

@@ -22,7 +22,8 @@ struct NormRopeSide {
 struct NormRopeParams {
     NormRopeSide side[2];
     RopeArgs r;
-    const int32_t* positions;    // [S] or [B, S]; null: 0 .. S - 1
+    AxesArgs axes;
+    const int32_t* positions;    // [S] or [B, S]; null: 0 .. S - 1 (with axes: of axis 0)
     long long positions_stride;  // between sequences (0: shared)
     float* part_dw;              // [workgroup][D]
     int B, S, D;

@@ -75,8 +75,14 @@ __device__ __forceinline__ long long position_of(const NormRopeParams& p, const 
     if (!p.positions) return at.s;
     return p.positions[at.b * p.positions_stride + at.s];
 }
+// The turn of a token's rows; AX: by several axes.
+template <bool AX, int EPC, bool IN>
+__device__ __forceinline__ void load_turn(RowTurn<EPC>& t, const NormRopeParams& p, const RowLane<EPC, IN>& l, const Place& at) {
+    if constexpr (AX) t.load_axes(p.r, p.axes, l, p.positions + at.b * p.positions_stride + at.s);
+    else t.load(p.r, l, position_of(p, at));
+}
 
-template <typename T, int EPC, int LPR, bool IN, int KU, bool NT>
+template <typename T, int EPC, int LPR, bool IN, int KU, bool NT, bool AX>
 __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_kernel(const NormRopeParams p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -98,7 +104,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_kernel(const NormRo
     for (int k = 0; k < KU; ++k)
         if (k < at.rows) load_row<T, EPC, IN, NT>(a[k], b[k], x + min(at.h + k * m.gpt, m.H - 1) * sd.xs.h, l);
     RowTurn<EPC> t;
-    t.load(p.r, l, position_of(p, at));
+    load_turn<AX>(t, p, l, at);
     float wa[EPC], wb[EPC];
     load_weight<T, EPC, IN>(wa, wb, sd.w, p.w32 != 0, l);
     RowFactors<EPC, IN> f;
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_kernel(const NormRo
 }
 
 // dx, and this workgroup's sum of dw (blocks of q before those of k).
-template <typename T, int EPC, int LPR, bool IN, int KU, bool NT>
+template <typename T, int EPC, int LPR, bool IN, int KU, bool NT, bool AX>
 __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const NormRopeParams p, const int blocks_q,
                                                                          const int blocks_k) {
     __shared__ float sums[kRopeWaves][2 * EPC * LPR];
@@ -148,7 +154,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void norm_rope_grad_kernel(const N
             load_row<T, EPC, IN, NT>(ya[k], yb[k], dy + h * sd.dys.h, l);
         }
         RowTurn<EPC> t;
-        t.load(p.r, l, position_of(p, at));
+        load_turn<AX>(t, p, l, at);
 #pragma unroll
         for (int k = 0; k < KU; ++k) {
             if (k >= at.rows) break;
@@ -301,7 +307,7 @@ bool past_caches(const NormRopeParams& p) {
     return (long long)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * (long long)sizeof(T) > (128LL << 20);
 }
 
-template <typename T>
+template <typename T, bool AX>
 hipError_t launch_norm_rope_t(const NormRopeParams& p, hipStream_t stream) {
     return with_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value;
@@ -314,9 +320,9 @@ hipError_t launch_norm_rope_t(const NormRopeParams& p, hipStream_t stream) {
             const dim3 grid = tile_grid((n + kRopeWaves - 1) / kRopeWaves, 64 * kRopeWaves);
             if constexpr (KU == 4) {
                 if (past_caches<T>(p))
-                    return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, true>>(grid, 64 * kRopeWaves, 0, stream, p);
+                    return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, true, AX>>(grid, 64 * kRopeWaves, 0, stream, p);
             }
-            return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, false>>(grid, 64 * kRopeWaves, 0, stream, p);
+            return launch_kernel<norm_rope_kernel<T, E, L, IN, KU, false, AX>>(grid, 64 * kRopeWaves, 0, stream, p);
         };
         const long long n4 = side_map<L, 4>(tokens, p.side[0].H).units + side_map<L, 4>(tokens, p.side[1].H).units;
         if (n4 >= kRopeFewWaves) return run(std::integral_constant<int, 4>{});
@@ -324,7 +330,7 @@ hipError_t launch_norm_rope_t(const NormRopeParams& p, hipStream_t stream) {
     });
 }
 
-template <typename T>
+template <typename T, bool AX>
 hipError_t launch_norm_rope_grad_t(const NormRopeParams& p, hipStream_t stream) {
     return with_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value, KU = 2;
@@ -335,9 +341,9 @@ hipError_t launch_norm_rope_grad_t(const NormRopeParams& p, hipStream_t stream) 
         hipError_t e = hipSuccess;
         const dim3 grid((unsigned)(bq + bk));
         if (bq + bk > 0)
-            e = past_caches<T>(p) ? launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, true>>(grid, 64 * kRopeWaves, 0,
+            e = past_caches<T>(p) ? launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, true, AX>>(grid, 64 * kRopeWaves, 0,
                                                                                                  stream, p, bq, bk)
-                                  : launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, false>>(grid, 64 * kRopeWaves, 0,
+                                  : launch_kernel<norm_rope_grad_kernel<T, E, L, IN, KU, false, AX>>(grid, 64 * kRopeWaves, 0,
                                                                                                   stream, p, bq, bk);
         if (e != hipSuccess || (!p.side[0].dw && !p.side[1].dw)) return e;
         return launch_kernel<norm_rope_dw_kernel<T>>(dim3((unsigned)((p.D + 15) / 16), 2), 1024, 0, stream, p, bq, bk);
@@ -347,12 +353,18 @@ hipError_t launch_norm_rope_grad_t(const NormRopeParams& p, hipStream_t stream) 
 }  // namespace
 
 hipError_t launch_norm_rope(const NormRopeParams& p, DType dtype, hipStream_t stream) {
-    return dtype == DType::F16 ? launch_norm_rope_t<half_t>(p, stream) : launch_norm_rope_t<float>(p, stream);
+    return with_bool(p.axes.used != 0, [&](auto ax) {
+        constexpr bool AX = decltype(ax)::value;
+        return dtype == DType::F16 ? launch_norm_rope_t<half_t, AX>(p, stream) : launch_norm_rope_t<float, AX>(p, stream);
+    });
 }
 
 hipError_t launch_norm_rope_grad(const NormRopeParams& p, DType dtype, hipStream_t stream) {
-    return dtype == DType::F16 ? launch_norm_rope_grad_t<half_t>(p, stream)
-                               : launch_norm_rope_grad_t<float>(p, stream);
+    return with_bool(p.axes.used != 0, [&](auto ax) {
+        constexpr bool AX = decltype(ax)::value;
+        return dtype == DType::F16 ? launch_norm_rope_grad_t<half_t, AX>(p, stream)
+                                   : launch_norm_rope_grad_t<float, AX>(p, stream);
+    });
 }
 
 }  // namespace sdpa

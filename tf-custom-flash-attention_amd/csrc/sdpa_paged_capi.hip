@@ -8,6 +8,7 @@
 #include "sdpa_kv_append.h"
 #include "sdpa_norm_rope.h"
 #include "sdpa_paged.h"
+#include "sdpa_reserve.h"
 
 namespace {
 
@@ -51,21 +52,44 @@ void add_rows(Chunks& c, const void* p, const sdpa::RowStrides& s) {
     c.stride(s.h);
 }
 
+// The axes of the rotated pairs, R / 2 bytes on the host; positions [n_axes][per_axis].
+int make_axes(sdpa::AxesArgs& a, const uint8_t* pair_axes, int n_axes, const int32_t* positions, long long per_axis, int R) {
+    a = sdpa::AxesArgs{};
+    if (n_axes < 0) return SDPA_ERR_NEGATIVE_DIM;
+    if (R == 0) return SDPA_OK;
+    if (!pair_axes || (per_axis > 0 && !positions)) return SDPA_ERR_NULL_POINTER;
+    for (int i = 0; i < R / 2; ++i) {
+        const int x = pair_axes[i];
+        if (x >= n_axes || x >= sdpa::kMaxAxes) return SDPA_ERR_AXES;
+        a.lo |= (uint64_t)(x & 1) << i;
+        a.hi |= (uint64_t)(x >> 1) << i;
+        a.used |= 1 << x;
+    }
+    a.positions = positions;
+    a.stride = per_axis;
+    return SDPA_OK;
+}
+
 int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64_t* const (&xs)[2],
                     const void* const (&dy)[2], const int64_t* const (&dys)[2], void* const (&y)[2],
                     const int64_t* const (&ys)[2], const void* const (&w)[2], void* const (&dw)[2], int weight_dtype,
                     const float* cos, const float* sin, int table_rows, const int32_t* positions,
                     int positions_per_batch, void* workspace, size_t workspace_bytes, int B, int S, int H_q, int H_kv,
-                    int D, int R, float eps, int norm, int interleaved, hipStream_t stream) {
+                    int D, int R, float eps, int norm, int interleaved, hipStream_t stream, bool by_axes = false,
+                    const uint8_t* pair_axes = nullptr, int n_axes = 0) {
     if (B < 0 || S < 0 || H_q < 0 || H_kv < 0) return SDPA_ERR_NEGATIVE_DIM;
     const bool any_dw = dw[0] || dw[1];
     int st = check_rows(dtype, weight_dtype, any_dw ? (dw[0] ? dw[0] : dw[1]) : w[0], w[1] ? w[1] : w[0], cos, sin,
                         table_rows, D, R, norm);
     if (st != SDPA_OK) return st;
     if (!rows_fit(B, S, 0) || !rows_fit((long long)B * S, H_q, H_kv)) return SDPA_ERR_TOO_LARGE;
+    sdpa::NormRopeParams p{};
+    if (by_axes) {
+        st = make_axes(p.axes, pair_axes, n_axes, positions, positions_per_batch ? (long long)B * S : S, R);
+        if (st != SDPA_OK) return st;
+    }
     if (D == 0) return SDPA_OK;
     const bool rows = B > 0 && S > 0;
-    sdpa::NormRopeParams p{};
     Chunks ch{dtype == SDPA_DTYPE_F16 ? 8 : 4};
     ch.features(D);
     ch.rotated(R, interleaved);
@@ -111,11 +135,15 @@ int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64
     return hip_status(grad ? sdpa::launch_norm_rope_grad(p, dt, stream) : sdpa::launch_norm_rope(p, dt, stream));
 }
 
+bool page_size_ok(int page_size) {
+    return page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0;
+}
+
 // Checks of a batch over a paged cache and its description.
 int make_batch(sdpa::PagedBatch& b, const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
                const int32_t* kv_lens, int N, int T, int width, int pages, int page_size) {
     if (N < 0 || T < 0 || width < 0 || pages < 0) return SDPA_ERR_NEGATIVE_DIM;
-    if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)) != 0) return SDPA_ERR_PAGE_SIZE;
+    if (!page_size_ok(page_size)) return SDPA_ERR_PAGE_SIZE;
     // token numbers of a sequence, and those of sequences a wave ahead, stay below 2^31
     if (N > 0x7FFFFFFF - 65536 || (long long)width * page_size > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     if (N > 0 && T > 0 && (!q_starts || !kv_lens || (width > 0 && !page_table))) return SDPA_ERR_NULL_POINTER;
@@ -136,48 +164,13 @@ void add_tokens(Chunks& c, const void* p, const sdpa::TokenStrides& s) {
     c.stride(s.h);
 }
 
-}  // namespace
-
-extern "C" {
-
-int sdpa_hip_qk_norm_rope(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                          void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
-                          const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
-                          const float* sin, int table_rows, const int32_t* positions, int positions_per_batch, int B,
-                          int S, int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
-                          hipStream_t stream) {
-    return norm_rope_entry(false, dtype, {q, k}, {q_strides, k_strides}, {nullptr, nullptr}, {nullptr, nullptr},
-                           {q_out, k_out}, {q_out_strides, k_out_strides}, {q_weight, k_weight}, {nullptr, nullptr},
-                           weight_dtype, cos, sin, table_rows, positions, positions_per_batch, nullptr, 0, B, S, H_q,
-                           H_kv, D, R, eps, norm, interleaved, stream);
-}
-
-size_t sdpa_hip_qk_norm_rope_grad_workspace_bytes(int D) {
-    return D <= 0 || D > 128 ? 0 : 2 * (size_t)sdpa::kGradBlocks * (size_t)D * sizeof(float);
-}
-
-int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_q_out_strides, const void* d_k_out,
-                               const int64_t* d_k_out_strides, const void* q, const int64_t* q_strides, const void* k,
-                               const int64_t* k_strides, void* dq, const int64_t* dq_strides, void* dk,
-                               const int64_t* dk_strides, void* dq_weight, void* dk_weight, const void* q_weight,
-                               const void* k_weight, int weight_dtype, const float* cos, const float* sin,
-                               int table_rows, const int32_t* positions, int positions_per_batch, void* workspace,
-                               size_t workspace_bytes, int B, int S, int H_q, int H_kv, int D, int R, float eps,
-                               int norm, int interleaved, hipStream_t stream) {
-    return norm_rope_entry(true, dtype, {q, k}, {q_strides, k_strides}, {d_q_out, d_k_out},
-                           {d_q_out_strides, d_k_out_strides}, {dq, dk}, {dq_strides, dk_strides},
-                           {q_weight, k_weight}, {dq_weight, dk_weight}, weight_dtype, cos, sin, table_rows, positions,
-                           positions_per_batch, workspace, workspace_bytes, B, S, H_q, H_kv, D, R, eps, norm,
-                           interleaved, stream);
-}
-
-int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                       void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
-                       const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
-                       const float* cos, const float* sin, int table_rows, const int32_t* page_table,
-                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
-                       int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
-                       int norm, int interleaved, hipStream_t stream) {
+int append_entry(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_cache,
+                 void* v_cache, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                 const void* q_weight, const void* k_weight, int weight_dtype, const float* cos, const float* sin,
+                 int table_rows, const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
+                 const int32_t* kv_lens, int N, int T, int width, int pages, int page_size, int H_q, int H_kv, int D_qk,
+                 int D_v, int R, float eps, int norm, int interleaved, hipStream_t stream, bool by_axes,
+                 const int32_t* positions, const uint8_t* pair_axes, int n_axes) {
     int st = check_rows(dtype, weight_dtype, q_weight, k_weight, cos, sin, table_rows, D_qk, R, norm);
     if (st != SDPA_OK) return st;
     if (H_q < 0 || H_kv < 0 || D_v < 0) return SDPA_ERR_NEGATIVE_DIM;
@@ -186,6 +179,10 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     st = make_batch(p.batch, page_table, page_table_stride, q_starts, kv_lens, N, T, width, pages, page_size);
     if (st != SDPA_OK) return st;
     if (!rows_fit(T, H_q, 2LL * H_kv)) return SDPA_ERR_TOO_LARGE;
+    if (by_axes) {
+        st = make_axes(p.axes, pair_axes, n_axes, positions, T, R);
+        if (st != SDPA_OK) return st;
+    }
     if (N == 0 || T == 0) return SDPA_OK;
     const bool has_k = H_kv > 0 && D_qk > 0, has_v = H_kv > 0 && D_v > 0, has_q = H_q > 0 && D_qk > 0;
     if ((has_k && (!k || (pages > 0 && !k_cache))) || (has_v && (!v || (pages > 0 && !v_cache))) ||
@@ -230,6 +227,129 @@ int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const
     if (has_v) add_tokens(ch, v, p.vs);
     p.vec = ch.ok;
     return hip_status(sdpa::launch_kv_append(p, (sdpa::DType)dtype, stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int sdpa_hip_qk_norm_rope(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                          const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                          const float* sin, int table_rows, const int32_t* positions, int positions_per_batch, int B,
+                          int S, int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
+                          hipStream_t stream) {
+    return norm_rope_entry(false, dtype, {q, k}, {q_strides, k_strides}, {nullptr, nullptr}, {nullptr, nullptr},
+                           {q_out, k_out}, {q_out_strides, k_out_strides}, {q_weight, k_weight}, {nullptr, nullptr},
+                           weight_dtype, cos, sin, table_rows, positions, positions_per_batch, nullptr, 0, B, S, H_q,
+                           H_kv, D, R, eps, norm, interleaved, stream);
+}
+
+size_t sdpa_hip_qk_norm_rope_grad_workspace_bytes(int D) {
+    return D <= 0 || D > 128 ? 0 : 2 * (size_t)sdpa::kGradBlocks * (size_t)D * sizeof(float);
+}
+
+int sdpa_hip_qk_norm_rope_grad(int dtype, const void* d_q_out, const int64_t* d_q_out_strides, const void* d_k_out,
+                               const int64_t* d_k_out_strides, const void* q, const int64_t* q_strides, const void* k,
+                               const int64_t* k_strides, void* dq, const int64_t* dq_strides, void* dk,
+                               const int64_t* dk_strides, void* dq_weight, void* dk_weight, const void* q_weight,
+                               const void* k_weight, int weight_dtype, const float* cos, const float* sin,
+                               int table_rows, const int32_t* positions, int positions_per_batch, void* workspace,
+                               size_t workspace_bytes, int B, int S, int H_q, int H_kv, int D, int R, float eps,
+                               int norm, int interleaved, hipStream_t stream) {
+    return norm_rope_entry(true, dtype, {q, k}, {q_strides, k_strides}, {d_q_out, d_k_out},
+                           {d_q_out_strides, d_k_out_strides}, {dq, dk}, {dq_strides, dk_strides},
+                           {q_weight, k_weight}, {dq_weight, dk_weight}, weight_dtype, cos, sin, table_rows, positions,
+                           positions_per_batch, workspace, workspace_bytes, B, S, H_q, H_kv, D, R, eps, norm,
+                           interleaved, stream);
+}
+
+int sdpa_hip_qk_norm_rope_axes(int dtype, const void* q, const int64_t* q_strides, const void* k,
+                               const int64_t* k_strides, void* q_out, const int64_t* q_out_strides, void* k_out,
+                               const int64_t* k_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                               const float* cos, const float* sin, int table_rows, const int32_t* positions,
+                               int positions_per_batch, const uint8_t* pair_axes, int n_axes, int B, int S, int H_q,
+                               int H_kv, int D, int R, float eps, int norm, int interleaved, hipStream_t stream) {
+    return norm_rope_entry(false, dtype, {q, k}, {q_strides, k_strides}, {nullptr, nullptr}, {nullptr, nullptr},
+                           {q_out, k_out}, {q_out_strides, k_out_strides}, {q_weight, k_weight}, {nullptr, nullptr},
+                           weight_dtype, cos, sin, table_rows, positions, positions_per_batch, nullptr, 0, B, S, H_q,
+                           H_kv, D, R, eps, norm, interleaved, stream, true, pair_axes, n_axes);
+}
+
+int sdpa_hip_qk_norm_rope_axes_grad(int dtype, const void* d_q_out, const int64_t* d_q_out_strides, const void* d_k_out,
+                                    const int64_t* d_k_out_strides, const void* q, const int64_t* q_strides, const void* k,
+                                    const int64_t* k_strides, void* dq, const int64_t* dq_strides, void* dk,
+                                    const int64_t* dk_strides, void* dq_weight, void* dk_weight, const void* q_weight,
+                                    const void* k_weight, int weight_dtype, const float* cos, const float* sin,
+                                    int table_rows, const int32_t* positions, int positions_per_batch,
+                                    const uint8_t* pair_axes, int n_axes, void* workspace, size_t workspace_bytes, int B,
+                                    int S, int H_q, int H_kv, int D, int R, float eps, int norm, int interleaved,
+                                    hipStream_t stream) {
+    return norm_rope_entry(true, dtype, {q, k}, {q_strides, k_strides}, {d_q_out, d_k_out},
+                           {d_q_out_strides, d_k_out_strides}, {dq, dk}, {dq_strides, dk_strides},
+                           {q_weight, k_weight}, {dq_weight, dk_weight}, weight_dtype, cos, sin, table_rows, positions,
+                           positions_per_batch, workspace, workspace_bytes, B, S, H_q, H_kv, D, R, eps, norm,
+                           interleaved, stream, true, pair_axes, n_axes);
+}
+
+int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens, const int32_t* new_lens,
+                        const uint8_t* finished, int32_t* free_pages, const int32_t* free_count, int32_t* q_starts,
+                        int32_t* kv_lens_out, int32_t* free_count_out, int32_t* positions, int64_t* slots, int N, int T,
+                        int width, int page_size, int capacity, hipStream_t stream) {
+    if (N < 0 || T < 0 || width < 0 || capacity < 0) return SDPA_ERR_NEGATIVE_DIM;
+    if (!page_size_ok(page_size)) return SDPA_ERR_PAGE_SIZE;
+    if (N > 0x7FFFFFFF - 65536 || T > 0x3FFFFFFF || (long long)width * page_size + T > 0x7FFFFFFFLL - 65536)
+        return SDPA_ERR_TOO_LARGE;
+    if (!q_starts || !free_count || !free_count_out || (N > 0 && (!kv_lens || !new_lens || !kv_lens_out)) ||
+        (N > 0 && width > 0 && !page_table) || (capacity > 0 && !free_pages) || (T > 0 && (!positions || !slots)))
+        return SDPA_ERR_NULL_POINTER;
+    if (N > 1 && page_table_stride < width) return SDPA_ERR_LAYOUT;
+    sdpa::ReserveParams p{};
+    p.page_table = page_table;
+    p.table_stride = page_table_stride;
+    p.kv_lens = kv_lens;
+    p.new_lens = new_lens;
+    p.finished = finished;
+    p.free_pages = free_pages;
+    p.free_count = free_count;
+    p.q_starts = q_starts;
+    p.kv_lens_out = kv_lens_out;
+    p.free_count_out = free_count_out;
+    p.positions = positions;
+    p.slots = slots;
+    p.N = N;
+    p.T = T;
+    p.width = width;
+    p.capacity = capacity;
+    while ((1 << p.page_log2) < page_size) ++p.page_log2;
+    return hip_status(sdpa::launch_kv_reserve(p, stream));
+}
+
+int sdpa_hip_kv_append(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
+                       const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                       const float* cos, const float* sin, int table_rows, const int32_t* page_table,
+                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
+                       int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
+                       int norm, int interleaved, hipStream_t stream) {
+    return append_entry(dtype, k, k_strides, v, v_strides, k_cache, v_cache, q, q_strides, q_out, q_out_strides, q_weight,
+                        k_weight, weight_dtype, cos, sin, table_rows, page_table, page_table_stride, q_starts, kv_lens, N, T,
+                        width, pages, page_size, H_q, H_kv, D_qk, D_v, R, eps, norm, interleaved, stream, false, nullptr,
+                        nullptr, 0);
+}
+
+int sdpa_hip_kv_append_axes(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                            void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
+                            const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                            const float* cos, const float* sin, int table_rows, const int32_t* positions,
+                            const uint8_t* pair_axes, int n_axes, const int32_t* page_table, int64_t page_table_stride,
+                            const int32_t* q_starts, const int32_t* kv_lens, int N, int T, int width, int pages,
+                            int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps, int norm,
+                            int interleaved, hipStream_t stream) {
+    return append_entry(dtype, k, k_strides, v, v_strides, k_cache, v_cache, q, q_strides, q_out, q_out_strides, q_weight,
+                        k_weight, weight_dtype, cos, sin, table_rows, page_table, page_table_stride, q_starts, kv_lens, N, T,
+                        width, pages, page_size, H_q, H_kv, D_qk, D_v, R, eps, norm, interleaved, stream, true, positions,
+                        pair_axes, n_axes);
 }
 
 }  // extern "C"

@@ -33,6 +33,16 @@ struct RopeArgs {
     float eps, inv_D;
 };
 
+// Positions with several axes (time, height, width): pair i is turned by the row of the
+// tables that the token's position on axis axis_of(i) names.
+constexpr int kMaxAxes = 4;
+struct AxesArgs {
+    const int32_t* positions;  // axis a of a token: a * stride behind its axis 0
+    long long stride;
+    uint64_t lo, hi;  // bits 0 and 1 of the axis of every pair
+    int used;         // bit a: some pair follows axis a (0: no axes)
+};
+
 namespace {
 
 // Pow2-sized groups of lanes per row, for D features in chunks of epc.
@@ -167,6 +177,53 @@ struct RowTurn {
                 load_table<HP>(h, p.sin + row + l.t + HP);
 #pragma unroll
                 for (int i = 0; i < HP; ++i) s[HP + i] = h[i];
+            }
+        }
+    }
+    // The same by axes; `pos`: the token's position on axis 0.
+    template <bool IN>
+    __device__ __forceinline__ void load_axes(const RopeArgs& p, const AxesArgs& ax, const RowLane<EPC, IN>& l,
+                                              const int32_t* pos) {
+        // pairs of this lane: t .. t + EPC (IN: the first half in a, the second in b)
+        constexpr int HP = IN ? EPC / 2 : EPC;
+        constexpr uint32_t kHalf = (1u << HP) - 1;
+        const uint32_t mine = (l.ra ? kHalf : 0u) | (IN && l.rb ? kHalf << HP : 0u);
+        const uint32_t lo = mine ? (uint32_t)(ax.lo >> l.t) : 0u, hi = mine ? (uint32_t)(ax.hi >> l.t) : 0u;
+        int32_t row[kMaxAxes];
+        bad = false;
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; ++a) {
+            row[a] = 0;
+            if (!((ax.used >> a) & 1)) continue;
+            row[a] = pos[a * ax.stride];
+            if (row[a] < 0 || row[a] >= p.rows) {
+                bad = true;
+                row[a] = 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < EPC; ++i) {
+            c[i] = 1.f;
+            s[i] = 0.f;
+        }
+        if (p.rows == 0) return;
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; ++a) {
+            const uint32_t on = mine & (a & 1 ? lo : ~lo) & (a & 2 ? hi : ~hi);
+            if (on == 0) continue;
+            const long long at = (long long)row[a] * (p.R / 2) + l.t;
+#pragma unroll
+            for (int h = 0; h < EPC; h += HP) {
+                if (!((mine >> h) & 1)) continue;
+                float x[HP], y[HP];
+                load_table<HP>(x, p.cos + at + h);
+                load_table<HP>(y, p.sin + at + h);
+#pragma unroll
+                for (int i = 0; i < HP; ++i)
+                    if ((on >> (h + i)) & 1) {
+                        c[h + i] = x[i];
+                        s[h + i] = y[i];
+                    }
             }
         }
     }

@@ -8,6 +8,7 @@ checked there, where they are used.
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 import functools
 
@@ -130,7 +131,34 @@ def _check_qk(q, k):
     _sizes_fit(q=q, k=k)
 
 
-def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
+@functools.lru_cache(maxsize=64)
+def _pair_axes(axes, pairs):
+    """The axis of every rotated pair, for the C entries, and the largest."""
+    if len(axes) != pairs:
+        _fail(f"axes has {len(axes)} entries, the tables {pairs} pairs")
+    if any(type(a) is not int or not 0 <= a < 4 for a in axes):
+        _fail("axes are 0, 1, 2 or 3")
+    return (ctypes.c_uint8 * max(1, pairs))(*axes), max(axes, default=-1)
+
+
+def _axes_args(axes, positions, cos, *shape):
+    """(axes of the pairs, number of axes) for the C entries; positions [axes, *shape]."""
+    if cos is None:
+        _fail("axes need cos and sin")
+    if not isinstance(positions, torch.Tensor):
+        _fail("axes need positions")
+    if cos.dim() != 2:
+        _fail("cos and sin must have one shape [positions, rotated features / 2]")
+    pairs, top = _pair_axes(tuple(axes), cos.shape[1])
+    n = positions.shape[0] if positions.dim() else 0
+    _int32("positions", positions, n, *shape)
+    if top >= n:
+        _fail(f"positions have {n} axes, axes names {top}")
+    _sizes_fit(positions=positions)
+    return pairs, n
+
+
+def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm, axes):
     """What ``_rope_args`` returns, of arguments that pass its checks by a few
     comparisons and need no copies; None of others, which go through them (the
     checks one by one took half of a small call's host time)."""
@@ -148,14 +176,21 @@ def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
         return None
     per_batch = 0
     if positions is None:
-        if S > sc[0]:
+        if S > sc[0] or axes is not None:
             return None
     else:
         sp = positions.shape
+        if axes is not None:
+            pairs, top = _pair_axes(axes if type(axes) is tuple else tuple(axes), sc[1])
+            if not 2 <= len(sp) <= 3 or not top < sp[0] <= _MOST:
+                return None
+            n_axes, sp = sp[0], sp[1:]
         per_batch = int(len(sp) == 2)
         if (sp != ((B, S) if per_batch else (S,)) or positions.dtype is not _I32 or positions.device != device
                 or not positions.is_contiguous()):
             return None
+        if axes is not None:
+            per_batch = (per_batch, pairs, n_axes)
     w_code = DTYPE_F32
     if w is not None or k_weight is not None:
         if (not norm or w is None or k_weight is None or w.dtype is not k_weight.dtype or w.dtype not in (T, _F32)
@@ -166,9 +201,9 @@ def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm):
     return code, (B, S, H_q, sk[2], D, 2 * sc[1]), (cos, sin, sc[0]), (w, k_weight, w_code), positions, per_batch
 
 
-def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm):
+def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm, axes=None):
     """Checks of what the forward and the gradient have in common."""
-    plain = _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm)
+    plain = _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm, axes)
     if plain is not None:
         return plain
     _check_qk(q, k)
@@ -177,7 +212,11 @@ def _rope_args(q, k, cos, sin, q_weight, k_weight, positions, norm):
     rows, R = _tables(cos, sin)
     w_code = _weight_dtype(q.dtype, D, q_weight, k_weight, norm)
     per_batch = 0
-    if positions is not None:
+    if axes is not None:
+        per_batch = int(isinstance(positions, torch.Tensor) and positions.dim() == 3)
+        per_batch = (per_batch,) + _axes_args(axes, positions, cos, *((B, S) if per_batch else (S,)))
+        positions = positions.contiguous()
+    elif positions is not None:
         per_batch = int(positions.dim() == 2)
         _int32("positions", positions, *((B, S) if per_batch else (S,)))
         positions = positions.contiguous()
@@ -196,7 +235,7 @@ def _out_rows(like, B, S, H, D, fold_heads):
 
 
 def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
-                 norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+                 norm: bool = True, interleaved: bool = False, fold_heads: bool = True, axes=None):
     """RMS norm of every head of q and k, and its rotation by position: ``(q_out, k_out)``.
 
     q [B, S, H_q, D] and k [B, S, H_kv, D] (fp16 or fp32; any strides, so both may be parts of one
@@ -206,22 +245,29 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, e
     cos and sin [P, R / 2]: pairs (i, i + R/2), or (2i, 2i + 1) if ``interleaved``; without tables
     (None) nothing is.  A position outside the tables makes its rows NaN.
 
+    ``axes``: tokens with several positions (time, height, width): the axis that each of the R/2 pairs
+    follows, as a sequence of numbers below 4 ((0,) * 16 + (1,) * 24 + (2,) * 24: the first 16 pairs time, and so on);
+    positions are then int32 [axes, S] or [axes, B, S].
+
     ``fold_heads``: results [B * H, S, D], the layout of ``sdpa``; else [B, S, H, D].
     """
     code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
-        q, k, cos, sin, q_weight, k_weight, positions, norm)
+        q, k, cos, sin, q_weight, k_weight, positions, norm, axes)
     q, k = _dense_features(q), _dense_features(k)
     q_out, qos = _out_rows(q, B, S, H_q, D, fold_heads)
     k_out, kos = _out_rows(k, B, S, H_kv, D, fold_heads)
-    _call(library().sdpa_hip_qk_norm_rope, q.device, code, q.data_ptr(), _strides3(q.stride()), k.data_ptr(), _strides3(k.stride()),
+    L = library()
+    entry = L.sdpa_hip_qk_norm_rope if axes is None else L.sdpa_hip_qk_norm_rope_axes
+    by = (per_batch,) if axes is None else per_batch
+    _call(entry, q.device, code, q.data_ptr(), _strides3(q.stride()), k.data_ptr(), _strides3(k.stride()),
           q_out.data_ptr(), qos, k_out.data_ptr(), kos, _ptr(weights[0]), _ptr(weights[1]), weights[2],
-          _ptr(tables[0]), _ptr(tables[1]), tables[2], _ptr(positions), per_batch, B, S, H_q, H_kv, D, R, float(eps),
+          _ptr(tables[0]), _ptr(tables[1]), tables[2], _ptr(positions), *by, B, S, H_q, H_kv, D, R, float(eps),
           int(bool(norm)), int(bool(interleaved)))
     return q_out, k_out
 
 
 def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=None, positions=None,
-                      eps: float = 1e-6, norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+                      eps: float = 1e-6, norm: bool = True, interleaved: bool = False, fold_heads: bool = True, axes=None):
     """Gradient of ``qk_norm_rope``: ``(dq, dk, dq_weight, dk_weight)``.
 
     ``d_q_out`` and ``d_k_out`` are laid out as its results; dq and dk come as
@@ -229,7 +275,7 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
     weight that was not given.
     """
     code, (B, S, H_q, H_kv, D, R), tables, weights, positions, per_batch = _rope_args(
-        q, k, cos, sin, q_weight, k_weight, positions, norm)
+        q, k, cos, sin, q_weight, k_weight, positions, norm, axes)
     L = library()
     _on_device(q.device, d_q_out=d_q_out, d_k_out=d_k_out)
     grads = []
@@ -248,10 +294,12 @@ def qk_norm_rope_grad(d_q_out, d_k_out, q, k, cos, sin, q_weight=None, k_weight=
     if dw[0] is not None or dw[1] is not None:
         ws_bytes = L.sdpa_hip_qk_norm_rope_grad_workspace_bytes(D)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
-    _call(L.sdpa_hip_qk_norm_rope_grad, q.device, code, grads[0][0].data_ptr(), grads[0][1], grads[1][0].data_ptr(),
+    entry = L.sdpa_hip_qk_norm_rope_grad if axes is None else L.sdpa_hip_qk_norm_rope_axes_grad
+    by = (per_batch,) if axes is None else per_batch
+    _call(entry, q.device, code, grads[0][0].data_ptr(), grads[0][1], grads[1][0].data_ptr(),
           grads[1][1], q.data_ptr(), _strides3(q.stride()), k.data_ptr(), _strides3(k.stride()), dq.data_ptr(), None, dk.data_ptr(),
           None, _ptr(dw[0]), _ptr(dw[1]), _ptr(weights[0]), _ptr(weights[1]), weights[2], _ptr(tables[0]),
-          _ptr(tables[1]), tables[2], _ptr(positions), per_batch, _ptr(ws), ws_bytes, B, S, H_q, H_kv, D, R,
+          _ptr(tables[1]), tables[2], _ptr(positions), *by, _ptr(ws), ws_bytes, B, S, H_q, H_kv, D, R,
           float(eps), int(bool(norm)), int(bool(interleaved)))
     return dq, dk, dw[0], dw[1]
 
@@ -262,16 +310,16 @@ def _make_function():
         """``qk_norm_rope`` with its gradient for q, k and the weights."""
 
         @staticmethod
-        def forward(ctx, q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads):
+        def forward(ctx, q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads, axes):
             ctx.save_for_backward(q, k, cos, sin, q_weight, k_weight, positions)
-            ctx.attrs = dict(eps=eps, norm=norm, interleaved=interleaved, fold_heads=fold_heads)
+            ctx.attrs = dict(eps=eps, norm=norm, interleaved=interleaved, fold_heads=fold_heads, axes=axes)
             return qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, **ctx.attrs)
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, d_q_out, d_k_out):
             dq, dk, dqw, dkw = qk_norm_rope_grad(d_q_out, d_k_out, *ctx.saved_tensors, **ctx.attrs)
-            return dq, dk, None, None, dqw, dkw, None, None, None, None, None
+            return dq, dk, None, None, dqw, dkw, None, None, None, None, None, None
 
     return QkNormRopeFunction
 
@@ -280,12 +328,12 @@ _fn = None
 
 
 def qk_norm_rope_autograd(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, eps: float = 1e-6,
-                          norm: bool = True, interleaved: bool = False, fold_heads: bool = True):
+                          norm: bool = True, interleaved: bool = False, fold_heads: bool = True, axes=None):
     """Differentiable ``qk_norm_rope`` (once; no gradient for the tables)."""
     global _fn
     if _fn is None:
         _fn = _make_function()
-    return _fn.apply(q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads)
+    return _fn.apply(q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads, axes)
 
 
 def _check_cache(k_cache, v_cache, T):
@@ -388,8 +436,86 @@ def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, nor
     return code, sc[0], 2 * sc[1], DTYPE_F32
 
 
+Reserved = collections.namedtuple("Reserved", "q_starts kv_lens free_count positions slots")
+
+
+def _vector(name, t, n, *dtypes):
+    """``t`` is a dense vector of n entries (None: of any number) of one of the dtypes."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        _fail(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}")
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        _fail(f"{name} must have shape [{'entries' if n is None else n}], got {list(t.shape)}")
+    if not t.is_contiguous():
+        _fail(f"{name} must be contiguous")
+
+
+def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size: int, total: int, finished=None,
+               in_place: bool = False):
+    """Pages for the new tokens of a batch, and where each token goes, all on the GPU.
+
+    page_table int32 [N, pages per sequence] and kv_lens int32 [N] say what the N sequences hold,
+    new_lens int32 [N] how many tokens each of them gets, free_pages int32 [capacity] is a stack of pages that
+    none holds: its first free_count (int32 [1]) entries.  Sequences with ``finished`` (bool or uint8 [N])
+    first give the pages of their tokens back; their length is 0 then (new tokens begin a new sequence there).
+    Every column that the new tokens are the first to need gets the page on top of the stack, in the order
+    sequence, column; once the stack is empty -1.  page_table and free_pages are changed in place.
+
+    Returns ``Reserved``: q_starts [N + 1] and kv_lens [N], as ``kv_append`` and ``paged_sdpa`` take them;
+    free_count [1]; and for the ``total`` packed tokens positions (int32, the place in the sequence) and
+    slots (int64, page * page_size + row; -1 without a page), -1 behind the last.  ``in_place``: kv_lens
+    and free_count are the tensors given, changed (for a captured step that is replayed).
+
+    More tokens than ``total`` have no rows: ``kv_append`` and ``paged_sdpa`` leave out sequences that reach past it.
+    """
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        _fail("page_table must be [sequences, pages per sequence]")
+    N, width = page_table.shape
+    _int32("page_table", page_table, N, width)
+    if (width > 1 and page_table.stride(1) != 1) or (N > 1 and page_table.stride(0) < width):
+        _fail("the rows of page_table must be contiguous and memory of their own")
+    _vector("kv_lens", kv_lens, N, _I32)
+    _vector("new_lens", new_lens, N, _I32)
+    _vector("free_pages", free_pages, None, _I32)
+    _vector("free_count", free_count, 1, _I32)
+    if finished is not None:
+        _vector("finished", finished, N, torch.bool, torch.uint8)
+    if type(page_size) is not int or type(total) is not int or not 0 <= total <= _MOST or not 0 < page_size <= _MOST:
+        _fail("page_size and total must be sizes")
+    _sizes_fit(page_table=page_table, free_pages=free_pages)
+    device = page_table.device
+    _on_device(device, kv_lens=kv_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count, finished=finished)
+    states = {"page_table": page_table, "free_pages": free_pages, "kv_lens": kv_lens, "free_count": free_count}
+    if _share_memory(free_pages, page_table) or any(
+            _share_memory(t, s) for t in (kv_lens, free_count, new_lens) + (() if finished is None else (finished,))
+            for s in (page_table, free_pages)):
+        _fail(f"{', '.join(states)} must not share memory")
+    if in_place and (_share_memory(kv_lens, free_count) or _share_memory(kv_lens, new_lens) or _share_memory(free_count, new_lens)
+                     or (finished is not None and (_share_memory(kv_lens, finished) or _share_memory(free_count, finished)))):
+        _fail("kv_lens and free_count must be memory of their own")
+    new = lambda n, dtype: torch.empty((n,), dtype=dtype, device=device)  # noqa: E731
+    out = Reserved(new(N + 1, _I32), kv_lens if in_place else new(N, _I32), free_count if in_place else new(1, _I32),
+                   new(total, _I32), new(total, torch.int64))
+    _call(library().sdpa_hip_kv_reserve, device, page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
+          new_lens.data_ptr(), _ptr(finished), free_pages.data_ptr(), free_count.data_ptr(), *(t.data_ptr() for t in out), N, total,
+          width, page_size, free_pages.shape[0])
+    return out
+
+
+def _append_positions(positions, axes, cos, n, device):
+    """Positions [axes, n] of the new tokens, the axes of the pairs and their number; [n]
+    without ``axes``: one axis."""
+    if axes is None:
+        if cos is None:
+            _fail("positions need cos and sin")
+        _int32("positions", positions, n)
+        positions, axes = positions[None], (0,) * cos.shape[1]
+    pairs, n_axes = _axes_args(axes, positions, cos, n)
+    _on_device(device, positions=positions)
+    return positions.contiguous(), pairs, n_axes
+
+
 def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, sin=None, q=None, q_weight=None,
-              k_weight=None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False):
+              k_weight=None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, positions=None, axes=None):
     """Appends new tokens to a paged cache, in place, and returns their rotated queries.
 
     k [T, H_kv, D_qk] and v [T, H_kv, D_v] are the packed new tokens of N sequences (any strides):
@@ -398,7 +524,8 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     page_table[s, j // page] (int32 [N, pages per sequence]) of the caches [pages, H_kv, page, D],
     page a power of two of at least 16.  On the way k is normed (``norm``, ``k_weight``) and rotated
     by j as in ``qk_norm_rope`` (cos and sin None: not), and so is q [T, H_q, D_qk], where given:
-    the result is [T, H_q, D_qk], else None.
+    the result is [T, H_q, D_qk], else None.  ``positions``: what the tokens are rotated by instead of their
+    places j: int32 [T], or [axes, T] with ``axes``, the axis of each rotated pair, as in ``qk_norm_rope``.
 
     Tokens behind the last sequence are skipped (their rows of the result are not written).  A token
     without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
@@ -406,6 +533,11 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     Any width up to 128 can be cached; ``paged_sdpa`` reads multiples of 8 (fp16) or 4 (fp32).
     """
     T, device = k.dtype, k.device
+    L = library()
+    entry, by = L.sdpa_hip_kv_append, ()
+    if positions is not None or axes is not None:
+        positions, pairs, n_axes = _append_positions(positions, axes, cos, k.shape[0], device)
+        entry, by = L.sdpa_hip_kv_append_axes, (positions.data_ptr(), pairs, n_axes)
     batch = _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
     checked = None
     if batch is not None:
@@ -425,9 +557,9 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     if q is not None:
         q = _dense_features(q)
         q_out = torch.empty((n, H_q, D_qk), dtype=T, device=device)
-    _call(library().sdpa_hip_kv_append, device, code, k.data_ptr(), _strides2(k.stride()), v.data_ptr(), _strides2(v.stride()),
+    _call(entry, device, code, k.data_ptr(), _strides2(k.stride()), v.data_ptr(), _strides2(v.stride()),
           k_cache.data_ptr(), v_cache.data_ptr(), _ptr(q), None if q is None else _strides2(q.stride()), _ptr(q_out), None,
-          _ptr(q_weight), _ptr(k_weight), w_code, _ptr(cos), _ptr(sin), rows, page_table.data_ptr(),
+          _ptr(q_weight), _ptr(k_weight), w_code, _ptr(cos), _ptr(sin), rows, *by, page_table.data_ptr(),
           page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, R, float(eps), int(bool(norm)), int(bool(interleaved)))
     return q_out
