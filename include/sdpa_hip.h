@@ -394,6 +394,41 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
                        int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int max_q_len, float scale,
                        int causal_mask, hipStream_t stream);
 
+/* ---- paged cache in 4 bits -------------------------------------------------------
+ * No counterpart in the reference.  A value is s c, c one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a
+ * sign (a code: sign 8, then the place in this list) and s a scale that 32 neighbouring
+ * features of a token and head share (a byte: the upper one of an fp16, e5m2).  s is the
+ * largest |x| of the 32 over 6, rounded to nearest even, at most 10240; c is x / s, rounded
+ * to nearest even, at most 6 in size (so what passes 61440 comes back as that).  Every
+ * value is exact in fp16.  32 features with an infinity or a NaN among them are NaN.
+ * k_cache and v_cache: bytes [pages, H_kv, page_size * 17 D / 32], 16-byte aligned, a page's
+ * head its codes, then its scales:
+ *   k  codes [page_size][D / 2], the feature before in the lower half; scales [page_size][D / 32]
+ *   v  codes [page_size / 8][D][4]: 8 tokens of a feature, the token before in the lower
+ *      half; scales [page_size / 8][D / 32][8]
+ * D_qk and D_v are 32, 64, 96 or 128.                                          */
+
+/* As sdpa_hip_kv_append (pair_axes NULL) or sdpa_hip_kv_append_axes, into such a cache.
+ * The keys' norm and rotation are formed in fp64 and rounded to fp32 before they are
+ * rounded to 4 bits.  The tokens 8 i .. 8 i + 7 of a page share words: no two sequences of
+ * a call may append to the same 8.  Other tokens of the 8 keep their values.       */
+int sdpa_hip_kv_append_fp4(int dtype, const void* k, const int64_t* k_strides, const void* v,
+                           const int64_t* v_strides, void* k_cache, void* v_cache, const void* q,
+                           const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* q_weight,
+                           const void* k_weight, int weight_dtype, const float* cos, const float* sin, int table_rows,
+                           const int32_t* positions, const uint8_t* pair_axes, int n_axes, const int32_t* page_table,
+                           int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T,
+                           int width, int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps,
+                           int norm, int interleaved, hipStream_t stream);
+
+/* The values of the T tokens of a batch out of such a cache: k [T, H_kv, D_qk] and v
+ * [T, H_kv, D_v] of dtype, dense, 16-byte aligned.  Rows of a token without a place are NaN,
+ * those of no sequence stay as they were.                                       */
+int sdpa_hip_kv_read_fp4(int dtype, const void* k_cache, const void* v_cache, void* k, void* v,
+                         const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
+                         const int32_t* kv_lens, int N, int T, int width, int pages, int page_size, int H_kv, int D_qk,
+                         int D_v, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

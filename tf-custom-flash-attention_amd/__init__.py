@@ -132,6 +132,10 @@ def library():
     L.sdpa_hip_kv_append_axes.restype = i32
     L.sdpa_hip_kv_append_axes.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + [i32p, vp, i32] + batch +
                                           [i32] * 10 + [f32, i32, i32, vp])
+    L.sdpa_hip_kv_append_fp4.restype = i32
+    L.sdpa_hip_kv_append_fp4.argtypes = L.sdpa_hip_kv_append_axes.argtypes
+    L.sdpa_hip_kv_read_fp4.restype = i32
+    L.sdpa_hip_kv_read_fp4.argtypes = [i32] + [vp] * 4 + batch + [i32] * 8 + [vp]
     L.sdpa_hip_paged_fwd_workspace_bytes.restype = sz
     L.sdpa_hip_paged_fwd_workspace_bytes.argtypes = [i32] * 10
     L.sdpa_hip_paged_fwd.restype = i32
@@ -369,7 +373,8 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
     return _fn.apply(q, k, v, seed, offset, dropout, scale, causal_mask)
 
 
-_HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_reserve", "Reserved", "kv_append", "paged_sdpa")
+_HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_reserve", "Reserved", "kv_append", "paged_sdpa", "fp4_cache",
+          "kv_append_fp4", "kv_read_fp4")
 
 
 def __getattr__(name):

@@ -49,4 +49,19 @@ struct AppendParams {
 
 hipError_t launch_kv_append(const AppendParams& p, DType dtype, hipStream_t stream);
 
+// The same into a cache in 4 bits (sdpa_kv_fp4.hip; all bytes of a page's head in
+// a row), and its tokens out again.  D_qk and D_v are multiples of 32.
+struct Fp4ReadParams {
+    PagedBatch batch;
+    const void* k_cache;
+    const void* v_cache;
+    void* k;  // [T, H_kv, D_qk]
+    void* v;  // [T, H_kv, D_v]
+    int H_kv, D_qk, D_v;
+};
+// From so many windows of 8 tokens (and heads) on a wave takes 8 tokens, else one.
+constexpr int kFp4FewWindows = 1024;
+hipError_t launch_kv_append_fp4(const AppendParams& p, DType dtype, hipStream_t stream);
+hipError_t launch_kv_read_fp4(const Fp4ReadParams& p, DType dtype, hipStream_t stream);
+
 }  // namespace sdpa

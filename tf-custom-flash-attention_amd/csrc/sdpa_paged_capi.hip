@@ -164,17 +164,22 @@ void add_tokens(Chunks& c, const void* p, const sdpa::TokenStrides& s) {
     c.stride(s.h);
 }
 
+// Feature sizes of a cache in 4 bits.
+bool fp4_width(int D) { return D > 0 && D % 32 == 0 && D <= 128; }
+bool aligned16(const void* a, const void* b) { return (((uintptr_t)a | (uintptr_t)b) & 15u) == 0; }
+
 int append_entry(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_cache,
                  void* v_cache, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
                  const void* q_weight, const void* k_weight, int weight_dtype, const float* cos, const float* sin,
                  int table_rows, const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
                  const int32_t* kv_lens, int N, int T, int width, int pages, int page_size, int H_q, int H_kv, int D_qk,
                  int D_v, int R, float eps, int norm, int interleaved, hipStream_t stream, bool by_axes,
-                 const int32_t* positions, const uint8_t* pair_axes, int n_axes) {
+                 const int32_t* positions, const uint8_t* pair_axes, int n_axes, bool fp4 = false) {
     int st = check_rows(dtype, weight_dtype, q_weight, k_weight, cos, sin, table_rows, D_qk, R, norm);
     if (st != SDPA_OK) return st;
     if (H_q < 0 || H_kv < 0 || D_v < 0) return SDPA_ERR_NEGATIVE_DIM;
     if (D_v > 128) return SDPA_ERR_FEATURE_TOO_LARGE;
+    if (fp4 && !(fp4_width(D_qk) && fp4_width(D_v))) return SDPA_ERR_FP4_WIDTH;
     sdpa::AppendParams p{};
     st = make_batch(p.batch, page_table, page_table_stride, q_starts, kv_lens, N, T, width, pages, page_size);
     if (st != SDPA_OK) return st;
@@ -217,6 +222,7 @@ int append_entry(int dtype, const void* k, const int64_t* k_strides, const void*
     ch.address(sin);
     ch.address(k_cache);
     ch.address(v_cache);
+    if (fp4 && !ch.ok && !aligned16(k_cache, v_cache)) return SDPA_ERR_LAYOUT;
     ch.address(q_weight);
     ch.address(k_weight);
     if (has_q) {
@@ -226,7 +232,8 @@ int append_entry(int dtype, const void* k, const int64_t* k_strides, const void*
     if (has_k) add_tokens(ch, k, p.ks);
     if (has_v) add_tokens(ch, v, p.vs);
     p.vec = ch.ok;
-    return hip_status(sdpa::launch_kv_append(p, (sdpa::DType)dtype, stream));
+    return hip_status(fp4 ? sdpa::launch_kv_append_fp4(p, (sdpa::DType)dtype, stream)
+                          : sdpa::launch_kv_append(p, (sdpa::DType)dtype, stream));
 }
 
 }  // namespace
@@ -430,6 +437,44 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     if (dtype == SDPA_DTYPE_F32)
         return hip_status(small ? sdpa::launch_paged_f32_small(p, stream) : sdpa::launch_paged_f32(p, stream));
     return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));
+}
+
+int sdpa_hip_kv_append_fp4(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                           void* k_cache, void* v_cache, const void* q, const int64_t* q_strides, void* q_out,
+                           const int64_t* q_out_strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                           const float* cos, const float* sin, int table_rows, const int32_t* positions,
+                           const uint8_t* pair_axes, int n_axes, const int32_t* page_table, int64_t page_table_stride,
+                           const int32_t* q_starts, const int32_t* kv_lens, int N, int T, int width, int pages,
+                           int page_size, int H_q, int H_kv, int D_qk, int D_v, int R, float eps, int norm,
+                           int interleaved, hipStream_t stream) {
+    return append_entry(dtype, k, k_strides, v, v_strides, k_cache, v_cache, q, q_strides, q_out, q_out_strides, q_weight,
+                        k_weight, weight_dtype, cos, sin, table_rows, page_table, page_table_stride, q_starts, kv_lens, N, T,
+                        width, pages, page_size, H_q, H_kv, D_qk, D_v, R, eps, norm, interleaved, stream, pair_axes != nullptr,
+                        positions, pair_axes, n_axes, true);
+}
+
+int sdpa_hip_kv_read_fp4(int dtype, const void* k_cache, const void* v_cache, void* k, void* v, const int32_t* page_table,
+                         int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, int N, int T, int width,
+                         int pages, int page_size, int H_kv, int D_qk, int D_v, hipStream_t stream) {
+    if (dtype != SDPA_DTYPE_F32 && dtype != SDPA_DTYPE_F16) return SDPA_ERR_DTYPE;
+    if (H_kv < 0 || D_qk < 0 || D_v < 0) return SDPA_ERR_NEGATIVE_DIM;
+    if (D_qk > 128 || D_v > 128) return SDPA_ERR_FEATURE_TOO_LARGE;
+    if (!fp4_width(D_qk) || !fp4_width(D_v)) return SDPA_ERR_FP4_WIDTH;
+    sdpa::Fp4ReadParams p{};
+    const int st = make_batch(p.batch, page_table, page_table_stride, q_starts, kv_lens, N, T, width, pages, page_size);
+    if (st != SDPA_OK) return st;
+    if (!rows_fit(T, 0, 2LL * H_kv)) return SDPA_ERR_TOO_LARGE;
+    if (N == 0 || T == 0 || H_kv == 0) return SDPA_OK;
+    if (!k || !v || (pages > 0 && (!k_cache || !v_cache))) return SDPA_ERR_NULL_POINTER;
+    if (!aligned16(k_cache, v_cache) || !aligned16(k, v)) return SDPA_ERR_LAYOUT;
+    p.k_cache = k_cache;
+    p.v_cache = v_cache;
+    p.k = k;
+    p.v = v;
+    p.H_kv = H_kv;
+    p.D_qk = D_qk;
+    p.D_v = D_v;
+    return hip_status(sdpa::launch_kv_read_fp4(p, (sdpa::DType)dtype, stream));
 }
 
 }  // extern "C"

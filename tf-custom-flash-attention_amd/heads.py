@@ -21,7 +21,7 @@ _Strides3 = ctypes.c_int64 * 3
 _Strides2 = ctypes.c_int64 * 2
 
 
-_F32, _I32 = torch.float32, torch.int32
+_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
 _MOST = 0x7FFFFFFF  # of any size: the C entries take them as int
 _CODES = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
 
@@ -342,7 +342,7 @@ def _check_cache(k_cache, v_cache, T):
     if k_cache.shape[:3] != v_cache.shape[:3]:
         _fail(f"k_cache {list(k_cache.shape)} and v_cache {list(v_cache.shape)} differ in pages, heads or page size")
     if k_cache.dtype != T or v_cache.dtype != T:
-        _fail("the caches must have the same dtype T as the tokens")
+        _fail("a cache in 4 bits is uint8 (fp4_cache)" if T is _U8 else "the caches must have the same dtype T as the tokens")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         _fail("k_cache and v_cache must be contiguous")
     _sizes_fit(k_cache=k_cache, v_cache=v_cache)
@@ -388,18 +388,19 @@ def _check_tokens(name, t, T, features=None):
         _sizes_fit(**{name: t})
 
 
-def _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm):
+def _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm, fp4):
     """Checks of ``kv_append``: (N, width) and (dtype code, table rows, rotated features, weights' code)."""
     T = k.dtype
     _check_tokens("k", k, T)
     _check_tokens("v", v, T)
     code = _dtype_code(k)
-    _check_cache(k_cache, v_cache, T)
+    _check_cache(k_cache, v_cache, _U8 if fp4 else T)
     batch = _check_batch(page_table, q_starts, kv_lens)
     n, H_kv, D_qk = k.shape
     if v.shape[:2] != k.shape[:2]:
         _fail(f"k {list(k.shape)} and v {list(v.shape)} differ in tokens or heads")
-    if k_cache.shape[1] != H_kv or k_cache.shape[3] != D_qk or v_cache.shape[3] != v.shape[2]:
+    row_k, row_v = (_fp4_bytes(D_qk), _fp4_bytes(v.shape[2])) if fp4 else (D_qk, v.shape[2])
+    if k_cache.shape[1] != H_kv or k_cache.shape[3] != row_k or v_cache.shape[3] != row_v or (fp4 and not (row_k and row_v)):
         _fail(f"the caches {list(k_cache.shape)}, {list(v_cache.shape)} do not hold rows of k {list(k.shape)} and v "
               f"{list(v.shape)}")
     if q is not None:
@@ -413,7 +414,7 @@ def _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, si
     return batch, (code, rows, R, w_code)
 
 
-def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, norm):
+def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, norm, fp4):
     """What ``_check_append`` returns second, of usual arguments that pass its
     checks by a few comparisons; None of others."""
     sk, sv, T, device = k.shape, v.shape, k.dtype, k.device
@@ -423,7 +424,8 @@ def _plain_append(k, v, sk_cache, sv_cache, cos, sin, q, q_weight, k_weight, nor
         return None
     n, H_kv, D = sk
     sq, sc = q.shape, cos.shape
-    if not (sv[0] == n and sv[1] == H_kv == sk_cache[1] and sk_cache[3] == D and sv_cache[3] == sv[2] and len(sq) == 3
+    row_k, row_v = (_fp4_bytes(D), _fp4_bytes(sv[2])) if fp4 else (D, sv[2])
+    if not (sv[0] == n and sv[1] == H_kv == sk_cache[1] and sk_cache[3] == row_k and sv_cache[3] == row_v and len(sq) == 3
             and sq[0] == n and sq[2] == D and len(sc) == 2 and sin.shape == sc and cos.dtype is _F32 and sin.dtype is _F32
             and sum(sq) + sum(sc) <= _MOST):
         return None
@@ -532,19 +534,27 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     of a call may have the same place.  D_qk or D_v may be 0 (a cache of keys or of values alone).
     Any width up to 128 can be cached; ``paged_sdpa`` reads multiples of 8 (fp16) or 4 (fp32).
     """
+    return _append(False, k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm, eps,
+                   interleaved, positions, axes)
+
+
+def _append(fp4, k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm, eps, interleaved,
+            positions, axes):
     T, device = k.dtype, k.device
     L = library()
-    entry, by = L.sdpa_hip_kv_append, ()
+    entry, by = (L.sdpa_hip_kv_append_fp4, (None, None, 0)) if fp4 else (L.sdpa_hip_kv_append, ())
     if positions is not None or axes is not None:
         positions, pairs, n_axes = _append_positions(positions, axes, cos, k.shape[0], device)
-        entry, by = L.sdpa_hip_kv_append_axes, (positions.data_ptr(), pairs, n_axes)
-    batch = _plain_batch(device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
+        by = (positions.data_ptr(), pairs, n_axes)
+        if not fp4:
+            entry = L.sdpa_hip_kv_append_axes
+    batch = _plain_batch(device, _U8 if fp4 else T, k_cache, v_cache, page_table, q_starts, kv_lens)
     checked = None
     if batch is not None:
-        checked = _plain_append(k, v, k_cache.shape, v_cache.shape, cos, sin, q, q_weight, k_weight, norm)
+        checked = _plain_append(k, v, k_cache.shape, v_cache.shape, cos, sin, q, q_weight, k_weight, norm, fp4)
     if checked is None:
         batch, checked = _check_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight,
-                                       k_weight, norm)
+                                       k_weight, norm, fp4)
     N, width = batch
     code, rows, R, w_code = checked
     n, H_kv, D_qk = k.shape
@@ -563,6 +573,72 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
           page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, R, float(eps), int(bool(norm)), int(bool(interleaved)))
     return q_out
+
+
+def _fp4_bytes(D):
+    """Bytes of a token's D features in a cache in 4 bits (0: no such width)."""
+    return D // 2 + D // 32 if D % 32 == 0 and 0 < D <= 128 else 0
+
+
+def _fp4_features(cache):
+    """Features of a cache in 4 bits."""
+    D = cache.shape[3] // 17 * 32
+    if not cache.shape[3] or _fp4_bytes(D) != cache.shape[3]:
+        _fail(f"a cache in 4 bits has 17, 34, 51 or 68 bytes a token and head, not {cache.shape[3]}")
+    return D
+
+
+def fp4_cache(pages: int, heads: int, page_size: int, D_qk: int, D_v: int, device="cuda"):
+    """An empty cache in 4 bits: ``(k_cache, v_cache)``, uint8 [pages, heads, page_size, 17 * D / 32].
+
+    32 neighbouring features of a token and head share a scale (8 bits), so a value takes 4.25 bits; D_qk and
+    D_v are 32, 64, 96 or 128.  What a value becomes, and where the bytes of a page lie, stands in
+    ``include/sdpa_hip.h``.  ``kv_append_fp4`` fills it, ``paged_sdpa_fp4`` attends over it, ``kv_read_fp4`` reads it.
+    """
+    for D in (D_qk, D_v):
+        if not _fp4_bytes(D):
+            _fail(f"feature sizes of a cache in 4 bits must be 32, 64, 96 or 128, got {D}")
+    if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+        _fail("tokens per page must be a power of two from 16 to 65536")
+    return tuple(torch.zeros((pages, heads, page_size, _fp4_bytes(D)), dtype=_U8, device=device) for D in (D_qk, D_v))
+
+
+def kv_append_fp4(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, sin=None, q=None, q_weight=None,
+                  k_weight=None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, positions=None, axes=None):
+    """``kv_append`` into a cache in 4 bits (``fp4_cache``), with the same arguments and result.
+
+    The keys are rounded after norm and rotation, which are formed in fp64 for them, so that a token's codes do
+    not depend on what else is in the call.  Groups of 32 features that hold an infinity or a NaN become
+    NaN, values beyond 61440 in size become that.  No two sequences of a call may append to the same 8 tokens (8 i .. 8 i + 7) of a page.
+    """
+    return _append(True, k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos, sin, q, q_weight, k_weight, norm, eps,
+                   interleaved, positions, axes)
+
+
+def kv_read_fp4(k_cache, v_cache, page_table, q_starts, kv_lens, total: int, dtype=torch.float16):
+    """The values of a batch's tokens out of a cache in 4 bits: ``(k, v)``, [total, H_kv, D] in ``dtype``.
+
+    The batch as in ``kv_append``: of sequence s its last q_starts[s + 1] - q_starts[s] cached tokens (all of them where that
+    is kv_lens[s]).  The values are exact (fp16 or fp32).  Rows of a token without a place are NaN,
+    those behind the last sequence arbitrary.
+    """
+    batch = _plain_batch(k_cache.device, _U8, k_cache, v_cache, page_table, q_starts, kv_lens)
+    if batch is None:
+        _check_cache(k_cache, v_cache, _U8)
+        batch = _check_batch(page_table, q_starts, kv_lens)
+        _on_device(k_cache.device, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
+    if type(total) is not int or not 0 <= total <= _MOST:
+        _fail("total must be a size")
+    if dtype not in _CODES:
+        _fail(f"T must be half or float, got {dtype}")
+    N, width = batch
+    pages, H_kv, page, _ = k_cache.shape
+    D_qk, D_v = _fp4_features(k_cache), _fp4_features(v_cache)
+    k, v = (torch.empty((total, H_kv, D), dtype=dtype, device=k_cache.device) for D in (D_qk, D_v))
+    _call(library().sdpa_hip_kv_read_fp4, k_cache.device, _CODES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(),
+          v.data_ptr(), page_table.data_ptr(), page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, total, width,
+          pages, page, H_kv, D_qk, D_v)
+    return k, v
 
 
 def _whole_chunks(t):
