@@ -429,6 +429,18 @@ int sdpa_hip_kv_read_fp4(int dtype, const void* k_cache, const void* v_cache, vo
                          const int32_t* kv_lens, int N, int T, int width, int pages, int page_size, int H_kv, int D_qk,
                          int D_v, hipStream_t stream);
 
+/* Attention of new tokens over such a cache: as sdpa_hip_paged_fwd, with queries and o
+ * of dtype, over the values.  A value is NaN where its scale is.                  */
+size_t sdpa_hip_paged_fwd_fp4_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
+                                              int D_qk, int D_v, int max_q_len);
+
+int sdpa_hip_paged_fwd_fp4(int dtype, const void* q, const int64_t* q_strides, const void* k_cache,
+                           const void* v_cache, void* o, const int64_t* o_strides, float* stats,
+                           const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
+                           const int32_t* kv_lens, void* workspace, size_t workspace_bytes, int N, int T, int width,
+                           int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int max_q_len, float scale,
+                           int causal_mask, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,3 +90,35 @@ def test_abi_refusals(pkg):
             assert fn(**kw) == code, (fn, kw)
         assert fn(T=0) == 0 and fn(N=0) == 0
     assert read(k=odd) == 29 and "32" in pkg.status_string(33)
+
+
+@pytest.mark.parametrize("change,message", CHANGES + [
+    (dict(k=(6, 2, 32)), "q has 32 features, k_cache 64"),
+    (dict(k=(6, 64)), "q must be"),
+])
+def test_paged_refusals(pkg, change, message):
+    t = _tensors(change)
+    q = t.pop("k")
+    del t["v"]
+    if t["k_cache"].dim() == 4 and t["k_cache"].shape[3] == 102:
+        message = "bytes a token"
+    _refused(pkg, message, pkg.paged_sdpa_fp4, q, **t)
+
+
+def test_paged_abi_refusals(pkg):
+    L = pkg.library()
+    some, odd = ctypes.c_void_p(64), ctypes.c_void_p(72)
+
+    def call(dtype=1, N=3, T=6, width=4, pages=9, page=16, H_q=4, H_kv=2, D=32, D_v=64, q=some, table=some, stats=some, k=some):
+        return L.sdpa_hip_paged_fwd_fp4(dtype, q, None, k, some, some, None, stats, table, width, some, some, None, 0, N, T,
+                                        width, pages, page, H_q, H_kv, D, D_v, 0, 0.5, 1, None)
+
+    for kw, code in ((dict(dtype=2), 18), (dict(N=-1), 19), (dict(width=-1), 19), (dict(H_q=-4), 19), (dict(D=160), 16),
+                     (dict(D=0), 33), (dict(D_v=16), 33), (dict(dtype=0, D_v=80), 33), (dict(H_q=3), 28), (dict(H_kv=0), 28),
+                     (dict(page=24), 27), (dict(q=None), 20), (dict(stats=None), 20), (dict(table=None), 20), (dict(k=None), 20),
+                     (dict(q=odd), 29), (dict(k=odd), 29), (dict(T=1 << 30), 30)):
+        assert call(**kw) == code, kw
+    assert call(T=0) == 0 and call(N=0) == 0 and call(H_q=0) == 0
+    need = lambda **k: L.sdpa_hip_paged_fwd_fp4_workspace_bytes(*dict(dict(dtype=1, N=3, T=6, width=400, page=16, H_q=4, H_kv=2,
+                                                                           D=32, D_v=64, most=1), **k).values())
+    assert need() > 0 and need(width=1) == 0 and need(H_q=3) == 0 and need(D=48) == 0

@@ -140,6 +140,10 @@ def library():
     L.sdpa_hip_paged_fwd_workspace_bytes.argtypes = [i32] * 10
     L.sdpa_hip_paged_fwd.restype = i32
     L.sdpa_hip_paged_fwd.argtypes = [i32, vp, i64p, vp, vp, vp, i64p, vp] + batch + [vp, sz] + [i32] * 10 + [f32, i32, vp]
+    L.sdpa_hip_paged_fwd_fp4_workspace_bytes.restype = sz
+    L.sdpa_hip_paged_fwd_fp4_workspace_bytes.argtypes = [i32] * 10
+    L.sdpa_hip_paged_fwd_fp4.restype = i32
+    L.sdpa_hip_paged_fwd_fp4.argtypes = L.sdpa_hip_paged_fwd.argtypes
     _lib = L
     return L
 
@@ -374,7 +378,7 @@ def sdpa_autograd(q, k, v, seed=0, offset=0, dropout: float = 0.0, scale: float 
 
 
 _HEADS = ("qk_norm_rope", "qk_norm_rope_grad", "qk_norm_rope_autograd", "kv_reserve", "Reserved", "kv_append", "paged_sdpa", "fp4_cache",
-          "kv_append_fp4", "kv_read_fp4")
+          "kv_append_fp4", "kv_read_fp4", "paged_sdpa_fp4")
 
 
 def __getattr__(name):

@@ -166,9 +166,13 @@ inline long long paged_most_rows(long long T, int G, int max_q_len) {
 inline bool paged_small(bool f16, long long most_rows) {
     return most_rows <= (f16 ? kPagedSmallRowsF16 : kPagedSmallRowsF32);
 }
-inline size_t paged_part_bytes(int D_v, int BM) {
-    return ((size_t)2 << kPagedTargetLog2) * BM * ((size_t)D_v + 2) * sizeof(float);
+inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
+    return ((size_t)2 << target_log2) * BM * ((size_t)D_v + 2) * sizeof(float);
 }
+
+// Attention over a cache in 4 bits: tiles of 16 rows, four workgroups a CU.
+constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 10;
+hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t stream);
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream);

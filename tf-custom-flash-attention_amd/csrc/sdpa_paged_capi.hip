@@ -363,39 +363,46 @@ int sdpa_hip_kv_append_axes(int dtype, const void* k, const int64_t* k_strides, 
 
 namespace {
 
+// Which kernel a call takes: by the rows of its sequences, as far as is known, and the cache.
+bool paged_is_small(bool fp4, int dtype, long long most_rows) {
+    if (fp4) return true;
+    return sdpa::paged_small(dtype == SDPA_DTYPE_F16, most_rows);
+}
+int paged_tile_rows(bool fp4, bool small) {
+    return !small ? sdpa::kPagedBM : fp4 ? sdpa::kPagedFp4SmallBM : sdpa::kPagedSmallBM;
+}
+int paged_target_log2(bool fp4, bool small) { return fp4 && small ? sdpa::kPagedFp4TargetLog2 : sdpa::kPagedTargetLog2; }
+
 // Whether the parts of divided tiles can come up at all, and their bytes.
-size_t paged_workspace(bool small, int width, int page_size, int D_v) {
+size_t paged_workspace(bool fp4, bool small, int width, int page_size, int D_v) {
     if ((long long)width * page_size <= 128) return 0;  // (one block of the smallest kind)
-    return sdpa::paged_part_bytes(D_v, small ? sdpa::kPagedSmallBM : sdpa::kPagedBM);
+    return sdpa::paged_part_bytes(D_v, paged_tile_rows(fp4, small), paged_target_log2(fp4, small));
 }
 
-int check_paged(int dtype, int H_q, int H_kv, int D_qk, int D_v) {
+int check_paged(bool fp4, int dtype, int H_q, int H_kv, int D_qk, int D_v) {
     if (dtype != SDPA_DTYPE_F32 && dtype != SDPA_DTYPE_F16) return SDPA_ERR_DTYPE;
     if (H_q < 0 || H_kv < 0 || D_qk < 0 || D_v < 0) return SDPA_ERR_NEGATIVE_DIM;
     if (D_qk > 128 || D_v > 128) return SDPA_ERR_FEATURE_TOO_LARGE;
+    if (fp4 && !(fp4_width(D_qk) && fp4_width(D_v))) return SDPA_ERR_FP4_WIDTH;
     const int epc = dtype == SDPA_DTYPE_F16 ? 8 : 4;
     if (D_qk == 0 || D_v == 0 || D_qk % epc != 0 || D_v % epc != 0) return SDPA_ERR_LAYOUT;
     if (H_q > 0 && (H_kv == 0 || H_q % H_kv != 0)) return SDPA_ERR_HEADS;
     return SDPA_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
-                                          int D_qk, int D_v, int max_q_len) {
-    if (check_paged(dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
+size_t paged_workspace_entry(bool fp4, int dtype, int N, int T, int width, int page_size, int H_q, int H_kv, int D_qk, int D_v,
+                             int max_q_len) {
+    if (check_paged(fp4, dtype, H_q, H_kv, D_qk, D_v) != SDPA_OK || N <= 0 || T <= 0 || width <= 0 || page_size <= 0 || H_q == 0)
         return 0;
-    return paged_workspace(sdpa::paged_small(dtype == SDPA_DTYPE_F16, sdpa::paged_most_rows(T, H_q / H_kv, max_q_len)), width, page_size, D_v);
+    return paged_workspace(fp4, paged_is_small(fp4, dtype, sdpa::paged_most_rows(T, H_q / H_kv, max_q_len)), width, page_size, D_v);
 }
 
-int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
-                       void* o, const int64_t* o_strides, float* stats, const int32_t* page_table,
-                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, void* workspace,
-                       size_t workspace_bytes, int N, int T, int width, int pages, int page_size, int H_q, int H_kv,
-                       int D_qk, int D_v, int max_q_len, float scale, int causal_mask, hipStream_t stream) {
-    int st = check_paged(dtype, H_q, H_kv, D_qk, D_v);
+int paged_entry(bool fp4, int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache, void* o,
+                const int64_t* o_strides, float* stats, const int32_t* page_table, int64_t page_table_stride,
+                const int32_t* q_starts, const int32_t* kv_lens, void* workspace, size_t workspace_bytes, int N, int T, int width,
+                int pages, int page_size, int H_q, int H_kv, int D_qk, int D_v, int max_q_len, float scale, int causal_mask,
+                hipStream_t stream) {
+    int st = check_paged(fp4, dtype, H_q, H_kv, D_qk, D_v);
     if (st != SDPA_OK) return st;
     sdpa::PagedParams p{};
     // without pages no column of the table holds any
@@ -426,17 +433,53 @@ int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const
     if ((long long)T * p.G > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
     // sequences of few rows, as far as is known here (either kernel takes any)
     p.most_rows = (int)sdpa::paged_most_rows(T, p.G, max_q_len);
-    const bool small = sdpa::paged_small(dtype == SDPA_DTYPE_F16, p.most_rows);
-    if (sdpa::paged_max_tiles(p, sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
-    const size_t need = paged_workspace(small, p.batch.width, page_size, D_v);
-    p.target_log2 = sdpa::kPagedTargetLog2;
+    const bool small = paged_is_small(fp4, dtype, p.most_rows);
+    if (sdpa::paged_max_tiles(p, fp4 ? sdpa::kPagedFp4SmallBM : sdpa::kPagedSmallBM) > 0x7FFFFFFFLL - 65536) return SDPA_ERR_TOO_LARGE;
+    const size_t need = paged_workspace(fp4, small, p.batch.width, page_size, D_v);
+    p.target_log2 = paged_target_log2(fp4, small);
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + ((size_t)2 << p.target_log2) * (small ? sdpa::kPagedSmallBM : sdpa::kPagedBM) * D_v;
+        p.part_ml = p.part_o + ((size_t)2 << p.target_log2) * paged_tile_rows(fp4, small) * D_v;
     }
+    const sdpa::DType dt = (sdpa::DType)dtype;
+    if (fp4) return hip_status(sdpa::launch_paged_fp4_small(p, dt, stream));
     if (dtype == SDPA_DTYPE_F32)
         return hip_status(small ? sdpa::launch_paged_f32_small(p, stream) : sdpa::launch_paged_f32(p, stream));
     return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sdpa_hip_paged_fwd_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
+                                          int D_qk, int D_v, int max_q_len) {
+    return paged_workspace_entry(false, dtype, N, T, width, page_size, H_q, H_kv, D_qk, D_v, max_q_len);
+}
+
+int sdpa_hip_paged_fwd(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
+                       void* o, const int64_t* o_strides, float* stats, const int32_t* page_table,
+                       int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, void* workspace,
+                       size_t workspace_bytes, int N, int T, int width, int pages, int page_size, int H_q, int H_kv,
+                       int D_qk, int D_v, int max_q_len, float scale, int causal_mask, hipStream_t stream) {
+    return paged_entry(false, dtype, q, q_strides, k_cache, v_cache, o, o_strides, stats, page_table, page_table_stride,
+                       q_starts, kv_lens, workspace, workspace_bytes, N, T, width, pages, page_size, H_q, H_kv, D_qk, D_v,
+                       max_q_len, scale, causal_mask, stream);
+}
+
+size_t sdpa_hip_paged_fwd_fp4_workspace_bytes(int dtype, int N, int T, int width, int page_size, int H_q, int H_kv,
+                                              int D_qk, int D_v, int max_q_len) {
+    return paged_workspace_entry(true, dtype, N, T, width, page_size, H_q, H_kv, D_qk, D_v, max_q_len);
+}
+
+int sdpa_hip_paged_fwd_fp4(int dtype, const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
+                           void* o, const int64_t* o_strides, float* stats, const int32_t* page_table,
+                           int64_t page_table_stride, const int32_t* q_starts, const int32_t* kv_lens, void* workspace,
+                           size_t workspace_bytes, int N, int T, int width, int pages, int page_size, int H_q, int H_kv,
+                           int D_qk, int D_v, int max_q_len, float scale, int causal_mask, hipStream_t stream) {
+    return paged_entry(true, dtype, q, q_strides, k_cache, v_cache, o, o_strides, stats, page_table, page_table_stride,
+                       q_starts, kv_lens, workspace, workspace_bytes, N, T, width, pages, page_size, H_q, H_kv, D_qk, D_v,
+                       max_q_len, scale, causal_mask, stream);
 }
 
 int sdpa_hip_kv_append_fp4(int dtype, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,

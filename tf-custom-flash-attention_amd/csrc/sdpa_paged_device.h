@@ -310,14 +310,15 @@ __device__ __forceinline__ int tile_keys(const PagedParams& p, const PagedItem& 
 struct CareRow {
     float m, l, o[2], extra[2];
 };
-template <typename T>
-__device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t* table, const PagedRows& K, const PagedRows& V,
-                                         const T* q, int lo, int hi) {
+// none: the query holds a NaN; dot(page, key): its product with a key; value(page, key,
+// column).
+template <typename D, typename V>
+__device__ __forceinline__ CareRow care_row_of(const PagedParams& p, const int32_t* table, int log2, bool none, int lo, int hi,
+                                            D&& dot, V&& value) {
     const int lane = threadIdx.x & 63;
     CareRow r{-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}};
     const float sl2 = p.scale * kLog2e;
     // (of a NaN query all that sees a key is NaN)
-    const bool none = (lane < p.D_qk && q[lane] != q[lane]) || (lane + 64 < p.D_qk && q[lane + 64] != q[lane + 64]);
     if (lo < hi && __builtin_amdgcn_ballot_w64(none) != 0) {
         r.l = __builtin_nanf("");
         return r;
@@ -327,15 +328,8 @@ __device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t*
         float s = -INFINITY;
         int page = 0;
         if (j < hi) {
-            page = table[j >> K.log2];
-            typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));
-            const chunk *k = reinterpret_cast<const chunk*>(K.at(page, j)), *qc = reinterpret_cast<const chunk*>(q);
-            constexpr int EPC = 16 / (int)sizeof(T);
-            float dot = 0.f;
-            for (int d = 0; d < p.D_qk / EPC; ++d)
-#pragma unroll
-                for (int e = 0; e < EPC; ++e) dot = __builtin_fmaf((float)qc[d][e], (float)k[d][e], dot);
-            s = dot * sl2;
+            page = table[j >> log2];
+            s = dot(page, j) * sl2;
         }
         float mx = s;
 #pragma unroll
@@ -351,12 +345,12 @@ __device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t*
         r.o[1] *= a;
         for (int i = 0; i < 64 && j0 + i < hi; ++i) {
             const float wi = __shfl(w, i);
-            const T* v = reinterpret_cast<const T*>(V.at(__shfl(page, i), j0 + i));
+            const int pg = __shfl(page, i);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int d = lane + 64 * c;
                 if (d >= p.D_v) continue;
-                const float x = (float)v[d];
+                const float x = value(pg, j0 + i, d);
                 if (__builtin_fabsf(x) < INFINITY) r.o[c] = __builtin_fmaf(wi, x, r.o[c]);
                 else r.extra[c] += x;
             }
@@ -365,6 +359,25 @@ __device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t*
     r.o[0] += r.extra[0];
     r.o[1] += r.extra[1];
     return r;
+}
+template <typename T>
+__device__ __forceinline__ CareRow care_row(const PagedParams& p, const int32_t* table, const PagedRows& K, const PagedRows& V,
+                                         const T* q, int lo, int hi) {
+    const int lane = threadIdx.x & 63;
+    const bool none = (lane < p.D_qk && q[lane] != q[lane]) || (lane + 64 < p.D_qk && q[lane + 64] != q[lane + 64]);
+    return care_row_of(
+        p, table, K.log2, none, lo, hi,
+        [&](int page, int j) {
+            typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));
+            const chunk *k = reinterpret_cast<const chunk*>(K.at(page, j)), *qc = reinterpret_cast<const chunk*>(q);
+            constexpr int EPC = 16 / (int)sizeof(T);
+            float dot = 0.f;
+            for (int d = 0; d < p.D_qk / EPC; ++d)
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) dot = __builtin_fmaf((float)qc[d][e], (float)k[d][e], dot);
+            return dot;
+        },
+        [&](int page, int j, int d) { return (float)reinterpret_cast<const T*>(V.at(page, j))[d]; });
 }
 
 // One row's results of one wave, column d at a time: to o and stats, or (the
@@ -466,35 +479,19 @@ __device__ __forceinline__ float add_part(float acc, float x, float w) {
     return __builtin_fabsf(x) < INFINITY ? __builtin_fmaf(x, w, acc) : acc + x;
 }
 
-// The sums of the NW waves of a workgroup, whose 32 rows and lanes are those of
-// an MFMA accumulator (lane l32: row; features 32 dt + 8 g + 4 hh + e), through
-// LDS in wave order: to o and stats, or to the workspace.  bad: a page of some
-// wave's keys is none; the rows are NaN.  [k0, k1): this workgroup's keys.
-template <typename T, int DV, int NW, int BM>
-__device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const PagedItem& it, float* lds,
-                                                  const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
-                                                  const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
-                                                  int k1) {
+// The sums of NW waves' accumulators in LDS ([wave][row][acc_stride(DV)], then their statistics, flags of
+// rows and of waves), in wave order: to o and stats, or to the workspace.  The
+// callers have written accumulators, statistics and `none`, and cleared `again`.
+// care(row in the tile): a wave does a row again.
+template <typename T, int DV, int NW, int BM, typename F>
+__device__ __forceinline__ void reduce_paged_waves(const PagedParams& p, const PagedItem& it, float* lds, int tid, F&& care) {
     constexpr int OS = acc_stride(DV), NT = 64 * NW, ITER = (BM * (DV / 4) + NT - 1) / NT;
-    static_assert(BM == 32 && BM * (DV / 4) % NT == 0, "one accumulator tile of rows");
-    // (opaque: what is formed from it below stays out of the callers' loops, whose
-    // registers it would take)
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* mml = lds + NW * BM * OS;
-    int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);  // rows to do again
-    int* none = again + BM;                                  // waves that met a page that is none
-    if (hh == 0) {
-        mml[(wave * BM + l32) * 2] = m_run;
-        mml[(wave * BM + l32) * 2 + 1] = l_tot;
-    }
-    if (tid < BM) again[tid] = 0;
-    if (lane == 0) none[wave] = bad;
-    acc_to_lds<DV>(lds, wave * BM + l32, oacc, hh);
+    int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);
+    int* none = again + BM;
     __syncthreads();
-    bad = false;
+    bool bad = false;
 #pragma unroll
     for (int w = 0; w < NW; ++w) bad = bad || none[w] != 0;
     // one thread per four columns of a row
@@ -556,13 +553,43 @@ __device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const Pa
             if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M[u] * kLn2 + logf(L[u]);
         }
     }
-    for (int r = wave; r < rows; r += NW) {
-        if (!__builtin_amdgcn_readfirstlane(again[r])) continue;
+    for (int r = wave; r < rows; r += NW)
+        if (__builtin_amdgcn_readfirstlane(again[r])) care(r);
+}
+
+// The sums of the NW waves of a workgroup, whose 32 rows and lanes are those of
+// an MFMA accumulator (lane l32: row; features 32 dt + 8 g + 4 hh + e), through
+// LDS in wave order: to o and stats, or to the workspace.  bad: a page of some
+// wave's keys is none; the rows are NaN.  [k0, k1): this workgroup's keys.
+template <typename T, int DV, int NW, int BM>
+__device__ __forceinline__ void merge_paged_waves(const PagedParams& p, const PagedItem& it, float* lds,
+                                                  const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
+                                                  const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
+                                                  int k1) {
+    constexpr int OS = acc_stride(DV);
+    static_assert(BM == 32, "one accumulator tile of rows");
+    // (opaque: what is formed from it below stays out of the callers' loops, whose
+    // registers it would take)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float* mml = lds + NW * BM * OS;
+    int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);  // rows to do again
+    int* none = again + BM;                                  // waves that met a page that is none
+    if (hh == 0) {
+        mml[(wave * BM + l32) * 2] = m_run;
+        mml[(wave * BM + l32) * 2 + 1] = l_tot;
+    }
+    if (tid < BM) again[tid] = 0;
+    if (lane == 0) none[wave] = bad;
+    acc_to_lds<DV>(lds, wave * BM + l32, oacc, hh);
+    reduce_paged_waves<T, DV, NW, BM>(p, it, lds, tid, [&](int r) {
         PagedRow row;
         row.init(p, it, it.tile * BM + r);
         const T* q = static_cast<const T*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h;
         put_care_row<T, BM>(p, it, row, r, care_row<T>(p, table, K, V, q, k0, min(k1, min(row.see, it.s.len))));
-    }
+    });
 }
 
 // The sums of a row's parts, four columns of them, as they come:

@@ -1,0 +1,307 @@
+// sdpa_paged_fp4_small.hip -- attention of few new tokens per sequence (generation, short
+// drafts) over a paged cache in 4 bits (sdpa_fp4.h), queries in fp16 or fp32, for gfx950.
+//
+// Tiles of 16 rows (tokens times the query heads of a key head) by equal shares of the key
+// blocks (sdpa_paged.h); the four waves of a workgroup take a tile's blocks of 32
+// keys in turn, each with sums of its own, merged through LDS at the tile's end.
+//   S^T = K Q^T, online softmax in the log2 domain, O^T += V^T P^T
+// on v_mfma_f32_16x16x32_f16, without LDS in the loop: a lane of the K operand is a key, 8
+// of whose features are one word of codes; a lane of the V operand is a feature, 8 keys of
+// which are one word; and the keys of a block are dealt to the rows of two K operands so
+// that a lane holds the scores of 8 keys in a row, which is the P operand as it stands.
+// A word becomes 8 fp16 values by four conversions (v_cvt_scalef32_pk_f16_fp4) and four
+// packed products with the scale, exactly.
+// P enters as two fp16 parts (22 bits): the matrix cores are idle beside the conversions.
+// fp32 queries are cut into three parts (33 bits), after a row's largest has been brought to
+// 2^14 by a power of two.
+#include "sdpa_launch.h"
+#include "sdpa_paged_fp4.h"
+
+namespace sdpa {
+namespace {
+
+template <typename T, int DQK, int DV>
+struct PagedFp4SmallCfg {
+    static constexpr int NP = sizeof(T) == 2 ? 1 : 3;  // parts of a query
+    static constexpr int NW = 4, NT = 64 * NW, BM = kPagedFp4SmallBM, BN = 32, PLAN = BN * NW;
+    static constexpr int OS = acc_stride(DV), MERGE = NW * BM * OS * 4 + NW * BM * 8 + (BM + NW) * 4;
+    static constexpr int PLAN_AT = (MERGE + 15) / 16 * 16;
+    static constexpr size_t LDS_BYTES = PLAN_AT + PagedShares<BM, PLAN>::LDS_BYTES;
+    static constexpr int WPE = NP == 3 && DQK + DV > 96 ? 2 : 4;
+    static_assert(WPE * LDS_BYTES <= 160 * 1024, "gfx950 LDS");
+};
+
+// A wave's part of a block of keys, as it lies in the cache.
+template <int DQK, int DV>
+struct Fp4Block {
+    static constexpr int KW = DQK / 32;              // words of a lane's key
+    static constexpr int V4 = DV / 64, V2 = DV / 32 % 2;  // pieces of 64 features, and one of 32
+    static constexpr int NV = V4 + V2;
+    uint32_t k[2][KW];
+    uint32_t ks[2][2];  // scales: of a lane's first and last word
+    uint32_t v[4 * V4 + 2 * V2];
+    uint2v vs[NV];
+
+    // groups of a lane's first and last word of a key
+    __device__ __forceinline__ static int group(int kb, int w) { return (KW * kb + w) / 4; }
+
+    __device__ __forceinline__ void load_keys(const Fp4Pages& K, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
+        const int m = lane & 15, kb = lane >> 4;
+        const unsigned char* head = K.log2 == 4 && m >= 8 ? p1 : p0;
+        const int slot = (K.log2 == 4 ? 0 : K.slot(kv0)) + 8 * (K.log2 == 4 ? (m >> 2) & 1 : m >> 2) + (m & 3);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const unsigned char* row = head + (slot + 4 * t) * (DQK / 2) + KW * 4 * kb;
+            if constexpr (KW == 4) {
+                const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(row));
+#pragma unroll
+                for (int w = 0; w < 4; ++w) k[t][w] = x[w];
+            } else if constexpr (KW == 2) {
+                const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(row));
+                k[t][0] = x[0];
+                k[t][1] = x[1];
+            } else {
+#pragma unroll
+                for (int w = 0; w < KW; ++w) k[t][w] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row) + w);
+            }
+            const unsigned char* scales = head + K.scales_at() + (slot + 4 * t) * (DQK / 32);
+            ks[t][0] = scales[group(kb, 0)];
+            if constexpr (KW == 3) ks[t][1] = scales[group(kb, 2)];
+        }
+    }
+    __device__ __forceinline__ half8 key(int t, int w, int lane) const {
+        const int kb = lane >> 4;
+        uint32_t s = ks[t][0];
+        if constexpr (KW == 3) s = group(kb, w) == group(kb, 0) ? s : ks[t][1];
+        return fp4_word(k[t][w], fp4_scale2<0>(s));
+    }
+    __device__ __forceinline__ void load_values(const Fp4Pages& V, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
+        const int i = lane & 15, kb = lane >> 4;
+        const unsigned char* head = V.log2 == 4 && kb >= 2 ? p1 : p0;
+        const int block = V.log2 == 4 ? kb & 1 : V.slot(kv0) / 8 + kb;
+        const unsigned char* words = head + block * DV * 4;
+        const unsigned char* scales = head + V.scales_at() + block * (DV / 32) * 8;
+#pragma unroll
+        for (int c = 0; c < V4; ++c) {
+            const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(words + 256 * c) + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * c + e] = x[e];
+            vs[c] = *(reinterpret_cast<const uint2v*>(scales + 16 * c) + (i >> 3));
+        }
+        if constexpr (V2) {
+            const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(words + 256 * V4) + i);
+            v[4 * V4] = x[0];
+            v[4 * V4 + 1] = x[1];
+            vs[V4] = *reinterpret_cast<const uint2v*>(scales + 16 * V4);
+        }
+    }
+};
+
+template <typename T, int DQK, int DV>
+__global__ __launch_bounds__((PagedFp4SmallCfg<T, DQK, DV>::NT))
+__attribute__((amdgpu_waves_per_eu(PagedFp4SmallCfg<T, DQK, DV>::WPE, PagedFp4SmallCfg<T, DQK, DV>::WPE)))
+void paged_fp4_small_kernel(const PagedParams p) {
+    using Cfg = PagedFp4SmallCfg<T, DQK, DV>;
+    using Block = Fp4Block<DQK, DV>;
+    constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW, NP = Cfg::NP, KW = Block::KW, NDT = DV / 16;
+    const PagedShares<BM, Cfg::PLAN> plan(p, smem + Cfg::PLAN_AT);
+    plan.each(tile_id(), [&](const PagedItem& it) __attribute__((always_inline)) {
+        int tid = threadIdx.x;  // (opaque: lane terms are formed for each tile, not held across them)
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, i16 = lane & 15, kb = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int kv_end = min(tile_keys(p, it, BM), it.s.len);
+        PagedRow row;
+        row.init(p, it, it.tile * BM + i16);
+        const int see = row.live ? row.see : 0x7FFFFFFF;  // (rows that are none need no mask)
+
+        // |scale| with negated queries for scale < 0; 1e-30 for 0: the running
+        // maximum is taken on raw scores, which needs a positive factor
+        const float sl2_raw = p.scale * kLog2e;
+        float sl2 = (sl2_raw == 0.f) ? 1e-30f : fabsf(sl2_raw);
+        half8 q[KW][NP];
+        {
+            const T* qrow = static_cast<const T*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h + 8 * KW * kb;
+            if constexpr (NP == 1) {
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    half8 v = half8{};
+                    if (row.live) v = *reinterpret_cast<const half8*>(qrow + 8 * w);
+                    q[w][0] = sl2_raw < 0.f ? -v : v;
+                }
+            } else {
+                float x[KW][8], most = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[w][e] = row.live ? qrow[8 * w + e] : 0.f;
+                        most = fmaxf(most, fabsf(x[w][e]));
+                    }
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                // (powers of two within what a float holds; queries below 2^-100 lose bits)
+                const int up = min(max(14 - (int)(__float_as_uint(most) >> 23) + 127, -113), 114);
+                const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+                sl2 *= __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[w][e] *= sl2_raw < 0.f ? -f : f;
+                    cut_queries(q[w], x[w]);
+                }
+            }
+        }
+
+        // this wave's blocks: lo + wave, lo + wave + NW, ... below hi
+        const int nblk = (kv_end + BN - 1) / BN;
+        const int lo = min(NW * it.u0, nblk), hi = min(NW * it.u1, nblk);
+        Fp4Pages K, V;
+        K.init(p.k_cache, p.H_kv, it.h, DQK, p.batch.page_log2);
+        V.init(p.v_cache, p.H_kv, it.h, DV, p.batch.page_log2);
+        PageWindow pw{uniform_ptr(p.batch.page_table + it.seq * p.batch.table_stride), p.batch.pages,
+                      (min(kv_end, hi * BN) + (1 << K.log2) - 1) >> K.log2};
+        Block b;
+        const auto pages_of = [&](int blk, int& p0, int& p1) __attribute__((always_inline)) {
+            const int c = (blk * BN) >> K.log2;
+            pw.need(c, lane);  // (a window holds whole blocks)
+            p0 = pw.held(c);
+            p1 = K.log2 == 4 ? pw.held(c + 1) : p0;
+        };
+        pw.load((lo * BN) >> K.log2, lane);
+        int p0 = 0, p1 = 0;
+        if (lo + wave < hi) {
+            pages_of(lo + wave, p0, p1);
+            b.load_keys(K, K.page(p0), K.page(p1), (lo + wave) * BN, lane);
+            b.load_values(V, V.page(p0), V.page(p1), (lo + wave) * BN, lane);
+        }
+        floatx4 oacc[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) oacc[dt] = floatx4{};
+        float m_run = -INFINITY, l_run = 0.f;
+
+        for (int blk = lo + wave; blk < hi; blk += NW) {
+            const int kv0 = blk * BN;
+            const bool more = blk + NW < hi;
+            floatx4 s[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    const half8 k = b.key(t, w, lane);
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; --n) s[t] = mfma16_f16(k, q[w][n], s[t]);
+                }
+            // the next keys fly while these are worked on, and below the next values
+            if (more) {
+                pages_of(blk + NW, p0, p1);
+                b.load_keys(K, K.page(p0), K.page(p1), kv0 + NW * BN, lane);
+            }
+            const int key0 = kv0 + 8 * kb;  // of this lane's 8 scores
+            if (wave_any(kv0 + BN > see)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key0 + 4 * t + r >= see) s[t][r] = -INFINITY;
+            }
+            float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+            for (int r = 1; r < 4; ++r) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
+            {
+                const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            }
+            mx = xhalf_max(mx) * sl2;
+            const float m_use = (mx > m_run + kTauP) ? mx - kTopP : m_run;
+            const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
+            const float nm = m_use == -INFINITY ? 0.f : -m_use;
+            float pf[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pf[j] = fast_exp2(__builtin_fmaf(s[j / 4][j % 4], sl2, nm));
+            if (wave_any(alpha != 1.f)) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) oacc[dt][r] *= alpha;
+            }
+            l_run = __builtin_fmaf(l_run, alpha, ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7])));
+            m_run = m_use;
+            half8 part[2];
+            cut_queries(part, pf);
+            if (kv0 + BN > kv_end)  // what lies behind the last key, whatever it is, is 0
+#pragma unroll
+                for (int c = 0; c < Block::NV; ++c) b.vs[c] = first_bytes(b.vs[c], kv_end - key0);
+#pragma unroll
+            for (int c = 0; c < Block::NV; ++c) {
+                half2v vs[4];
+                fp4_scales(vs, b.vs[c]);
+#pragma unroll
+                for (int e = 0; e < (c < Block::V4 ? 4 : 2); ++e) {
+                    const half8 v = fp4_word(b.v[4 * c + e], vs);
+                    oacc[4 * c + e] = mfma16_f16(v, part[1], oacc[4 * c + e]);
+                    oacc[4 * c + e] = mfma16_f16(v, part[0], oacc[4 * c + e]);
+                }
+            }
+            if (more) b.load_values(V, V.page(p0), V.page(p1), kv0 + NW * BN, lane);
+        }
+
+        // ---- merge the four waves.  Lane (row i16, kb): features 64 c + 16 kb + 4 r + e, of a
+        // piece of 32 features 64 c + 8 kb + 2 r + e
+        l_run += __shfl_xor(l_run, 16);
+        l_run += __shfl_xor(l_run, 32);
+        float* lds = reinterpret_cast<float*>(smem);
+        float* mml = lds + NW * BM * Cfg::OS;
+        int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);
+        int* none = again + BM;
+        const int at = wave * BM + i16;
+        if (kb == 0) {
+            mml[2 * at] = m_run;
+            mml[2 * at + 1] = l_run;
+        }
+        if (tid < BM) again[tid] = 0;
+        if (lane == 0) none[wave] = pw.bad || it.s.bad;
+#pragma unroll
+        for (int c = 0; c < Block::V4; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 16 * kb + 4 * r) =
+                    (floatx4){oacc[4 * c][r], oacc[4 * c + 1][r], oacc[4 * c + 2][r], oacc[4 * c + 3][r]};
+        if constexpr (Block::V2) {
+            constexpr int c = Block::V4;
+#pragma unroll
+            for (int r = 0; r < 4; r += 2)
+                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 8 * kb + 2 * r) =
+                    (floatx4){oacc[4 * c][r], oacc[4 * c + 1][r], oacc[4 * c][r + 1], oacc[4 * c + 1][r + 1]};
+        }
+        reduce_paged_waves<T, DV, NW, BM>(p, it, lds, tid, [&](int r) {
+            PagedRow rr;
+            rr.init(p, it, it.tile * BM + r);
+            const T* qr = static_cast<const T*>(p.q) + rr.tok * p.qs.t + rr.head * p.qs.h;
+            put_care_row<T, BM>(p, it, rr, r, care_row_fp4<T>(p, pw.row, K, V, qr, lo * BN, min(hi * BN, min(rr.see, it.s.len))));
+        });
+        __syncthreads();
+    });
+}
+
+}  // namespace
+
+hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t stream) {
+    const auto run = [&](auto t) {
+        using T = decltype(t);
+        return with_fp4_dim(p.D_qk, [&](auto dqk) {
+            return with_fp4_dim(p.D_v, [&](auto dv) {
+                constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
+                using Cfg = PagedFp4SmallCfg<T, DQK, DV>;
+                hipError_t e = launch_kernel<paged_fp4_small_kernel<T, DQK, DV>>(dim3(1u << p.target_log2), Cfg::NT, Cfg::LDS_BYTES,
+                                                                                stream, p);
+                return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
+                           ? launch_paged_share_merge<T, Cfg::BM, Cfg::PLAN>(p, stream)
+                           : e;
+            });
+        });
+    };
+    return dtype == DType::F16 ? run(half_t{}) : run(float{});
+}
+
+}  // namespace sdpa

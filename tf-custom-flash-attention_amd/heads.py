@@ -671,19 +671,36 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
     kernels only.  ``out``: (o, stats) to write into, memory of their own; rows of tokens of no sequence stay as they were
     (in new ones they are arbitrary).  Feature sizes are multiples of 8 (fp16) or 4 (fp32), up to 128.
     """
+    return _paged(False, q, k_cache, v_cache, page_table, q_starts, kv_lens, scale, causal_mask, max_q_len, out)
+
+
+def paged_sdpa_fp4(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float = 1.0, causal_mask: bool = True,
+                   max_q_len=None, out=None):
+    """``paged_sdpa`` over a cache in 4 bits (``fp4_cache``, ``kv_append_fp4``): ``(o, stats)``.
+
+    Arguments and results as there; the queries are fp16 or fp32, and the cache's values exact in either.
+    """
+    return _paged(True, q, k_cache, v_cache, page_table, q_starts, kv_lens, scale, causal_mask, max_q_len, out)
+
+
+def _paged(fp4, q, k_cache, v_cache, page_table, q_starts, kv_lens, scale, causal_mask, max_q_len, out):
     T = q.dtype
     _check_tokens("q", q, T)
     code = _dtype_code(q)
-    plain = _plain_batch(q.device, T, k_cache, v_cache, page_table, q_starts, kv_lens)
+    of = _U8 if fp4 else T
+    plain = _plain_batch(q.device, of, k_cache, v_cache, page_table, q_starts, kv_lens)
     known = plain is not None
     if not known:
-        _check_cache(k_cache, v_cache, T)
+        _check_cache(k_cache, v_cache, of)
         plain = _check_batch(page_table, q_starts, kv_lens)
     N, width = plain
     n, H_q, D_qk = q.shape
     pages, H_kv, page, D_v = v_cache.shape
-    if k_cache.shape[3] != D_qk:
-        _fail(f"q has {D_qk} features, k_cache {k_cache.shape[3]}")
+    D_k = k_cache.shape[3]
+    if fp4:
+        D_k, D_v = _fp4_features(k_cache), _fp4_features(v_cache)
+    if D_k != D_qk:
+        _fail(f"q has {D_qk} features, k_cache {D_k}")
     if out is None:
         if not known:
             _on_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
@@ -703,11 +720,13 @@ def paged_sdpa(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: float 
         if _share_memory(o, stats):
             _fail("the tensors of out must not share memory")
     L = library()
+    size, entry = ((L.sdpa_hip_paged_fwd_fp4_workspace_bytes, L.sdpa_hip_paged_fwd_fp4) if fp4 else
+                   (L.sdpa_hip_paged_fwd_workspace_bytes, L.sdpa_hip_paged_fwd))
     longest = 0 if max_q_len is None else int(max_q_len)
-    ws_bytes = L.sdpa_hip_paged_fwd_workspace_bytes(code, N, n, width, page, H_q, H_kv, D_qk, D_v, longest)
+    ws_bytes = size(code, N, n, width, page, H_q, H_kv, D_qk, D_v, longest)
     ws = _workspace(torch, ws_bytes, q.device) if ws_bytes else None
     q = _whole_chunks(q)
-    _call(L.sdpa_hip_paged_fwd, q.device, code, q.data_ptr(), _strides2(q.stride()), k_cache.data_ptr(), v_cache.data_ptr(),
+    _call(entry, q.device, code, q.data_ptr(), _strides2(q.stride()), k_cache.data_ptr(), v_cache.data_ptr(),
           o.data_ptr(), None, stats.data_ptr(), page_table.data_ptr(), page_table.stride(0), q_starts.data_ptr(),
           kv_lens.data_ptr(), _ptr(ws), ws_bytes if ws is not None else 0, N, n, width, pages, page, H_q, H_kv, D_qk,
           D_v, longest, float(scale), int(bool(causal_mask)))
