@@ -170,9 +170,12 @@ inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
     return ((size_t)2 << target_log2) * BM * ((size_t)D_v + 2) * sizeof(float);
 }
 
-// Attention over a cache in 4 bits: tiles of 16 rows, four workgroups a CU.
+// Attention over a cache in 4 bits: sequences of up to so many rows by tiles of 16 rows,
+// four workgroups a CU, others by tiles of 128.
 constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 10;
+constexpr int kPagedFp4SmallRows = 16;
 hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t stream);
+hipError_t launch_paged_fp4(const PagedParams& p, DType dtype, hipStream_t stream);
 
 hipError_t launch_paged_f16_small(const PagedParams& p, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedParams& p, hipStream_t stream);

@@ -365,7 +365,7 @@ namespace {
 
 // Which kernel a call takes: by the rows of its sequences, as far as is known, and the cache.
 bool paged_is_small(bool fp4, int dtype, long long most_rows) {
-    if (fp4) return true;
+    if (fp4) return most_rows <= sdpa::kPagedFp4SmallRows;
     return sdpa::paged_small(dtype == SDPA_DTYPE_F16, most_rows);
 }
 int paged_tile_rows(bool fp4, bool small) {
@@ -442,7 +442,7 @@ int paged_entry(bool fp4, int dtype, const void* q, const int64_t* q_strides, co
         p.part_ml = p.part_o + ((size_t)2 << p.target_log2) * paged_tile_rows(fp4, small) * D_v;
     }
     const sdpa::DType dt = (sdpa::DType)dtype;
-    if (fp4) return hip_status(sdpa::launch_paged_fp4_small(p, dt, stream));
+    if (fp4) return hip_status(small ? sdpa::launch_paged_fp4_small(p, dt, stream) : sdpa::launch_paged_fp4(p, dt, stream));
     if (dtype == SDPA_DTYPE_F32)
         return hip_status(small ? sdpa::launch_paged_f32_small(p, stream) : sdpa::launch_paged_f32(p, stream));
     return hip_status(small ? sdpa::launch_paged_f16_small(p, stream) : sdpa::launch_paged_f16(p, stream));

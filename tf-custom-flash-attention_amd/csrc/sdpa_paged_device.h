@@ -417,14 +417,12 @@ __device__ __forceinline__ bool any_nonfinite(const floatx16 (&acc)[N]) {
 }
 
 // Results of a wave of 32 rows (lane l32: row; accumulator tiles over features) of a
-// kernel of 128-row tiles: to o and stats, or to the workspace.  CARE: rows whose sums
-// hold a NaN or an infinity, or whose scores do, again with care.  [k0, k1): this
-// workgroup's keys.
-template <typename T, int DV, int BM, bool CARE>
-__device__ __forceinline__ void put_paged_rows(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
-                                               const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
-                                               const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
-                                               int k1) {
+// kernel of 128-row tiles: to o and stats, or to the workspace.  PER: features of one tile are
+// PER apart (tile dt: features PER m + dt; 1: 32 dt + m).  CARE: rows whose sums
+// hold a NaN or an infinity, or whose scores do, again with care: care(item's row, row in the tile).
+template <typename T, int DV, int BM, bool CARE, int PER, typename F>
+__device__ __forceinline__ void put_paged_rows_by(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
+                                                  const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad, F&& care) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, in_tile = 32 * wave + l32, D_v = p.D_v;
     uint32_t again = 0;
     if constexpr (CARE) {
@@ -445,19 +443,24 @@ __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const Paged
         }
         typedef T t4 __attribute__((ext_vector_type(4)));
         T* o = static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h;
+        static_assert(PER == 1 || PER == DV / 32, "the tiles' features in turn, or each its own");
 #pragma unroll
         for (int dt = 0; dt < DV / 32; ++dt)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int d0 = 32 * dt + 8 * g + 4 * hh;
+                // four neighbouring features: of one tile, or of PER tiles and 4 / PER registers
+                const int i = PER == 4 ? 4 * dt + g : PER == 2 ? 8 * dt + 2 * g : 4 * g;
+                const int d0 = PER == 1 ? 32 * dt + 8 * g + 4 * hh : PER * (8 * (i >> 2) + 4 * hh + (i & 3));
                 if (d0 >= D_v) continue;
+                floatx4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = PER == 1 ? oacc[dt][i + e] : oacc[e % PER][i + e / PER];
                 if (it.divided) {
-                    *reinterpret_cast<floatx4*>(p.part_o + at * D_v + d0) =
-                        (floatx4){oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
+                    *reinterpret_cast<floatx4*>(p.part_o + at * D_v + d0) = x;
                 } else {
                     t4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = (T)(oacc[dt][4 * g + e] * f);
+                    for (int e = 0; e < 4; ++e) v[e] = (T)(x[e] * f);
                     *reinterpret_cast<t4*>(o + d0) = v;
                 }
             }
@@ -467,9 +470,20 @@ __device__ __forceinline__ void put_paged_rows(const PagedParams& p, const Paged
         const int r = 32 * wave + __builtin_ctz(todo);
         PagedRow rr;
         rr.init(p, it, it.tile * BM + r);
+        care(rr, r);
+    }
+}
+
+// The same with the features in order, over a cache of T.  [k0, k1): this workgroup's keys.
+template <typename T, int DV, int BM, bool CARE>
+__device__ __forceinline__ void put_paged_rows(const PagedParams& p, const PagedItem& it, int wave, const PagedRow& row,
+                                               const floatx16 (&oacc)[DV / 32], float m_run, float l_tot, bool bad,
+                                               const int32_t* table, const PagedRows& K, const PagedRows& V, int k0,
+                                               int k1) {
+    put_paged_rows_by<T, DV, BM, CARE, 1>(p, it, wave, row, oacc, m_run, l_tot, bad, [&](const PagedRow& rr, int r) {
         const T* q = static_cast<const T*>(p.q) + rr.tok * p.qs.t + rr.head * p.qs.h;
         put_care_row<T, BM>(p, it, rr, r, care_row<T>(p, table, K, V, q, k0, min(k1, min(rr.see, it.s.len))));
-    }
+    });
 }
 
 // Weight 2^(m - M) of a part (0 where both are -inf: nothing was seen).

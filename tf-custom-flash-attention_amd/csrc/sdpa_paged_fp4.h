@@ -90,6 +90,39 @@ __device__ __forceinline__ CareRow care_row_fp4(const PagedParams& p, const int3
         });
 }
 
+// A lane's words of a K operand: KW = DQK / 32 neighbouring ones, those from KW part on, of a
+// key's 4 KW, and their scales.
+template <int KW>
+struct Fp4Keys {
+    uint32_t words[KW];
+    uint32_t first, last;  // scales of the first and the last word
+    __device__ __forceinline__ static int group(int part, int w) { return (KW * part + w) / 4; }
+    // head: the page's bytes
+    __device__ __forceinline__ void load(const unsigned char* head, int scales_at, int slot, int part) {
+        const unsigned char* row = head + slot * (16 * KW) + 4 * KW * part;
+        if constexpr (KW == 4) {
+            const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(row));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) words[w] = x[w];
+        } else if constexpr (KW == 2) {
+            const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(row));
+            words[0] = x[0];
+            words[1] = x[1];
+        } else {
+#pragma unroll
+            for (int w = 0; w < KW; ++w) words[w] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row) + w);
+        }
+        const unsigned char* scales = head + scales_at + slot * KW;
+        first = scales[group(part, 0)];
+        if constexpr (KW == 3) last = scales[group(part, 2)];
+    }
+    __device__ __forceinline__ half8 word(int w, int part) const {
+        uint32_t s = first;
+        if constexpr (KW == 3) s = group(part, w) == group(part, 0) ? s : last;
+        return fp4_word(words[w], fp4_scale2<0>(s));
+    }
+};
+
 // 8 queries as N fp16 parts, the first the nearest fp16 and so on.
 template <int N>
 __device__ __forceinline__ void cut_queries(half8 (&part)[N], float (&x)[8]) {
@@ -100,6 +133,14 @@ __device__ __forceinline__ void cut_queries(half8 (&part)[N], float (&x)[8]) {
             part[n][e] = (half_t)x[e];
             x[e] -= (float)part[n][e];
         }
+}
+
+// Power of two that brings a row's largest |query| near 2^14 (within what a float
+// holds; queries below 2^-100 lose bits), and its inverse.
+__device__ __forceinline__ void query_factor(float most, float& f, float& inv) {
+    const int up = min(max(14 - (int)(__float_as_uint(most) >> 23) + 127, -113), 114);
+    f = __uint_as_float((uint32_t)(127 + up) << 23);
+    inv = __uint_as_float((uint32_t)(127 - up) << 23);
 }
 
 }  // namespace

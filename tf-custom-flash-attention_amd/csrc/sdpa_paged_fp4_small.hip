@@ -37,43 +37,16 @@ struct Fp4Block {
     static constexpr int KW = DQK / 32;              // words of a lane's key
     static constexpr int V4 = DV / 64, V2 = DV / 32 % 2;  // pieces of 64 features, and one of 32
     static constexpr int NV = V4 + V2;
-    uint32_t k[2][KW];
-    uint32_t ks[2][2];  // scales: of a lane's first and last word
+    Fp4Keys<KW> k[2];
     uint32_t v[4 * V4 + 2 * V2];
     uint2v vs[NV];
-
-    // groups of a lane's first and last word of a key
-    __device__ __forceinline__ static int group(int kb, int w) { return (KW * kb + w) / 4; }
 
     __device__ __forceinline__ void load_keys(const Fp4Pages& K, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
         const int m = lane & 15, kb = lane >> 4;
         const unsigned char* head = K.log2 == 4 && m >= 8 ? p1 : p0;
         const int slot = (K.log2 == 4 ? 0 : K.slot(kv0)) + 8 * (K.log2 == 4 ? (m >> 2) & 1 : m >> 2) + (m & 3);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const unsigned char* row = head + (slot + 4 * t) * (DQK / 2) + KW * 4 * kb;
-            if constexpr (KW == 4) {
-                const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(row));
-#pragma unroll
-                for (int w = 0; w < 4; ++w) k[t][w] = x[w];
-            } else if constexpr (KW == 2) {
-                const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(row));
-                k[t][0] = x[0];
-                k[t][1] = x[1];
-            } else {
-#pragma unroll
-                for (int w = 0; w < KW; ++w) k[t][w] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row) + w);
-            }
-            const unsigned char* scales = head + K.scales_at() + (slot + 4 * t) * (DQK / 32);
-            ks[t][0] = scales[group(kb, 0)];
-            if constexpr (KW == 3) ks[t][1] = scales[group(kb, 2)];
-        }
-    }
-    __device__ __forceinline__ half8 key(int t, int w, int lane) const {
-        const int kb = lane >> 4;
-        uint32_t s = ks[t][0];
-        if constexpr (KW == 3) s = group(kb, w) == group(kb, 0) ? s : ks[t][1];
-        return fp4_word(k[t][w], fp4_scale2<0>(s));
+        for (int t = 0; t < 2; ++t) k[t].load(head, K.scales_at(), slot + 4 * t, kb);
     }
     __device__ __forceinline__ void load_values(const Fp4Pages& V, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
         const int i = lane & 15, kb = lane >> 4;
@@ -140,10 +113,9 @@ void paged_fp4_small_kernel(const PagedParams p) {
                     }
                 most = fmaxf(most, __shfl_xor(most, 16));
                 most = fmaxf(most, __shfl_xor(most, 32));
-                // (powers of two within what a float holds; queries below 2^-100 lose bits)
-                const int up = min(max(14 - (int)(__float_as_uint(most) >> 23) + 127, -113), 114);
-                const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-                sl2 *= __uint_as_float((uint32_t)(127 - up) << 23);
+                float f, inv;
+                query_factor(most, f, inv);
+                sl2 *= inv;
 #pragma unroll
                 for (int w = 0; w < KW; ++w) {
 #pragma unroll
@@ -188,7 +160,7 @@ void paged_fp4_small_kernel(const PagedParams p) {
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int w = 0; w < KW; ++w) {
-                    const half8 k = b.key(t, w, lane);
+                    const half8 k = b.k[t].word(w, kb);
 #pragma unroll
                     for (int n = NP - 1; n >= 0; --n) s[t] = mfma16_f16(k, q[w][n], s[t]);
                 }
