@@ -30,6 +30,18 @@ __host__ __device__ inline long long fp4_scales_at(int D, int page_log2) { retur
 
 namespace {
 
+// A cache's bytes in device memory: pointers that went through scalar registers are
+// taken for any memory otherwise, and loads from those wait for LDS too.
+typedef __attribute__((address_space(1))) const unsigned char* fp4_ptr;
+template <typename V>
+__device__ __forceinline__ V fp4_load(fp4_ptr p) {
+    return *reinterpret_cast<__attribute__((address_space(1))) const V*>(p);
+}
+template <typename V>  // past the caches
+__device__ __forceinline__ V fp4_load_nt(fp4_ptr p) {
+    return __builtin_nontemporal_load(reinterpret_cast<__attribute__((address_space(1))) const V*>(p));
+}
+
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 

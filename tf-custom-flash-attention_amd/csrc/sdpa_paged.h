@@ -35,6 +35,7 @@ struct PagedParams {
     TokenStrides qs, os;
     float* part_o;   // [slot][BM][D_v]: unnormalised O of a part
     float* part_ml;  // [slot][BM][2]: the reference of its weights (log2) and their sum
+    struct CutTile* cut;  // (cache in 4 bits, shares) what each workgroup leaves to merge
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
@@ -174,6 +175,11 @@ inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
 // four workgroups a CU, others by tiles of 128.
 constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 10;
 constexpr int kPagedFp4SmallRows = 16;
+// The tile that a workgroup's share begins and does not end, for the merge: its rows
+// are row0 .. row0 + rows - 1 of the sequence from token q0 on and key head h, its parts np (0: none).
+struct CutTile {
+    int np, rows, row0, q0, h, pad[3];
+};
 hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t stream);
 hipError_t launch_paged_fp4(const PagedParams& p, DType dtype, hipStream_t stream);
 

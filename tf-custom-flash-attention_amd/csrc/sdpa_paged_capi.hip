@@ -376,7 +376,8 @@ int paged_target_log2(bool fp4, bool small) { return fp4 && small ? sdpa::kPaged
 // Whether the parts of divided tiles can come up at all, and their bytes.
 size_t paged_workspace(bool fp4, bool small, int width, int page_size, int D_v) {
     if ((long long)width * page_size <= 128) return 0;  // (one block of the smallest kind)
-    return sdpa::paged_part_bytes(D_v, paged_tile_rows(fp4, small), paged_target_log2(fp4, small));
+    const size_t parts = sdpa::paged_part_bytes(D_v, paged_tile_rows(fp4, small), paged_target_log2(fp4, small));
+    return parts + (fp4 && small ? sizeof(sdpa::CutTile) << sdpa::kPagedFp4TargetLog2 : 0);
 }
 
 int check_paged(bool fp4, int dtype, int H_q, int H_kv, int D_qk, int D_v) {
@@ -439,7 +440,9 @@ int paged_entry(bool fp4, int dtype, const void* q, const int64_t* q_strides, co
     p.target_log2 = paged_target_log2(fp4, small);
     if (need > 0 && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need) {
         p.part_o = static_cast<float*>(workspace);
-        p.part_ml = p.part_o + ((size_t)2 << p.target_log2) * paged_tile_rows(fp4, small) * D_v;
+        const size_t rows = ((size_t)2 << p.target_log2) * paged_tile_rows(fp4, small);
+        p.part_ml = p.part_o + rows * D_v;
+        if (fp4 && small) p.cut = reinterpret_cast<sdpa::CutTile*>(p.part_ml + 2 * rows);
     }
     const sdpa::DType dt = (sdpa::DType)dtype;
     if (fp4) return hip_status(small ? sdpa::launch_paged_fp4_small(p, dt, stream) : sdpa::launch_paged_fp4(p, dt, stream));

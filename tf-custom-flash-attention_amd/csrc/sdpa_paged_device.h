@@ -619,18 +619,24 @@ struct MergedRow {
         for (int e = 0; e < 4; ++e) acc[e] = add_part(add_part(0.f, acc[e], a), o[e], b);
         M = Mn;
     }
-    // columns c .. c + 3 of row r of a tile
-    template <typename T, int BM>
-    __device__ __forceinline__ void put(const PagedParams& p, const PagedItem& it, int r, int c) const {
-        PagedRow row;
-        row.init(p, it, it.tile * BM + r);
+    // four columns to o, the statistics (null: another thread's) to stats
+    template <typename T>
+    __device__ __forceinline__ void write(const PagedParams& p, T* o, float* stats) const {
         const float inv = L == 0.f ? 0.f : 1.f / L;
         typedef T t4 __attribute__((ext_vector_type(4)));
         t4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (T)(acc[e] * inv);
-        *reinterpret_cast<t4*>(static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c) = v;
-        if (c == 0) p.stats[(size_t)row.tok * p.H_kv * p.G + row.head] = M * kLn2 + logf(L);
+        *reinterpret_cast<t4*>(o) = v;
+        if (stats) *stats = M * kLn2 + logf(L);
+    }
+    // columns c .. c + 3 of row r of a tile
+    template <typename T, int BM>
+    __device__ __forceinline__ void put(const PagedParams& p, const PagedItem& it, int r, int c) const {
+        PagedRow row;
+        row.init(p, it, it.tile * BM + r);
+        write(p, static_cast<T*>(p.o) + row.tok * p.os.t + row.head * p.os.h + c,
+              c == 0 ? p.stats + (size_t)row.tok * p.H_kv * p.G + row.head : nullptr);
     }
 };
 

@@ -20,19 +20,27 @@ hipError_t with_fp4_dim(int d, F&& f) {
     return with_dim(d, f);
 }
 
+// The same in scalar registers.
+__device__ __forceinline__ fp4_ptr uniform(fp4_ptr p) {
+    const uint64_t a = (uint64_t)p;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+    return (fp4_ptr)(((uint64_t)hi << 32) | lo);
+}
+
 // One head's bytes in the pages of a cache.
 struct Fp4Pages {
-    const unsigned char* base;  // of page 0
-    long long stride;           // between pages
+    fp4_ptr base;      // of page 0
+    long long stride;  // between pages
     int D, log2;
     __device__ __forceinline__ void init(const void* cache, int H_kv, int h, int D_, int page_log2) {
         D = D_;
         log2 = page_log2;
         const long long bytes = fp4_head_bytes(D, log2);
         stride = bytes * H_kv;
-        base = uniform_ptr(static_cast<const unsigned char*>(cache) + bytes * h);
+        base = (fp4_ptr)uniform_ptr(static_cast<const unsigned char*>(cache) + bytes * h);
     }
-    __device__ __forceinline__ const unsigned char* page(int id) const { return base + id * stride; }
+    __device__ __forceinline__ fp4_ptr page(int id) const { return base + id * stride; }
     __device__ __forceinline__ int slot(int key) const { return key & ((1 << log2) - 1); }
     __device__ __forceinline__ int scales_at() const { return (D / 2) << log2; }
 };
@@ -70,19 +78,18 @@ __device__ __forceinline__ CareRow care_row_fp4(const PagedParams& p, const int3
     return care_row_of(
         p, table, K.log2, none, lo, hi,
         [&](int page, int j) {
-            const unsigned char* head = K.page(page);
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(head + (long long)K.slot(j) * (p.D_qk / 2));
-            const unsigned char* scales = head + K.scales_at() + (long long)K.slot(j) * (p.D_qk / 32);
+            const fp4_ptr words = K.page(page) + (long long)K.slot(j) * (p.D_qk / 2);
+            const fp4_ptr scales = K.page(page) + K.scales_at() + (long long)K.slot(j) * (p.D_qk / 32);
             float dot = 0.f;
             for (int w = 0; w < p.D_qk / 8; ++w) {
-                const half8 k = fp4_word(words[w], fp4_scale2<0>(scales[w / 4]));
+                const half8 k = fp4_word(fp4_load<uint32_t>(words + 4 * w), fp4_scale2<0>(scales[w / 4]));
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dot = __builtin_fmaf((float)q[8 * w + e], (float)k[e], dot);
             }
             return dot;
         },
         [&](int page, int j, int d) {
-            const unsigned char* head = V.page(page);
+            const fp4_ptr head = V.page(page);
             const int slot = V.slot(j), block = slot / 8, at = slot % 8;
             const uint32_t byte = head[((long long)block * p.D_v + d) * 4 + at / 2];
             const uint32_t scale = head[V.scales_at() + ((long long)block * (p.D_v / 32) + d / 32) * 8 + at];
@@ -97,24 +104,24 @@ struct Fp4Keys {
     uint32_t words[KW];
     uint32_t first, last;  // scales of the first and the last word
     __device__ __forceinline__ static int group(int part, int w) { return (KW * part + w) / 4; }
-    // head: the page's bytes
-    __device__ __forceinline__ void load(const unsigned char* head, int scales_at, int slot, int part) {
-        const unsigned char* row = head + slot * (16 * KW) + 4 * KW * part;
+    // bytes from the page's (or a block's) codes and scales on: of key `slot`, from word KW part on
+    __device__ __forceinline__ static uint32_t codes_at(int slot, int part) { return (uint32_t)(slot * (16 * KW) + 4 * KW * part); }
+    __device__ __forceinline__ static uint32_t scale_at(int slot, int part) { return (uint32_t)(slot * KW + group(part, 0)); }
+    __device__ __forceinline__ void load(fp4_ptr row, fp4_ptr scale, int part) {
         if constexpr (KW == 4) {
-            const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(row));
+            const uint4v x = fp4_load_nt<uint4v>(row);
 #pragma unroll
             for (int w = 0; w < 4; ++w) words[w] = x[w];
         } else if constexpr (KW == 2) {
-            const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(row));
+            const uint2v x = fp4_load_nt<uint2v>(row);
             words[0] = x[0];
             words[1] = x[1];
         } else {
 #pragma unroll
-            for (int w = 0; w < KW; ++w) words[w] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row) + w);
+            for (int w = 0; w < KW; ++w) words[w] = fp4_load_nt<uint32_t>(row + 4 * w);
         }
-        const unsigned char* scales = head + scales_at + slot * KW;
-        first = scales[group(part, 0)];
-        if constexpr (KW == 3) last = scales[group(part, 2)];
+        first = scale[0];
+        if constexpr (KW == 3) last = scale[group(part, 2) - group(part, 0)];
     }
     __device__ __forceinline__ half8 word(int w, int part) const {
         uint32_t s = first;
@@ -131,7 +138,7 @@ __device__ __forceinline__ void cut_queries(half8 (&part)[N], float (&x)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             part[n][e] = (half_t)x[e];
-            x[e] -= (float)part[n][e];
+            x[e] = __builtin_fmaf((float)part[n][e], -1.f, x[e]);  // (one instruction, on the half as it is)
         }
 }
 

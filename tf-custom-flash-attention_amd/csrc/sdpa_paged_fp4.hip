@@ -119,26 +119,28 @@ void paged_fp4_kernel(const PagedParams p) {
         const int kv0 = step * BN + 16 * wave;
         pw.need((step * BN) >> K.log2, lane);  // (a window holds whole blocks)
         const int page = pw.held(kv0 >> K.log2);
-        kr.load(K.page(page), K.scales_at(), K.slot(kv0) + key, part);
-        const unsigned char* head = V.page(page);
-        const int block = V.slot(kv0) / 8 + hh;
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(head) + block * DV;
-        const uint2v* scales = reinterpret_cast<const uint2v*>(head + V.scales_at()) + block * (DV / 32);
+        const int slot = K.slot(kv0);
+        const fp4_ptr codes = uniform(K.page(page) + slot * (DQK / 2));
+        kr.load(codes + Fp4Keys<KW>::codes_at(key, part),
+                codes + (K.scales_at() + slot * (KW - DQK / 2)) + Fp4Keys<KW>::scale_at(key, part), part);
+        const fp4_ptr first = uniform(V.page(page) + slot * (DV / 2));
+        const fp4_ptr words = first + (uint32_t)(hh * DV * 4);
+        const fp4_ptr scales = first + (V.scales_at() + slot * (DV / 32 - DV / 2)) + (uint32_t)(hh * (DV / 4));
         if constexpr (PER == 4) {
-            const uint4v x = *(reinterpret_cast<const uint4v*>(words) + l32);
+            const uint4v x = fp4_load<uint4v>(words + 16 * l32);
 #pragma unroll
             for (int e = 0; e < 4; ++e) vr[e] = x[e];
-            vsr[0] = scales[l32 / 8];
+            vsr[0] = fp4_load<uint2v>(scales + 8 * (l32 / 8));
         } else if constexpr (PER == 2) {
-            const uint2v x = *(reinterpret_cast<const uint2v*>(words) + l32);
+            const uint2v x = fp4_load<uint2v>(words + 8 * l32);
             vr[0] = x[0];
             vr[1] = x[1];
-            vsr[0] = scales[l32 / 16];
+            vsr[0] = fp4_load<uint2v>(scales + 8 * (l32 / 16));
         } else {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
-                vr[dt] = words[32 * dt + l32];
-                vsr[dt] = scales[dt];
+                vr[dt] = fp4_load<uint32_t>(words + 4 * (32 * dt + l32));
+                vsr[dt] = fp4_load<uint2v>(scales + 8 * dt);
             }
         }
     };

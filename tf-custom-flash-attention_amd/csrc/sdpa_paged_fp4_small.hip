@@ -41,36 +41,50 @@ struct Fp4Block {
     uint32_t v[4 * V4 + 2 * V2];
     uint2v vs[NV];
 
-    __device__ __forceinline__ void load_keys(const Fp4Pages& K, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
-        const int m = lane & 15, kb = lane >> 4;
-        const unsigned char* head = K.log2 == 4 && m >= 8 ? p1 : p0;
-        const int slot = (K.log2 == 4 ? 0 : K.slot(kv0)) + 8 * (K.log2 == 4 ? (m >> 2) & 1 : m >> 2) + (m & 3);
+    // Of the block from key kv0 on, in page `a` or, where pages hold 16 tokens, its second half in
+    // page b.  Addresses are a page's in scalar registers and a lane's offset.
+    template <bool HALVES>
+    __device__ __forceinline__ void load_keys(const Fp4Pages& K, int a, int b, int kv0, int lane) {
+        const int m = lane & 15, kb = lane >> 4, r = 8 * (HALVES ? (m >> 2) & 1 : m >> 2) + (m & 3);
+        const int slot = HALVES ? 0 : K.slot(kv0);
+        fp4_ptr codes = uniform(K.page(a) + slot * (DQK / 2)), scales = codes + (K.scales_at() + slot * (KW - DQK / 2));
+        if constexpr (HALVES) {
+            const fp4_ptr second = uniform(K.page(b));
+            codes = m >= 8 ? second : codes;
+            scales = codes + K.scales_at();
+        }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) k[t].load(head, K.scales_at(), slot + 4 * t, kb);
+        for (int t = 0; t < 2; ++t)
+            k[t].load(codes + Fp4Keys<KW>::codes_at(r + 4 * t, kb), scales + Fp4Keys<KW>::scale_at(r + 4 * t, kb), kb);
     }
-    __device__ __forceinline__ void load_values(const Fp4Pages& V, const unsigned char* p0, const unsigned char* p1, int kv0, int lane) {
-        const int i = lane & 15, kb = lane >> 4;
-        const unsigned char* head = V.log2 == 4 && kb >= 2 ? p1 : p0;
-        const int block = V.log2 == 4 ? kb & 1 : V.slot(kv0) / 8 + kb;
-        const unsigned char* words = head + block * DV * 4;
-        const unsigned char* scales = head + V.scales_at() + block * (DV / 32) * 8;
+    template <bool HALVES>
+    __device__ __forceinline__ void load_values(const Fp4Pages& V, int a, int b, int kv0, int lane) {
+        const int i = lane & 15, kb = lane >> 4, block = HALVES ? kb & 1 : kb, first = HALVES ? 0 : V.slot(kv0) / 8;
+        fp4_ptr words = uniform(V.page(a) + first * (DV * 4)), scales = words + (V.scales_at() + first * (DV / 4 - DV * 4));
+        if constexpr (HALVES) {
+            const fp4_ptr second = uniform(V.page(b));
+            words = kb >= 2 ? second : words;
+            scales = words + V.scales_at();
+        }
+        const uint32_t w0 = (uint32_t)(block * DV * 4), s0 = (uint32_t)(block * (DV / 4));
 #pragma unroll
         for (int c = 0; c < V4; ++c) {
-            const uint4v x = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(words + 256 * c) + i);
+            const uint4v x = fp4_load_nt<uint4v>(words + (w0 + 256 * c + 16 * i));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[4 * c + e] = x[e];
-            vs[c] = *(reinterpret_cast<const uint2v*>(scales + 16 * c) + (i >> 3));
+            vs[c] = fp4_load<uint2v>(scales + (s0 + 16 * c + 8 * (i >> 3)));
         }
         if constexpr (V2) {
-            const uint2v x = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(words + 256 * V4) + i);
+            const uint2v x = fp4_load_nt<uint2v>(words + (w0 + 256 * V4 + 8 * i));
             v[4 * V4] = x[0];
             v[4 * V4 + 1] = x[1];
-            vs[V4] = *reinterpret_cast<const uint2v*>(scales + 16 * V4);
+            vs[V4] = fp4_load<uint2v>(scales + (s0 + 16 * V4));
         }
     }
 };
 
-template <typename T, int DQK, int DV>
+// HALVES: pages of 16 tokens, two to a block of keys.
+template <typename T, int DQK, int DV, bool HALVES>
 __global__ __launch_bounds__((PagedFp4SmallCfg<T, DQK, DV>::NT))
 __attribute__((amdgpu_waves_per_eu(PagedFp4SmallCfg<T, DQK, DV>::WPE, PagedFp4SmallCfg<T, DQK, DV>::WPE)))
 void paged_fp4_small_kernel(const PagedParams p) {
@@ -78,7 +92,9 @@ void paged_fp4_small_kernel(const PagedParams p) {
     using Block = Fp4Block<DQK, DV>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW, NP = Cfg::NP, KW = Block::KW, NDT = DV / 16;
     const PagedShares<BM, Cfg::PLAN> plan(p, smem + Cfg::PLAN_AT);
-    plan.each(tile_id(), [&](const PagedItem& it) __attribute__((always_inline)) {
+    const int w = (int)blockIdx.x;
+    if (p.cut && threadIdx.x == 0) p.cut[w].np = 0;
+    plan.each(w, [&](const PagedItem& it) __attribute__((always_inline)) {
         int tid = threadIdx.x;  // (opaque: lane terms are formed for each tile, not held across them)
         asm volatile("" : "+v"(tid));
         const int lane = tid & 63, i16 = lane & 15, kb = lane >> 4;
@@ -88,40 +104,23 @@ void paged_fp4_small_kernel(const PagedParams p) {
         row.init(p, it, it.tile * BM + i16);
         const int see = row.live ? row.see : 0x7FFFFFFF;  // (rows that are none need no mask)
 
-        // |scale| with negated queries for scale < 0; 1e-30 for 0: the running
-        // maximum is taken on raw scores, which needs a positive factor
-        const float sl2_raw = p.scale * kLog2e;
-        float sl2 = (sl2_raw == 0.f) ? 1e-30f : fabsf(sl2_raw);
+        // the queries, before it is known where the keys are
         half8 q[KW][NP];
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        typedef T t4 __attribute__((ext_vector_type(16 / sizeof(T))));
+        t8 raw[KW];
         {
             const T* qrow = static_cast<const T*>(p.q) + row.tok * p.qs.t + row.head * p.qs.h + 8 * KW * kb;
-            if constexpr (NP == 1) {
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    half8 v = half8{};
-                    if (row.live) v = *reinterpret_cast<const half8*>(qrow + 8 * w);
-                    q[w][0] = sl2_raw < 0.f ? -v : v;
-                }
-            } else {
-                float x[KW][8], most = 0.f;
+            for (int w8 = 0; w8 < KW; ++w8) {
+                raw[w8] = t8{};
+                if (row.live)
 #pragma unroll
-                for (int w = 0; w < KW; ++w)
+                    for (int e = 0; e < 8; e += 16 / (int)sizeof(T)) {
+                        const t4 x = *reinterpret_cast<const t4*>(qrow + 8 * w8 + e);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[w][e] = row.live ? qrow[8 * w + e] : 0.f;
-                        most = fmaxf(most, fabsf(x[w][e]));
+                        for (int i = 0; i < 16 / (int)sizeof(T); ++i) raw[w8][e + i] = x[i];
                     }
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                float f, inv;
-                query_factor(most, f, inv);
-                sl2 *= inv;
-#pragma unroll
-                for (int w = 0; w < KW; ++w) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[w][e] *= sl2_raw < 0.f ? -f : f;
-                    cut_queries(q[w], x[w]);
-                }
             }
         }
 
@@ -138,14 +137,52 @@ void paged_fp4_small_kernel(const PagedParams p) {
             const int c = (blk * BN) >> K.log2;
             pw.need(c, lane);  // (a window holds whole blocks)
             p0 = pw.held(c);
-            p1 = K.log2 == 4 ? pw.held(c + 1) : p0;
+            p1 = HALVES ? pw.held(c + 1) : p0;
+        };
+        int p0 = 0, p1 = 0;
+        const auto load_keys = [&](int blk) __attribute__((always_inline)) {
+            b.template load_keys<HALVES>(K, p0, p1, blk * BN, lane);
+        };
+        const auto load_values = [&](int blk) __attribute__((always_inline)) {
+            b.template load_values<HALVES>(V, p0, p1, blk * BN, lane);
         };
         pw.load((lo * BN) >> K.log2, lane);
-        int p0 = 0, p1 = 0;
         if (lo + wave < hi) {
             pages_of(lo + wave, p0, p1);
-            b.load_keys(K, K.page(p0), K.page(p1), (lo + wave) * BN, lane);
-            b.load_values(V, V.page(p0), V.page(p1), (lo + wave) * BN, lane);
+            load_keys(lo + wave);
+            load_values(lo + wave);
+        }
+        // |scale| with negated queries for scale < 0; 1e-30 for 0: the running
+        // maximum is taken on raw scores, which needs a positive factor
+        const float sl2_raw = p.scale * kLog2e;
+        float sl2 = (sl2_raw == 0.f) ? 1e-30f : fabsf(sl2_raw);
+        if constexpr (NP == 1) {
+#pragma unroll
+            for (int w8 = 0; w8 < KW; ++w8) q[w8][0] = sl2_raw < 0.f ? -raw[w8] : raw[w8];
+        } else {
+            float most = 0.f;
+#pragma unroll
+            for (int w8 = 0; w8 < KW; ++w8)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)raw[w8][e]));
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            float f, inv;
+            query_factor(most, f, inv);
+            sl2 *= inv;
+#pragma unroll
+            for (int w8 = 0; w8 < KW; ++w8) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = (float)raw[w8][e] * (sl2_raw < 0.f ? -f : f);
+                cut_queries(q[w8], x);
+            }
+        }
+        // a tile that goes on in the next share: what the merge has to know
+        if (p.cut && tid == 0 && it.divided && it.u0 == 0) {
+            const long long first = share_begin(plan.total, w + 1, plan.n, p.target_log2) - it.u1;  // of the tile's blocks
+            p.cut[w] = CutTile{share_owner(plan.total, first + it.s.blocks - 1, plan.n, p.target_log2) - w + 1,
+                               min(BM, it.s.n * p.G - it.tile * BM), it.tile * BM, it.s.q0, it.h, {0, 0, 0}};
         }
         floatx4 oacc[NDT];
 #pragma unroll
@@ -167,7 +204,7 @@ void paged_fp4_small_kernel(const PagedParams p) {
             // the next keys fly while these are worked on, and below the next values
             if (more) {
                 pages_of(blk + NW, p0, p1);
-                b.load_keys(K, K.page(p0), K.page(p1), kv0 + NW * BN, lane);
+                load_keys(blk + NW);
             }
             const int key0 = kv0 + 8 * kb;  // of this lane's 8 scores
             if (wave_any(kv0 + BN > see)) {
@@ -177,14 +214,14 @@ void paged_fp4_small_kernel(const PagedParams p) {
                     for (int r = 0; r < 4; ++r)
                         if (key0 + 4 * t + r >= see) s[t][r] = -INFINITY;
             }
-            float mx = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-            for (int r = 1; r < 4; ++r) mx = fmaxf(fmaxf(mx, s[0][r]), s[1][r]);
+            float mx = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]),
+                            __builtin_elementwise_maximum(s[1][2], s[1][3]));
             {
                 const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+                mx = __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+                const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = __builtin_elementwise_maximum(__uint_as_float(h[0]), __uint_as_float(h[1])) * sl2;
             }
-            mx = xhalf_max(mx) * sl2;
             const float m_use = (mx > m_run + kTauP) ? mx - kTopP : m_run;
             const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
             const float nm = m_use == -INFINITY ? 0.f : -m_use;
@@ -210,12 +247,13 @@ void paged_fp4_small_kernel(const PagedParams p) {
                 fp4_scales(vs, b.vs[c]);
 #pragma unroll
                 for (int e = 0; e < (c < Block::V4 ? 4 : 2); ++e) {
+                    if (e % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const half8 v = fp4_word(b.v[4 * c + e], vs);
                     oacc[4 * c + e] = mfma16_f16(v, part[1], oacc[4 * c + e]);
                     oacc[4 * c + e] = mfma16_f16(v, part[0], oacc[4 * c + e]);
                 }
             }
-            if (more) b.load_values(V, V.page(p0), V.page(p1), kv0 + NW * BN, lane);
+            if (more) load_values(blk + NW);
         }
 
         // ---- merge the four waves.  Lane (row i16, kb): features 64 c + 16 kb + 4 r + e, of a
@@ -256,6 +294,52 @@ void paged_fp4_small_kernel(const PagedParams p) {
     });
 }
 
+// Merge of the tiles that shares cut, a workgroup a share: four columns of a row a thread, and where
+// a tile has fewer of them than there are threads its parts dealt over groups of
+// threads, whose sums meet in LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_fp4_merge_kernel(const PagedParams p) {
+    __shared__ MergeLds lds;
+    constexpr int BM = kPagedFp4SmallBM, U = 4;
+    const int w = (int)blockIdx.x, tid = (int)threadIdx.x;
+    const CutTile cut = p.cut[w];
+    const int np = cut.np;
+    if (np == 0) return;
+    const int cpr = p.D_v / 4, items = cut.rows * cpr;
+    const int groups = items >= 256 ? 1 : 256 / items;
+    for (int i0 = 0; i0 < items; i0 += 256) {
+        const int group = groups > 1 ? tid / items : 0, i = groups > 1 ? tid - group * items : i0 + tid;
+        const int r = i / cpr, c = 4 * (i - r * cpr);
+        const bool mine = i < items && group < groups;
+        MergedRow x;
+        if (mine)
+            for (int k0 = group; k0 < np; k0 += U * groups) {
+                floatx2 ml[U];
+                floatx4 o[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const size_t row = (size_t)share_slot(w, min(k0 + u * groups, np - 1)) * BM + r;
+                    ml[u] = *reinterpret_cast<const floatx2*>(p.part_ml + 2 * row);
+                    o[u] = *reinterpret_cast<const floatx4*>(p.part_o + row * p.D_v + c);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (k0 + u * groups < np) x.add(ml[u][0], ml[u][1], o[u]);
+            }
+        if (groups > 1) {
+            lds.sum[tid] = x.acc;
+            lds.ml[tid] = (floatx2){x.M, x.L};
+            __syncthreads();
+            if (!mine || group != 0) return;
+            for (int g = 1; g < min(groups, np); ++g) x.add(lds.ml[g * items + i][0], lds.ml[g * items + i][1], lds.sum[g * items + i]);
+        }
+        if (!mine) continue;
+        const int row = cut.row0 + r, t = (int)((unsigned)row / (unsigned)p.G);
+        const int tok = cut.q0 + t, head = cut.h * p.G + (row - t * p.G);
+        x.write(p, static_cast<T*>(p.o) + tok * p.os.t + head * p.os.h + c, c == 0 ? p.stats + (size_t)tok * p.H_kv * p.G + head : nullptr);
+    }
+}
+
 }  // namespace
 
 hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t stream) {
@@ -263,13 +347,15 @@ hipError_t launch_paged_fp4_small(const PagedParams& p, DType dtype, hipStream_t
         using T = decltype(t);
         return with_fp4_dim(p.D_qk, [&](auto dqk) {
             return with_fp4_dim(p.D_v, [&](auto dv) {
-                constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
-                using Cfg = PagedFp4SmallCfg<T, DQK, DV>;
-                hipError_t e = launch_kernel<paged_fp4_small_kernel<T, DQK, DV>>(dim3(1u << p.target_log2), Cfg::NT, Cfg::LDS_BYTES,
-                                                                                stream, p);
-                return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
-                           ? launch_paged_share_merge<T, Cfg::BM, Cfg::PLAN>(p, stream)
-                           : e;
+                return with_bool(p.batch.page_log2 == 4, [&](auto halves) {
+                    constexpr int DQK = decltype(dqk)::value, DV = decltype(dv)::value;
+                    using Cfg = PagedFp4SmallCfg<T, DQK, DV>;
+                    hipError_t e = launch_kernel<paged_fp4_small_kernel<T, DQK, DV, decltype(halves)::value>>(
+                        dim3(1u << p.target_log2), Cfg::NT, Cfg::LDS_BYTES, stream, p);
+                    return e == hipSuccess && paged_shares_divide(p, Cfg::PLAN)
+                               ? launch_kernel<paged_fp4_merge_kernel<T>>(dim3((1u << p.target_log2) - 1), 256, 0, stream, p)
+                               : e;
+                });
             });
         });
     };
