@@ -258,33 +258,39 @@ void paged_fp4_small_kernel(const PagedParams p) {
 
         // ---- merge the four waves.  Lane (row i16, kb): features 64 c + 16 kb + 4 r + e, of a
         // piece of 32 features 64 c + 8 kb + 2 r + e
-        l_run += __shfl_xor(l_run, 16);
-        l_run += __shfl_xor(l_run, 32);
+        {
+            const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+            l_run = xhalf_sum(__uint_as_float(h[0]) + __uint_as_float(h[1]));
+        }
         float* lds = reinterpret_cast<float*>(smem);
+        // (opaque: what is formed from it stays out of the loop, whose registers it would take)
+        int end_tid = threadIdx.x;
+        asm volatile("" : "+v"(end_tid));
+        const int end_lane = end_tid & 63, er = end_lane & 15, ek = end_lane >> 4;
         float* mml = lds + NW * BM * Cfg::OS;
         int* again = reinterpret_cast<int*>(mml + 2 * NW * BM);
         int* none = again + BM;
-        const int at = wave * BM + i16;
-        if (kb == 0) {
+        const int at = wave * BM + er;
+        if (ek == 0) {
             mml[2 * at] = m_run;
             mml[2 * at + 1] = l_run;
         }
-        if (tid < BM) again[tid] = 0;
-        if (lane == 0) none[wave] = pw.bad || it.s.bad;
+        if (end_tid < BM) again[end_tid] = 0;
+        if (end_lane == 0) none[wave] = pw.bad || it.s.bad;
 #pragma unroll
         for (int c = 0; c < Block::V4; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 16 * kb + 4 * r) =
+                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 16 * ek + 4 * r) =
                     (floatx4){oacc[4 * c][r], oacc[4 * c + 1][r], oacc[4 * c + 2][r], oacc[4 * c + 3][r]};
         if constexpr (Block::V2) {
             constexpr int c = Block::V4;
 #pragma unroll
             for (int r = 0; r < 4; r += 2)
-                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 8 * kb + 2 * r) =
+                *reinterpret_cast<floatx4*>(lds + at * Cfg::OS + 64 * c + 8 * ek + 2 * r) =
                     (floatx4){oacc[4 * c][r], oacc[4 * c + 1][r], oacc[4 * c][r + 1], oacc[4 * c + 1][r + 1]};
         }
-        reduce_paged_waves<T, DV, NW, BM>(p, it, lds, tid, [&](int r) {
+        reduce_paged_waves<T, DV, NW, BM>(p, it, lds, end_tid, [&](int r) {
             PagedRow rr;
             rr.init(p, it, it.tile * BM + r);
             const T* qr = static_cast<const T*>(p.q) + rr.tok * p.qs.t + rr.head * p.qs.h;
