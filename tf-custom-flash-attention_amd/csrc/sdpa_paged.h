@@ -172,8 +172,8 @@ inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
 }
 
 // Attention over a cache in 4 bits: sequences of up to so many rows by tiles of 16 rows,
-// four workgroups a CU, others by tiles of 128.
-constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 10;
+// two workgroups a CU, others by tiles of 128.
+constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 9;
 constexpr int kPagedFp4SmallRows = 16;
 // The tile that a workgroup's share begins and does not end, for the merge: its rows
 // are row0 .. row0 + rows - 1 of the sequence from token q0 on and key head h, its parts np (0: none).

@@ -2,7 +2,7 @@
 // drafts) over a paged cache in 4 bits (sdpa_fp4.h), queries in fp16 or fp32, for gfx950.
 //
 // Tiles of 16 rows (tokens times the query heads of a key head) by equal shares of the key
-// blocks (sdpa_paged.h); the four waves of a workgroup take a tile's blocks of 32
+// blocks (sdpa_paged.h); the four waves of a workgroup take a tile's blocks of 64
 // keys in turn, each with sums of its own, merged through LDS at the tile's end.
 //   S^T = K Q^T, online softmax in the log2 domain, O^T += V^T P^T
 // on v_mfma_f32_16x16x32_f16, without LDS in the loop: a lane of the K operand is a key, 8
@@ -12,6 +12,7 @@
 // A word becomes 8 fp16 values by four conversions (v_cvt_scalef32_pk_f16_fp4) and four
 // packed products with the scale, exactly.
 // P enters as two fp16 parts (22 bits): the matrix cores are idle beside the conversions.
+// A wave loads its next block's words as soon as this one's are used up.
 // fp32 queries are cut into three parts (33 bits), after a row's largest has been brought to
 // 2^14 by a power of two.
 #include "sdpa_launch.h"
@@ -23,15 +24,15 @@ namespace {
 template <typename T, int DQK, int DV>
 struct PagedFp4SmallCfg {
     static constexpr int NP = sizeof(T) == 2 ? 1 : 3;  // parts of a query
-    static constexpr int NW = 4, NT = 64 * NW, BM = kPagedFp4SmallBM, BN = 32, PLAN = BN * NW;
+    static constexpr int NW = 4, NT = 64 * NW, BM = kPagedFp4SmallBM, BN = 64, PLAN = BN * NW;
     static constexpr int OS = acc_stride(DV), MERGE = NW * BM * OS * 4 + NW * BM * 8 + (BM + NW) * 4;
     static constexpr int PLAN_AT = (MERGE + 15) / 16 * 16;
     static constexpr size_t LDS_BYTES = PLAN_AT + PagedShares<BM, PLAN>::LDS_BYTES;
-    static constexpr int WPE = NP == 3 && DQK + DV > 96 ? 2 : 4;
+    static constexpr int WPE = 2;
     static_assert(WPE * LDS_BYTES <= 160 * 1024, "gfx950 LDS");
 };
 
-// A wave's part of a block of keys, as it lies in the cache.
+// A lane's words of 32 keys, as they lie in the cache.
 template <int DQK, int DV>
 struct Fp4Block {
     static constexpr int KW = DQK / 32;              // words of a lane's key
@@ -132,23 +133,26 @@ void paged_fp4_small_kernel(const PagedParams p) {
         V.init(p.v_cache, p.H_kv, it.h, DV, p.batch.page_log2);
         PageWindow pw{uniform_ptr(p.batch.page_table + it.seq * p.batch.table_stride), p.batch.pages,
                       (min(kv_end, hi * BN) + (1 << K.log2) - 1) >> K.log2};
-        Block b;
-        const auto pages_of = [&](int blk, int& p0, int& p1) __attribute__((always_inline)) {
-            const int c = (blk * BN) >> K.log2;
-            pw.need(c, lane);  // (a window holds whole blocks)
-            p0 = pw.held(c);
-            p1 = HALVES ? pw.held(c + 1) : p0;
-        };
-        int p0 = 0, p1 = 0;
+        // A block's 64 keys in two halves, whose sums do not wait for each other's.
+        Block half[2];
+        int page[2][2];  // of a half (HALVES: of 16 keys each)
         const auto load_keys = [&](int blk) __attribute__((always_inline)) {
-            b.template load_keys<HALVES>(K, p0, p1, blk * BN, lane);
+            pw.need((blk * BN) >> K.log2, lane);  // (a window holds whole blocks)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int kv0 = blk * BN + 32 * h, c = kv0 >> K.log2;
+                page[h][0] = pw.held(c);
+                page[h][1] = HALVES ? pw.held(c + 1) : 0;
+                half[h].template load_keys<HALVES>(K, page[h][0], page[h][1], kv0, lane);
+            }
         };
         const auto load_values = [&](int blk) __attribute__((always_inline)) {
-            b.template load_values<HALVES>(V, p0, p1, blk * BN, lane);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                half[h].template load_values<HALVES>(V, page[h][0], page[h][1], blk * BN + 32 * h, lane);
         };
         pw.load((lo * BN) >> K.log2, lane);
         if (lo + wave < hi) {
-            pages_of(lo + wave, p0, p1);
             load_keys(lo + wave);
             load_values(lo + wave);
         }
@@ -192,30 +196,33 @@ void paged_fp4_small_kernel(const PagedParams p) {
         for (int blk = lo + wave; blk < hi; blk += NW) {
             const int kv0 = blk * BN;
             const bool more = blk + NW < hi;
-            floatx4 s[2] = {floatx4{}, floatx4{}};
+            floatx4 s[2][2] = {};  // [half][tile]
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int w8 = 0; w8 < KW; ++w8)
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    const half8 k = b.k[t].word(w, kb);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; --n) s[t] = mfma16_f16(k, q[w][n], s[t]);
-                }
-            // the next keys fly while these are worked on, and below the next values
-            if (more) {
-                pages_of(blk + NW, p0, p1);
-                load_keys(blk + NW);
-            }
-            const int key0 = kv0 + 8 * kb;  // of this lane's 8 scores
+                    for (int t = 0; t < 2; ++t) {
+                        const half8 k = half[h].k[t].word(w8, kb);
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) s[h][t] = mfma16_f16(k, q[w8][n], s[h][t]);
+                    }
+            if (more) load_keys(blk + NW);
+            const int key0 = kv0 + 8 * kb;  // of this lane's 8 scores of each half
             if (wave_any(kv0 + BN > see)) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (key0 + 4 * t + r >= see) s[t][r] = -INFINITY;
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (key0 + 32 * h + 4 * t + r >= see) s[h][t][r] = -INFINITY;
             }
-            float mx = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]),
-                            __builtin_elementwise_maximum(s[1][2], s[1][3]));
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) mx = max3(mx, max3(s[h][t][0], s[h][t][1], s[h][t][2]), s[h][t][3]);
             {
                 const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
                 mx = __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -225,34 +232,41 @@ void paged_fp4_small_kernel(const PagedParams p) {
             const float m_use = (mx > m_run + kTauP) ? mx - kTopP : m_run;
             const float alpha = m_use == m_run ? 1.f : fast_exp2(m_run - m_use);
             const float nm = m_use == -INFINITY ? 0.f : -m_use;
-            float pf[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) pf[j] = fast_exp2(__builtin_fmaf(s[j / 4][j % 4], sl2, nm));
             if (wave_any(alpha != 1.f)) {
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) oacc[dt][r] *= alpha;
             }
-            l_run = __builtin_fmaf(l_run, alpha, ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7])));
             m_run = m_use;
-            half8 part[2];
-            cut_queries(part, pf);
+            l_run *= alpha;
+            half8 part[2][2];  // [half][part]
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float pf[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pf[j] = fast_exp2(__builtin_fmaf(s[h][j / 4][j % 4], sl2, nm));
+                l_run += ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7]));
+                cut_queries(part[h], pf);
+            }
             if (kv0 + BN > kv_end)  // what lies behind the last key, whatever it is, is 0
 #pragma unroll
-                for (int c = 0; c < Block::NV; ++c) b.vs[c] = first_bytes(b.vs[c], kv_end - key0);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int c = 0; c < Block::NV; ++c) {
-                half2v vs[4];
-                fp4_scales(vs, b.vs[c]);
+                    for (int c = 0; c < Block::NV; ++c) half[h].vs[c] = first_bytes(half[h].vs[c], kv_end - key0 - 32 * h);
 #pragma unroll
-                for (int e = 0; e < (c < Block::V4 ? 4 : 2); ++e) {
-                    if (e % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-                    const half8 v = fp4_word(b.v[4 * c + e], vs);
-                    oacc[4 * c + e] = mfma16_f16(v, part[1], oacc[4 * c + e]);
-                    oacc[4 * c + e] = mfma16_f16(v, part[0], oacc[4 * c + e]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < Block::NV; ++c) {
+                    half2v vs[4];
+                    fp4_scales(vs, half[h].vs[c]);
+#pragma unroll
+                    for (int e = 0; e < (c < Block::V4 ? 4 : 2); ++e) {
+                        const half8 v = fp4_word(half[h].v[4 * c + e], vs);
+#pragma unroll
+                        for (int n = 1; n >= 0; --n) oacc[4 * c + e] = mfma16_f16(v, part[h][n], oacc[4 * c + e]);
+                    }
                 }
-            }
             if (more) load_values(blk + NW);
         }
 
