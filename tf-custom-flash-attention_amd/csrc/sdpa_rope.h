@@ -180,7 +180,9 @@ struct RowTurn {
             }
         }
     }
-    // The same by axes; `pos`: the token's position on axis 0.
+    // The same by axes; `pos`: the token's position on axis 0.  A lane whose pairs all follow one
+    // axis reads that row of the tables, as with one position; where some lane's do not, all
+    // read the rows of every axis and choose pair by pair.
     template <bool IN>
     __device__ __forceinline__ void load_axes(const RopeArgs& p, const AxesArgs& ax, const RowLane<EPC, IN>& l,
                                               const int32_t* pos) {
@@ -188,43 +190,52 @@ struct RowTurn {
         constexpr int HP = IN ? EPC / 2 : EPC;
         constexpr uint32_t kHalf = (1u << HP) - 1;
         const uint32_t mine = (l.ra ? kHalf : 0u) | (IN && l.rb ? kHalf << HP : 0u);
-        const uint32_t lo = mine ? (uint32_t)(ax.lo >> l.t) : 0u, hi = mine ? (uint32_t)(ax.hi >> l.t) : 0u;
+        const uint32_t lo = mine ? (uint32_t)(ax.lo >> l.t) & mine : 0u, hi = mine ? (uint32_t)(ax.hi >> l.t) & mine : 0u;
         int32_t row[kMaxAxes];
+        const int any = __builtin_ctz((unsigned)ax.used);
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; ++a) row[a] = pos[((ax.used >> a) & 1 ? a : any) * ax.stride];
         bad = false;
 #pragma unroll
-        for (int a = 0; a < kMaxAxes; ++a) {
-            row[a] = 0;
-            if (!((ax.used >> a) & 1)) continue;
-            row[a] = pos[a * ax.stride];
-            if (row[a] < 0 || row[a] >= p.rows) {
-                bad = true;
-                row[a] = 0;
-            }
-        }
+        for (int a = 0; a < kMaxAxes; ++a) bad = bad || (uint32_t)row[a] >= (uint32_t)p.rows;
 #pragma unroll
         for (int i = 0; i < EPC; ++i) {
             c[i] = 1.f;
             s[i] = 0.f;
         }
         if (p.rows == 0) return;
+        const auto load = [&](int32_t r, float (&x)[EPC], float (&y)[EPC]) __attribute__((always_inline)) {
+            const long long at = (long long)(bad ? 0 : r) * (p.R / 2) + l.t;
+#pragma unroll
+            for (int h = 0; h < EPC; h += HP)
+                if ((mine >> h) & 1) {
+                    float u[HP], v[HP];
+                    load_table<HP>(u, p.cos + at + h);
+                    load_table<HP>(v, p.sin + at + h);
+#pragma unroll
+                    for (int i = 0; i < HP; ++i) {
+                        x[h + i] = u[i];
+                        y[h + i] = v[i];
+                    }
+                }
+        };
+        const bool mixed = (lo != 0 && lo != mine) || (hi != 0 && hi != mine);
+        if (!wave_any(mixed)) {
+            load(lo ? (hi ? row[3] : row[1]) : (hi ? row[2] : row[0]), c, s);
+            return;
+        }
 #pragma unroll
         for (int a = 0; a < kMaxAxes; ++a) {
+            if (!((ax.used >> a) & 1)) continue;
+            float x[EPC] = {}, y[EPC] = {};
+            load(row[a], x, y);
             const uint32_t on = mine & (a & 1 ? lo : ~lo) & (a & 2 ? hi : ~hi);
-            if (on == 0) continue;
-            const long long at = (long long)row[a] * (p.R / 2) + l.t;
 #pragma unroll
-            for (int h = 0; h < EPC; h += HP) {
-                if (!((mine >> h) & 1)) continue;
-                float x[HP], y[HP];
-                load_table<HP>(x, p.cos + at + h);
-                load_table<HP>(y, p.sin + at + h);
-#pragma unroll
-                for (int i = 0; i < HP; ++i)
-                    if ((on >> (h + i)) & 1) {
-                        c[h + i] = x[i];
-                        s[h + i] = y[i];
-                    }
-            }
+            for (int i = 0; i < EPC; ++i)
+                if ((on >> i) & 1) {
+                    c[i] = x[i];
+                    s[i] = y[i];
+                }
         }
     }
     // The pairs of (a, b) turned back by the angle.
