@@ -2,7 +2,8 @@
 // (sdpa_fp4.h), keys normed (where asked) and rotated on the way, the queries of the same
 // tokens beside them in one launch; and tokens out of such pages again.  For gfx950.
 //
-// Queries go as in sdpa_kv_append.hip.  8 tokens of a head share the words of the
+// Queries go as in sdpa_kv_append.hip, where calls are large by its kernel (which
+// needs half the registers, and waits for memory).  8 tokens of a head share the words of the
 // values' codes, so a wave takes those new tokens of one head that lie in the same 8 places
 // of a sequence; of a window of W packed tokens it takes each run of such that begins in it.
 // The words of a run that does not fill its 8 places are read, and the other tokens' codes
@@ -196,16 +197,18 @@ __device__ __forceinline__ void append_values(const AppendParams& p, const Fp4Ru
 template <int W>
 __host__ __device__ inline long long fp4_units(int T, int H_kv) { return ((long long)T + W - 1) / W * H_kv; }
 
-template <typename T, int EPC, int LPR, bool IN, bool AX, int W>
-__global__ __launch_bounds__(64 * kAppendWaves) void kv_append_fp4_kernel(const AppendParams p) {
+// QUERIES: those of the tokens too, behind the keys and values, which are the longer chains.
+template <typename T, int EPC, int LPR, bool IN, bool AX, int W, bool QUERIES>
+__global__ __launch_bounds__(64 * kAppendWaves, W > 1 ? 4 : 1) void kv_append_fp4_kernel(const AppendParams p) {
     __shared__ Fp4Lds lds[kAppendWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    long long u = (long long)tile_id() * kAppendWaves + wave;
-    // keys and values first: they are the longer chains
     const long long n = fp4_units<W>(p.batch.T, p.H_kv);
+    long long u = (long long)tile_id() * kAppendWaves + wave;
     if (u >= 2 * n) {
-        const AppendMap m = append_map<LPR>(p.batch.T, p.H_q);
-        if (u - 2 * n < m.units) append_rows<T, EPC, LPR, IN, AX>(p, m, u - 2 * n, 0);
+        if constexpr (QUERIES) {
+            const AppendMap m = append_map<LPR>(p.batch.T, p.H_q);
+            if (u - 2 * n < m.units) append_rows<T, EPC, LPR, IN, AX>(p, m, u - 2 * n, 0);
+        }
         return;
     }
     const bool values = u >= n;
@@ -223,15 +226,20 @@ hipError_t launch_kv_append_fp4_t(const AppendParams& p, hipStream_t stream) {
     return with_append_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value;
         constexpr bool IN = decltype(in)::value;
-        const auto run = [&](auto w) {
+        const auto run = [&](auto w, auto queries) {
             constexpr int W = decltype(w)::value;
-            const long long n = append_map<L>(p.batch.T, p.H_q).units + 2 * fp4_units<W>(p.batch.T, p.H_kv);
+            constexpr bool Q = decltype(queries)::value;
+            const long long n = 2 * fp4_units<W>(p.batch.T, p.H_kv) + (Q ? append_map<L>(p.batch.T, p.H_q).units : 0);
             if (n == 0) return hipSuccess;
-            return launch_kernel<kv_append_fp4_kernel<T, E, L, IN, AX, W>>(
+            return launch_kernel<kv_append_fp4_kernel<T, E, L, IN, AX, W, Q>>(
                 tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves), 64 * kAppendWaves, 0, stream, p);
         };
-        if (fp4_units<kFp4Run>(p.batch.T, p.H_kv) >= kFp4FewWindows) return run(std::integral_constant<int, kFp4Run>{});
-        return run(std::integral_constant<int, 1>{});
+        if (fp4_units<kFp4Run>(p.batch.T, p.H_kv) < kFp4FewWindows) return run(std::integral_constant<int, 1>{}, std::true_type{});
+        const hipError_t e = run(std::integral_constant<int, kFp4Run>{}, std::false_type{});
+        if (e != hipSuccess || p.H_q == 0) return e;
+        AppendParams q = p;
+        q.H_k = q.H_v = 0;
+        return launch_kv_append(q, sizeof(T) == 2 ? DType::F16 : DType::F32, stream);
     });
 }
 

@@ -52,9 +52,13 @@ def _on_device(device, **tensors):
             _fail(f"{name} is on {t.device}, not on {device}")
 
 
+# (what torch.cuda.current_device does once the GPU is in use, as it is where its tensors are)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(entry, device, *args):
     """``entry(*args, stream)`` with ``device`` current."""
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         code = entry(*args, _stream_handle(device))
     else:
         with torch.cuda.device(device):
@@ -469,9 +473,56 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
 
     More tokens than ``total`` have no rows: ``kv_append`` and ``paged_sdpa`` leave out sequences that reach past it.
     """
+    N, width, capacity, device = _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished)
+    table, lens, fresh, pages, count, ended = (page_table.data_ptr(), kv_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
+                                               free_count.data_ptr(), _ptr(finished))
+    # what is written shares memory with nothing else
+    stride = page_table.stride(0)
+    reads = [(lens, 4 * N), (fresh, 4 * N), (count, 4)]
+    if ended is not None:
+        reads.append((ended, N))
+    table_bytes = 4 * ((N - 1) * stride + width) if N and width else 0
+    for start, size in reads:
+        if (start < table + table_bytes and table < start + size) or (start < pages + 4 * capacity and pages < start + size):
+            _fail("page_table, free_pages, kv_lens and free_count must not share memory")
+    if pages < table + table_bytes and table < pages + 4 * capacity:
+        _fail("page_table, free_pages, kv_lens and free_count must not share memory")
+    new = kv_lens.new_empty
+    if in_place:
+        for start, size in reads[1:]:
+            if start < lens + 4 * N and lens < start + size:
+                _fail("kv_lens and free_count must be memory of their own")
+        for start, size in reads[1:2] + reads[3:]:
+            if start < count + 4 and count < start + size:
+                _fail("kv_lens and free_count must be memory of their own")
+        out = Reserved(new(N + 1), kv_lens, free_count, new(total), new(total, dtype=torch.int64))
+    else:
+        out = Reserved(new(N + 1), new(N), new(1), new(total), new(total, dtype=torch.int64))
+    _call(library().sdpa_hip_kv_reserve, device, table, stride, lens, fresh, ended, pages, count, out[0].data_ptr(),
+          out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), N, total, width, page_size, capacity)
+    return out
+
+
+def _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished):
+    """Checks of ``kv_reserve`` but for shared memory: (N, width, capacity, device)."""
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
         _fail("page_table must be [sequences, pages per sequence]")
     N, width = page_table.shape
+    device = page_table.device
+    one, sizes = (N,), type(page_size) is int and type(total) is int and 0 <= total <= _MOST and 0 < page_size <= _MOST
+    # (usual arguments by a few comparisons, others one by one)
+    if (sizes and page_table.dtype is _I32 and page_table.is_contiguous() and device.type == "cuda"
+            and isinstance(kv_lens, torch.Tensor) and isinstance(new_lens, torch.Tensor) and isinstance(free_pages, torch.Tensor)
+            and isinstance(free_count, torch.Tensor)
+            and kv_lens.dtype is _I32 and new_lens.dtype is _I32 and free_pages.dtype is _I32 and free_count.dtype is _I32
+            and kv_lens.shape == one and new_lens.shape == one and free_count.shape == (1,) and free_pages.dim() == 1
+            and kv_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+            and kv_lens.device == device and new_lens.device == device and free_pages.device == device and free_count.device == device
+            and (finished is None or (isinstance(finished, torch.Tensor) and finished.dtype in (torch.bool, _U8)
+                                      and finished.shape == one and finished.is_contiguous() and finished.device == device))):
+        capacity = free_pages.shape[0]
+        if N + width + capacity <= _MOST:
+            return N, width, capacity, device
     _int32("page_table", page_table, N, width)
     if (width > 1 and page_table.stride(1) != 1) or (N > 1 and page_table.stride(0) < width):
         _fail("the rows of page_table must be contiguous and memory of their own")
@@ -480,27 +531,12 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
     _vector("free_pages", free_pages, None, _I32)
     _vector("free_count", free_count, 1, _I32)
     if finished is not None:
-        _vector("finished", finished, N, torch.bool, torch.uint8)
-    if type(page_size) is not int or type(total) is not int or not 0 <= total <= _MOST or not 0 < page_size <= _MOST:
+        _vector("finished", finished, N, torch.bool, _U8)
+    if not sizes:
         _fail("page_size and total must be sizes")
     _sizes_fit(page_table=page_table, free_pages=free_pages)
-    device = page_table.device
     _on_device(device, kv_lens=kv_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count, finished=finished)
-    states = {"page_table": page_table, "free_pages": free_pages, "kv_lens": kv_lens, "free_count": free_count}
-    if _share_memory(free_pages, page_table) or any(
-            _share_memory(t, s) for t in (kv_lens, free_count, new_lens) + (() if finished is None else (finished,))
-            for s in (page_table, free_pages)):
-        _fail(f"{', '.join(states)} must not share memory")
-    if in_place and (_share_memory(kv_lens, free_count) or _share_memory(kv_lens, new_lens) or _share_memory(free_count, new_lens)
-                     or (finished is not None and (_share_memory(kv_lens, finished) or _share_memory(free_count, finished)))):
-        _fail("kv_lens and free_count must be memory of their own")
-    new = lambda n, dtype: torch.empty((n,), dtype=dtype, device=device)  # noqa: E731
-    out = Reserved(new(N + 1, _I32), kv_lens if in_place else new(N, _I32), free_count if in_place else new(1, _I32),
-                   new(total, _I32), new(total, torch.int64))
-    _call(library().sdpa_hip_kv_reserve, device, page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
-          new_lens.data_ptr(), _ptr(finished), free_pages.data_ptr(), free_count.data_ptr(), *(t.data_ptr() for t in out), N, total,
-          width, page_size, free_pages.shape[0])
-    return out
+    return N, width, free_pages.shape[0], device
 
 
 def _append_positions(positions, axes, cos, n, device):
