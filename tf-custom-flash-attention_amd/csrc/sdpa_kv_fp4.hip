@@ -204,10 +204,11 @@ __global__ __launch_bounds__(64 * kAppendWaves, W > 1 ? 4 : 1) void kv_append_fp
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long n = fp4_units<W>(p.batch.T, p.H_kv);
     long long u = (long long)tile_id() * kAppendWaves + wave;
-    if (u >= 2 * n) {
+    constexpr int KINDS = W > 1 ? 1 : 2;  // keys and values by waves of their own, or by one after the other
+    if (u >= KINDS * n) {
         if constexpr (QUERIES) {
             const AppendMap m = append_map<LPR>(p.batch.T, p.H_q);
-            if (u - 2 * n < m.units) append_rows<T, EPC, LPR, IN, AX>(p, m, u - 2 * n, 0);
+            if (u - KINDS * n < m.units) append_rows<T, EPC, LPR, IN, AX>(p, m, u - KINDS * n, 0);
         }
         return;
     }
@@ -216,8 +217,8 @@ __global__ __launch_bounds__(64 * kAppendWaves, W > 1 ? 4 : 1) void kv_append_fp
     const int window = (int)(u / (unsigned)p.H_kv), h = (int)(u - (long long)window * p.H_kv);
     each_run<W>(p.batch, window * W, [&](const Fp4Run& run) __attribute__((always_inline)) {
         if (run.page < 0) return;
-        if (values) append_values<T, (EPC > 1)>(p, run, h, lds[wave]);
-        else append_keys<T, EPC, LPR, IN, AX>(p, run, h, lds[wave]);
+        if (KINDS == 1 || values) append_values<T, (EPC > 1)>(p, run, h, lds[wave]);
+        if (KINDS == 1 || !values) append_keys<T, EPC, LPR, IN, AX>(p, run, h, lds[wave]);
     });
 }
 
@@ -229,7 +230,7 @@ hipError_t launch_kv_append_fp4_t(const AppendParams& p, hipStream_t stream) {
         const auto run = [&](auto w, auto queries) {
             constexpr int W = decltype(w)::value;
             constexpr bool Q = decltype(queries)::value;
-            const long long n = 2 * fp4_units<W>(p.batch.T, p.H_kv) + (Q ? append_map<L>(p.batch.T, p.H_q).units : 0);
+            const long long n = (W > 1 ? 1 : 2) * fp4_units<W>(p.batch.T, p.H_kv) + (Q ? append_map<L>(p.batch.T, p.H_q).units : 0);
             if (n == 0) return hipSuccess;
             return launch_kernel<kv_append_fp4_kernel<T, E, L, IN, AX, W, Q>>(
                 tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves), 64 * kAppendWaves, 0, stream, p);
