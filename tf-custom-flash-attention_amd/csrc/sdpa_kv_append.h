@@ -47,6 +47,8 @@ struct AppendParams {
     int interleaved, w32, vec;
 };
 
+// From so many waves of four rows per group of lanes on queries without keys are taken so.
+constexpr int kAppendFewWaves = 2048;
 hipError_t launch_kv_append(const AppendParams& p, DType dtype, hipStream_t stream);
 
 // The same into a cache in 4 bits (sdpa_kv_fp4.hip; all bytes of a page's head in

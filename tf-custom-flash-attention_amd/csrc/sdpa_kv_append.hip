@@ -23,25 +23,25 @@
 namespace sdpa {
 namespace {
 
-template <typename T, int EPC, int LPR, bool IN, bool AX>
+template <typename T, int EPC, int LPR, bool IN, bool AX, int KU>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(const AppendParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const PagedBatch& bt = p.batch;
     long long u = (long long)tile_id() * kAppendWaves + wave;
-    AppendMap m = append_map<LPR>(bt.T, p.H_q);
+    AppendMap m = append_map<LPR, KU>(bt.T, p.H_q);
     int kind = 0;  // 0: q, 1: k, 2: v
     if (u >= m.units) {
         u -= m.units;
-        m = append_map<LPR>(bt.T, p.H_k);
+        m = append_map<LPR, KU>(bt.T, p.H_k);
         kind = 1;
         if (u >= m.units) {
             u -= m.units;
-            m = append_map<LPR>(bt.T, p.H_v);
+            m = append_map<LPR, KU>(bt.T, p.H_v);
             kind = 2;
             if (u >= m.units) return;
         }
     }
-    append_rows<T, EPC, LPR, IN, AX>(p, m, u, kind);
+    append_rows<T, EPC, LPR, IN, AX, KU>(p, m, u, kind);
 }
 
 template <typename T, bool AX>
@@ -49,11 +49,17 @@ hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
     return with_append_row<T>(p, [&](auto epc, auto lpr, auto in) {
         constexpr int E = decltype(epc)::value, L = decltype(lpr)::value;
         constexpr bool IN = decltype(in)::value;
-        const long long n = append_map<L>(p.batch.T, p.H_q).units + append_map<L>(p.batch.T, p.H_k).units +
-                            append_map<L>(p.batch.T, p.H_v).units;
-        if (n == 0) return hipSuccess;
-        return launch_kernel<kv_append_kernel<T, E, L, IN, AX>>(tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves),
-                                                            64 * kAppendWaves, 0, stream, p);
+        const auto run = [&](auto ku) {
+            constexpr int KU = decltype(ku)::value;
+            const long long n = append_map<L, KU>(p.batch.T, p.H_q).units + append_map<L, KU>(p.batch.T, p.H_k).units +
+                                append_map<L, KU>(p.batch.T, p.H_v).units;
+            if (n == 0) return hipSuccess;
+            return launch_kernel<kv_append_kernel<T, E, L, IN, AX, KU>>(tile_grid((n + kAppendWaves - 1) / kAppendWaves, 64 * kAppendWaves),
+                                                                        64 * kAppendWaves, 0, stream, p);
+        };
+        // (queries alone, many of them: of the append in 4 bits)
+        if (p.H_k == 0 && p.H_v == 0 && append_map<L, 4>(p.batch.T, p.H_q).units >= kAppendFewWaves) return run(std::integral_constant<int, 4>{});
+        return run(std::integral_constant<int, 1>{});
     });
 }
 

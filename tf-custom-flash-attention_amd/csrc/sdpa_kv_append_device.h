@@ -17,27 +17,28 @@ struct AppendMap {
     int H, gpt, tpw, splits;
     long long units;
 };
-template <int LPR>
+// KU: rows of a group of lanes.
+template <int LPR, int KU = 1>
 __host__ __device__ inline AppendMap append_map(int tokens, int H) {
     constexpr int RG = 64 / LPR;
     AppendMap m{H, 1, 1, 0, 0};
     if (H <= 0 || tokens <= 0) return m;
     while (m.gpt < H && m.gpt < RG) m.gpt *= 2;
     m.tpw = RG / m.gpt;
-    m.splits = (H + m.gpt - 1) / m.gpt;
+    m.splits = (H + m.gpt * KU - 1) / (m.gpt * KU);
     m.units = ((long long)tokens + m.tpw - 1) / m.tpw * m.splits;
     return m;
 }
 
 // Unit u of the rows of q (kind 0), k (1) or v (2).
-template <typename T, int EPC, int LPR, bool IN, bool AX>
+template <typename T, int EPC, int LPR, bool IN, bool AX, int KU = 1>
 __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendMap& m, long long u, int kind) {
     const int lane = threadIdx.x & 63;
     const PagedBatch& bt = p.batch;
     const unsigned uu = (unsigned)u, tg = uu / (unsigned)m.splits;
     const int group = lane / LPR, tok0 = (int)(tg * (unsigned)m.tpw), mine = group / m.gpt;
     const long long tok = (long long)tok0 + mine;
-    const int h = (int)(uu - tg * (unsigned)m.splits) * m.gpt + group % m.gpt;
+    const int h = (int)(uu - tg * (unsigned)m.splits) * m.gpt * KU + group % m.gpt;  // and further ones, gpt apart
     const bool in_batch = tok < bt.T;
 
     // the row, before it is known where it goes
@@ -46,8 +47,13 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendM
     l.init(lane % LPR, D, kind == 2 ? 0 : p.r.R, p.interleaved != 0);
     const T* x = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v);
     const TokenStrides xs = kind == 0 ? p.qs : kind == 1 ? p.ks : p.vs;
-    chunk_t<T, EPC> a, b;
-    load_row<T, EPC, IN>(a, b, x + (in_batch ? tok : bt.T - 1) * xs.t + min(h, m.H - 1) * xs.h, l);
+    chunk_t<T, EPC> a[KU], b[KU];
+#pragma unroll
+    for (int i = 0; i < KU; ++i)
+        load_row<T, EPC, IN>(a[i], b[i], x + (in_batch ? tok : bt.T - 1) * xs.t + min(h + i * m.gpt, m.H - 1) * xs.h, l);
+    RowTurn<EPC> t;
+    if constexpr (AX)
+        if (kind != 2) t.load_axes(p.r, p.axes, l, p.axes.positions + (in_batch ? tok : bt.T - 1));
 
     // sequence of the token: the last that begins at or before it
     int count = 0;
@@ -68,11 +74,8 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendM
     if (pos >= 0 && pg < bt.width) page = bt.page_table[s * bt.table_stride + pg];
     const bool placed = page >= 0 && page < bt.pages;
 
-    RowTurn<EPC> t;
-    if (kind != 2) {
-        if constexpr (AX) t.load_axes(p.r, p.axes, l, p.axes.positions + tok);
-        else t.load(p.r, l, pos);
-    }
+    if constexpr (!AX)
+        if (kind != 2) t.load(p.r, l, pos);
     float wa[EPC], wb[EPC];
     load_weight<T, EPC, IN>(wa, wb, kind == 2 ? nullptr : kind == 0 ? p.q_weight : p.k_weight, p.w32 != 0, l);
     const long long slot = pos & ((1LL << bt.page_log2) - 1);
@@ -86,14 +89,17 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendM
         hs = (long long)D << bt.page_log2;
         y = static_cast<T*>(kind == 1 ? p.k_cache : p.v_cache) + (long long)page * p.H_kv * hs + slot * D;
     }
-    if (kind != 2) {
-        RowFactors<EPC, IN> f;
-        f.init(l, t, wa, wb);
-        float r = p.r.norm ? row_rnorm<T, LPR, EPC, IN>(a, b, l, p.r) : 1.f;
-        if (t.bad || !placed) r = __builtin_nanf("");
-        f.template apply<T>(l, a, b, r);
+    RowFactors<EPC, IN> f;
+    if (kind != 2) f.init(l, t, wa, wb);
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+        if (kind != 2) {
+            float r = p.r.norm ? row_rnorm<T, LPR, EPC, IN>(a[i], b[i], l, p.r) : 1.f;
+            if (t.bad || !placed) r = __builtin_nanf("");
+            f.template apply<T>(l, a[i], b[i], r);
+        }
+        store_row<T, EPC, IN>(y + (h + i * m.gpt) * hs, a[i], b[i], h + i * m.gpt < m.H, l);
     }
-    store_row<T, EPC, IN>(y + h * hs, a, b, h < m.H, l);
 }
 
 // f<EPC, LPR, IN>() for the chunks these rows allow.
