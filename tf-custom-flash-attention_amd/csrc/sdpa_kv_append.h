@@ -47,7 +47,8 @@ struct AppendParams {
     int interleaved, w32, vec;
 };
 
-// From so many waves of four rows per group of lanes on queries without keys are taken so.
+// From so many waves of four rows per group of lanes on queries without keys are taken so: 8643 tokens
+// of 32 heads of 128, fp16, one row a group 35.6 us, two 33.9, four 32.3.
 constexpr int kAppendFewWaves = 2048;
 hipError_t launch_kv_append(const AppendParams& p, DType dtype, hipStream_t stream);
 
@@ -61,7 +62,10 @@ struct Fp4ReadParams {
     void* v;  // [T, H_kv, D_v]
     int H_kv, D_qk, D_v;
 };
-// From so many windows of 8 tokens (and heads) on a wave takes 8 tokens, else one.
+// From so many windows of 8 tokens (and heads) on a wave takes 8 tokens, else one.  us of the
+// append by one token and by 8, 32 query heads on 8, D 128: a prompt of 512 tokens (512 windows) 18 and
+// 21, 1024 23 and 20.5, 2048 44 and 23; single tokens of as many sequences 18 and 35, 38 and 41,
+// 102 and 69.
 constexpr int kFp4FewWindows = 1024;
 hipError_t launch_kv_append_fp4(const AppendParams& p, DType dtype, hipStream_t stream);
 hipError_t launch_kv_read_fp4(const Fp4ReadParams& p, DType dtype, hipStream_t stream);

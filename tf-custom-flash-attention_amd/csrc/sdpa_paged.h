@@ -171,10 +171,17 @@ inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
     return ((size_t)2 << target_log2) * BM * ((size_t)D_v + 2) * sizeof(float);
 }
 
-// Attention over a cache in 4 bits: sequences of up to so many rows by tiles of 16 rows,
-// two workgroups a CU, others by tiles of 128.
+// Attention over a cache in 4 bits.  Sequences of up to so many rows, as far as is known, go by
+// tiles of 16 rows (two workgroups a CU), others by tiles of 128.  us a call by 16-row and by
+// 128-row tiles, 4 key heads, D 128, sequences of 600 to 16384 tokens (64), 4 x 2000, 32 x 4096,
+// 256 x 500, one of 30000, 8 x 300:
+//   fp16, 32 rows: 102, 132; 19, 22; 37, 46; 54, 55; 59, 27; 19, 22
+//   fp16, 64 rows: 187, 150; 22, 24; 60, 55; 101, 63; 43, 30; 19, 23
+//   fp32, 32 rows (from 4 x 2000 on): 20, 28; 44, 89; 64, 124; 60, 34; 19, 26
+//   fp32, 64 rows: 25, 30; 72, 94; 119, 133; 46, 37; 19, 27
+// One long sequence alone loses by the small tiles; lengths are on the device.
 constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 9;
-constexpr int kPagedFp4SmallRows = 16;
+constexpr int kPagedFp4SmallRowsF16 = 32, kPagedFp4SmallRowsF32 = 64;
 // The tile that a workgroup's share begins and does not end, for the merge: its rows
 // are row0 .. row0 + rows - 1 of the sequence from token q0 on and key head h, its parts np (0: none).
 struct CutTile {

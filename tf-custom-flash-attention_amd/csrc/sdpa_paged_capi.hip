@@ -365,7 +365,7 @@ namespace {
 
 // Which kernel a call takes: by the rows of its sequences, as far as is known, and the cache.
 bool paged_is_small(bool fp4, int dtype, long long most_rows) {
-    if (fp4) return most_rows <= sdpa::kPagedFp4SmallRows;
+    if (fp4) return most_rows <= (dtype == SDPA_DTYPE_F16 ? sdpa::kPagedFp4SmallRowsF16 : sdpa::kPagedFp4SmallRowsF32);
     return sdpa::paged_small(dtype == SDPA_DTYPE_F16, most_rows);
 }
 int paged_tile_rows(bool fp4, bool small) {

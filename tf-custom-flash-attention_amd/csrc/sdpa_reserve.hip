@@ -18,7 +18,10 @@ namespace sdpa {
 namespace {
 
 constexpr int kReserveThreads = 1024, kReserveWaves = kReserveThreads / 64;
-constexpr int kReserveFill = 4096;
+// us a call by one kernel and by two: one sequence, 4096 tokens 13.8 and 15.8, 8192 24 and 15.8; 8
+// sequences, 4096 15.6 and 15.8, 16384 45 and 15.7; 1024 sequences of one token 13.3 and 15.7, of four
+// 29.8 and 16.4.  (13.3 is the host's time of a call.)
+constexpr int kReserveFill = 2048;
 
 // Sums over the workgroup: x becomes the sum over the threads before, the sum over
 // all is returned.  Two barriers; `lds` is free again after the next ones.
