@@ -40,11 +40,11 @@ struct AppendParams {
     const void* k_weight;
     TokenStrides qs, qos, ks, vs;
     RopeArgs r;
-    AxesArgs axes;      // (positions [axes][T] instead of the places, where some are used)
     int H_kv;           // heads of the caches
     int H_q, H_k, H_v;  // heads whose rows are taken: none of those without features
     int D_qk, D_v;
     int interleaved, w32, vec;
+    AxesArgs axes;  // (positions [axes][T] instead of the places, where some are used)
 };
 
 // From so many waves of four rows per group of lanes on queries without keys are taken so: 8643 tokens

@@ -89,17 +89,19 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendM
         hs = (long long)D << bt.page_log2;
         y = static_cast<T*>(kind == 1 ? p.k_cache : p.v_cache) + (long long)page * p.H_kv * hs + slot * D;
     }
-    RowFactors<EPC, IN> f;
-    if (kind != 2) f.init(l, t, wa, wb);
+    // (several rows of a group of lanes are queries', and each is stored as it is done)
+    if (KU > 1 || kind != 2) {
+        RowFactors<EPC, IN> f;
+        f.init(l, t, wa, wb);
 #pragma unroll
-    for (int i = 0; i < KU; ++i) {
-        if (kind != 2) {
+        for (int i = 0; i < KU; ++i) {
             float r = p.r.norm ? row_rnorm<T, LPR, EPC, IN>(a[i], b[i], l, p.r) : 1.f;
             if (t.bad || !placed) r = __builtin_nanf("");
             f.template apply<T>(l, a[i], b[i], r);
+            if constexpr (KU > 1) store_row<T, EPC, IN>(y + (h + i * m.gpt) * hs, a[i], b[i], h + i * m.gpt < m.H, l);
         }
-        store_row<T, EPC, IN>(y + (h + i * m.gpt) * hs, a[i], b[i], h + i * m.gpt < m.H, l);
     }
+    if constexpr (KU == 1) store_row<T, EPC, IN>(y + h * hs, a[0], b[0], h < m.H, l);
 }
 
 // f<EPC, LPR, IN>() for the chunks these rows allow.

@@ -22,7 +22,6 @@ struct NormRopeSide {
 struct NormRopeParams {
     NormRopeSide side[2];
     RopeArgs r;
-    AxesArgs axes;
     const int32_t* positions;    // [S] or [B, S]; null: 0 .. S - 1 (with axes: of axis 0)
     long long positions_stride;  // between sequences (0: shared)
     float* part_dw;              // [workgroup][D]
@@ -30,6 +29,7 @@ struct NormRopeParams {
     int interleaved;  // pairs (2i, 2i + 1), else (i, i + R/2)
     int w32;          // weights are float, else T
     int vec;          // every row in whole aligned 16-byte chunks, pairs in them
+    AxesArgs axes;
 };
 
 // Workgroups that share a side's rows in the gradient, at most: the weight's

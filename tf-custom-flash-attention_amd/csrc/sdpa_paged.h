@@ -35,7 +35,6 @@ struct PagedParams {
     TokenStrides qs, os;
     float* part_o;   // [slot][BM][D_v]: unnormalised O of a part
     float* part_ml;  // [slot][BM][2]: the reference of its weights (log2) and their sum
-    struct CutTile* cut;  // (cache in 4 bits, shares) what each workgroup leaves to merge
     int H_kv, G, D_qk, D_v;
     float scale;
     int causal;
@@ -44,6 +43,7 @@ struct PagedParams {
     int divide;       // parts: whether tiles may be divided
     int min_chunk;    // parts: key blocks of a part, at least
     int one_per_cu;   // parts: chunks up to this come for half the workgroups (0: not)
+    struct CutTile* cut;  // (cache in 4 bits, shares) what each workgroup leaves to merge
 };
 
 // Key blocks of 64 of a part, at least.  16 tokens of 8 heads on one, D 128, over 2300:
