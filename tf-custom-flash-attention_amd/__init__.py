@@ -16,8 +16,9 @@ CPU fallback: if the library is missing, every entry point raises.
 
 Around the op (:mod:`.heads`): ``qk_norm_rope`` and its gradient norm and
 rotate the queries and keys of a layer into the layout that ``sdpa`` reads;
-``kv_append`` puts new tokens into the pages of a cache and ``paged_sdpa``
-attends over them.
+``kv_reserve`` gives new tokens pages of a cache, ``kv_append`` puts them there and
+``paged_sdpa`` attends over them; ``kv_append_fp4``, ``kv_read_fp4`` and
+``paged_sdpa_fp4`` do so with a cache in 4 bits (``fp4_cache``).
 """
 from __future__ import annotations
 

@@ -8,6 +8,10 @@
 // of a sequence; of a window of W packed tokens it takes each run of such that begins in it.
 // The words of a run that does not fill its 8 places are read, and the other tokens' codes
 // kept.
+// 8643 tokens of 4 sequences, 32 + 8 + 8 heads of 128, fp16, three positions: keys and values 27 us
+// (45 MB), most of it the keys' fp64, queries 32 (142 MB, 4.4 TB/s) by a kernel of their own (one
+// kernel for both 76 us where two took 68).  64 single tokens, without norm: 5.4 us, a chain of
+// loads.  The read of 8643 tokens: 14.7 us (45 MB).
 // Keys: norm and rotation in fp64, then rounded to fp32 and to 4 bits.  A code changes
 // by a whole step where a value crosses a border, so with fp32 sums the codes of a token would go
 // by the order of the additions, one in some 10^6 values; in fp64 they do not, in

@@ -15,6 +15,12 @@
 // A wave loads its next block's words as soon as this one's are used up.
 // fp32 queries are cut into three parts (33 bits), after a row's largest has been brought to
 // 2^14 by a power of two.
+//
+// Bound by memory between a start and an end that do not read: 64 sequences of 600 to 16384 tokens, 32
+// heads on 8, D 128 (298 MB): 69 us and the merge 4.6, 4.3 TB/s, some 6 in the loop (over fp16 pages 217
+// and 9).  11 vector instructions a matrix instruction, matrix cores busy 13 %.  4 sequences of
+// 4096, 16 heads (36 MB): 13.9 and 3.9, mostly a chain: plan, page table, queries, first block, merge.
+// Four workgroups a CU with blocks of 32 keys: 71 and 17 us; two blocks ahead: no change.
 #include "sdpa_launch.h"
 #include "sdpa_paged_fp4.h"
 

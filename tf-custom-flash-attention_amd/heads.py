@@ -1,5 +1,6 @@
 """The steps around ``sdpa`` of a layer of a language model: norm and rotation
-of queries and keys (with the gradient), and a paged cache of keys and values.
+of queries and keys (with the gradient), and a paged cache of keys and values, in
+fp16, fp32 or 4 bits.
 
 As with the op itself, torch tensors are device memory and streams only; the
 arithmetic runs in the HIP kernels behind ``include/sdpa_hip.h``, fp16 or fp32.
