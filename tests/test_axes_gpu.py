@@ -223,3 +223,19 @@ def test_captured(pkg):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+
+
+def test_axes_that_change_before_the_backward_pass(pkg):
+    """The gradient is that of the call, whatever becomes of the list that the axes came in."""
+    T, B, S, H_q, H_kv, D = F32, 1, 9, 2, 1, 64
+    g = torch.Generator().manual_seed(3)
+    q, k, dq, dk = (torch.randn(s, generator=g).to(DEV) for s in ((B, S, H_q, D), (B, S, H_kv, D), (H_q, S, D), (H_kv, S, D)))
+    cos, sin = (t.to(DEV) for t in R64.tables(40, D))
+    pos = torch.randint(0, 40, (3, S), generator=g, dtype=torch.int32).to(DEV)
+    axes = [0, 1] * 16
+    want = pkg.qk_norm_rope_grad(dq, dk, q, k, cos, sin, positions=pos, axes=tuple(axes))
+    x = [t.clone().requires_grad_() for t in (q, k)]
+    out = pkg.qk_norm_rope_autograd(*x, cos, sin, positions=pos, axes=axes)
+    axes[:] = [2] * 32
+    got = torch.autograd.grad(out, x, (dq, dk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

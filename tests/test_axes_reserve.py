@@ -41,6 +41,22 @@ def test_axes_refusals(pkg, axes, positions, dtype, tables, message):
         _refused(pkg, message, fn, *d, q, k, cos, cos, **kw)
 
 
+@pytest.mark.parametrize("one", [True, 1.0, [1], None])
+def test_axes_that_equal_numbers(pkg, one):
+    """What is no integer is refused, also where integers of its value came before it."""
+    q, cos, pos = _meta(2, 5, 4, 32), _meta(7, 16, dtype=torch.float32), _meta(2, 5, dtype=I32)
+    for axes, message in ((((0, 1) * 8), "on the GPU"), ((0, 1) * 7 + (0, one), "0, 1, 2 or 3")):
+        _refused(pkg, message, pkg.qk_norm_rope, q, q, cos, cos, positions=pos, axes=axes)
+
+
+def test_append_positions_need_whole_tables(pkg):
+    cache, table = _meta(4, 2, 16, 32), _meta(7, dtype=torch.float32)
+    batch = _meta(1, 3, dtype=I32), _meta(2, dtype=I32), _meta(1, dtype=I32)
+    for axes in (None, (0,) * 16):
+        _refused(pkg, "cos and sin must have one shape", pkg.kv_append, _meta(6, 2, 32), _meta(6, 2, 32), cache, cache, *batch, table,
+                 table, positions=_meta(*((6,) if axes is None else (1, 6)), dtype=I32), axes=axes)
+
+
 @pytest.mark.parametrize("axes,positions,message", [
     (None, (3, 6), "must have shape"),
     ((0, 1) * 8, (6,), "must have shape"),

@@ -136,12 +136,20 @@ def _check_qk(q, k):
     _sizes_fit(q=q, k=k)
 
 
-@functools.lru_cache(maxsize=64)
 def _pair_axes(axes, pairs):
     """The axis of every rotated pair, for the C entries, and the largest."""
+    axes = tuple(axes)
+    # (before the numbers are looked up, among which 1, True and 1.0 are one key)
+    if set(map(type, axes)) - {int}:
+        _fail("axes are 0, 1, 2 or 3")
+    return _axes_bytes(axes, pairs)
+
+
+@functools.lru_cache(maxsize=64)
+def _axes_bytes(axes, pairs):
     if len(axes) != pairs:
         _fail(f"axes has {len(axes)} entries, the tables {pairs} pairs")
-    if any(type(a) is not int or not 0 <= a < 4 for a in axes):
+    if any(not 0 <= a < 4 for a in axes):
         _fail("axes are 0, 1, 2 or 3")
     return (ctypes.c_uint8 * max(1, pairs))(*axes), max(axes, default=-1)
 
@@ -154,7 +162,7 @@ def _axes_args(axes, positions, cos, *shape):
         _fail("axes need positions")
     if cos.dim() != 2:
         _fail("cos and sin must have one shape [positions, rotated features / 2]")
-    pairs, top = _pair_axes(tuple(axes), cos.shape[1])
+    pairs, top = _pair_axes(axes, cos.shape[1])
     n = positions.shape[0] if positions.dim() else 0
     _int32("positions", positions, n, *shape)
     if top >= n:
@@ -186,7 +194,7 @@ def _plain_rope(q, k, cos, sin, q_weight, k_weight, positions, norm, axes):
     else:
         sp = positions.shape
         if axes is not None:
-            pairs, top = _pair_axes(axes if type(axes) is tuple else tuple(axes), sc[1])
+            pairs, top = _pair_axes(axes, sc[1])
             if not 2 <= len(sp) <= 3 or not top < sp[0] <= _MOST:
                 return None
             n_axes, sp = sp[0], sp[1:]
@@ -338,6 +346,8 @@ def qk_norm_rope_autograd(q, k, cos, sin, q_weight=None, k_weight=None, position
     global _fn
     if _fn is None:
         _fn = _make_function()
+    if axes is not None:
+        axes = tuple(axes)  # (a list may change before the backward pass)
     return _fn.apply(q, k, cos, sin, q_weight, k_weight, positions, eps, norm, interleaved, fold_heads, axes)
 
 
@@ -546,6 +556,8 @@ def _append_positions(positions, axes, cos, n, device):
     if axes is None:
         if cos is None:
             _fail("positions need cos and sin")
+        if cos.dim() != 2:
+            _fail("cos and sin must have one shape [positions, rotated features / 2]")
         _int32("positions", positions, n)
         positions, axes = positions[None], (0,) * cos.shape[1]
     pairs, n_axes = _axes_args(axes, positions, cos, n)
