@@ -16,7 +16,7 @@
 //
 // Bound by issue, as the kernel over fp16 pages is: 10 vector instructions a matrix instruction
 // (there 7.3), matrix cores busy 36 %.  512 tokens over 16000, 32 heads on 8, D 128: 164 us a call, 806
-// TFLOP/s (over fp16 pages 157 to 159; a product of 8192^3 1212), 12 of it the merge.  300 tokens over 2300
+// TFLOP/s (172 in another run; over fp16 pages 157 to 159; a product of 8192^3 1212), 12 of it the merge.  300 tokens over 2300
 // and 3 single ones, 16 heads on 4, D 64, fp32: 24 and 7 us (over fp32 pages 33 and 7).
 #include "sdpa_launch.h"
 #include "sdpa_paged_fp4.h"
