@@ -142,12 +142,19 @@ __device__ __forceinline__ void cut_queries(half8 (&part)[N], float (&x)[8]) {
         }
 }
 
-// Power of two that brings a row's largest |query| near 2^14 (within what a float
-// holds; queries below 2^-100 lose bits), and its inverse.
-__device__ __forceinline__ void query_factor(float most, float& f, float& inv) {
+// The power of two that brings a row's largest |query| near 2^14 (within what a float holds; queries
+// below 2^-100 lose bits), negated for a scale below 0, and the scale (log2 units) of the products of such
+// queries.  That one stays a normal number, as 0 times the -inf of a masked score is NaN: the
+// scores, below 2^14 128 61440 < 2^37, are 0 by 2^-126 as by what is less.  Scale 0: the queries are 0.
+__device__ __forceinline__ void query_factor(float most, float sl2_raw, float& f, float& sl2) {
     const int up = min(max(14 - (int)(__float_as_uint(most) >> 23) + 127, -113), 114);
-    f = __uint_as_float((uint32_t)(127 + up) << 23);
-    inv = __uint_as_float((uint32_t)(127 - up) << 23);
+    f = __builtin_copysignf(__uint_as_float((uint32_t)(127 + up) << 23), sl2_raw);
+    sl2 = fabsf(sl2_raw) * __uint_as_float((uint32_t)(127 - up) << 23);
+    sl2 = sl2 < 0x1p-126f ? 0x1p-126f : sl2;  // (NaN stays)
+    if (sl2_raw == 0.f) {
+        f = 0.f;
+        sl2 = 1.f;
+    }
 }
 
 }  // namespace

@@ -93,13 +93,12 @@ void paged_fp4_kernel(const PagedParams p) {
                         most = fmaxf(most, fabsf(v[e]));
                     }
                 }
-            float f, inv;
-            query_factor(xhalf_max(most), f, inv);
-            sl2 *= inv;
+            float f;
+            query_factor(xhalf_max(most), sl2_raw, f, sl2);
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[ks][e] *= neg ? -f : f;
+                for (int e = 0; e < 8; ++e) x[ks][e] *= f;
                 cut_queries(q[ks], x[ks]);
             }
         }

@@ -177,14 +177,13 @@ void paged_fp4_small_kernel(const PagedParams p) {
                 for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)raw[w8][e]));
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
-            float f, inv;
-            query_factor(most, f, inv);
-            sl2 *= inv;
+            float f;
+            query_factor(most, sl2_raw, f, sl2);
 #pragma unroll
             for (int w8 = 0; w8 < KW; ++w8) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (float)raw[w8][e] * (sl2_raw < 0.f ? -f : f);
+                for (int e = 0; e < 8; ++e) x[e] = (float)raw[w8][e] * f;
                 cut_queries(q[w8], x);
             }
         }
