@@ -123,7 +123,7 @@ int norm_rope_entry(bool grad, int dtype, const void* const (&x)[2], const int64
         p.part_dw = static_cast<float*>(workspace);
     }
     p.r = sdpa::RopeArgs{cos, sin, table_rows, R, norm != 0, eps, 1.f / (float)D};
-    p.positions = positions;
+    p.positions = R > 0 ? positions : nullptr;  // (on no axis there are none to read)
     p.positions_stride = positions_per_batch ? S : 0;
     p.B = B;
     p.S = S;
