@@ -299,7 +299,8 @@ int sdpa_hip_qk_norm_rope_axes_grad(int dtype, const void* d_q_out, const int64_
  * dense matrix as the op's k and v are.  T new tokens are packed, sequence after
  * sequence; device arrays of int32 say what belongs where:
  *   q_starts [N + 1]    sequence s has the new tokens q_starts[s] ..
- *                       q_starts[s + 1] - 1 (none: not in this call);
+ *                       q_starts[s + 1] - 1 (none, or not all of them among the
+ *                       T: append and attention leave the sequence out);
  *   kv_lens [N]         its cached tokens, the new ones among them, last;
  *   page_table [N, width] (rows page_table_stride apart): token j of s is row
  *                       j % page_size of page page_table[s][j / page_size].
@@ -321,7 +322,8 @@ int sdpa_hip_qk_norm_rope_axes_grad(int dtype, const void* d_q_out, const int64_
  * Out: q_starts [N + 1] and kv_lens_out [N] as below (kv_lens_out may be kv_lens);
  * free_count_out (may be free_count); for every one of the T packed tokens its
  * place in the sequence, positions [T], and slots [T], page * page_size + row, -1 for
- * a token without a page; both -1 behind the last sequence.  Lengths below 0 count as
+ * a token without a page; both -1 behind the last sequence.  (With fewer than q_starts[N] tokens T
+ * the sequences that reach past them have their pages and lengths all the same.)  Lengths below 0 count as
  * 0, cached ones above width * page_size and new ones above T as those.  No two
  * rows of the table may overlap.  T <= 2^30 - 1, width * page_size + T below 2^31.  */
 int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
@@ -334,7 +336,7 @@ int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const in
  * rotated by its place in the sequence on the way as above (R = 0: not
  * rotated), and the queries of the same tokens, normed and rotated, to q_out
  * (H_q = 0: none).  q, k, v, q_out: [T, H, D] with dense features and strides
- * {token, head} in elements.  q_out may be q.  Tokens behind the last sequence leave
+ * {token, head} in elements.  q_out may be q.  Tokens of no sequence leave
  * everything as it was; a token whose place is outside of the table's columns or
  * of the pages is not appended, and its row of q_out is NaN.  Two tokens of one
  * call must not have the same place.  D_qk or D_v may be 0: nothing of that width
@@ -423,7 +425,8 @@ int sdpa_hip_kv_append_fp4(int dtype, const void* k, const int64_t* k_strides, c
 
 /* The values of the T tokens of a batch out of such a cache: k [T, H_kv, D_qk] and v
  * [T, H_kv, D_v] of dtype, dense, 16-byte aligned.  Rows of a token without a place are NaN,
- * those of no sequence stay as they were.                                       */
+ * those of no sequence stay as they were; of a sequence that reaches past the T tokens those
+ * that lie among them are read.                                                 */
 int sdpa_hip_kv_read_fp4(int dtype, const void* k_cache, const void* v_cache, void* k, void* v,
                          const int32_t* page_table, int64_t page_table_stride, const int32_t* q_starts,
                          const int32_t* kv_lens, int N, int T, int width, int pages, int page_size, int H_kv, int D_qk,

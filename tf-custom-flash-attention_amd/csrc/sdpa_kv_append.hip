@@ -14,7 +14,8 @@
 // writes are alike, reaches 5.9 with loads past the caches; here they have not been tried.
 // 64 single tokens: 4.6 us.
 //
-// A token of no sequence (behind the last) leaves everything as it was.  One
+// A token of no sequence (behind the last), or of one that reaches past the T tokens,
+// leaves everything as it was.  One
 // whose place is outside the table's columns or the cache's pages is not
 // appended, and its query row is NaN; a position outside the rotation tables
 // makes the rotated rows NaN.

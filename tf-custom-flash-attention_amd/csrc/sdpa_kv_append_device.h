@@ -67,7 +67,7 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendM
     }
     if (!in_batch || count == 0) return;
     const int s = count - 1, qs = bt.q_starts[s], qe = bt.q_starts[s + 1];
-    if (tok < qs || tok >= qe) return;
+    if (tok < qs || tok >= qe || qs < 0 || qe > bt.T) return;  // (as attention leaves them out)
     const long long pos = (long long)bt.kv_lens[s] - qe + tok;
     const long long pg = pos >> bt.page_log2;
     int page = -1;

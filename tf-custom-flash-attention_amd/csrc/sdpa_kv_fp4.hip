@@ -34,8 +34,9 @@ struct Fp4Run {
 };
 
 // work(run) for every run that begins in the window of W packed tokens from tok0 on.  The wave's
-// lanes look for them together: lane i < W has token tok0 + i.
-template <int W, typename F>
+// lanes look for them together: lane i < W has token tok0 + i.  WHOLE: sequences that do not lie
+// in the T tokens are left out, else those of their tokens that do are taken.
+template <int W, bool WHOLE, typename F>
 __device__ __forceinline__ void each_run(const PagedBatch& bt, int tok0, F&& work) {
     const int lane = threadIdx.x & 63;
     int count = 0;  // sequences that begin at or before the lane's token
@@ -52,7 +53,7 @@ __device__ __forceinline__ void each_run(const PagedBatch& bt, int tok0, F&& wor
     long long pos = 0;
     if (lane < W && tok < bt.T && count > 0) {
         const int s = count - 1, qs = bt.q_starts[s], qe = bt.q_starts[s + 1];
-        if (tok >= qs && tok < qe) {
+        if (tok >= qs && tok < qe && !(WHOLE && (qs < 0 || qe > bt.T))) {
             pos = (long long)bt.kv_lens[s] - qe + tok;
             const long long pg = pos >> bt.page_log2;
             if (pos >= 0 && pg < bt.width) page = bt.page_table[s * bt.table_stride + pg];
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(64 * kAppendWaves, W > 1 ? 4 : 1) void kv_append_fp
     const bool values = u >= n;
     if (values) u -= n;
     const int window = (int)(u / (unsigned)p.H_kv), h = (int)(u - (long long)window * p.H_kv);
-    each_run<W>(p.batch, window * W, [&](const Fp4Run& run) __attribute__((always_inline)) {
+    each_run<W, true>(p.batch, window * W, [&](const Fp4Run& run) __attribute__((always_inline)) {
         if (run.page < 0) return;
         if (KINDS == 1 || values) append_values<T, (EPC > 1)>(p, run, h, lds[wave]);
         if (KINDS == 1 || !values) append_keys<T, EPC, LPR, IN, AX>(p, run, h, lds[wave]);
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_read_fp4_kernel(const Fp
     const int D = values ? p.D_v : p.D_qk, log2 = p.batch.page_log2;
     T* const out = static_cast<T*>(values ? p.v : p.k) + (long long)h * D;
     const long long token = (long long)p.H_kv * D;  // elements between tokens
-    each_run<W>(p.batch, window * W, [&](const Fp4Run& run) __attribute__((always_inline)) {
+    each_run<W, false>(p.batch, window * W, [&](const Fp4Run& run) __attribute__((always_inline)) {
         const bool none = run.page < 0;
         const unsigned char* head = static_cast<const unsigned char*>(values ? p.v_cache : p.k_cache) +
                                     ((long long)(none ? 0 : run.page) * p.H_kv + h) * fp4_head_bytes(D, log2);

@@ -482,7 +482,9 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
     slots (int64, page * page_size + row; -1 without a page), -1 behind the last.  ``in_place``: kv_lens
     and free_count are the tensors given, changed (for a captured step that is replayed).
 
-    More tokens than ``total`` have no rows: ``kv_append`` and ``paged_sdpa`` leave out sequences that reach past it.
+    More tokens than ``total`` have no rows: ``kv_append`` and ``paged_sdpa`` leave out the sequences that reach past it, whole.
+    Those have their pages and lengths all the same (of a sequence's new tokens ``total`` count at most), so that their new
+    tokens are to be appended, by a further call with q_starts of its own, before anything is attended over them.
     """
     N, width, capacity, device = _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished)
     table, lens, fresh, pages, count, ended = (page_table.data_ptr(), kv_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
@@ -578,7 +580,8 @@ def kv_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos=None, s
     the result is [T, H_q, D_qk], else None.  ``positions``: what the tokens are rotated by instead of their
     places j: int32 [T], or [axes, T] with ``axes``, the axis of each rotated pair, as in ``qk_norm_rope``.
 
-    Tokens behind the last sequence are skipped (their rows of the result are not written).  A token
+    Tokens behind the last sequence are skipped (their rows of the result are not written), and so are those of a
+    sequence that reaches past the T tokens.  A token
     without a place in the table or the cache is not appended and its query row is NaN.  No two tokens
     of a call may have the same place.  D_qk or D_v may be 0 (a cache of keys or of values alone).
     Any width up to 128 can be cached; ``paged_sdpa`` reads multiples of 8 (fp16) or 4 (fp32).
@@ -668,8 +671,8 @@ def kv_read_fp4(k_cache, v_cache, page_table, q_starts, kv_lens, total: int, dty
     """The values of a batch's tokens out of a cache in 4 bits: ``(k, v)``, [total, H_kv, D] in ``dtype``.
 
     The batch as in ``kv_append``: of sequence s its last q_starts[s + 1] - q_starts[s] cached tokens (all of them where that
-    is kv_lens[s]).  The values are exact (fp16 or fp32).  Rows of a token without a place are NaN,
-    those behind the last sequence arbitrary.
+    is kv_lens[s]; those that lie in the first ``total`` rows).  The values are exact (fp16 or fp32).  Rows of a token
+    without a place are NaN, those behind the last sequence arbitrary.
     """
     batch = _plain_batch(k_cache.device, _U8, k_cache, v_cache, page_table, q_starts, kv_lens)
     if batch is None:
