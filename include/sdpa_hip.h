@@ -332,6 +332,18 @@ int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const in
                         int32_t* positions, int64_t* slots, int N, int T, int width, int page_size, int capacity,
                         hipStream_t stream);
 
+/* The same, and *pages_short (NULL: not wanted): the pages that the stack lacked, that is the columns
+ * that got -1 for want of one.  A column that got -1 stays so (tokens that belong there are in no
+ * page, and rows that see them NaN) until its sequence is finished, which gives back the pages it has.
+ * Where kv_lens_out and free_count_out are memory of their own, a call may also be taken back, by a call with the
+ * same kv_lens and free_count: with other new_lens, with more sequences finished, but with none
+ * that was finished and got new tokens.                                         */
+int sdpa_hip_kv_reserve_counted(int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                                const int32_t* new_lens, const uint8_t* finished, int32_t* free_pages,
+                                const int32_t* free_count, int32_t* q_starts, int32_t* kv_lens_out,
+                                int32_t* free_count_out, int32_t* pages_short, int32_t* positions, int64_t* slots, int N,
+                                int T, int width, int page_size, int capacity, hipStream_t stream);
+
 /* Keys and values of the new tokens into their places, k normed (norm) and
  * rotated by its place in the sequence on the way as above (R = 0: not
  * rotated), and the queries of the same tokens, normed and rotated, to q_out

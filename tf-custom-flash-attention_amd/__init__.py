@@ -127,6 +127,8 @@ def library():
     batch = [i32p, ctypes.c_int64, i32p, i32p]  # page table and its row stride, q_starts, kv_lens
     L.sdpa_hip_kv_reserve.restype = i32
     L.sdpa_hip_kv_reserve.argtypes = [i32p, ctypes.c_int64] + [vp] * 10 + [i32] * 5 + [vp]
+    L.sdpa_hip_kv_reserve_counted.restype = i32
+    L.sdpa_hip_kv_reserve_counted.argtypes = [i32p, ctypes.c_int64] + [vp] * 11 + [i32] * 5 + [vp]
     L.sdpa_hip_kv_append.restype = i32
     L.sdpa_hip_kv_append.argtypes = ([i32] + [vp, i64p] * 2 + [vp, vp] + [vp, i64p] * 2 + rope + batch + [i32] * 10 +
                                      [f32, i32, i32, vp])

@@ -303,6 +303,15 @@ int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const in
                         const uint8_t* finished, int32_t* free_pages, const int32_t* free_count, int32_t* q_starts,
                         int32_t* kv_lens_out, int32_t* free_count_out, int32_t* positions, int64_t* slots, int N, int T,
                         int width, int page_size, int capacity, hipStream_t stream) {
+    return sdpa_hip_kv_reserve_counted(page_table, page_table_stride, kv_lens, new_lens, finished, free_pages, free_count, q_starts,
+                                       kv_lens_out, free_count_out, nullptr, positions, slots, N, T, width, page_size, capacity,
+                                       stream);
+}
+
+int sdpa_hip_kv_reserve_counted(int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens, const int32_t* new_lens,
+                                const uint8_t* finished, int32_t* free_pages, const int32_t* free_count, int32_t* q_starts,
+                                int32_t* kv_lens_out, int32_t* free_count_out, int32_t* pages_short, int32_t* positions,
+                                int64_t* slots, int N, int T, int width, int page_size, int capacity, hipStream_t stream) {
     if (N < 0 || T < 0 || width < 0 || capacity < 0) return SDPA_ERR_NEGATIVE_DIM;
     if (!page_size_ok(page_size)) return SDPA_ERR_PAGE_SIZE;
     if (N > 0x7FFFFFFF - 65536 || T > 0x3FFFFFFF || (long long)width * page_size + T > 0x7FFFFFFFLL - 65536)
@@ -322,6 +331,7 @@ int sdpa_hip_kv_reserve(int32_t* page_table, int64_t page_table_stride, const in
     p.q_starts = q_starts;
     p.kv_lens_out = kv_lens_out;
     p.free_count_out = free_count_out;
+    p.pages_short = pages_short;
     p.positions = positions;
     p.slots = slots;
     p.N = N;

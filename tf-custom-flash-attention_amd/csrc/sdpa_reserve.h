@@ -17,6 +17,7 @@ struct ReserveParams {
     int32_t* q_starts;        // [N + 1]
     int32_t* kv_lens_out;     // [N], maybe kv_lens
     int32_t* free_count_out;  // [1], maybe free_count
+    int32_t* pages_short;     // [1] or null
     int32_t* positions;       // [T]
     int64_t* slots;           // [T]
     int N, T, width, capacity, page_log2;

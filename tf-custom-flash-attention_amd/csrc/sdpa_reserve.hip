@@ -141,6 +141,7 @@ __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(const ReserveP
     if (tid == 0) {
         p.q_starts[p.N] = (int32_t)min(tokens, 0x7FFFFFFFLL);
         *p.free_count_out = (int32_t)max(count - taken, 0LL);
+        if (p.pages_short) *p.pages_short = (int32_t)min(max(taken - count, 0LL), 0x7FFFFFFFLL);
     }
     if (p.fill)
         for (long long t = tokens + tid; t < p.T; t += kReserveThreads) {

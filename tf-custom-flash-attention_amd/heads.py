@@ -467,7 +467,7 @@ def _vector(name, t, n, *dtypes):
 
 
 def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size: int, total: int, finished=None,
-               in_place: bool = False):
+               in_place: bool = False, short=None):
     """Pages for the new tokens of a batch, and where each token goes, all on the GPU.
 
     page_table int32 [N, pages per sequence] and kv_lens int32 [N] say what the N sequences hold,
@@ -482,11 +482,17 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
     slots (int64, page * page_size + row; -1 without a page), -1 behind the last.  ``in_place``: kv_lens
     and free_count are the tensors given, changed (for a captured step that is replayed).
 
+    ``short`` (int32 [1]) receives how many pages the stack lacked.  A column that got -1 for want of one stays so, and
+    what sees its tokens is NaN, until its sequence is finished: that gives back the pages it has, and it
+    can begin anew at once.  Where not ``in_place``, the call can also be made again, with the same kv_lens and free_count,
+    fewer new_lens or more of ``finished``, as long as no sequence that was finished got new tokens.
+
     More tokens than ``total`` have no rows: ``kv_append`` and ``paged_sdpa`` leave out the sequences that reach past it, whole.
     Those have their pages and lengths all the same (of a sequence's new tokens ``total`` count at most), so that their new
     tokens are to be appended, by a further call with q_starts of its own, before anything is attended over them.
     """
-    N, width, capacity, device = _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished)
+    N, width, capacity, device = _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished,
+                                                short)
     table, lens, fresh, pages, count, ended = (page_table.data_ptr(), kv_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
                                                free_count.data_ptr(), _ptr(finished))
     # what is written shares memory with nothing else
@@ -500,6 +506,11 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
             _fail("page_table, free_pages, kv_lens and free_count must not share memory")
     if pages < table + table_bytes and table < pages + 4 * capacity:
         _fail("page_table, free_pages, kv_lens and free_count must not share memory")
+    if short is not None:
+        lack = short.data_ptr()
+        for start, size in reads + [(table, table_bytes), (pages, 4 * capacity)]:
+            if start < lack + 4 and lack < start + size:
+                _fail("short must be memory of its own")
     new = kv_lens.new_empty
     if in_place:
         for start, size in reads[1:]:
@@ -511,17 +522,21 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
         out = Reserved(new(N + 1), kv_lens, free_count, new(total), new(total, dtype=torch.int64))
     else:
         out = Reserved(new(N + 1), new(N), new(1), new(total), new(total, dtype=torch.int64))
-    _call(library().sdpa_hip_kv_reserve, device, table, stride, lens, fresh, ended, pages, count, out[0].data_ptr(),
-          out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), N, total, width, page_size, capacity)
+    L = library()
+    entry, lacks = (L.sdpa_hip_kv_reserve, ()) if short is None else (L.sdpa_hip_kv_reserve_counted, (short.data_ptr(),))
+    _call(entry, device, table, stride, lens, fresh, ended, pages, count, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+          *lacks, out[3].data_ptr(), out[4].data_ptr(), N, total, width, page_size, capacity)
     return out
 
 
-def _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished):
+def _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size, total, finished, short):
     """Checks of ``kv_reserve`` but for shared memory: (N, width, capacity, device)."""
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
         _fail("page_table must be [sequences, pages per sequence]")
     N, width = page_table.shape
     device = page_table.device
+    if short is not None:
+        _vector("short", short, 1, _I32)
     one, sizes = (N,), type(page_size) is int and type(total) is int and 0 <= total <= _MOST and 0 < page_size <= _MOST
     # (usual arguments by a few comparisons, others one by one)
     if (sizes and page_table.dtype is _I32 and page_table.is_contiguous() and device.type == "cuda"
@@ -532,7 +547,8 @@ def _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_s
             and kv_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
             and kv_lens.device == device and new_lens.device == device and free_pages.device == device and free_count.device == device
             and (finished is None or (isinstance(finished, torch.Tensor) and finished.dtype in (torch.bool, _U8)
-                                      and finished.shape == one and finished.is_contiguous() and finished.device == device))):
+                                      and finished.shape == one and finished.is_contiguous() and finished.device == device))
+            and (short is None or short.device == device)):
         capacity = free_pages.shape[0]
         if N + width + capacity <= _MOST:
             return N, width, capacity, device
@@ -548,7 +564,8 @@ def _check_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_s
     if not sizes:
         _fail("page_size and total must be sizes")
     _sizes_fit(page_table=page_table, free_pages=free_pages)
-    _on_device(device, kv_lens=kv_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count, finished=finished)
+    _on_device(device, kv_lens=kv_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count, finished=finished,
+               short=short)
     return N, width, free_pages.shape[0], device
 
 
