@@ -692,9 +692,12 @@ def kv_read_fp4(k_cache, v_cache, page_table, q_starts, kv_lens, total: int, dty
     without a place are NaN, those behind the last sequence arbitrary.
     """
     batch = _plain_batch(k_cache.device, _U8, k_cache, v_cache, page_table, q_starts, kv_lens)
-    if batch is None:
+    plain = batch is not None
+    if not plain:
         _check_cache(k_cache, v_cache, _U8)
         batch = _check_batch(page_table, q_starts, kv_lens)
+    D_qk, D_v = _fp4_features(k_cache), _fp4_features(v_cache)
+    if not plain:
         _on_device(k_cache.device, v_cache=v_cache, page_table=page_table, q_starts=q_starts, kv_lens=kv_lens)
     if type(total) is not int or not 0 <= total <= _MOST:
         _fail("total must be a size")
@@ -702,7 +705,6 @@ def kv_read_fp4(k_cache, v_cache, page_table, q_starts, kv_lens, total: int, dty
         _fail(f"T must be half or float, got {dtype}")
     N, width = batch
     pages, H_kv, page, _ = k_cache.shape
-    D_qk, D_v = _fp4_features(k_cache), _fp4_features(v_cache)
     k, v = (torch.empty((total, H_kv, D), dtype=dtype, device=k_cache.device) for D in (D_qk, D_v))
     _call(library().sdpa_hip_kv_read_fp4, k_cache.device, _CODES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(),
           v.data_ptr(), page_table.data_ptr(), page_table.stride(0), q_starts.data_ptr(), kv_lens.data_ptr(), N, total, width,
