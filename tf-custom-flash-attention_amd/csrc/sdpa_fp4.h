@@ -21,7 +21,6 @@
 
 namespace sdpa {
 
-constexpr int kFp4Group = 32;    // features that share a scale
 constexpr float kFp4Most = 10240.f;  // the largest scale
 
 // Bytes of one head of a page, and where its scales begin.

@@ -8,8 +8,6 @@
 namespace sdpa {
 namespace {
 
-typedef uint32_t uint3v __attribute__((ext_vector_type(3)));
-
 __device__ __forceinline__ floatx4 mfma16_f16(const half8& a, const half8& b, const floatx4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -20,7 +18,7 @@ hipError_t with_fp4_dim(int d, F&& f) {
     return with_dim(d, f);
 }
 
-// The same in scalar registers.
+// An address that is the same in every lane, in scalar registers.
 __device__ __forceinline__ fp4_ptr uniform(fp4_ptr p) {
     const uint64_t a = (uint64_t)p;
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
