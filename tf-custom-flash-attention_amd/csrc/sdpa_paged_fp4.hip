@@ -12,7 +12,10 @@
 // neither is swizzled or transposed, but that the keys are dealt to the rows of the K operand in
 // the order in which a lane holds 8 neighbouring scores (which meet 8 tokens of a V word), and K words are
 // written 4 lanes apart by the part of the key (whose lanes would meet in a bank).
-// fp32 queries are cut into three fp16 parts, and weights into two.
+// fp32 queries are cut into three fp16 parts, and weights into two.  With fp16 queries weights are one
+// part, 11 bits, and two only where few keys carry a row (kSplitLog2), the rule of every tile of
+// 128 rows over fp16: 512 tokens over 16000, 32 heads on 8, D 128, 170 us, o off by 2.9e-4 of its norm
+// (its own rounding is 2.1e-4 of that); two parts throughout 213 us and 2.1e-4.
 //
 // Bound by issue, as the kernel over fp16 pages is: 10 vector instructions a matrix instruction
 // (there 7.3), matrix cores busy 36 %.  512 tokens over 16000, 32 heads on 8, D 128: 164 us a call, 806

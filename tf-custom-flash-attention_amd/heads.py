@@ -749,7 +749,9 @@ def paged_sdpa_fp4(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale: fl
                    max_q_len=None, out=None):
     """``paged_sdpa`` over a cache in 4 bits (``fp4_cache``, ``kv_append_fp4``): ``(o, stats)``.
 
-    Arguments and results as there; the queries are fp16 or fp32, and the cache's values exact in either.
+    Arguments and results as there; the queries are fp16 or fp32, and the cache's values exact in either.  The weights
+    enter the product with the values in 22 bits, but in 11 for fp16 queries of more than 32 rows (tokens times the
+    query heads of a key head; unless few keys carry a row), as with ``paged_sdpa``.
     """
     return _paged(True, q, k_cache, v_cache, page_table, q_starts, kv_lens, scale, causal_mask, max_q_len, out)
 
