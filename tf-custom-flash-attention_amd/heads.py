@@ -53,13 +53,9 @@ def _on_device(device, **tensors):
             _fail(f"{name} is on {t.device}, not on {device}")
 
 
-# (what torch.cuda.current_device does once the GPU is in use, as it is where its tensors are)
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
 def _call(entry, device, *args):
     """``entry(*args, stream)`` with ``device`` current."""
-    if _current_device() == device.index:
+    if torch.cuda.current_device() == device.index:
         code = entry(*args, _stream_handle(device))
     else:
         with torch.cuda.device(device):
