@@ -47,8 +47,12 @@ struct AppendParams {
     AxesArgs axes;  // (positions [axes][T] instead of the places, where some are used)
 };
 
-// From so many waves of four rows per group of lanes on queries without keys are taken so: 8643 tokens
-// of 32 heads of 128, fp16, one row a group 35.6 us, two 33.9, four 32.3.
+// Queries without keys are taken by four rows per group of lanes from so many waves of such on,
+// where seven eighths of the rows are heads.  us by one row and by four, D 128:
+//   waves (fp16, 32 heads): 512 4.8 and 5.6, 1024 6.5 and 7.1, 2048 11.7 and 10.7, 4096 18.0 and 14.7, 8643 35.4 and
+//     33.9; fp32 (two waves a token): 1024 6.0 and 6.4, 2048 10.1 and 10.0, 4096 16.1 and 14.1
+//   heads (fp16, 32 rows a wave, 8643 tokens): 8 11.8 and 16.4, 16 18.5 and 20.6, 24 25.2 and 24.2, 28 29.3 and
+//     27.0, 40 43 and 43, 48 50 and 48.7, 96 97 and 88; 2100 tokens: 24 9.1 and 9.9, 28 11.2 and 10.6, 40 12.5 and 13.9
 constexpr int kAppendFewWaves = 2048;
 hipError_t launch_kv_append(const AppendParams& p, DType dtype, hipStream_t stream);
 

@@ -59,7 +59,7 @@ hipError_t launch_kv_append_t(const AppendParams& p, hipStream_t stream) {
                                                                         64 * kAppendWaves, 0, stream, p);
         };
         // (queries alone, many of them: of the append in 4 bits)
-        if (p.H_k == 0 && p.H_v == 0 && append_map<L, 4>(p.batch.T, p.H_q).units >= kAppendFewWaves) return run(std::integral_constant<int, 4>{});
+        if (p.H_k == 0 && p.H_v == 0 && append_four_rows<L>(p.batch.T, p.H_q)) return run(std::integral_constant<int, 4>{});
         return run(std::integral_constant<int, 1>{});
     });
 }

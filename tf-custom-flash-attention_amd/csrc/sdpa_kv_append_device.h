@@ -30,6 +30,13 @@ __host__ __device__ inline AppendMap append_map(int tokens, int H) {
     return m;
 }
 
+// Whether queries alone go by four rows per group of lanes (sdpa_kv_append.h).
+template <int LPR>
+inline bool append_four_rows(int tokens, int H) {
+    const AppendMap m = append_map<LPR, 4>(tokens, H);
+    return m.units >= kAppendFewWaves && 8LL * H >= 7LL * 4 * m.gpt * m.splits;
+}
+
 // Unit u of the rows of q (kind 0), k (1) or v (2).
 template <typename T, int EPC, int LPR, bool IN, bool AX, int KU = 1>
 __device__ __forceinline__ void append_rows(const AppendParams& p, const AppendMap& m, long long u, int kind) {
