@@ -12,6 +12,7 @@
 // TB/s, where the rows lie in the last-level cache, 53 us, 4.1 TB/s, from HBM; up to four
 // rows per group of lanes 45 and 53.  The forward of sdpa_norm_rope.hip, whose reads and
 // writes are alike, reaches 5.9 with loads past the caches; here they have not been tried.
+// By positions of the tokens' own, three axes in sections, 56 us from HBM (fp32 93, 434 MB), axes in turn 63.
 // 64 single tokens: 4.6 us.
 //
 // A token of no sequence (behind the last), or of one that reaches past the T tokens,

@@ -9,9 +9,12 @@
 // The words of a run that does not fill its 8 places are read, and the other tokens' codes
 // kept.
 // 8643 tokens of 4 sequences, 32 + 8 + 8 heads of 128, fp16, three positions: keys and values 27 us
-// (45 MB), most of it the keys' fp64, queries 32 (142 MB, 4.4 TB/s) by a kernel of their own (one
-// kernel for both 76 us where two took 68).  64 single tokens, without norm: 5.4 us, a chain of
-// loads.  The read of 8643 tokens: 14.7 us (45 MB).
+// (25 alone; 45 MB, 9 us at a copy's rate), queries 32 (142 MB, 4.4 TB/s) by a kernel of their own
+// (one kernel for both 76 us where two took 68); fp32 34 (27 alone) and 58 (283 MB, 4.9 TB/s).  fp32 in place of
+// the keys' fp64 takes 3.4 us off; by places and without norm they are 30 us, as 22 registers
+// spill there (16 with fp32).  The rest is work that every wave does again for its head: the search for
+// the run, the turn, the weights.  64 single tokens, without norm: 5.4 us, a chain of loads.  The read of 8643 tokens: 14
+// us (45 MB; fp32 22, 80 MB), with the search for each head and for keys and values apart.
 // Keys: norm and rotation in fp64, then rounded to fp32 and to 4 bits.  A code changes
 // by a whole step where a value crosses a border, so with fp32 sums the codes of a token would go
 // by the order of the additions, one in some 10^6 values; in fp64 they do not, in

@@ -179,7 +179,12 @@ inline size_t paged_part_bytes(int D_v, int BM, int target_log2) {
 //   fp16, 64 rows: 187, 150; 22, 24; 60, 55; 101, 63; 43, 30; 19, 23
 //   fp32, 32 rows (from 4 x 2000 on): 20, 28; 44, 89; 64, 124; 60, 34; 19, 26
 //   fp32, 64 rows: 25, 30; 72, 94; 119, 133; 46, 37; 19, 27
-// One long sequence alone loses by the small tiles; lengths are on the device.
+// One sequence alone, 8 and 32 rows, of 1000, 4000, 30000, 120000 tokens:
+//   fp16: 10.5, 17; 14, 18; 45, 28; 60, 45 and 13, 18; 21, 19; 58, 29; 73, 48
+//   fp32: 11.6, 22; 15, 23; 46, 34; 62, 83 and 14, 22; 21, 23; 59, 36; 76, 84
+// so that a long one alone loses by the small tiles where key heads are few (with 8 of them and 4 rows 26 us
+// and 33 at 30000, with 16 22 and 45).  Rows are all that the rule asks: how many tiles there may be, and how long,
+// the host knows too (sequences, key heads, columns of the table), the lengths it does not.
 constexpr int kPagedFp4SmallBM = 16, kPagedFp4TargetLog2 = 9;
 constexpr int kPagedFp4SmallRowsF16 = 32, kPagedFp4SmallRowsF32 = 64;
 // The tile that a workgroup's share begins and does not end, for the merge: its rows
