@@ -208,3 +208,23 @@ def test_steps_that_run_out(pkg, fp4):
         ref = (torch.softmax(z, -1) @ V).transpose(0, 1)
         # (fp16 weights and results: 2^-11 of the values, twice)
         assert float((o[ends[s]:ends[s + 1]].double().cpu() - ref).abs().max()) <= 2.0 ** -10 * float(V.abs().max())
+
+
+@pytest.mark.gpu
+def test_entry_without_a_count(pkg):
+    """The C entry that reports nothing does the same."""
+    page, width, total = 16, 4, 40
+    lens, new, stack, count = [3, 0, 60], [14, 20, 3], [4, 7, 8, 9, 5], 4
+    table = [[0, -1, -1, -1], [-1] * 4, [1, 2, 3, 6]]
+    t, l, n, f, c = _i32(table), _i32(lens), _i32(new), _i32(stack), _i32([count])
+    starts, out, left, places = _i32([0] * 4), _i32([0] * 3), _i32([0]), _i32([0] * total)
+    slots = torch.zeros(total, dtype=torch.int64, device=DEV)
+    rc = pkg.library().sdpa_hip_kv_reserve(t.data_ptr(), width, *(x.data_ptr() for x in (l, n)), None,
+                                           *(x.data_ptr() for x in (f, c, starts, out, left, places, slots)), 3, total, width, page, 5,
+                                           torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    want = reserve(table, lens, new, stack, count, page, total)
+    for g, w in zip((starts, out, left, places, slots), want):
+        assert g.tolist() == (w if isinstance(w, list) else [w])
+    assert t.tolist() == table and f.tolist() == stack

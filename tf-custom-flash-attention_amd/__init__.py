@@ -194,12 +194,18 @@ def _dtype_code(t) -> int:
     raise InvalidArgumentError(f"T must be half or float, got {t.dtype}")
 
 
+_raw_stream = 0  # torch's function of that kind, or None (0: not looked up yet)
+
+
 def _stream_handle(device) -> int:
-    import torch
     # the handle of torch.cuda.current_stream(device) without the Stream object
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None and device.index is not None:
-        return raw(device.index)
+    global _raw_stream
+    if _raw_stream == 0:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
+    import torch
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -53,9 +53,12 @@ def _on_device(device, **tensors):
             _fail(f"{name} is on {t.device}, not on {device}")
 
 
+_current_device = torch.cuda.current_device
+
+
 def _call(entry, device, *args):
     """``entry(*args, stream)`` with ``device`` current."""
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         code = entry(*args, _stream_handle(device))
     else:
         with torch.cuda.device(device):
@@ -502,6 +505,7 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
             _fail("page_table, free_pages, kv_lens and free_count must not share memory")
     if pages < table + table_bytes and table < pages + 4 * capacity:
         _fail("page_table, free_pages, kv_lens and free_count must not share memory")
+    lack = None
     if short is not None:
         lack = short.data_ptr()
         for start, size in reads + [(table, table_bytes), (pages, 4 * capacity)]:
@@ -518,10 +522,8 @@ def kv_reserve(page_table, kv_lens, new_lens, free_pages, free_count, page_size:
         out = Reserved(new(N + 1), kv_lens, free_count, new(total), new(total, dtype=torch.int64))
     else:
         out = Reserved(new(N + 1), new(N), new(1), new(total), new(total, dtype=torch.int64))
-    L = library()
-    entry, lacks = (L.sdpa_hip_kv_reserve, ()) if short is None else (L.sdpa_hip_kv_reserve_counted, (short.data_ptr(),))
-    _call(entry, device, table, stride, lens, fresh, ended, pages, count, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
-          *lacks, out[3].data_ptr(), out[4].data_ptr(), N, total, width, page_size, capacity)
+    _call(library().sdpa_hip_kv_reserve_counted, device, table, stride, lens, fresh, ended, pages, count, out[0].data_ptr(),
+          out[1].data_ptr(), out[2].data_ptr(), lack, out[3].data_ptr(), out[4].data_ptr(), N, total, width, page_size, capacity)
     return out
 
 
